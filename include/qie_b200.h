@@ -160,6 +160,99 @@ int qie_attention_prefill_tc(const qie_kv_view* kv, int layer, const qie_bf16* Q
                              const int* slot, const int* block_table, int max_pages, int n_tok, int n_q_heads, int variant,
                              qie_stream st);
 
+/* ---- a serving step over the paged cache, without the host knowing its lengths ------------------------------------
+ * The reference keeps one sequence's page list on the host (src/iengine.cu:25-96) and one state per call
+ * (include/iengine.cuh:23-37); these operators take a step of many requests, decode rows beside ragged portions of
+ * prompts, whose lengths are device data: one captured graph of them serves every step of up to max_tokens rows.
+ * They are written one after another on a stream; arrays that one writes are what the next one reads.  Values in device
+ * arrays that make no sense (lengths, offsets, page ids, rows outside their range) never lead outside the arrays named
+ * here; what they say is then not defined, except where a function's comment does. */
+typedef struct {
+  int n_req;              /* requests of the step, 0 .. QIE_BATCH_MAX_REQ */
+  int max_tokens;         /* rows of pos / slot / row; qie_attention_batch: rows of Q and out */
+  int max_seqs, max_pages; /* block_table[max_seqs][max_pages] */
+  int n_pages, page_size;  /* of the pool; n_pages * page_size < 2^31, max_pages * page_size < 2^31 */
+  const int* cached;      /* [n_req] positions of the request that are in the cache */
+  const int* n_new;       /* [n_req] tokens of this step, 0: none, -1: the request is over and its pages go back */
+  const int* slots;       /* [n_req] row of the block table, each at most once; NULL: request i has row i */
+  int* block_table;
+  int* free_ring;         /* [n_pages] ids of free pages, at ring_in[0], ring_in[0] + 1, ... modulo n_pages; none of them in a request's row */
+  const int* ring_in;     /* {first, count} */
+  int* ring_out;          /* the same behind the step; may be ring_in */
+  int* q_start;           /* [n_req + 1] first row of each request in the step's tokens, and their number */
+  int* kv_len;            /* [n_req] positions behind the step: cached + n_new (0 for a request that is over) */
+  int *pos, *slot, *row;  /* [max_tokens] position, block-table row and cache row (page * page_size + place) of each token; -1 behind the last */
+  int* status;            /* [2] QIE_BATCH_* flags, pages that are missing */
+  void* work;             /* qie_attention_batch: qie_attention_batch_work() bytes on a 16-byte boundary, of one call at a time */
+  size_t work_bytes;
+} qie_batch;
+#define QIE_BATCH_MAX_REQ 8192
+#define QIE_BATCH_NO_PAGES 1   /* more pages needed than the ring has */
+#define QIE_BATCH_TOO_LONG 2   /* a request is longer than its row of the block table */
+#define QIE_BATCH_TOO_MANY 4   /* more tokens than max_tokens */
+#define QIE_BATCH_BAD_VALUE 8  /* a length below zero (n_new: below -1), a slot outside the table, a ring that is none or would hold more than n_pages */
+
+/* The step's layout.  Reads cached, n_new, slots, the ring and the block table; takes the pages that the new tokens need out of the ring, in
+ * the requests' order, into their rows of the block table; puts the pages of requests that are over behind the ring's last, in their order;
+ * writes q_start, kv_len, pos, slot, row, ring_out and status.  All or nothing: with a flag set no page changes hands, q_start and
+ * kv_len are 0 and pos, slot and row -1, so that the operators below have nothing to do, and ring_out is ring_in. */
+int qie_batch_layout(const qie_batch* b, qie_stream st);
+
+/* Rotary positions of any frequencies: the first `rotated` (even) of head_dim elements of a head turn in pairs, (2i, 2i + 1) with
+ * `neighbours` (as qie_rope) or (i, i + rotated / 2) without: (a, b) -> (a c - b s, b c + a s) with c, s = factor * cos, sin(pos * freq[i]).
+ * freq: DEVICE double[rotated / 2], radians a position.  The angle is computed in 64 bits, so any position has its own and no table is read. */
+typedef struct {
+  const double* freq;
+  int rotated, neighbours;
+  float factor;
+} qie_rope_plan;
+#define QIE_ROPE_PLAIN 0   /* base^(-2i / rotated) */
+#define QIE_ROPE_LINEAR 1  /* the same / scale */
+#define QIE_ROPE_NTK 2     /* base * scale^(rotated / (rotated - 2)) as the base */
+#define QIE_ROPE_YARN 3    /* by the turns over `original` positions: more than a (32) kept, fewer than b (1) / scale, a ramp over i between; factor 0.1 ln(scale) + 1 */
+#define QIE_ROPE_PARTS 4   /* by the turns over `original` positions: more than b (4) kept, fewer than a (1) / scale, a ramp over the turns between */
+/* HOST only: h_freq[rotated / 2] and *h_factor.  scale >= 1; a, b: 0 for the numbers in brackets. */
+int qie_rope_frequencies(double* h_freq, float* h_factor, int rotated, double base, int kind, double scale, int original, double a, double b);
+/* x [n_tok, n_heads * head_dim] -> out, rows `stride` elements apart (may be the same array); rows whose pos is below 0 are left as they are. */
+int qie_rope_rows(const qie_bf16* x, size_t x_stride, qie_bf16* out, size_t out_stride, const qie_rope_plan* rope, const int* pos, int n_tok,
+                  int n_heads, int head_dim, qie_stream st);
+/* The same for q, and in the same launch k (rotated) and v into the cache rows row[t] of `layer`; q, k and v are rows `stride` apart, so they may be
+ * parts of one array.  A token whose pos is below 0 has no q written, one whose row is outside the pool no k and v. */
+int qie_rope_store(const qie_kv_view* kv, int layer, const qie_bf16* q, size_t q_stride, qie_bf16* q_out, size_t q_out_stride, const qie_bf16* k,
+                   size_t k_stride, const qie_bf16* v, size_t v_stride, const qie_rope_plan* rope, const int* pos, const int* row, int n_tok,
+                   int n_q_heads, qie_stream st);
+
+/* Attention of the step's rows over the cache (fast numerics): row q_start[i] + j of request i is position kv_len[i] - n_i + j (n_i = q_start[i + 1]
+ * - q_start[i]) and sees the positions up to its own; with window > 0 the last `window` of them.  scale 0: 1 / sqrt(head_dim).  Reads n_req,
+ * max_tokens, max_seqs, max_pages, slots, block_table, q_start, kv_len, work of the batch.  head_dim 64 or 128, at most 128 query heads
+ * a kv head; Q and out are rows `stride` elements apart on 16-byte boundaries.  Rows that no request owns are left as they are. */
+int qie_attention_batch(const qie_kv_view* kv, int layer, const qie_batch* b, const qie_bf16* Q, size_t q_stride, qie_bf16* out, size_t out_stride,
+                        int n_q_heads, int window, float scale, qie_stream st);
+/* bytes of qie_batch.work on the current device (0: a geometry that qie_attention_batch refuses) */
+size_t qie_attention_batch_work(const qie_kv_view* kv, int n_q_heads);
+
+/* Rules for rows of logits, in front of the sampler.  Row i has the tokens [tok_start[i], tok_start[i + 1]), of which those from gen_start[i] on
+ * are generated ones.  In this order, in fp32 with one rounding at the end:
+ *   a token of the row's list:      x = x > 0 ? x / repetition[i] : x * repetition[i]   (qie_repetition_penalty)
+ *   a generated one, n times:       x = x - frequency[i] * n, x = x - presence[i]
+ *   entries [bias_start[i], ..):    x = x + the sum of the entries of this token
+ *   mask row mask_row[i], bit 0:    x = -infinity  (bit t % 32 of word t / 32; a mask_row outside [0, n_masks): every token is allowed)
+ * Any pointer may be NULL (no such rule; gen_start NULL: all are generated ones; mask_row NULL: row i has mask i).  Tokens outside the
+ * vocabulary are ignored. */
+typedef struct {
+  const int *tok_start, *tokens, *gen_start;
+  const float *repetition, *presence, *frequency;
+  const int *bias_start, *bias_ids;
+  const float* bias;
+  const uint32_t* mask;
+  const int* mask_row;
+  int n_tokens, n_bias;       /* elements of tokens and of bias_ids / bias */
+  int mask_words, n_masks;    /* mask[n_masks][mask_words] */
+} qie_logit_rules;
+/* dtype: QIE_DTYPE_BF16 or QIE_DTYPE_F32.  out may be logits. */
+int qie_logits_process(const void* logits, size_t stride, void* out, size_t out_stride, int dtype, int n_rows, int vocab,
+                       const qie_logit_rules* rules, qie_stream st);
+
 /* ------------------------------------------------------------------------------------
  * (2) driver level
  * ---------------------------------------------------------------------------------- */

@@ -40,6 +40,21 @@ class KvView(C.Structure):
                 ("n_layers", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int)]
 
 
+class BatchView(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("n_req", "max_tokens", "max_seqs", "max_pages", "n_pages", "page_size")] + \
+               [(n, C.c_void_p) for n in ("cached", "n_new", "slots", "block_table", "free_ring", "ring_in", "ring_out", "q_start", "kv_len",
+                                          "pos", "slot", "row", "status", "work")] + [("work_bytes", C.c_size_t)]
+
+
+class RopePlan(C.Structure):
+    _fields_ = [("freq", C.c_void_p), ("rotated", C.c_int), ("neighbours", C.c_int), ("factor", C.c_float)]
+
+
+class LogitRulesView(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("tok_start", "tokens", "gen_start", "repetition", "presence", "frequency", "bias_start", "bias_ids",
+                                          "bias", "mask", "mask_row")] + [(n, C.c_int) for n in ("n_tokens", "n_bias", "mask_words", "n_masks")]
+
+
 def declared_symbols(header=HEADER_PATH):
     """Every function name declared in include/qie_b200.h."""
     src = open(header).read()
@@ -85,6 +100,13 @@ def lib():
         "qie_attention_prefill_tc": (i32, [C.POINTER(KvView), i32, vp, vp, vp, vp, vp, i32, i32, i32, i32, vp]),
         "qie_attention_prefill_fast": (i32, [C.POINTER(KvView), i32, vp, vp, vp, vp, vp, i32, i32, i32, vp]),
         "qie_attention_decode_fast": (i32, [C.POINTER(KvView), i32, vp, vp, vp, vp, vp, i32, i32, i32, i32, vp]),
+        "qie_batch_layout": (i32, [vp, vp]),
+        "qie_rope_frequencies": (i32, [vp, vp, i32, C.c_double, i32, C.c_double, i32, C.c_double, C.c_double]),
+        "qie_rope_rows": (i32, [vp, sz, vp, sz, vp, vp, i32, i32, i32, vp]),
+        "qie_rope_store": (i32, [vp, i32, vp, sz, vp, sz, vp, sz, vp, sz, vp, vp, vp, i32, i32, vp]),
+        "qie_attention_batch": (i32, [vp, i32, vp, vp, sz, vp, sz, i32, i32, f32, vp]),
+        "qie_attention_batch_work": (sz, [vp, i32]),
+        "qie_logits_process": (i32, [vp, sz, vp, sz, i32, i32, i32, vp, vp]),
         "qie_engine_opts_default": (None, [C.POINTER(EngineOpts)]),
         "qie_synth_checkpoint_write": (i32, [C.POINTER(Config), u64, C.c_char_p, C.c_char_p]),
         "qie_convert_safetensors": (i32, [C.POINTER(C.c_char_p), i32, C.c_char_p, C.c_char_p, i32, C.POINTER(sz), C.POINTER(i32)]),

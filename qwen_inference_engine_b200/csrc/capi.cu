@@ -410,6 +410,151 @@ int qie_attention_prefill_tc(const qie_kv_view* kv, int layer, const qie_bf16* Q
   return QIE_OK;
 }
 
+// ---------------------------------------------------------------- a serving step
+// a table of `rows` positions a page that offsets of 32 bits name
+static bool batch_sizes_ok(const qie_batch* b) {
+  return b && b->n_req >= 0 && b->n_req <= QIE_BATCH_MAX_REQ && b->max_tokens >= 0 && b->max_seqs >= 0 && b->max_pages > 0 && b->page_size > 0 &&
+         (long long)b->max_pages * b->page_size < (1ll << 31) && (b->n_req == 0 || b->max_seqs > 0);
+}
+int qie_batch_layout(const qie_batch* b, qie_stream st) {
+  static_assert(BATCH_MAX_REQ == QIE_BATCH_MAX_REQ, "one limit");
+  if (!batch_sizes_ok(b) || b->n_pages <= 0 || (long long)b->n_pages * b->page_size >= (1ll << 31))
+    return fail(QIE_EINVAL, "batch_layout: need 0 to %d requests, and n_pages and max_pages above 0 with less than 2^31 positions", QIE_BATCH_MAX_REQ);
+  if (!b->free_ring || !b->ring_in || !b->ring_out || !b->q_start || !b->status || (b->n_req && (!b->cached || !b->n_new || !b->block_table || !b->kv_len)) ||
+      (b->max_tokens && (!b->pos || !b->slot || !b->row)))
+    return fail(QIE_EINVAL, "batch_layout: an array is missing");
+  if (!b->slots && b->n_req > b->max_seqs) return fail(QIE_EINVAL, "batch_layout: %d requests on %d rows of the block table", b->n_req, b->max_seqs);
+  BatchArgs a{};
+  a.n_req = b->n_req, a.max_tokens = b->max_tokens, a.max_seqs = b->max_seqs, a.max_pages = b->max_pages, a.n_pages = b->n_pages, a.page_size = b->page_size;
+  a.cached = b->cached, a.n_new = b->n_new, a.slots = b->slots;
+  a.block_table = b->block_table, a.free_ring = b->free_ring, a.ring_in = b->ring_in, a.ring_out = b->ring_out;
+  a.q_start = b->q_start, a.kv_len = b->kv_len, a.pos = b->pos, a.slot = b->slot, a.row = b->row, a.status = b->status;
+  CU(launch_batch_layout(a, (cudaStream_t)st));
+  return QIE_OK;
+}
+
+int qie_rope_frequencies(double* h_freq, float* h_factor, int rotated, double base, int kind, double scale, int original, double a, double b) {
+  const double pi = 3.14159265358979323846;
+  if (!h_freq || !h_factor || rotated < 2 || (rotated & 1) || !(base > 1.0) || kind < QIE_ROPE_PLAIN || kind > QIE_ROPE_PARTS)
+    return fail(QIE_EINVAL, "rope_frequencies: need an even number of rotated elements, a base above 1 and a known kind");
+  if (kind != QIE_ROPE_PLAIN && !(scale >= 1.0 && scale < 1e9)) return fail(QIE_EINVAL, "rope_frequencies: need a scale of at least 1");
+  if (kind == QIE_ROPE_NTK && rotated < 4) return fail(QIE_EINVAL, "rope_frequencies: need 4 rotated elements");
+  if (kind >= QIE_ROPE_YARN) {
+    if (original < 1) return fail(QIE_EINVAL, "rope_frequencies: need the number of original positions");
+    if (a == 0) a = kind == QIE_ROPE_YARN ? 32 : 1;
+    if (b == 0) b = kind == QIE_ROPE_YARN ? 1 : 4;
+    if (!(a > 0) || !(b > 0) || (kind == QIE_ROPE_YARN ? a < b : a >= b)) return fail(QIE_EINVAL, "rope_frequencies: the two numbers of turns are in the wrong order");
+  }
+  *h_factor = kind == QIE_ROPE_YARN && scale > 1 ? (float)(0.1 * log(scale) + 1) : 1.f;
+  if (kind == QIE_ROPE_NTK) base *= pow(scale, (double)rotated / (rotated - 2));
+  double lo = 0, hi = 0;
+  if (kind == QIE_ROPE_YARN) {  // the pair that makes so many turns over the original positions
+    auto at = [&](double turns) { return rotated * log(original / (turns * 2 * pi)) / (2 * log(base)); };
+    lo = std::max(0.0, floor(at(a))), hi = std::min((double)(rotated - 1), ceil(at(b)));
+    if (hi - lo < 1e-3) hi = lo + 1e-3;
+  }
+  for (int i = 0; i < rotated / 2; ++i) {
+    const double w = pow(base, -2.0 * i / rotated);
+    double keep = 1;  // the share of the unscaled frequency
+    if (kind == QIE_ROPE_LINEAR) keep = 0;
+    if (kind == QIE_ROPE_YARN) keep = 1 - std::min(1.0, std::max(0.0, (i - lo) / (hi - lo)));
+    if (kind == QIE_ROPE_PARTS) keep = std::min(1.0, std::max(0.0, (original * w / (2 * pi) - a) / (b - a)));
+    h_freq[i] = keep == 1 ? w : w * keep + w / scale * (1 - keep);
+  }
+  return QIE_OK;
+}
+static bool rope_ok(const qie_rope_plan* r, int head_dim) { return r && r->freq && r->rotated >= 2 && !(r->rotated & 1) && r->rotated <= head_dim && head_dim <= 1024; }
+int qie_rope_rows(const qie_bf16* x, size_t x_stride, qie_bf16* out, size_t out_stride, const qie_rope_plan* rope, const int* pos, int n_tok, int n_heads,
+                  int head_dim, qie_stream st) {
+  if (!rope_ok(rope, head_dim)) return fail(QIE_EINVAL, "rope_rows: need an even number of rotated elements, at most head_dim, and head_dim up to 1024");
+  if (n_tok < 0 || n_heads < 0 || (n_tok && n_heads && (!x || !out || !pos))) return fail(QIE_EINVAL, "rope_rows: bad argument");
+  const size_t wide = (size_t)n_heads * head_dim;
+  if (n_tok > 1 && (x_stride < wide || out_stride < wide)) return fail(QIE_EINVAL, "rope_rows: rows of %zu elements overlap", wide);
+  if (n_tok > 1 && x == out && x_stride != out_stride) return fail(QIE_EINVAL, "rope_rows: in place with rows at other places");
+  if (n_tok == 0 || n_heads == 0) return QIE_OK;
+  RopeArgs a{};
+  a.q = (const bf16*)x, a.q_out = (bf16*)out, a.q_stride = x_stride, a.q_out_stride = out_stride;
+  a.freq = rope->freq, a.rotated = rope->rotated, a.neighbours = rope->neighbours, a.factor = rope->factor;
+  a.pos = pos, a.n_tok = n_tok, a.n_q = n_heads, a.kv.hd = head_dim;
+  CU(launch_rope_store(a, (cudaStream_t)st));
+  return QIE_OK;
+}
+int qie_rope_store(const qie_kv_view* kv, int layer, const qie_bf16* q, size_t q_stride, qie_bf16* q_out, size_t q_out_stride, const qie_bf16* k,
+                   size_t k_stride, const qie_bf16* v, size_t v_stride, const qie_rope_plan* rope, const int* pos, const int* row, int n_tok, int n_q_heads,
+                   qie_stream st) {
+  if (!kv || !kv->pool || layer < 0 || layer >= kv->n_layers || kv->n_pages <= 0 || kv->page_size <= 0 || kv->n_kv_heads <= 0 ||
+      (long long)kv->n_pages * kv->page_size >= (1ll << 31))
+    return fail(QIE_EINVAL, "rope_store: bad pool or layer");
+  if (!rope_ok(rope, kv->head_dim)) return fail(QIE_EINVAL, "rope_store: need an even number of rotated elements, at most head_dim, and head_dim up to 1024");
+  if (n_tok < 0 || n_q_heads < 0 || (n_tok && (!k || !v || !pos || !row || (n_q_heads && (!q || !q_out))))) return fail(QIE_EINVAL, "rope_store: bad argument");
+  const size_t wide = (size_t)n_q_heads * kv->head_dim, kv_wide = (size_t)kv->n_kv_heads * kv->head_dim;
+  if (n_tok > 1 && (k_stride < kv_wide || v_stride < kv_wide || (n_q_heads && (q_stride < wide || q_out_stride < wide))))
+    return fail(QIE_EINVAL, "rope_store: rows overlap");
+  if (n_tok > 1 && n_q_heads && q == q_out && q_stride != q_out_stride) return fail(QIE_EINVAL, "rope_store: in place with rows at other places");
+  if (n_tok == 0) return QIE_OK;
+  RopeArgs a{};
+  a.q = (const bf16*)q, a.q_out = (bf16*)q_out, a.q_stride = q_stride, a.q_out_stride = q_out_stride;
+  a.k = (const bf16*)k, a.v = (const bf16*)v, a.k_stride = k_stride, a.v_stride = v_stride;
+  a.freq = rope->freq, a.rotated = rope->rotated, a.neighbours = rope->neighbours, a.factor = rope->factor;
+  a.pos = pos, a.row = row, a.n_tok = n_tok, a.n_q = n_q_heads, a.layer = layer, a.kv = geom_of(kv);
+  CU(launch_rope_store(a, (cudaStream_t)st));
+  return QIE_OK;
+}
+
+static bool batch_heads_ok(const qie_kv_view* kv, int n_q) {
+  return kv && heads_ok(n_q, kv->n_kv_heads) && n_q / kv->n_kv_heads <= 128 && (kv->head_dim == 64 || kv->head_dim == 128);
+}
+size_t qie_attention_batch_work(const qie_kv_view* kv, int n_q_heads) {
+  int sms = 0;
+  if (!batch_heads_ok(kv, n_q_heads) || sm_count(&sms) != cudaSuccess) return 0;
+  return attention_batch_work(kv->head_dim, sms);
+}
+int qie_attention_batch(const qie_kv_view* kv, int layer, const qie_batch* b, const qie_bf16* Q, size_t q_stride, qie_bf16* out, size_t out_stride, int n_q_heads,
+                        int window, float scale, qie_stream st) {
+  if (!kv || !kv->pool || layer < 0 || layer >= kv->n_layers || kv->n_pages <= 0 || kv->page_size <= 0) return fail(QIE_EINVAL, "attention_batch: bad pool or layer");
+  if (!batch_heads_ok(kv, n_q_heads)) return fail(QIE_EINVAL, "attention_batch: need n_q %% n_kv == 0, n_q / n_kv <= 128 and head_dim 64 or 128");
+  if (!batch_sizes_ok(b) || b->page_size != kv->page_size || b->n_pages != kv->n_pages) return fail(QIE_EINVAL, "attention_batch: a batch of other pages, or of sizes out of range");
+  if (!b->slots && b->n_req > b->max_seqs) return fail(QIE_EINVAL, "attention_batch: %d requests on %d rows of the block table", b->n_req, b->max_seqs);
+  if (window < 0 || !(scale >= 0.f) || scale > 1e6f) return fail(QIE_EINVAL, "attention_batch: window and scale must not be below 0");
+  if (b->n_req == 0 || b->max_tokens == 0) return QIE_OK;
+  if (!b->q_start || !b->kv_len || !b->block_table || !Q || !out) return fail(QIE_EINVAL, "attention_batch: an array is missing");
+  const size_t wide = (size_t)n_q_heads * kv->head_dim;
+  if (q_stride < wide || out_stride < wide || q_stride % 8 || out_stride % 8 || q_stride >= (1ull << 38)) return fail(QIE_EINVAL, "attention_batch: rows of Q and out are multiples of 8 elements, %zu at least", wide);
+  if (!aligned(16, {kv->pool, Q, out, b->work})) return fail(QIE_EINVAL, "attention_batch: the pool, Q, out and the work area must start on a 16-byte boundary");
+  OP_STATUS(status);
+  BatchAttnArgs a{};
+  CU(sm_count(&a.num_sms));
+  if (!b->work || b->work_bytes < attention_batch_work(kv->head_dim, a.num_sms)) return fail(QIE_EINVAL, "attention_batch: needs a work area of %zu bytes", attention_batch_work(kv->head_dim, a.num_sms));
+  a.q = (const bf16*)Q, a.out = (bf16*)out, a.q_stride = q_stride, a.out_stride = out_stride;
+  a.q_start = b->q_start, a.kv_len = b->kv_len, a.slots = b->slots, a.block_table = b->block_table;
+  a.n_req = b->n_req, a.n_tok = b->max_tokens, a.max_seqs = b->max_seqs, a.max_pages = b->max_pages, a.n_q = n_q_heads, a.layer = layer, a.window = window;
+  a.scale_log2 = 1.4426950408889634f * (scale > 0.f ? scale : 1.f / sqrtf((float)kv->head_dim));
+  a.kv = geom_of(kv), a.work = b->work, a.status = status;
+  CU(launch_attention_batch(a, (cudaStream_t)st));
+  return QIE_OK;
+}
+
+int qie_logits_process(const void* logits, size_t stride, void* out, size_t out_stride, int dtype, int n_rows, int vocab, const qie_logit_rules* rules, qie_stream st) {
+  if (dtype != QIE_DTYPE_BF16 && dtype != QIE_DTYPE_F32) return fail(QIE_EINVAL, "logits_process: bf16 or fp32 logits");
+  if (!rules || n_rows < 0 || n_rows > 65535 || vocab <= 0 || (n_rows && (!logits || !out))) return fail(QIE_EINVAL, "logits_process: bad argument (at most 65535 rows)");
+  if (n_rows > 1 && (stride < (size_t)vocab || out_stride < (size_t)vocab)) return fail(QIE_EINVAL, "logits_process: rows of %d elements overlap", vocab);
+  if (n_rows > 1 && logits == out && stride != out_stride) return fail(QIE_EINVAL, "logits_process: in place with rows at other places");
+  if (!aligned(dtype == QIE_DTYPE_F32 ? 4 : 2, {logits, out})) return fail(QIE_EINVAL, "logits_process: logits off their type's boundary");
+  const qie_logit_rules& r = *rules;
+  if (r.n_tokens < 0 || r.n_bias < 0 || (r.gen_start && !r.tok_start) || (r.tok_start && !r.tokens && r.n_tokens) ||
+      (r.bias_start && r.n_bias && (!r.bias_ids || !r.bias)) || ((r.repetition || r.presence || r.frequency) && !r.tok_start) || (r.bias && !r.bias_start))
+    return fail(QIE_EINVAL, "logits_process: a rule without its lists");
+  if (r.mask && (r.n_masks < 0 || (long long)r.mask_words * 32 < vocab)) return fail(QIE_EINVAL, "logits_process: masks of %d words for %d tokens", r.mask_words, vocab);
+  if (n_rows == 0) return QIE_OK;
+  LogitArgs a{};
+  a.in = logits, a.out = out, a.stride = stride, a.out_stride = out_stride, a.f32 = dtype == QIE_DTYPE_F32, a.n_rows = n_rows, a.vocab = vocab;
+  a.tok_start = r.tok_start, a.tokens = r.tokens, a.gen_start = r.gen_start, a.repetition = r.repetition, a.presence = r.presence, a.frequency = r.frequency;
+  a.bias_start = r.bias ? r.bias_start : nullptr, a.bias_ids = r.bias_ids, a.bias = r.bias, a.mask = r.mask, a.mask_row = r.mask_row;
+  a.n_tokens = r.n_tokens, a.n_bias = r.n_bias, a.mask_words = r.mask_words, a.n_masks = r.n_masks;
+  CU(launch_logit_rules(a, (cudaStream_t)st));
+  return QIE_OK;
+}
+
 int qie_kernel_status(void) { return take_status(g_op_status.load(std::memory_order_acquire)) ? wait_failed("an earlier operator call") : QIE_OK; }
 int qie_wait_selftest(qie_engine* e, qie_stream st) {
   if (e) {

@@ -170,6 +170,60 @@ cudaError_t launch_attention_prompt_tc(const FastAttnArgs& a, int two_term, cuda
 // the same with one bf16 term per weight, head_dim 128: attn_prompt_tc.cu, or for pages of other than 16 positions attn_prefill_tc.cu
 cudaError_t launch_attention_prefill_tc(const FastAttnArgs& a, cudaStream_t st);
 
+// ---------------------------------------------------------------- a serving step (qie_batch in qie_b200.h)
+struct BatchArgs {
+  int n_req, max_tokens, max_seqs, max_pages, n_pages, page_size;
+  const int *cached, *n_new, *slots;
+  int *block_table, *free_ring;
+  const int* ring_in;
+  int *ring_out, *q_start, *kv_len, *pos, *slot, *row, *status;
+};
+constexpr int BATCH_MAX_REQ = 8192;
+cudaError_t launch_batch_layout(const BatchArgs& a, cudaStream_t st);
+
+struct RopeArgs {
+  const bf16 *q, *k, *v;  // rows of heads, strides in elements; k null: q only
+  bf16* q_out;
+  size_t q_stride, q_out_stride, k_stride, v_stride;
+  const double* freq;
+  int rotated, neighbours;
+  float factor;
+  const int *pos, *row;
+  int n_tok, n_q, layer;
+  KvGeom kv;  // hd also where k is null
+};
+cudaError_t launch_rope_store(const RopeArgs& a, cudaStream_t st);
+
+struct BatchAttnArgs {
+  const bf16* q;
+  bf16* out;
+  size_t q_stride, out_stride;
+  const int *q_start, *kv_len, *slots, *block_table;
+  int n_req, n_tok, max_seqs, max_pages, n_q, layer, window;
+  float scale_log2;  // log2(e) * scale
+  KvGeom kv;
+  void* work;
+  int num_sms;
+  int* status;  // see FastAttnArgs
+};
+size_t attention_batch_work(int hd, int num_sms);
+cudaError_t launch_attention_batch(const BatchAttnArgs& a, cudaStream_t st);
+
+struct LogitArgs {
+  const void* in;
+  void* out;
+  size_t stride, out_stride;
+  int f32, n_rows, vocab;
+  const int *tok_start, *tokens, *gen_start;
+  const float *repetition, *presence, *frequency;
+  const int *bias_start, *bias_ids;
+  const float* bias;
+  const uint32_t* mask;
+  const int* mask_row;
+  int n_tokens, n_bias, mask_words, n_masks;
+};
+cudaError_t launch_logit_rules(const LogitArgs& a, cudaStream_t st);
+
 // tcgen05 GEMM (fast numerics; without a split over K also the reference's order)
 struct TensorMap2D {
   alignas(64) unsigned char opaque[128];  // CUtensorMap

@@ -13,7 +13,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import KvView, check
+from ._lib import BatchView, KvView, LogitRulesView, RopePlan, check
 
 
 def _p(t):
@@ -92,6 +92,17 @@ class KvPool:
             bt[s, :len(ids)] = ids
         self.block_table = torch.from_numpy(bt).cuda()
 
+    @classmethod
+    def over(cls, pool, block_table=None):
+        """the same over a caller's pool [page][layer][k|v][kv_head][slot][head_dim] and, for the operators that take it from here, block table"""
+        assert pool.dim() == 6 and pool.shape[2] == 2 and pool.dtype == torch.bfloat16
+        n_pages, n_layers, _, n_kv_heads, page_size, head_dim = pool.shape
+        self = cls.__new__(cls)
+        self.pool, self.block_table = pool, block_table
+        self.view = KvView(_p(pool), n_pages, page_size, n_layers, n_kv_heads, head_dim)
+        self.max_pages = n_pages if block_table is None else block_table.shape[1]
+        return self
+
     def store(self, layer, K, V, pos, slot):
         check(_lib.lib().qie_kv_store(C.byref(self.view), layer, _p(K), _p(V), _p(pos), _p(slot),
                                       _p(self.block_table), self.max_pages, pos.numel(), _st()))
@@ -145,3 +156,134 @@ def launch_attn_prefill_tc(Q, out, pool, layer, pos, slot, n_q_heads, variant=0)
     check(_lib.lib().qie_attention_prefill_tc(C.byref(pool.view), layer, _p(Q), _p(out), _p(pos), _p(slot),
                                               _p(pool.block_table), pool.max_pages, pos.numel(), n_q_heads, variant,
                                               _st()))
+
+
+# ---- a serving step over the paged cache (see qie_batch in include/qie_b200.h) ----------------
+def _here(t):
+    assert t.device.index == torch.cuda.current_device(), "a tensor of another device than the current one"
+
+
+def _ints(t, n, name):
+    """pointer of n int32 on the current device"""
+    assert t.dtype == torch.int32 and t.numel() >= n, f"{name}: {n} int32 expected"
+    _here(t)
+    return _p(t)
+
+
+def _rows(t):
+    """(pointer, row stride) of rows whose elements lie side by side"""
+    assert t.is_cuda and t.dim() == 2 and (t.shape[1] == 1 or t.stride(1) == 1), "device-resident rows of contiguous elements expected"
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+class Batch:
+    """A step of n_req requests and up to max_tokens rows: the arrays of qie_batch.  Those of the layout that are not given are made here; the
+    object holds what it points to and is used step after step, its arrays changed in place."""
+
+    def __init__(self, block_table, page_size, n_pages, n_req, max_tokens, *, slots=None, cached=None, n_new=None, free_ring=None, ring_in=None,
+                 ring_out=None, q_start=None, kv_len=None, pos=None, slot=None, row=None, status=None):
+        def ints(t, n):
+            return torch.zeros(n, dtype=torch.int32, device=block_table.device) if t is None else t
+
+        assert block_table.dim() == 2
+        self.block_table, self.slots, self.cached, self.n_new, self.free_ring, self.ring_in = block_table, slots, cached, n_new, free_ring, ring_in
+        self.ring_out, self.q_start, self.kv_len, self.status = ints(ring_out, 2), ints(q_start, n_req + 1), ints(kv_len, n_req), ints(status, 2)
+        self.pos, self.slot, self.row = ints(pos, max_tokens), ints(slot, max_tokens), ints(row, max_tokens)
+        self.work = None
+        b = self.view = BatchView(n_req=n_req, max_tokens=max_tokens, max_seqs=block_table.shape[0], max_pages=block_table.shape[1], n_pages=n_pages,
+                                  page_size=page_size)
+        for name, n in (("block_table", 0), ("slots", n_req), ("cached", n_req), ("n_new", n_req), ("free_ring", n_pages), ("ring_in", 2), ("ring_out", 2),
+                        ("q_start", n_req + 1), ("kv_len", n_req), ("pos", max_tokens), ("slot", max_tokens), ("row", max_tokens), ("status", 2)):
+            t = getattr(self, name)
+            if t is not None:
+                setattr(b, name, _ints(t, n, name))
+        self.ref = C.byref(b)
+
+    def reserve(self, pool, n_q_heads):
+        """the work area of launch_attn_batch; one call at a time uses it"""
+        n = _lib.lib().qie_attention_batch_work(C.byref(pool.view), n_q_heads)
+        if self.work is None or self.work.numel() < n:
+            self.work = torch.empty(n, dtype=torch.uint8, device=self.block_table.device)
+            self.view.work, self.view.work_bytes = self.work.data_ptr(), n
+
+
+def launch_batch_layout(batch):
+    check(_lib.lib().qie_batch_layout(batch.ref, _st()))
+
+
+class Rope:
+    """rotary frequencies on the device: freq, float64 radians a position of each pair"""
+    KINDS = {"plain": 0, "linear": 1, "ntk": 2, "yarn": 3, "parts": 4}
+
+    def __init__(self, freq, factor=1.0, neighbours=False):
+        assert freq.dtype == torch.float64 and freq.dim() == 1
+        _here(freq)
+        self.freq = freq
+        self.plan = RopePlan(_p(freq), 2 * freq.numel(), int(neighbours), float(factor))
+        self.ref = C.byref(self.plan)
+
+    @staticmethod
+    def frequencies(rotated, base=1000000.0, kind="plain", scale=1.0, original=0, a=0.0, b=0.0):
+        """host: (float64 array of rotated / 2, factor), see qie_rope_frequencies"""
+        w, f = np.zeros(max(1, rotated // 2)), C.c_float()
+        check(_lib.lib().qie_rope_frequencies(w.ctypes.data, C.byref(f), rotated, base, Rope.KINDS[kind], scale, original, a, b))
+        return w, f.value
+
+
+def launch_rope_rows(x, out, pos, rope, n_heads, head_dim):
+    """rows [n_tok, n_heads * head_dim] -> out (may be x), token t at position pos[t]"""
+    assert x.dtype == out.dtype == torch.bfloat16 and x.shape == out.shape and x.shape[1] == n_heads * head_dim
+    _here(x)
+    check(_lib.lib().qie_rope_rows(*_rows(x), *_rows(out), rope.ref, _ints(pos, x.shape[0], "pos"), x.shape[0], n_heads, head_dim, _st()))
+
+
+def launch_rope_store(q, k, v, q_out, pool, layer, pos, row, rope, n_q_heads):
+    """q -> q_out, k and v -> the cache rows row[t] of the pool's layer"""
+    view, n = pool.view, q.shape[0]
+    assert q.dtype == k.dtype == v.dtype == q_out.dtype == torch.bfloat16
+    assert q.shape == q_out.shape and k.shape == v.shape == (n, view.n_kv_heads * view.head_dim) and q.shape[1] == n_q_heads * view.head_dim
+    _here(q)
+    check(_lib.lib().qie_rope_store(C.byref(view), layer, *_rows(q), *_rows(q_out), *_rows(k), *_rows(v), rope.ref, _ints(pos, n, "pos"), _ints(row, n, "row"), n,
+                                    n_q_heads, _st()))
+
+
+def launch_attn_batch(Q, out, pool, layer, batch, n_q_heads, window=0, scale=0.0):
+    """attention of the batch's rows over the pool, ragged over its requests (fast numerics)"""
+    assert Q.dtype == out.dtype == torch.bfloat16 and Q.shape == out.shape == (batch.view.max_tokens, n_q_heads * pool.view.head_dim)
+    if batch.work is None:
+        batch.reserve(pool, n_q_heads)
+    _here(Q)
+    check(_lib.lib().qie_attention_batch(C.byref(pool.view), layer, batch.ref, *_rows(Q), *_rows(out), n_q_heads, window, scale, _st()))
+
+
+class LogitRules:
+    """the lists and parameters of qie_logit_rules; None: no such rule"""
+
+    def __init__(self, tok_start=None, tokens=None, *, gen_start=None, repetition=None, presence=None, frequency=None, bias_start=None, bias_ids=None, bias=None,
+                 mask=None, mask_row=None):
+        self.held = dict(tok_start=tok_start, tokens=tokens, gen_start=gen_start, repetition=repetition, presence=presence, frequency=frequency,
+                         bias_start=bias_start, bias_ids=bias_ids, bias=bias, mask=mask, mask_row=mask_row)
+        self.n_rows = None  # rows that every list has
+        for name, t in self.held.items():
+            if t is None:
+                continue
+            assert t.dtype == (torch.float32 if name in ("repetition", "presence", "frequency", "bias") else torch.int32), f"{name}: {t.dtype}"
+            _here(t)
+            n = {"tokens": None, "bias_ids": None, "bias": None, "tok_start": t.numel() - 1, "bias_start": t.numel() - 1,
+                 "mask": t.shape[0] if mask_row is None else None}.get(name, t.numel())
+            if n is not None:
+                self.n_rows = n if self.n_rows is None else min(self.n_rows, n)
+        assert mask is None or mask.dim() == 2, "mask [masks][words]"
+        assert bias is None or (bias_ids is not None and bias_ids.numel() == bias.numel()), "a bias for each id"
+        r = self.view = LogitRulesView(**{name: _p(t) for name, t in self.held.items() if t is not None})
+        r.n_tokens, r.n_bias = 0 if tokens is None else tokens.numel(), 0 if bias is None else bias.numel()
+        r.n_masks, r.mask_words = (0, 0) if mask is None else mask.shape
+        self.ref = C.byref(r)
+
+
+def launch_logits(logits, out, rules):
+    """the rules over rows [n_rows, vocab] of bfloat16 or float32 logits -> out (may be logits)"""
+    assert logits.dtype == out.dtype and logits.shape == out.shape and logits.dtype in (torch.bfloat16, torch.float32)
+    assert rules.n_rows is None or rules.n_rows >= logits.shape[0], "rules for fewer rows"
+    _here(logits)
+    check(_lib.lib().qie_logits_process(*_rows(logits), *_rows(out), int(logits.dtype == torch.float32), logits.shape[0], logits.shape[1], rules.ref, _st()))
