@@ -1,60 +1,585 @@
-// attn_batch.cu -- attention of a step's rows over the paged cache: requests with any number of rows, causal behind their cached positions, with an
-// optional window (qie_attention_batch).
+// attn_batch.cu -- attention of a step's rows over the paged cache on tcgen05 / TMEM: requests with any number of rows, causal behind their cached positions,
+// with an optional window (qie_attention_batch).
 //
 //   out_t = sum_j 2^(s (q_t . k_j) - m) v_j / sum_j 2^(s (q_t . k_j) - m) over the positions j that row t sees, m their running maximum
+//
+// An item is a kv head of a request and a block of its tokens: the rows of a tile are (token, query head of the group), so keys and values are read once
+// for the whole group and a decode row costs the tiles of its context alone.  The tiles of all items, one after the other, are cut into equal stretches,
+// one a CTA (two CTAs an SM; the host knows no lengths, so every CTA adds the requests up itself).  An item that is cut leaves its parts (rows of O, maximum,
+// sum, in fp32) in the work area, and a second kernel joins them.
+// Within a CTA:
+//   S = Q K^T  : tcgen05.mma, 128 x 64 fp32 in one of two TMEM buffers, issued two tiles ahead of its softmax, across items
+//   softmax    : warps 0-3, a thread a row (= TMEM lane).  The weights go back over the scores as bf16: the product's A operand (2^-8 of each weight; sums take
+//                them unrounded).  Warps without rows only pass the barriers on.
+//   O += P V   : accumulates in TMEM; rows scale it when their maximum grows
+//   warp 4     : the products.  warp 5: queries and 64-column boxes of the pages by TMA with the 128-byte swizzle, or, for pages of other than multiples of 16
+//                positions and pools of 2^31 rows, 16-byte copies to the same places.
+// Values of keys that some row of a tile does not see must not meet its zero weight when they are no numbers: tiles at the edges of what rows see are
+// looked over, such values are put aside, and rows that see them get them at the end.
+// Every wait has a limit; when one runs out the CTA's results are not numbers and it reports it.
+#include <cuda.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "attn_batch_plan.cuh"
 #include "common.cuh"
 #include "kernels.h"
 #include "launch.h"
+#include "pack.cuh"
+#include "tc_ptx.cuh"
 
 namespace qie {
 namespace {
 
-// a warp a row and query head, one pass over the keys
+constexpr int TQ = AB_TQ, TK = AB_TK;
+constexpr int QBLK = TQ * 128, KBLK = TK * 128;  // [rows][64 columns] bf16 in 8-row swizzle atoms
+constexpr int NSOFT = 128, NTHR = NSOFT + 64;
+constexpr uint32_t TMEM_COLS = 256;  // two tiles of scores, O
+constexpr int EDGES = 6;             // tiles of an item at the edges of what its rows see: tokens span at most 128 positions, so three at either end
+
 template <int HD>
-__global__ void __launch_bounds__(256) attn_batch_kernel(BatchAttnArgs a) {
-  constexpr int E = HD / 32;
+struct Smem {
+  static constexpr int NB = HD / 64, ST = HD == 64 ? 4 : 2;  // column blocks; stages of K and of V
+  static constexpr int TILE = NB * KBLK;
+  static constexpr int Q = 0, K = NB * QBLK, V = K + ST * TILE, ODD = V + ST * TILE, BAR = ODD + EDGES * HD * 16, END = BAR + 256 + 1024;
+  // (three CTAs an SM would wait for TMEM columns: see attn_prompt_tc.cu)
+  static constexpr int TOTAL = END > 76 * 1024 ? END : 76 * 1024;
+  static_assert(512 / TMEM_COLS == 2 && 3 * (TOTAL + 1024) > 228 * 1024 && 2 * (TOTAL + 2048) <= 228 * 1024, "two CTAs an SM");
+};
+// a part of an item in the work area: O rows, then maxima and sums
+template <int HD>
+constexpr int PART = TQ * HD + 2 * TQ;  // floats
+struct JoinInfo {
+  int t0, tokens, kvh, parts;  // rows t0 .. t0 + tokens of Q; parts 0: nothing to join
+};
+
+__device__ __forceinline__ void ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,"
+      "%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
+      "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
+      ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+      "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// two scores at once: x * s + n, and a + b
+__device__ __forceinline__ void fma2(float& x, float& y, unsigned long long s, unsigned long long n) {
+  asm("{\n\t.reg .b64 v;\n\tmov.b64 v, {%0, %1};\n\tfma.rn.f32x2 v, v, %2, %3;\n\tmov.b64 {%0, %1}, v;\n\t}" : "+f"(x), "+f"(y) : "l"(s), "l"(n));
+}
+__device__ __forceinline__ void add2(float& a, float& b, float x, float y) {
+  asm("{\n\t.reg .b64 u, v;\n\tmov.b64 u, {%0, %1};\n\tmov.b64 v, {%2, %3};\n\tadd.rn.f32x2 u, u, v;\n\tmov.b64 {%0, %1}, u;\n\t}"
+      : "+f"(a), "+f"(b) : "f"(x), "f"(y));
+}
+__device__ __forceinline__ unsigned long long twice(float x) {
+  unsigned long long v;
+  asm("mov.b64 %0, {%1, %1};" : "=l"(v) : "f"(x));
+  return v;
+}
+
+struct Shape {
+  int g, tt;  // query heads of a group; tokens of a block
+};
+// sum over the block of a 64-bit value a thread: what the threads below have, and all
+__device__ __forceinline__ long long block_scan(long long v, long long* warp_sums, long long& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long run = v;
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long o = __shfl_up_sync(0xffffffffu, run, d);
+    if (lane >= d) run += o;
+  }
+  if (lane == 31) warp_sums[warp] = run;
+  __syncthreads();
+  long long before = 0;
+  total = 0;
+  for (int w = 0; w < NTHR / 32; ++w) {
+    if (w == warp) before = total;
+    total += warp_sums[w];
+  }
+  return before + run - v;
+}
+
+template <int HD, bool TMA>
+__global__ void __launch_bounds__(NTHR, 2) attn_batch_kernel(BatchAttnArgs a, Shape sh, int box, const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap kvm) {
+  using SM = Smem<HD>;
+  constexpr int NB = SM::NB, ST = SM::ST;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  __shared__ long long s_sums[NTHR / 32], s_rest;
+  __shared__ int dead_s, s_req, s_kvh, s_block, s_skip, s_odd[2], s_edge[EDGES];  // s_odd, by the item's parity: there are values put aside; s_edge: first keys of the edge tiles
+  volatile int* dead = &dead_s;
   pdl_wait();
   pdl_trigger();
-  const int t = blockIdx.x, h = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (h >= a.n_q) return;
-  // the request that owns the row
-  int lo = 0, hi = a.n_req;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.q_start[mid] <= t) lo = mid;
-    else hi = mid;
+  const uint32_t s0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  // barriers: of S, P and O in pairs by the tile's parity; of the queries and of K and V a stage each, full and free
+  const uint32_t bar_s = s0 + SM::BAR, bar_p = bar_s + 16, bar_o = bar_s + 32, bar_q = bar_s + 48, slot = bar_s + 56, bar_k = bar_s + 64, bar_v = bar_k + 8 * ST,
+                 free_k = bar_v + 8 * ST, free_v = free_k + 8 * ST, free_q = free_v + 8 * ST;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, tt = sh.tt, G = sh.g;
+  if (tid == 0) {
+    dead_s = 0, s_odd[0] = s_odd[1] = 0, s_req = a.n_req;
+    for (int i = 0; i < 2; ++i) mbar_init_tc(bar_s + 8 * i, 1), mbar_init_tc(bar_p + 8 * i, NSOFT), mbar_init_tc(bar_o + 8 * i, 1);
+    mbar_init_tc(bar_q, 1), mbar_init_tc(free_q, 1);
+    for (int i = 0; i < ST; ++i) mbar_init_tc(bar_k + 8 * i, 1), mbar_init_tc(bar_v + 8 * i, 1), mbar_init_tc(free_k + 8 * i, 1), mbar_init_tc(free_v + 8 * i, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  const int t0 = a.q_start[lo], t1 = a.q_start[lo + 1], slot = a.slots ? a.slots[lo] : lo;
-  if (t < t0 || t >= t1 || slot < 0 || slot >= a.max_seqs) return;
-  const long long most = (long long)a.max_pages * a.kv.page_size;
-  const int len = (int)min((long long)max(a.kv_len[lo], 0), most), pos = min(len - 1, max(len - (t1 - t0), 0) + t - t0);
-  const int kvh = h / (a.n_q / a.kv.n_kv);
-  const int* bt = a.block_table + (size_t)slot * a.max_pages;
-  float q[E], o[E], m = -INFINITY, l = 0.f;
-  const bf16* src = a.q + t * a.q_stride + (size_t)h * HD + lane * E;
-  for (int e = 0; e < E; ++e) q[e] = bf2f(src[e]), o[e] = 0.f;
-  for (int j = a.window > 0 ? max(0, pos - a.window + 1) : 0; j <= pos; ++j) {
-    const int page = bt[j / a.kv.page_size], at = j % a.kv.page_size;
-    if (page < 0 || page >= a.kv.n_pages) continue;
-    const bf16 *k = a.kv.chunk(page, a.layer, 0, kvh) + (size_t)at * HD + lane * E, *v = a.kv.chunk(page, a.layer, 1, kvh) + (size_t)at * HD + lane * E;
-    float s = 0.f;
-    for (int e = 0; e < E; ++e) s += q[e] * bf2f(k[e]);
-    s = warp_sum(s) * a.scale_log2;
-    const float top = fmaxf(m, s), f = exp2f(m - top), p = exp2f(s - top);
-    l = l * f + p, m = top;
-    for (int e = 0; e < E; ++e) o[e] = o[e] * f + p * bf2f(v[e]);
+  if (warp == NSOFT / 32) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(TMEM_COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  bf16* dst = a.out + t * a.out_stride + (size_t)h * HD + lane * E;
-  for (int e = 0; e < E; ++e) dst[e] = f2bf(o[e] / l);
+  for (int i = tid; i < EDGES * HD; i += NTHR) asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(s0 + SM::ODD + i * 16), "r"(0u) : "memory");
+  // ---- this CTA's stretch
+  const int per = (a.n_req + NTHR - 1) / NTHR, r0 = min(a.n_req, tid * per), r1 = min(a.n_req, r0 + per);
+  long long mine = 0, total;
+  for (int i = r0; i < r1; ++i) {
+    const Raw w = request(a, i, tt);
+    mine += a.kv.n_kv * ab_cost(w.r, w.r.nb, tt, a.window);
+  }
+  const long long below = block_scan(mine, s_sums, total);
+  const long long share = (total + gridDim.x - 1) / gridDim.x, x0 = min(total, share * blockIdx.x), x1 = min(total, x0 + share);
+  if (x0 < x1 && below <= x0 && x0 < below + mine) {  // one thread: the request in which it begins
+    long long at = below;
+    for (int i = r0; i < r1; ++i) {
+      const Raw w = request(a, i, tt);
+      const long long c = a.kv.n_kv * ab_cost(w.r, w.r.nb, tt, a.window);
+      if (x0 < at + c) {
+        s_req = i, s_rest = x0 - at;
+        break;
+      }
+      at += c;
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  if (warp == 0 && s_req < a.n_req) {  // the block in which it begins: the last one whose cost of blocks before is not above the rest, 32 at a time
+    const Raw w = request(a, s_req, tt);
+    const long long head = ab_cost(w.r, w.r.nb, tt, a.window), rest = s_rest % head;
+    int lo = 0, hi = w.r.nb;
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 31) / 32, x = lo + lane * step;
+      const unsigned in = __ballot_sync(0xffffffffu, x < hi && ab_cost(w.r, x, tt, a.window) <= rest);
+      const int k = 31 - __clz(in);  // (lane 0's is)
+      hi = min(hi, lo + (k + 1) * step), lo += k * step;
+    }
+    if (lane == 0) s_kvh = (int)(s_rest / head), s_block = lo, s_skip = (int)(rest - ab_cost(w.r, lo, tt, a.window));
+  }
+  __syncthreads();
+  Walk walk;
+  walk.req = s_req, walk.kvh = s_kvh, walk.block = s_block, walk.skip = s_skip, walk.left = s_req < a.n_req ? x1 - x0 : 0;
+  if (walk.left > 0) walk.w = request(a, walk.req, tt);
+  uint32_t tmem;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(slot));
+  const uint32_t t_o = tmem + 128;  // scores: columns 0 .. 63 and 64 .. 127, the weights over them
+  JoinInfo* info = reinterpret_cast<JoinInfo*>(a.work);
+  unsigned long long* odd_bits = reinterpret_cast<unsigned long long*>(smem_raw + (s0 - smem_u32(smem_raw)) + SM::ODD);  // [edge tile][column][2]
+  float* parts = reinterpret_cast<float*>(info + gridDim.x) + (size_t)blockIdx.x * 2 * PART<HD>;
+
+  if (warp == NSOFT / 32 + 1) {
+    // ---- copies
+    const int P = a.kv.page_size, chunks = TK / box;  // of a tile
+    const uint32_t q_bytes = (uint32_t)(NB * tt * G * 128);
+    const int none = a.kv.n_pages * a.kv.n_layers * 2 * a.kv.n_kv * P;  // (TMA) a row behind the pool: zeros
+    Piece p;
+    int T = 0;  // tiles so far
+    for (int item = 0; walk.next(a, tt, p); ++item) {
+      const int* bt = a.block_table + (size_t)p.slot * a.max_pages;
+      const int last_page = (p.limit - 1) / P;
+      if (item > 0) mbar_wait_tc(free_q, (uint32_t)((item - 1) & 1), dead);
+      if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar_q), "r"(q_bytes) : "memory");
+      __syncwarp();
+      if (lane < NB)
+        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                     ::"r"(s0 + SM::Q + lane * QBLK), "l"(&qm), "r"(bar_q), "r"(lane * 64), "r"(p.kvh * G), "r"(p.t0)
+                     : "memory");
+      __syncwarp();
+      const int c0 = p.key0 / box;  // chunks of `box` keys; a lane holds the page of chunk `held` + lane
+      int held = -1000, page_of = 0;
+      for (int i = p.begin; i < p.end; ++i, ++T) {
+        const uint32_t st = (uint32_t)(T % ST);
+        if constexpr (TMA) {
+          const int ch = c0 + i * chunks;
+          if (ch < held || ch + chunks > held + 32) {
+            held = ch;
+            page_of = bt[min((ch + lane) * box / P, last_page)];  // chunks behind the last page repeat it (their keys are masked)
+          }
+          const int j = lane / NB, nb = lane % NB, page = __shfl_sync(0xffffffffu, page_of, (ch - held + j) & 31);
+          const int at = min((ch + j) * box, last_page * P + P - box) % P;  // (positions end at 2^30)
+          const bool in = page >= 0 && page < a.kv.n_pages;
+#pragma unroll
+          for (int is_v = 0; is_v < 2; ++is_v) {
+            if (T >= ST) mbar_wait_tc((is_v ? free_v : free_k) + 8u * st, (uint32_t)((T / ST - 1) & 1), dead);
+            const uint32_t bar = (is_v ? bar_v : bar_k) + 8u * st, dst = s0 + (is_v ? SM::V : SM::K) + st * SM::TILE + nb * KBLK + j * box * 128;
+            const int row = in ? (((page * a.kv.n_layers + a.layer) * 2 + is_v) * a.kv.n_kv + p.kvh) * P + at : none;
+            if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"((uint32_t)SM::TILE) : "memory");
+            __syncwarp();
+            if (lane < chunks * NB)
+              asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                           ::"r"(dst), "l"(&kvm), "r"(bar), "r"(nb * 64), "r"(row)
+                           : "memory");
+            __syncwarp();
+          }
+        } else {
+#pragma unroll
+          for (int is_v = 0; is_v < 2; ++is_v) {
+            if (T >= ST) mbar_wait_tc((is_v ? free_v : free_k) + 8u * st, (uint32_t)((T / ST - 1) & 1), dead);
+            const uint32_t dst = s0 + (is_v ? SM::V : SM::K) + st * SM::TILE;
+            const int c = lane & 7;
+            for (int k = lane >> 3; k < TK; k += 4) {  // eight lanes a row
+              const int key = min(p.key0 + i * TK + k, p.limit - 1), pg = key / P, page = bt[pg];
+              const bool in = page >= 0 && page < a.kv.n_pages;
+              const bf16* src = a.kv.chunk(in ? page : 0, a.layer, is_v, p.kvh) + (size_t)(key - pg * P) * HD + c * 8;
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb) cp_async16(dst + nb * KBLK + k * 128 + ((c ^ (k & 7)) << 4), src + nb * 64);
+            }
+            cp_async_commit();
+            cp_async_wait<0>();
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive_tc((is_v ? bar_v : bar_k) + 8u * st);
+          }
+        }
+      }
+    }
+  } else if (warp == NSOFT / 32) {
+    // ---- products
+    const uint32_t id_s = idesc_tc(TQ, TK, false), id_o = idesc_tc(TQ, HD, true);
+    const uint64_t dq = desc_k_tc(s0 + SM::Q), dk = desc_k_tc(s0 + SM::K), dv = desc_mn_tc(s0 + SM::V, KBLK);  // (steps are sums: in units of 16 bytes)
+    Walk ahead = walk;
+    Piece p;
+    int TS = 0, s_left = 0, items = 0;  // tiles of S issued; of the item they are in, left; items begun
+    auto issue_s = [&]() {              // the next tile's scores, if there is one
+      if (s_left == 0) {
+        Piece n;
+        if (!ahead.next(a, tt, n)) {
+          s_left = -1;
+          return;
+        }
+        s_left = n.count();
+        mbar_wait_tc(bar_q, (uint32_t)(items & 1), dead);
+        ++items;
+      }
+      if (s_left < 0) return;
+      const uint64_t k = dk + (uint64_t)((TS % ST) * (SM::TILE >> 4));
+      mbar_wait_tc(bar_k + 8u * (uint32_t)(TS % ST), (uint32_t)((TS / ST) & 1), dead);
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (elect_tc()) {
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk)
+          umma_tc(tmem + (uint32_t)((TS & 1) * TK), dq + (uint64_t)(((kk >> 2) * QBLK + (kk & 3) * 32) >> 4), k + (uint64_t)(((kk >> 2) * KBLK + (kk & 3) * 32) >> 4), id_s,
+                  kk != 0);
+        umma_commit_tc(bar_s + 8u * (uint32_t)(TS & 1));
+        umma_commit_tc(free_k + 8u * (uint32_t)(TS % ST));
+        if (s_left == 1) umma_commit_tc(free_q);
+      }
+      __syncwarp();
+      ++TS, --s_left;
+    };
+    issue_s();
+    issue_s();
+    for (int T = 0; walk.next(a, tt, p);)
+      for (int i = 0; i < p.count(); ++i, ++T) {
+        const uint32_t b = 8u * (uint32_t)(T & 1), ph = (uint32_t)((T >> 1) & 1), st = (uint32_t)(T % ST);
+        mbar_wait_tc(bar_v + 8u * st, (uint32_t)((T / ST) & 1), dead);
+        mbar_wait_tc(bar_p + b, ph, dead);
+        const uint32_t w = tmem + (uint32_t)((T & 1) * TK);
+        const uint64_t v = dv + (uint64_t)(st * (SM::TILE >> 4));
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (elect_tc()) {
+#pragma unroll
+          for (int kk = 0; kk < TK / 16; ++kk) umma_ts_tc(t_o, w + (uint32_t)(kk * 8), v + (uint64_t)(kk * 128), id_o, i > 0 || kk > 0);
+          umma_commit_tc(bar_o + b);
+          umma_commit_tc(free_v + 8u * st);
+        }
+        __syncwarp();
+        if (s_left >= 0) {
+          mbar_wait_tc(bar_o + b, ph, dead);  // S(T + 2) goes over the weights that P V(T) reads
+          issue_s();
+        }
+      }
+  } else {
+    // ---- softmax: this thread's row
+    const int row = tid, tok = row / G, g = row - tok * G;
+    const uint32_t la = (uint32_t)(warp * 32) << 16;
+    const float sl2 = a.scale_log2;
+    Piece p;
+    int T = 0;
+    if (tid == 0) info[blockIdx.x].parts = 0;
+    for (int item = 0; walk.next(a, tt, p); ++item) {
+      const bool some = warp * 32 < p.tokens * G;  // the warp has rows
+      const int my_pos = p.pos0 + min(tok, p.tokens - 1), my_low = a.window > 0 ? max(0, my_pos - a.window + 1) : 0;
+      const int low0 = a.window > 0 ? max(0, p.pos0 - a.window + 1) : 0, low1 = a.window > 0 ? max(0, p.pos0 + p.tokens - a.window) : 0;  // of the first and the last token
+      float m_ref = -INFINITY, l_run = 0.f;
+      int edge = 0;
+      for (int i = p.begin; i < p.end; ++i, ++T) {
+        const uint32_t b = 8u * (uint32_t)(T & 1), ph = (uint32_t)((T >> 1) & 1), ts = tmem + la + (uint32_t)((T & 1) * TK), st = (uint32_t)(T % ST);
+        const int key = p.key0 + i * TK, last = my_pos - key, low = my_low - key;  // the first key of the tile; the last and the first that the row sees
+        mbar_wait_tc(bar_s + b, ph, dead);
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (some) {
+          uint32_t r[64];
+          ld32(ts, r);
+          ld32(ts + 32, r + 32);
+          wait_ld();
+          if (last < TK - 1) {
+#pragma unroll
+            for (int j = 0; j < TK; ++j)
+              if (j > last) r[j] = 0xff800000u;  // -inf
+          }
+          if (low > 0) {
+#pragma unroll
+            for (int j = 0; j < TK; ++j)
+              if (j < low) r[j] = 0xff800000u;
+          }
+          float mx[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx[e] = max3(__uint_as_float(r[e]), __uint_as_float(r[e + 4]), __uint_as_float(r[e + 8]));
+#pragma unroll
+          for (int j = 12; j + 8 <= TK; j += 8)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(r[j + e]), __uint_as_float(r[j + 4 + e]));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(r[60 + e]));
+          const float m_new = fmaxf(m_ref, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2);
+          const bool grow = __any_sync(0xffffffffu, m_new > m_ref);
+          const float f = m_new > -INFINITY ? ex2_tc(m_ref - m_new) : 1.f;
+          m_ref = m_new;
+          const unsigned long long s2 = twice(sl2), n2 = twice(m_new > -INFINITY ? -m_new : 0.f);
+          float rs[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < TK; c += 32) {
+            uint32_t w[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              float e0 = __uint_as_float(r[c + 2 * e]), e1 = __uint_as_float(r[c + 2 * e + 1]);
+              fma2(e0, e1, s2, n2);
+              e0 = ex2_tc(e0), e1 = ex2_tc(e1);
+              add2(rs[2 * (e & 1)], rs[2 * (e & 1) + 1], e0, e1);
+              w[e] = pack2f(e0, e1);
+            }
+            tmem_st16_tc(ts + c / 2, w);
+          }
+          l_run = l_run * f + ((rs[0] + rs[1]) + (rs[2] + rs[3]));
+          if (grow && i > p.begin) {  // scale O by the new reference; behind the exponentials the product of the tile before is in
+            mbar_wait_tc(bar_o + (b ^ 8u), (uint32_t)(((T - 1) >> 1) & 1), dead);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+            for (int c = 0; c < HD; c += 64) {
+              uint32_t o[64];
+              ld32(t_o + la + c, o);
+              ld32(t_o + la + c + 32, o + 32);
+              wait_ld();
+#pragma unroll
+              for (int j = 0; j < 64; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+              st32(t_o + la + c, o);
+              st32(t_o + la + c + 32, o + 32);
+            }
+          }
+        }
+        if ((key + TK > p.pos0 + 1 || key < low1) && edge < EDGES) {  // some row does not see some key of the tile
+          mbar_wait_tc(bar_v + 8u * st, (uint32_t)((T / ST) & 1), dead);
+          if (tid == 0) s_edge[edge] = key;
+          for (int e = tid; e < TK * NB * 8; e += NSOFT) {
+            const int nb = e / (TK * 8), k = (e >> 3) & (TK - 1), c = e & 7, at = key + k;
+            const uint32_t addr = s0 + SM::V + st * SM::TILE + (uint32_t)(nb * KBLK + k * 128 + (c << 4));
+            uint32_t x[4];
+            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(addr));
+            bool odd = false;
+#pragma unroll
+            for (int y = 0; y < 4; ++y) odd |= (x[y] & 0x7f80u) == 0x7f80u || (x[y] & 0x7f800000u) == 0x7f800000u;
+            if (!odd) continue;
+            if (at >= p.pos0 + p.tokens || at < low0) {  // no row of the item sees the key
+              x[0] = x[1] = x[2] = x[3] = 0;
+            } else {
+              s_odd[item & 1] = 1;
+#pragma unroll
+              for (int y = 0; y < 8; ++y) {
+                const uint32_t v = (y & 1 ? x[y >> 1] >> 16 : x[y >> 1]) & 0xffffu;
+                if ((v & 0x7f80u) != 0x7f80u) continue;
+                x[y >> 1] &= y & 1 ? 0xffffu : 0xffff0000u;
+                // a bit a key: in the first word +infinity, in the second -infinity, in both no number
+                unsigned long long* to = odd_bits + 2 * (edge * HD + nb * 64 + ((c ^ (k & 7)) << 3) + y);
+                if (v != 0xff80u) atomicOr(to, 1ull << k);
+                if (v != 0x7f80u) atomicOr(to + 1, 1ull << k);
+              }
+            }
+            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          ++edge;
+        }
+        wait_st();
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        mbar_arrive_tc(bar_p + b);
+      }
+      // ---- the item's rows
+      mbar_wait_tc(bar_o + 8u * (uint32_t)((T - 1) & 1), (uint32_t)(((T - 1) >> 1) & 1), dead);
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const bool whole = p.whole();
+      const int odd = *(volatile int*)&s_odd[item & 1];  // (a thread may be in the next item already, none in the one behind it)
+      if (some) {
+        const float scale = *dead ? __int_as_float(0x7fc00000) : !whole ? 1.f : l_run > 0.f ? 1.f / l_run : l_run;
+        bf16* dst = a.out + (size_t)(p.t0 + tok) * a.out_stride + (size_t)(p.kvh * G + g) * HD;
+        float* part = parts + (p.begin > 0 ? 0 : PART<HD>);
+        if (!whole) part[TQ * HD + row] = m_ref, part[TQ * HD + TQ + row] = *dead ? __int_as_float(0x7fc00000) : l_run;
+#pragma unroll
+        for (int c = 0; c < HD; c += 32) {
+          uint32_t r[32];
+          ld32(t_o + la + c, r);
+          wait_ld();
+          if (odd)
+            for (int n = 0; n < edge; ++n) {
+              // the keys of the edge tile that the row sees
+              const int from = max(0, my_low - s_edge[n]), to = min(TK - 1, my_pos - s_edge[n]);
+              const unsigned long long sees = from > to ? 0ull : (~0ull >> (TK - 1 - to)) & (~0ull << from);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                const unsigned long long* bits = odd_bits + 2 * (n * HD + c + j);
+                if (bits[0] & sees) r[j] = __float_as_uint(__uint_as_float(r[j]) + INFINITY);
+                if (bits[1] & sees) r[j] = __float_as_uint(__uint_as_float(r[j]) - INFINITY);
+              }
+            }
+          if (tok >= p.tokens) continue;
+          if (whole) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 8) {
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) w[e] = pack2f(__uint_as_float(r[j + 2 * e]) * scale, __uint_as_float(r[j + 2 * e + 1]) * scale);
+              *reinterpret_cast<uint4*>(dst + c + j) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) *reinterpret_cast<uint4*>(part + row * HD + c + j) = make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
+          }
+        }
+      }
+      if (tid == 0 && !whole && p.begin == 0) {  // this CTA's last item goes on in the CTAs behind
+        const long long end = x0 + ((x1 - x0) - p.end) + p.tiles - 1;  // (the stretch ends with the piece) place of the item's last tile
+        info[blockIdx.x] = JoinInfo{p.t0, p.tokens, p.kvh, (int)(end / share) - (int)blockIdx.x + 1};
+      }
+      if (odd) {  // the same in every thread: arrivals at bar_p lie between the writes and this
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        for (int e = tid; e < EDGES * HD; e += NSOFT) odd_bits[2 * e] = odd_bits[2 * e + 1] = 0;
+        if (tid == 0) s_odd[item & 1] = 0;
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+      }
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == NSOFT / 32) {
+    drain_tc(dead);
+    if (lane == 0) report_tc(dead, a.status);
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+  }
+}
+
+// The parts of an item that was cut: CTA k joins the one that CTA k of the kernel above began and did not end.  A group of warps a row, each with a share of
+// the parts; their sums meet in shared memory, in a fixed order.
+constexpr int JOIN_THR = 512, JOIN_WARPS = JOIN_THR / 32;
+template <int HD>
+__global__ void __launch_bounds__(JOIN_THR) attn_batch_join_kernel(BatchAttnArgs a, int G, int n_cta) {
+  constexpr int E = HD / 32;
+  __shared__ float s_o[JOIN_WARPS][HD], s_m[JOIN_WARPS], s_l[JOIN_WARPS];
+  pdl_wait();
+  pdl_trigger();
+  const JoinInfo* info = reinterpret_cast<const JoinInfo*>(a.work);
+  const JoinInfo in = info[blockIdx.x];
+  const float* base = reinterpret_cast<const float*>(info + n_cta);
+  const int rows = in.tokens * G, parts = in.parts, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // (a work area that two calls used at once must not lead outside)
+  if (parts <= 0 || parts > n_cta - (int)blockIdx.x || rows <= 0 || rows > TQ || in.t0 < 0 || in.t0 > a.n_tok - in.tokens || in.kvh < 0 || in.kvh >= a.kv.n_kv) return;
+  int wpr = 1;  // warps a row
+  while (wpr * 2 * rows <= JOIN_WARPS && wpr < parts) wpr *= 2;
+  const int groups = JOIN_WARPS / wpr, group = warp / wpr, sub = warp % wpr;
+  for (int r0 = 0; r0 < rows; r0 += groups) {
+    const int row = r0 + group;
+    float m = -INFINITY, l = 0.f, o[E];
+    for (int e = 0; e < E; ++e) o[e] = 0.f;
+    if (row < rows)
+      for (int q = sub; q < parts; q += wpr) {
+        const float* part = base + ((size_t)(blockIdx.x + q) * 2 + (q == 0)) * PART<HD>;
+        const float pm = part[TQ * HD + row], pl = part[TQ * HD + TQ + row];
+        float x[E];
+        for (int e = 0; e < E; ++e) x[e] = part[(size_t)row * HD + lane * E + e];
+        const float top = fmaxf(m, pm), f = m > -INFINITY ? ex2_tc(m - top) : 0.f, pf = pl != pl ? pl : pm > -INFINITY ? ex2_tc(pm - top) : 0.f;
+        m = top;
+        l = l * f + pl * pf;
+        for (int e = 0; e < E; ++e) o[e] = o[e] * f + (pf != 0.f ? x[e] * pf : 0.f);
+      }
+    if (wpr > 1) {
+      __syncthreads();
+      for (int e = 0; e < E; ++e) s_o[warp][lane * E + e] = o[e];
+      if (lane == 0) s_m[warp] = m, s_l[warp] = l;
+      __syncthreads();
+      if (sub == 0) {
+        float top = m;
+        for (int w = 1; w < wpr; ++w) top = fmaxf(top, s_m[warp + w]);
+        float sum = 0.f;
+        for (int e = 0; e < E; ++e) o[e] = 0.f;
+        for (int w = 0; w < wpr; ++w) {
+          const float wl = s_l[warp + w], wm = s_m[warp + w], f = wl != wl ? wl : wm > -INFINITY ? ex2_tc(wm - top) : 0.f;
+          sum += wl * f;
+          for (int e = 0; e < E; ++e) o[e] += f != 0.f ? s_o[warp + w][lane * E + e] * f : 0.f;
+        }
+        l = sum;
+      }
+    }
+    if (row < rows && sub == 0) {
+      const float inv = l > 0.f ? 1.f / l : l;
+      bf16* dst = a.out + (size_t)(in.t0 + row / G) * a.out_stride + (size_t)(in.kvh * G + row % G) * HD + lane * E;
+      for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack2f(o[e] * inv, o[e + 1] * inv);
+    }
+  }
+}
+
+template <int HD, bool TMA>
+cudaError_t launch_hd(const BatchAttnArgs& a, const TensorMap2D& qm, const TensorMap2D& kvm, int box, cudaStream_t st) {
+  static PerDeviceOnce set;
+  if (set.need()) {
+    const cudaError_t e = cudaFuncSetAttribute(attn_batch_kernel<HD, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<HD>::TOTAL);
+    if (e != cudaSuccess) return e;
+    set.done();
+  }
+  const int G = a.n_q / a.kv.n_kv, ctas = 2 * a.num_sms;
+  const cudaError_t e = launched(launch_k(attn_batch_kernel<HD, TMA>, dim3(ctas), dim3(NTHR), Smem<HD>::TOTAL, st, a, Shape{G, TQ / G}, box,
+                                          *reinterpret_cast<const CUtensorMap*>(&qm), *reinterpret_cast<const CUtensorMap*>(&kvm)));
+  if (e != cudaSuccess) return e;
+  return launched(launch_k(attn_batch_join_kernel<HD>, dim3(ctas), dim3(JOIN_THR), 0, st, a, G, ctas));
 }
 
 }  // namespace
 
-size_t attention_batch_work(int, int) { return 16; }
+size_t attention_batch_work(int hd, int num_sms) { return (size_t)2 * num_sms * (sizeof(JoinInfo) + 2 * (hd == 64 ? PART<64> : PART<128>) * sizeof(float)); }
 
 cudaError_t launch_attention_batch(const BatchAttnArgs& a, cudaStream_t st) {
-  const dim3 grid(a.n_tok, (a.n_q + 7) / 8);
-  return launched(a.kv.hd == 64 ? launch_k(attn_batch_kernel<64>, grid, dim3(256), 0, st, a) : launch_k(attn_batch_kernel<128>, grid, dim3(256), 0, st, a));
+  const int G = a.n_q / a.kv.n_kv, P = a.kv.page_size;
+  TensorMap2D qm, kvm{};
+  cudaError_t e = make_tensor_map_heads(&qm, a.q, a.kv.hd, a.n_q, a.n_tok, a.q_stride, G, TQ / G);
+  if (e != cudaSuccess) return e;
+  const unsigned long long rows = (unsigned long long)a.kv.n_pages * a.kv.n_layers * 2ull * a.kv.n_kv * P;
+  const bool tma = P % 16 == 0 && rows < (1ull << 31);
+  const int box = !tma ? TK : P % 64 == 0 ? 64 : P % 32 == 0 ? 32 : 16;  // the largest that divides a page and a tile
+  if (tma && (e = make_tensor_map_kv(&kvm, a.kv.pool, rows, a.kv.hd, box)) != cudaSuccess) return e;
+  if (a.kv.hd == 64) return tma ? launch_hd<64, true>(a, qm, kvm, box, st) : launch_hd<64, false>(a, qm, kvm, box, st);
+  return tma ? launch_hd<128, true>(a, qm, kvm, box, st) : launch_hd<128, false>(a, qm, kvm, box, st);
 }
 
 }  // namespace qie

@@ -411,15 +411,14 @@ int qie_attention_prefill_tc(const qie_kv_view* kv, int layer, const qie_bf16* Q
 }
 
 // ---------------------------------------------------------------- a serving step
-// a table of `rows` positions a page that offsets of 32 bits name
 static bool batch_sizes_ok(const qie_batch* b) {
   return b && b->n_req >= 0 && b->n_req <= QIE_BATCH_MAX_REQ && b->max_tokens >= 0 && b->max_seqs >= 0 && b->max_pages > 0 && b->page_size > 0 &&
-         (long long)b->max_pages * b->page_size < (1ll << 31) && (b->n_req == 0 || b->max_seqs > 0);
+         (long long)b->max_pages * b->page_size <= (1ll << 30) && (b->n_req == 0 || b->max_seqs > 0);
 }
 int qie_batch_layout(const qie_batch* b, qie_stream st) {
   static_assert(BATCH_MAX_REQ == QIE_BATCH_MAX_REQ, "one limit");
   if (!batch_sizes_ok(b) || b->n_pages <= 0 || (long long)b->n_pages * b->page_size >= (1ll << 31))
-    return fail(QIE_EINVAL, "batch_layout: need 0 to %d requests, and n_pages and max_pages above 0 with less than 2^31 positions", QIE_BATCH_MAX_REQ);
+    return fail(QIE_EINVAL, "batch_layout: need 0 to %d requests, and n_pages and max_pages above 0 with less than 2^31 and at most 2^30 positions", QIE_BATCH_MAX_REQ);
   if (!b->free_ring || !b->ring_in || !b->ring_out || !b->q_start || !b->status || (b->n_req && (!b->cached || !b->n_new || !b->block_table || !b->kv_len)) ||
       (b->max_tokens && (!b->pos || !b->slot || !b->row)))
     return fail(QIE_EINVAL, "batch_layout: an array is missing");
@@ -517,6 +516,7 @@ int qie_attention_batch(const qie_kv_view* kv, int layer, const qie_batch* b, co
   if (!b->slots && b->n_req > b->max_seqs) return fail(QIE_EINVAL, "attention_batch: %d requests on %d rows of the block table", b->n_req, b->max_seqs);
   if (window < 0 || !(scale >= 0.f) || scale > 1e6f) return fail(QIE_EINVAL, "attention_batch: window and scale must not be below 0");
   if (b->n_req == 0 || b->max_tokens == 0) return QIE_OK;
+  if (b->max_tokens >= 1 << 24) return fail(QIE_EINVAL, "attention_batch: at most 2^24 - 1 rows");
   if (!b->q_start || !b->kv_len || !b->block_table || !Q || !out) return fail(QIE_EINVAL, "attention_batch: an array is missing");
   const size_t wide = (size_t)n_q_heads * kv->head_dim;
   if (q_stride < wide || out_stride < wide || q_stride % 8 || out_stride % 8 || q_stride >= (1ull << 38)) return fail(QIE_EINVAL, "attention_batch: rows of Q and out are multiples of 8 elements, %zu at least", wide);

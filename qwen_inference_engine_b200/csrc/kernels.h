@@ -235,6 +235,8 @@ cudaError_t make_tensor_map_kv(TensorMap2D* out, const bf16* pool, unsigned long
 // cache rows of one layer as a 3-D tensor {row elements, positions of a page, pages} (page stride page_elems): box = 64 elements x box_rows
 // positions of one page, 128-byte swizzle
 cudaError_t make_tensor_map_pages(TensorMap2D* out, const bf16* base, int row_elems, int page_size, int n_pages, size_t page_elems, int box_rows);
+// rows of heads as a 3-D tensor {head_dim, heads, rows} (row stride in elements): box = 64 elements x box_heads x box_rows, 128-byte swizzle
+cudaError_t make_tensor_map_heads(TensorMap2D* out, const bf16* base, int hd, int heads, int rows, size_t stride, int box_heads, int box_rows);
 struct TcGemm {
   const TensorMap2D* w[3];   // weight maps, box rows = 128 (EPI_SILU_MUL: 64)
   const TensorMap2D* w2[3];  // the same of two k-blocks (make_tensor_map_w3d, kc = 128)
