@@ -4,6 +4,9 @@
 //   n_i = max(new_i, 0), had_i = ceil(cached_i / P), need_i = ceil((cached_i + n_i) / P) - had_i, back_i = had_i where the request is over
 //   token t of request i (t in [sum n_<i, sum n_<=i)): position p = cached_i + t - sum n_<i, its page the request's p / P -th:
 //   the block table's where p / P < had_i, else ring[(first + sum need_<i + p / P - had_i) mod n_pages], which the table gets too
+#include <algorithm>
+
+#include "cluster.cuh"
 #include "common.cuh"
 #include "kernels.h"
 #include "launch.h"
@@ -11,7 +14,7 @@
 namespace qie {
 namespace {
 
-constexpr int NTHR = 1024;
+constexpr int MOST_THR = 512, MOST_CTA = 8, MOST_GRID = 128;
 
 struct Sums {
   long long tok, need, back;
@@ -21,21 +24,26 @@ __device__ __forceinline__ Sums from_below(Sums v, int d) {
   return {__shfl_up_sync(0xffffffffu, v.tok, d), __shfl_up_sync(0xffffffffu, v.need, d), __shfl_up_sync(0xffffffffu, v.back, d)};
 }
 
+// what the CTA keeps of each request in shared memory: running sums of tokens, pages needed and pages given back, positions, row of the block table
+struct Kept {
+  int *tok, *need, *back, *cached, *slot;
+  __device__ Kept(int* p, int n) : tok(p), need(p + n + 1), back(p + 2 * (n + 1)), cached(p + 3 * (n + 1)), slot(p + 4 * (n + 1)) {}
+};
 struct Request {
-  int tok, need, back, had, flags;
+  int n, slot, cached, flags;
+  Sums s;
 };
 __device__ __forceinline__ Request request(const BatchArgs& a, int i) {
-  const int c = a.cached[i], n = a.n_new[i], slot = a.slots ? a.slots[i] : i;
-  Request r{0, 0, 0, 0, 0};
-  if (c < 0 || n < -1 || slot < 0 || slot >= a.max_seqs) {
+  Request r{a.n_new[i], a.slots ? a.slots[i] : i, a.cached[i], 0, {0, 0, 0}};
+  if (r.cached < 0 || r.n < -1 || r.slot < 0 || r.slot >= a.max_seqs) {
     r.flags = 8;
-  } else if ((long long)c + max(n, 0) > (long long)a.max_pages * a.page_size) {
+  } else if ((long long)r.cached + max(r.n, 0) > a.max_pages * a.page_size) {
     r.flags = 2;
   } else {
-    r.had = (int)(((long long)c + a.page_size - 1) / a.page_size);
-    r.tok = max(n, 0);
-    r.need = n > 0 ? (int)(((long long)c + n + a.page_size - 1) / a.page_size) - r.had : 0;
-    r.back = n < 0 ? r.had : 0;
+    const int had = (r.cached + a.page_size - 1) / a.page_size;
+    r.s.tok = max(r.n, 0);
+    r.s.need = r.n > 0 ? (r.cached + r.n + a.page_size - 1) / a.page_size - had : 0;
+    r.s.back = r.n < 0 ? had : 0;
   }
   return r;
 }
@@ -50,25 +58,26 @@ __device__ __forceinline__ int holder(const int* s, int n, int x) {
   return lo;
 }
 
-__global__ void __launch_bounds__(NTHR) batch_layout_kernel(BatchArgs a) {
-  extern __shared__ int sums[];
-  __shared__ Sums warp_sums[NTHR / 32];
+__global__ void __launch_bounds__(MOST_THR) batch_layout_kernel(BatchArgs a, int wide, int cluster) {
+  extern __shared__ int kept_s[];
+  __shared__ Sums warp_sums[MOST_THR / 32];
   __shared__ int flags_s;
-  int *tok = sums, *need = tok + a.n_req + 1, *back = need + a.n_req + 1;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const Kept kept(kept_s, a.n_req);
+  const int tid = threadIdx.x, thr = blockDim.x, lane = tid & 31, warp = tid >> 5;
+  const int all = gridDim.x * thr, me = blockIdx.x * thr + tid;  // of all threads
   pdl_wait();
   pdl_trigger();
   if (tid == 0) flags_s = 0;
   const int first = a.ring_in[0], count = a.ring_in[1];
-  __syncthreads();
-  // ---- running sums over the requests, a stretch of them a thread
-  const int per = (a.n_req + NTHR - 1) / NTHR, i0 = min(a.n_req, tid * per), i1 = min(a.n_req, i0 + per);
+  // ---- running sums over the requests, a stretch of them a thread; every CTA for itself
+  const int per = (a.n_req + thr - 1) / thr, i0 = min(a.n_req, tid * per), i1 = min(a.n_req, i0 + per);
   Sums mine{0, 0, 0};
   int flags = 0;
+  Request one{};
   for (int i = i0; i < i1; ++i) {
-    const Request r = request(a, i);
-    mine = add(mine, Sums{r.tok, r.need, r.back});
-    flags |= r.flags;
+    one = request(a, i);
+    mine = add(mine, one.s);
+    flags |= one.flags;
   }
   Sums run = mine;
   for (int d = 1; d < 32; d <<= 1) {
@@ -76,68 +85,96 @@ __global__ void __launch_bounds__(NTHR) batch_layout_kernel(BatchArgs a) {
     if (lane >= d) run = add(run, o);
   }
   if (lane == 31) warp_sums[warp] = run;
-  if (flags) atomicOr(&flags_s, flags);
   __syncthreads();
+  if (flags) atomicOr(&flags_s, flags);
   Sums before{0, 0, 0}, total{0, 0, 0};
-  for (int w = 0; w < NTHR / 32; ++w) {
+  for (int w = 0; w < thr / 32; ++w) {
     if (w == warp) before = total;
     total = add(total, warp_sums[w]);
   }
+  Sums at{before.tok + run.tok - mine.tok, before.need + run.need - mine.need, before.back + run.back - mine.back};
+  for (int i = i0; i < i1; ++i) {  // (a flag makes these sums useless, and nothing uses them)
+    const Request r = per == 1 ? one : request(a, i);
+    kept.tok[i] = (int)at.tok, kept.need[i] = (int)at.need, kept.back[i] = (int)at.back;
+    kept.cached[i] = r.cached, kept.slot[i] = r.slot;
+    if (blockIdx.x == 0) a.kv_len[i] = r.n < 0 ? 0 : r.cached + r.n, a.q_start[i] = (int)at.tok;
+    at = add(at, r.s);
+  }
+  if (tid == 0) {
+    kept.tok[a.n_req] = (int)total.tok, kept.need[a.n_req] = (int)total.need, kept.back[a.n_req] = (int)total.back;
+    if (blockIdx.x == 0) a.q_start[a.n_req] = (int)total.tok;
+  }
+  __syncthreads();
   flags = flags_s;
   if (first < 0 || first >= a.n_pages || count < 0 || count > a.n_pages) flags |= 8;
   else if (total.need > count) flags |= 1;
   else if (count + total.back > a.n_pages) flags |= 8;
   if (total.tok > a.max_tokens) flags |= 4;
-  if (tid == 0) {
+  const int n_tok = flags ? 0 : (int)total.tok, n_back = flags ? 0 : (int)total.back;
+  if (flags && blockIdx.x == 0) {  // nothing to do for anybody
+    for (int i = tid; i <= a.n_req; i += thr) a.q_start[i] = 0;
+    for (int i = tid; i < a.n_req; i += thr) a.kv_len[i] = 0;
+  }
+  auto ring_at = [&](int i) {  // first + i modulo n_pages, i <= 2 n_pages
+    long long x = (long long)first + i;
+    while (x >= a.n_pages) x -= a.n_pages;
+    return (int)x;
+  };
+  // ---- pages given back: behind the ring's last, so at none of the places that are read below
+  for (int b = 4 * me; b < n_back; b += 4 * all) {
+    int i = holder(kept.back, a.n_req, b), page[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (b + e < n_back) {
+        while (kept.back[i + 1] <= b + e) ++i;
+        page[e] = a.block_table[(size_t)kept.slot[i] * a.max_pages + b + e - kept.back[i]];
+      }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (b + e < n_back) a.free_ring[ring_at(count + b + e)] = page[e];
+  }
+  // ---- tokens, four a thread and step.  The one that begins a page takes it into the block table.
+  for (int b = 4 * me; b < a.max_tokens; b += 4 * all) {
+    int pos[4], slot[4], row[4];
+    int i = -1, end = 0, from = -1, page = 0;  // the request and its end; the first position of the page at hand
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int t = b + e;
+      pos[e] = slot[e] = row[e] = -1;
+      if (t >= n_tok) continue;
+      if (t >= end) {
+        i = e == 0 ? holder(kept.tok, a.n_req, t) : i + 1;
+        while (kept.tok[i + 1] <= t) ++i;
+        end = kept.tok[i + 1], from = -1;
+      }
+      const int p = kept.cached[i] + t - kept.tok[i];
+      slot[e] = kept.slot[i];
+      if (from < 0 || p - from >= a.page_size) {
+        const int pg = p / a.page_size, had = (kept.cached[i] + a.page_size - 1) / a.page_size;
+        int* at = a.block_table + (size_t)slot[e] * a.max_pages + pg;
+        from = pg * a.page_size;
+        page = pg < had ? *at : a.free_ring[ring_at(kept.need[i] + pg - had)];
+        if (pg >= had && p == from) *at = page;
+      }
+      pos[e] = p;
+      row[e] = (int)((unsigned)page * a.page_size + (unsigned)(p - from));
+    }
+    if (wide && b + 4 <= a.max_tokens) {
+      *reinterpret_cast<int4*>(a.pos + b) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+      *reinterpret_cast<int4*>(a.slot + b) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+      *reinterpret_cast<int4*>(a.row + b) = make_int4(row[0], row[1], row[2], row[3]);
+    } else {
+      for (int e = 0; e < 4 && b + e < a.max_tokens; ++e) a.pos[b + e] = pos[e], a.slot[b + e] = slot[e], a.row[b + e] = row[e];
+    }
+  }
+  // ---- the ring's state, which may be the word that the others read
+  if (cluster) cluster_sync_all();
+  if (me == 0) {
     a.status[0] = flags;
     a.status[1] = flags & 1 ? (int)min(total.need - count, 0x7fffffffll) : 0;
+    a.ring_out[0] = flags ? first : ring_at((int)total.need);
+    a.ring_out[1] = flags ? count : count - (int)total.need + n_back;
   }
-  if (flags) {  // nothing to do for anybody
-    for (int i = tid; i <= a.n_req; i += NTHR) a.q_start[i] = 0;
-    for (int i = tid; i < a.n_req; i += NTHR) a.kv_len[i] = 0;
-    for (int t = tid; t < a.max_tokens; t += NTHR) a.pos[t] = a.slot[t] = a.row[t] = -1;
-    if (tid == 0) a.ring_out[0] = first, a.ring_out[1] = count;
-    return;
-  }
-  Sums at{before.tok + run.tok - mine.tok, before.need + run.need - mine.need, before.back + run.back - mine.back};
-  for (int i = i0; i < i1; ++i) {
-    const Request r = request(a, i);
-    tok[i] = (int)at.tok, need[i] = (int)at.need, back[i] = (int)at.back;
-    a.q_start[i] = (int)at.tok;
-    a.kv_len[i] = a.n_new[i] < 0 ? 0 : a.cached[i] + r.tok;
-    at = add(at, Sums{r.tok, r.need, r.back});
-  }
-  if (tid == 0) {
-    tok[a.n_req] = (int)total.tok, need[a.n_req] = (int)total.need, back[a.n_req] = (int)total.back;
-    a.q_start[a.n_req] = (int)total.tok;
-  }
-  __syncthreads();
-  // ---- pages taken and given back.  The places written in the ring are behind its last page, so none that is read.
-  auto ring_at = [&](int i) { return (int)(((long long)first + i) % a.n_pages); };
-  auto row_of = [&](int i) { return a.block_table + (size_t)(a.slots ? a.slots[i] : i) * a.max_pages; };
-  auto had_of = [&](int i) { return (int)(((long long)a.cached[i] + a.page_size - 1) / a.page_size); };
-  for (int j = tid; j < (int)total.need; j += NTHR) {
-    const int i = holder(need, a.n_req, j);
-    row_of(i)[had_of(i) + j - need[i]] = a.free_ring[ring_at(j)];
-  }
-  for (int j = tid; j < (int)total.back; j += NTHR) {
-    const int i = holder(back, a.n_req, j);
-    a.free_ring[ring_at(count + j)] = row_of(i)[j - back[i]];
-  }
-  // ---- tokens
-  for (int t = tid; t < a.max_tokens; t += NTHR) {
-    int pos = -1, slot = -1, row = -1;
-    if (t < (int)total.tok) {
-      const int i = holder(tok, a.n_req, t);
-      pos = a.cached[i] + t - tok[i];
-      slot = a.slots ? a.slots[i] : i;
-      const int had = had_of(i), pg = pos / a.page_size;
-      const int page = pg < had ? row_of(i)[pg] : a.free_ring[ring_at(need[i] + pg - had)];
-      row = page * a.page_size + pos - pg * a.page_size;
-    }
-    a.pos[t] = pos, a.slot[t] = slot, a.row[t] = row;
-  }
-  if (tid == 0) a.ring_out[0] = ring_at((int)total.need), a.ring_out[1] = count - (int)total.need + (int)total.back;
 }
 
 }  // namespace
@@ -145,11 +182,36 @@ __global__ void __launch_bounds__(NTHR) batch_layout_kernel(BatchArgs a) {
 cudaError_t launch_batch_layout(const BatchArgs& a, cudaStream_t st) {
   static PerDeviceOnce set;
   if (set.need()) {
-    const cudaError_t e = cudaFuncSetAttribute(batch_layout_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 * (BATCH_MAX_REQ + 1) * (int)sizeof(int));
+    const cudaError_t e = cudaFuncSetAttribute(batch_layout_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 5 * (BATCH_MAX_REQ + 1) * (int)sizeof(int));
     if (e != cudaSuccess) return e;
     set.done();
   }
-  return launched(launch_k(batch_layout_kernel, dim3(1), dim3(NTHR), 3 * (a.n_req + 1) * sizeof(int), st, a));
+  // A thread for four tokens and for a request.  Where the ring's state is updated in place the CTAs are one cluster (of eight at most): none may write it before all have read it.
+  const int thr = std::min(MOST_THR, std::max(128, (std::max((a.max_tokens + 3) / 4, a.n_req) + 31) / 32 * 32));
+  const bool in_place = a.ring_in == a.ring_out || a.ring_in + 1 == a.ring_out || a.ring_in == a.ring_out + 1;
+  const int ctas = std::max(1, std::min(in_place ? MOST_CTA : MOST_GRID, (a.max_tokens / 4 + thr - 1) / thr));
+  const bool wide = ((reinterpret_cast<uintptr_t>(a.pos) | reinterpret_cast<uintptr_t>(a.slot) | reinterpret_cast<uintptr_t>(a.row)) & 15) == 0;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(thr);
+  cfg.dynamicSmemBytes = 5 * (a.n_req + 1) * sizeof(int);
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  int na = 0;
+  if (in_place && ctas > 1) {
+    at[na].id = cudaLaunchAttributeClusterDimension;
+    at[na].val.clusterDim.x = ctas;
+    at[na].val.clusterDim.y = at[na].val.clusterDim.z = 1;
+    ++na;
+  }
+  if (g_use_pdl) {
+    at[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[na].val.programmaticStreamSerializationAllowed = 1;
+    ++na;
+  }
+  cfg.attrs = at;
+  cfg.numAttrs = na;
+  return launched(cudaLaunchKernelEx(&cfg, batch_layout_kernel, a, (int)wide, (int)(in_place && ctas > 1)));
 }
 
 }  // namespace qie
