@@ -84,6 +84,7 @@ class KvPool:
         self.pool = torch.zeros(n_pages, n_layers, 2, n_kv_heads, page_size, head_dim, dtype=torch.bfloat16,
                                 device="cuda")
         self.view = KvView(self.pool.data_ptr(), n_pages, page_size, n_layers, n_kv_heads, head_dim)
+        self.ref = C.byref(self.view)
         self.max_pages = n_pages
         # identity-ish block table: sequence s owns pages s, s+max_seqs, ... (deliberately non-contiguous)
         bt = np.zeros((max_seqs, n_pages), np.int32)
@@ -100,6 +101,7 @@ class KvPool:
         self = cls.__new__(cls)
         self.pool, self.block_table = pool, block_table
         self.view = KvView(_p(pool), n_pages, page_size, n_layers, n_kv_heads, head_dim)
+        self.ref = C.byref(self.view)
         self.max_pages = n_pages if block_table is None else block_table.shape[1]
         return self
 
@@ -160,20 +162,26 @@ def launch_attn_prefill_tc(Q, out, pool, layer, pos, slot, n_q_heads, variant=0)
 
 # ---- a serving step over the paged cache (see qie_batch in include/qie_b200.h) ----------------
 def _here(t):
-    assert t.device.index == torch.cuda.current_device(), "a tensor of another device than the current one"
+    """a tensor on the current device (torch's raw name, or the public way where torch does not have it: see _st)"""
+    try:
+        dev = torch._C._cuda_getDevice()
+    except AttributeError:
+        dev = torch.cuda.current_device()
+    assert t.get_device() == dev, "a tensor of another device than the current one, or of the host"
 
 
 def _ints(t, n, name):
-    """pointer of n int32 on the current device"""
-    assert t.dtype == torch.int32 and t.numel() >= n, f"{name}: {n} int32 expected"
-    _here(t)
-    return _p(t)
+    """pointer of n int32"""
+    assert t.dtype is torch.int32 and t.numel() >= n and t.is_cuda and t.is_contiguous(), f"{name}: {n} contiguous int32 on the device expected"
+    return t.data_ptr()
 
 
 def _rows(t):
-    """(pointer, row stride) of rows whose elements lie side by side"""
-    assert t.is_cuda and t.dim() == 2 and (t.shape[1] == 1 or t.stride(1) == 1), "device-resident rows of contiguous elements expected"
-    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    """(pointer, row stride) of rows of contiguous elements"""
+    n, wide = t.shape
+    stride, one = t.stride()
+    assert t.is_cuda and (one == 1 or wide == 1), "device-resident rows of contiguous elements expected"
+    return t.data_ptr(), stride if n > 1 else wide
 
 
 class Batch:
@@ -196,6 +204,7 @@ class Batch:
                         ("q_start", n_req + 1), ("kv_len", n_req), ("pos", max_tokens), ("slot", max_tokens), ("row", max_tokens), ("status", 2)):
             t = getattr(self, name)
             if t is not None:
+                _here(t)
                 setattr(b, name, _ints(t, n, name))
         self.ref = C.byref(b)
 
@@ -232,28 +241,30 @@ class Rope:
 
 def launch_rope_rows(x, out, pos, rope, n_heads, head_dim):
     """rows [n_tok, n_heads * head_dim] -> out (may be x), token t at position pos[t]"""
-    assert x.dtype == out.dtype == torch.bfloat16 and x.shape == out.shape and x.shape[1] == n_heads * head_dim
+    n, wide = x.shape
+    assert x.dtype is out.dtype is torch.bfloat16 and x.shape == out.shape and wide == n_heads * head_dim, "bfloat16 rows of n_heads * head_dim expected"
     _here(x)
-    check(_lib.lib().qie_rope_rows(*_rows(x), *_rows(out), rope.ref, _ints(pos, x.shape[0], "pos"), x.shape[0], n_heads, head_dim, _st()))
+    check(_lib.lib().qie_rope_rows(*_rows(x), *_rows(out), rope.ref, _ints(pos, n, "pos"), n, n_heads, head_dim, _st()))
 
 
 def launch_rope_store(q, k, v, q_out, pool, layer, pos, row, rope, n_q_heads):
     """q -> q_out, k and v -> the cache rows row[t] of the pool's layer"""
-    view, n = pool.view, q.shape[0]
-    assert q.dtype == k.dtype == v.dtype == q_out.dtype == torch.bfloat16
-    assert q.shape == q_out.shape and k.shape == v.shape == (n, view.n_kv_heads * view.head_dim) and q.shape[1] == n_q_heads * view.head_dim
+    view, (n, wide) = pool.view, q.shape
+    kv = (n, view.n_kv_heads * view.head_dim)
+    assert q.dtype is k.dtype is v.dtype is q_out.dtype is torch.bfloat16, "bfloat16 rows expected"
+    assert q_out.shape == q.shape and k.shape == kv and v.shape == kv and wide == n_q_heads * view.head_dim, "rows of the heads of as many tokens expected"
     _here(q)
-    check(_lib.lib().qie_rope_store(C.byref(view), layer, *_rows(q), *_rows(q_out), *_rows(k), *_rows(v), rope.ref, _ints(pos, n, "pos"), _ints(row, n, "row"), n,
+    check(_lib.lib().qie_rope_store(pool.ref, layer, *_rows(q), *_rows(q_out), *_rows(k), *_rows(v), rope.ref, _ints(pos, n, "pos"), _ints(row, n, "row"), n,
                                     n_q_heads, _st()))
 
 
 def launch_attn_batch(Q, out, pool, layer, batch, n_q_heads, window=0, scale=0.0):
     """attention of the batch's rows over the pool, ragged over its requests (fast numerics)"""
-    assert Q.dtype == out.dtype == torch.bfloat16 and Q.shape == out.shape == (batch.view.max_tokens, n_q_heads * pool.view.head_dim)
+    assert Q.dtype is out.dtype is torch.bfloat16 and Q.shape == out.shape == (batch.view.max_tokens, n_q_heads * pool.view.head_dim), "bfloat16 rows of the batch expected"
     if batch.work is None:
         batch.reserve(pool, n_q_heads)
     _here(Q)
-    check(_lib.lib().qie_attention_batch(C.byref(pool.view), layer, batch.ref, *_rows(Q), *_rows(out), n_q_heads, window, scale, _st()))
+    check(_lib.lib().qie_attention_batch(pool.ref, layer, batch.ref, *_rows(Q), *_rows(out), n_q_heads, window, scale, _st()))
 
 
 class LogitRules:
@@ -283,7 +294,8 @@ class LogitRules:
 
 def launch_logits(logits, out, rules):
     """the rules over rows [n_rows, vocab] of bfloat16 or float32 logits -> out (may be logits)"""
-    assert logits.dtype == out.dtype and logits.shape == out.shape and logits.dtype in (torch.bfloat16, torch.float32)
-    assert rules.n_rows is None or rules.n_rows >= logits.shape[0], "rules for fewer rows"
+    (n, vocab), kind = logits.shape, logits.dtype
+    assert kind is out.dtype and out.shape == logits.shape and (kind is torch.bfloat16 or kind is torch.float32), "bfloat16 or float32 logits, and out like them"
+    assert rules.n_rows is None or rules.n_rows >= n, "rules for fewer rows"
     _here(logits)
-    check(_lib.lib().qie_logits_process(*_rows(logits), *_rows(out), int(logits.dtype == torch.float32), logits.shape[0], logits.shape[1], rules.ref, _st()))
+    check(_lib.lib().qie_logits_process(*_rows(logits), *_rows(out), int(kind is torch.float32), n, vocab, rules.ref, _st()))
