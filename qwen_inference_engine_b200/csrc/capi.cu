@@ -536,12 +536,13 @@ int qie_attention_batch(const qie_kv_view* kv, int layer, const qie_batch* b, co
 
 int qie_logits_process(const void* logits, size_t stride, void* out, size_t out_stride, int dtype, int n_rows, int vocab, const qie_logit_rules* rules, qie_stream st) {
   if (dtype != QIE_DTYPE_BF16 && dtype != QIE_DTYPE_F32) return fail(QIE_EINVAL, "logits_process: bf16 or fp32 logits");
-  if (!rules || n_rows < 0 || n_rows > 65535 || vocab <= 0 || (n_rows && (!logits || !out))) return fail(QIE_EINVAL, "logits_process: bad argument (at most 65535 rows)");
+  if (!rules || n_rows < 0 || n_rows > 65535 || vocab <= 0 || vocab > 1 << 27 || (n_rows && (!logits || !out)))
+    return fail(QIE_EINVAL, "logits_process: bad argument (at most 65535 rows of 2^27)");
   if (n_rows > 1 && (stride < (size_t)vocab || out_stride < (size_t)vocab)) return fail(QIE_EINVAL, "logits_process: rows of %d elements overlap", vocab);
   if (n_rows > 1 && logits == out && stride != out_stride) return fail(QIE_EINVAL, "logits_process: in place with rows at other places");
   if (!aligned(dtype == QIE_DTYPE_F32 ? 4 : 2, {logits, out})) return fail(QIE_EINVAL, "logits_process: logits off their type's boundary");
   const qie_logit_rules& r = *rules;
-  if (r.n_tokens < 0 || r.n_bias < 0 || (r.gen_start && !r.tok_start) || (r.tok_start && !r.tokens && r.n_tokens) ||
+  if (r.n_tokens < 0 || r.n_bias < 0 || r.n_tokens > 1 << 30 || r.n_bias > 1 << 30 || (r.gen_start && !r.tok_start) || (r.tok_start && !r.tokens && r.n_tokens) ||
       (r.bias_start && r.n_bias && (!r.bias_ids || !r.bias)) || ((r.repetition || r.presence || r.frequency) && !r.tok_start) || (r.bias && !r.bias_start))
     return fail(QIE_EINVAL, "logits_process: a rule without its lists");
   if (r.mask && (r.n_masks < 0 || (long long)r.mask_words * 32 < vocab)) return fail(QIE_EINVAL, "logits_process: masks of %d words for %d tokens", r.mask_words, vocab);

@@ -1,9 +1,12 @@
 // logit_rules.cu -- penalties for tokens that were there, biases and masks over rows of logits (qie_logits_process).
 //
-// A CTA takes a stretch of one row's vocabulary.  It passes the logits through, 16 bytes at a time, with the mask; beside that it reads the row's lists and
-// counts, in shared memory, how often they have each token of the stretch (whole numbers, so the order does not matter).  The first one to meet a token notes
-// it, and at the end the noted tokens, few of the stretch, are computed from the input and written over what was passed through.  A token with several
-// biases gets their sum in the order of the list.
+// A CTA has a share of one row's vocabulary, chunks of 256 tokens in turn with the row's other CTAs (frequent tokens have low numbers).  It starts copies of all its
+// chunks into shared memory; while they are on their way it reads the row's lists and collects the share's tokens in a hash table: how often a token is there (whole
+// numbers, so their order does not matter) and the first entry of its biases.  Then those tokens, a few thousand of a row, are computed in the chunks, and the chunks are
+// written out, masked.  A token with several biases gets their sum in the order of the list.  In place, a row without a mask has its tokens computed where they are.
+// Bound by memory: 64 rows of 151936 bf16 are 39 MB.
+#include <algorithm>
+
 #include "common.cuh"
 #include "kernels.h"
 #include "launch.h"
@@ -11,10 +14,40 @@
 namespace qie {
 namespace {
 
+constexpr int THR = 512, CHUNK_BITS = 8;
+constexpr int SLOT_BITS = 11, SLOTS = 1 << SLOT_BITS, MOST_PROBES = 64, MOST_SHARE = 6, TILE_BYTES = 80 * 1024;
+constexpr uint32_t EMPTY = 0xffffffffu, NONE = 0x7fffffffu;
 // a token's word: how often it is among the generated ones, and
 constexpr uint32_t LISTED = 1u << 31, BIASED = 1u << 30, MORE = 1u << 29, TIMES = MORE - 1;  // in the row's list; has a bias; has several
-constexpr uint32_t NONE = 0x7fffffffu;
 
+// [from, to) of a list of n, whatever the offsets say
+__device__ __forceinline__ int2 span(const int* start, int i, int n) {
+  const int from = min(max(start[i], 0), n);
+  return make_int2(from, min(max(start[i + 1], from), n));
+}
+// a thread's next tokens of a list, U of them in steps of the CTA's threads; those behind the end are -1
+template <int U>
+struct Next {
+  int id[U];
+  __device__ __forceinline__ Next(const int* p, int2 s, int at) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) id[u] = at + u * THR < s.y - s.x ? p[s.x + at + u * THR] : -1;
+  }
+  // hit(place in the list, token) for those that are `mine`: a warp goes round as often as one of its threads has some
+  template <typename M, typename F>
+  __device__ __forceinline__ void each(int at, M mine, F hit) const {
+    unsigned hits = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) hits |= (unsigned)mine(id[u]) << u;
+    for (; hits; hits &= hits - 1) {
+      const int u = __ffs(hits) - 1;
+      int x = id[0];
+#pragma unroll
+      for (int e = 1; e < U; ++e) x = u == e ? id[e] : x;
+      hit(at + u * THR, x);
+    }
+  }
+};
 template <typename T>
 __device__ __forceinline__ float load(const T* p) {
   if constexpr (sizeof(T) == 2) return bf2f(*p);
@@ -25,155 +58,225 @@ __device__ __forceinline__ void store(T* p, float v) {
   if constexpr (sizeof(T) == 2) *p = f2bf(v);
   else *p = v;
 }
-// [from, to) of a list of n, whatever the offsets say
-__device__ __forceinline__ int2 span(const int* start, int i, int n) {
-  const int from = min(max(start[i], 0), n);
-  return make_int2(from, min(max(start[i + 1], from), n));
-}
-// f(index, value) for a thread's share of p[s.x .. s.y), 16 bytes at a time
-template <typename F>
-__device__ __forceinline__ void each(const int* p, int2 s, F f) {
-  int from = s.x;
-  const int lead = (int)((16 - (reinterpret_cast<uintptr_t>(p + s.x) & 15)) & 15) / 4, head = min(s.y, s.x + lead);
-  if ((int)threadIdx.x < head - from) f(from + threadIdx.x, p[from + threadIdx.x]);
-  from = head;
-  const int quads = (s.y - from) / 4;
-  for (int q = threadIdx.x; q < quads; q += blockDim.x) {
-    const int4 v = *reinterpret_cast<const int4*>(p + from + 4 * q);
-    f(from + 4 * q, v.x), f(from + 4 * q + 1, v.y), f(from + 4 * q + 2, v.z), f(from + 4 * q + 3, v.w);
-  }
-  from += 4 * quads;
-  if ((int)threadIdx.x < s.y - from) f(from + threadIdx.x, p[from + threadIdx.x]);
-}
+constexpr int CHUNK = 1 << CHUNK_BITS, CHUNK_WORDS = CHUNK / 32 + 1;  // mask words that a chunk at any place touches
+template <typename T>
+constexpr size_t chunk_bytes = CHUNK * sizeof(T) + CHUNK_WORDS * 4;
 
-// G groups of 16 bytes a thread.  A stretch begins on a 16-byte boundary of the row's input, so `shift` elements ahead of where a row on a boundary had it.
-template <typename T, int THR, int G>
-__global__ void __launch_bounds__(THR) logit_rules_kernel(LogitArgs a) {
-  constexpr int E = 16 / sizeof(T), STRETCH = G * THR * E;
-  extern __shared__ __align__(16) uint32_t seen[];  // [STRETCH], then (16 bits each) the noted tokens, then, where there are biases, the first one of each token
-  uint16_t* noted = reinterpret_cast<uint16_t*>(seen + STRETCH);
-  uint32_t* entry = seen + STRETCH + STRETCH / 2;
-  __shared__ int n_noted;
+// CTA y of 2^share of a row has the chunks whose number's lowest `share` bits are y.  Chunks begin on 16-byte boundaries of the row's input, so `shift` elements ahead
+// of where a row on a boundary has them.
+template <typename T>
+__global__ void __launch_bounds__(THR) logit_rules_kernel(LogitArgs a, int share, int most) {  // most: chunks that a CTA has at most
+  constexpr int E = 16 / sizeof(T), GROUPS = CHUNK / E;  // 16-byte groups of a chunk
+  extern __shared__ __align__(16) unsigned char tile[];
+  __shared__ __align__(16) uint32_t key[SLOTS], word[SLOTS], entry[SLOTS];  // the token, its word, the first of its biases
+  __shared__ uint16_t used[SLOTS];  // the slots in use
+  __shared__ int full, n_used;
   pdl_wait();
   pdl_trigger();
-  const int row = blockIdx.y, tid = threadIdx.x;
+  const int row = blockIdx.x, tid = threadIdx.x;
   const T* in = (const T*)a.in + (size_t)row * a.stride;
   T* out = (T*)a.out + (size_t)row * a.out_stride;
-  const int shift = (int)((reinterpret_cast<uintptr_t>(in) & 15) / sizeof(T)), lo = blockIdx.x * STRETCH - shift;
-  const bool out16 = ((reinterpret_cast<uintptr_t>(out) / sizeof(T) - shift) * sizeof(T) & 15) == 0;
+  const int shift = (int)((reinterpret_cast<uintptr_t>(in) & 15) / sizeof(T));
+  const bool lists = a.tok_start || a.bias_start;
+  int depth = share;
+  unsigned low = blockIdx.y;
+  // Tokens of the class (depth, low): the lowest `depth` bits of the place, its chunk's number first.  A class that finds no room in the table is taken in halves; at the
+  // latest one with no more tokens than probes fits.
+  auto place = [&](int id) { return __funnelshift_r((unsigned)(id + shift), (unsigned)(id + shift), CHUNK_BITS); };
+  auto mine = [&](int id) { return (unsigned)id < (unsigned)a.vocab && (place(id) & ((1u << depth) - 1)) == low; };
+  auto slot_of = [&](int id) {  // below 0: there is none
+    unsigned k = (place(id) >> depth) * 2654435769u >> (32 - SLOT_BITS);
+    for (int n = 0; n < MOST_PROBES; ++n, k = (k + 1) & (SLOTS - 1)) {
+      const uint32_t have = atomicCAS(&key[k], EMPTY, (uint32_t)id);
+      if (have == EMPTY || have == (uint32_t)id) return (int)k;
+    }
+    full = 1;
+    return -1;
+  };
+  auto clear = [&] {
+    for (int i = tid; i < SLOTS / 4; i += THR) {
+      reinterpret_cast<uint4*>(key)[i] = make_uint4(EMPTY, EMPTY, EMPTY, EMPTY);
+      reinterpret_cast<uint4*>(word)[i] = make_uint4(0, 0, 0, 0);
+      reinterpret_cast<uint4*>(entry)[i] = make_uint4(NONE, NONE, NONE, NONE);
+    }
+    if (tid == 0) full = n_used = 0;
+  };
+  // ---- the chunks into shared memory, and the words of the mask
+  const bool copy = a.in != a.out;
+  const int chunks = (((a.vocab + shift + CHUNK - 1) >> CHUNK_BITS) - (int)blockIdx.y + (1 << share) - 1) >> share;
+  uint32_t* words = reinterpret_cast<uint32_t*>(tile + (size_t)most * CHUNK * sizeof(T));  // [chunk][CHUNK_WORDS]
+  auto first_of = [&](int c) { return (((c << share) + (int)blockIdx.y) << CHUNK_BITS) - shift; };  // the chunk's first token
+  auto read = [&] {
+    for (int g = tid; g < chunks * GROUPS; g += THR) {
+      const int c = g / GROUPS, t0 = first_of(c) + (g - c * GROUPS) * E;
+      T* to = reinterpret_cast<T*>(tile) + (size_t)g * E;
+      if (t0 >= 0 && t0 + E <= a.vocab) cp_async16(smem_u32(to), in + t0);
+      else
+        for (int e = 0; e < E; ++e)
+          if (t0 + e >= 0 && t0 + e < a.vocab) to[e] = in[t0 + e];
+    }
+    cp_async_commit();
+  };
+  if (copy) read();
   const int m = a.mask ? (a.mask_row ? a.mask_row[row] : row) : -1;
   const uint32_t* mask = m >= 0 && m < a.n_masks ? a.mask + (size_t)m * a.mask_words : nullptr;
-  auto allowed = [&](int t) { return !mask || (mask[t >> 5] >> (t & 31) & 1); };
-  uint4 x[G];
-#pragma unroll
-  for (int g = 0; g < G; ++g) {
-    const int t = lo + (g * THR + tid) * E;
-    if (t >= 0 && t + E <= a.vocab) x[g] = *reinterpret_cast<const uint4*>(in + t);
-  }
-  const bool biases = a.bias_start != nullptr, lists = a.tok_start != nullptr;
-  if (lists || biases)
-    for (int i = tid; i < STRETCH / 4; i += THR) {
-      reinterpret_cast<uint4*>(seen)[i] = make_uint4(0, 0, 0, 0);
-      if (biases) reinterpret_cast<uint4*>(entry)[i] = make_uint4(NONE, NONE, NONE, NONE);
+  const bool staged = copy || mask;
+  if (!copy && mask) read();
+  // ---- the lists
+  const int2 ts = a.tok_start ? span(a.tok_start, row, a.n_tokens) : make_int2(0, 0), bs = a.bias_start ? span(a.bias_start, row, a.n_bias) : make_int2(0, 0);
+  const int gen = (a.gen_start && a.tok_start ? a.gen_start[row] : ts.x) - ts.x;
+  const float rep = a.repetition ? a.repetition[row] : 1.f, pres = a.presence ? a.presence[row] : 0.f, freq = a.frequency ? a.frequency[row] : 0.f;
+  constexpr int UT = 8, UB = 1;
+  auto collect = [&](auto&& ready) {  // `ready` between the loads and their use
+    Next<UT> t(a.tokens, ts, tid);
+    Next<UB> b(a.bias_ids, bs, tid);
+    if (tid < bs.y - bs.x) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.bias + bs.x + tid));
+    ready();
+    for (int i = tid;;) {
+      t.each(i, mine, [&](int j, int id) {
+        const int k = slot_of(id);
+        if (k < 0) return;
+        if (j >= gen) atomicAdd(&word[k], 1u);
+        else atomicOr(&word[k], LISTED);
+      });
+      if (ts.y - ts.x - i <= UT * THR) break;
+      i += UT * THR;
+      t = Next<UT>(a.tokens, ts, i);
     }
-  if (tid == 0) n_noted = 0;
-  __syncthreads();
-  auto note = [&](unsigned i, uint32_t before) {
-    if (before == 0) noted[atomicAdd(&n_noted, 1)] = (uint16_t)i;
+    for (int i = tid;;) {
+      b.each(i, mine, [&](int j, int id) {
+        const int k = slot_of(id);
+        if (k >= 0) atomicOr(&word[k], atomicMin(&entry[k], (uint32_t)j) != NONE ? BIASED | MORE : BIASED);
+      });
+      if (bs.y - bs.x - i <= UB * THR) break;
+      i += UB * THR;
+      b = Next<UB>(a.bias_ids, bs, i);
+    }
   };
-  if (lists) {
-    const int2 s = span(a.tok_start, row, a.n_tokens);
-    const int gen = a.gen_start ? a.gen_start[row] : s.x;
-    each(a.tokens, s, [&](int j, int id) {
-      const unsigned i = (unsigned)id - (unsigned)lo;
-      if (i < (unsigned)STRETCH && (unsigned)id < (unsigned)a.vocab) note(i, j >= gen ? atomicAdd(&seen[i], 1u) : atomicOr(&seen[i], LISTED));
+  if (lists)
+    collect([&] {
+      clear();
+      __syncthreads();
     });
-  }
-  const int2 bs = biases ? span(a.bias_start, row, a.n_bias) : make_int2(0, 0);
-  if (biases)
-    each(a.bias_ids, bs, [&](int j, int id) {
-      const unsigned i = (unsigned)id - (unsigned)lo;
-      if (i < (unsigned)STRETCH && (unsigned)id < (unsigned)a.vocab) {
-        const bool more = atomicMin(&entry[i], (uint32_t)j) != NONE;
-        note(i, atomicOr(&seen[i], more ? BIASED | MORE : BIASED));
+  if (mask)
+    for (int i = tid; i < chunks * CHUNK_WORDS; i += THR) {
+      const int c = i / CHUNK_WORDS, w = (first_of(c) >> 5) + i - c * CHUNK_WORDS;
+      words[i] = w >= 0 && w < (a.vocab + 31) >> 5 ? mask[w] : 0;
+    }
+  if (staged) cp_async_wait<0>();
+  __syncthreads();
+  // ---- the tokens of the lists
+  auto place_of = [&](int id) {  // in the chunks
+    const int v = id + shift;
+    return ((v >> (CHUNK_BITS + share)) << CHUNK_BITS) + (v & (CHUNK - 1));
+  };
+  while (lists) {
+    if (full) {
+      ++depth;
+    } else {
+      // the slots in use, side by side
+      constexpr int MINE = SLOTS / THR;
+      unsigned have[MINE];
+      int before = 0;
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) have[i] = __ballot_sync(0xffffffffu, key[i * THR + tid] != EMPTY), before += __popc(have[i]);
+      if ((tid & 31) == 0) before = atomicAdd(&n_used, before);
+      before = __shfl_sync(0xffffffffu, before, 0);
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) {
+        if (have[i] >> (tid & 31) & 1) used[before + __popc(have[i] & ((1u << (tid & 31)) - 1))] = (uint16_t)(i * THR + tid);
+        before += __popc(have[i]);
       }
-    });
-  // ---- the logits with the mask
-#pragma unroll
-  for (int g = 0; g < G; ++g) {
-    const int t0 = lo + (g * THR + tid) * E;
-    if (t0 >= a.vocab || t0 + E <= 0) continue;
-    if (t0 >= 0 && t0 + E <= a.vocab) {
-      uint32_t* w = reinterpret_cast<uint32_t*>(&x[g]);
-      if (mask) {
-        const uint32_t bits = __funnelshift_r(mask[t0 >> 5], mask[(t0 + E - 1) >> 5], t0 & 31);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const bool no = !(bits >> e & 1);
-          if constexpr (sizeof(T) == 4) w[e] = no ? 0xff800000u : w[e];
-          else w[e / 2] = no ? (e & 1 ? (w[e / 2] & 0xffffu) | 0xff800000u : (w[e / 2] & 0xffff0000u) | 0xff80u) : w[e / 2];
+      __syncthreads();
+      for (int n = tid; n < n_used; n += THR) {
+        const int k = used[n], id = (int)key[k];
+        const uint32_t w = word[k], times = w & TIMES;
+        T* at = staged ? reinterpret_cast<T*>(tile) + place_of(id) : out + id;
+        float v = load(at);
+        if ((times || w & LISTED) && a.repetition) v = v > 0.f ? v / rep : v * rep;
+        if (times) {
+          v -= freq * (float)times;
+          v -= pres;
         }
+        if (w & BIASED) {
+          const int j = (int)entry[k];
+          float sum = a.bias[bs.x + j];
+          if (w & MORE)
+            for (int i = bs.x + j + 1; i < bs.y; ++i)
+              if (a.bias_ids[i] == id) sum += a.bias[i];
+          v += sum;
+        }
+        store(at, v);
       }
-      if (out16) {
-        *reinterpret_cast<uint4*>(out + t0) = x[g];
+      // the next class
+      while (depth > share && (low >> (depth - 1) & 1)) --depth, low &= (1u << depth) - 1;
+      if (depth == share) break;
+      low |= 1u << (depth - 1);
+    }
+    __syncthreads();
+    clear();
+    __syncthreads();
+    collect([] {});
+    __syncthreads();
+  }
+  if (!staged) return;
+  __syncthreads();
+  // ---- the chunks out
+  const bool out16 = ((reinterpret_cast<uintptr_t>(out) / sizeof(T) - shift) * sizeof(T) & 15) == 0;
+  for (int g = tid; g < chunks * GROUPS; g += THR) {
+    const int c = g / GROUPS, first = first_of(c), t0 = first + (g - c * GROUPS) * E;
+    uint4 x = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(tile) + (size_t)g * E);
+    uint32_t* w = reinterpret_cast<uint32_t*>(&x);
+    if (mask) {
+      const uint32_t* p = words + c * CHUNK_WORDS + (t0 >> 5) - (first >> 5);
+      const uint32_t bits = (t0 & 31) + E <= 32 ? *p >> (t0 & 31) : __funnelshift_r(p[0], p[1], t0 & 31);
+      if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) w[e] = bits >> e & 1 ? w[e] : 0xff800000u;
       } else {
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          if constexpr (sizeof(T) == 4) out[t0 + e] = __uint_as_float(w[e]);
-          else out[t0 + e] = __ushort_as_bfloat16((unsigned short)(w[e / 2] >> (e & 1 ? 16 : 0)));
+        for (int e = 0; e < E / 2; ++e) {  // a pair's bits as 16 bits each
+          const uint32_t two = bits >> (2 * e), keep = ((two & 1) | (two & 2) << 15) * 0xffffu;
+          w[e] = (w[e] & keep) | (0xff80ff80u & ~keep);
         }
       }
+    }
+    if (out16 && t0 >= 0 && t0 + E <= a.vocab) {
+      *reinterpret_cast<uint4*>(out + t0) = x;
     } else {
-      for (int t = max(t0, 0); t < min(t0 + E, a.vocab); ++t) out[t] = allowed(t) ? in[t] : (T)(-INFINITY);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if (t0 + e < 0 || t0 + e >= a.vocab) continue;
+        if constexpr (sizeof(T) == 4) out[t0 + e] = __uint_as_float(w[e]);
+        else out[t0 + e] = __ushort_as_bfloat16((unsigned short)(w[e / 2] >> (e & 1 ? 16 : 0)));
+      }
     }
-  }
-  if (!lists && !biases) return;
-  __syncthreads();
-  // ---- the noted tokens.  (In place: their logits are as they were, or masked.)
-  const float rep = a.repetition ? a.repetition[row] : 1.f, pres = a.presence ? a.presence[row] : 0.f, freq = a.frequency ? a.frequency[row] : 0.f;
-  for (int k = tid; k < n_noted; k += THR) {
-    const int i = noted[k], id = lo + i;
-    if (!allowed(id)) continue;
-    const uint32_t w = seen[i], times = w & TIMES;
-    float v = load(in + id);
-    if ((times || w & LISTED) && a.repetition) v = v > 0.f ? v / rep : v * rep;
-    if (times) {
-      v -= freq * (float)times;
-      v -= pres;
-    }
-    if (w & BIASED) {
-      const int j = (int)entry[i];
-      float sum = a.bias[j];
-      if (w & MORE)
-        for (int n = j + 1; n < bs.y; ++n)
-          if (a.bias_ids[n] == id) sum += a.bias[n];
-      v += sum;
-    }
-    store(out + id, v);
   }
 }
 
-template <typename T, int THR, int G>
-cudaError_t launch_g(const LogitArgs& a, cudaStream_t st) {
-  constexpr int E = 16 / sizeof(T), STRETCH = G * THR * E;
-  static_assert(STRETCH <= 65536, "noted in 16 bits");
+template <typename T>
+cudaError_t launch_t(const LogitArgs& a, cudaStream_t st) {
+  if (!a.mask && a.in == a.out && !a.tok_start && !a.bias_start) return cudaSuccess;
   static PerDeviceOnce set;
   if (set.need()) {
-    const cudaError_t e = cudaFuncSetAttribute(logit_rules_kernel<T, THR, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, STRETCH * 10);
+    const cudaError_t e = cudaFuncSetAttribute(logit_rules_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, TILE_BYTES);
     if (e != cudaSuccess) return e;
     set.done();
   }
-  const dim3 grid((a.vocab + E - 2) / STRETCH + 1, a.n_rows);
-  return launched(launch_k(logit_rules_kernel<T, THR, G>, grid, dim3(THR), a.bias_start ? STRETCH * 10 : a.tok_start ? STRETCH * 6 : 0, st, a));
+  int share = 0, dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const bool staged = a.mask || a.in != a.out;
+  const long long chunks = ((long long)a.vocab + 16 / sizeof(T) + CHUNK - 1) >> CHUNK_BITS;
+  auto most = [&] { return (chunks + (1 << share) - 1) >> share; };  // of a CTA
+  // CTAs a row: as many as their chunks need for room, two CTAs an SM, then as many as find room at once
+  while (staged && most() * chunk_bytes<T> > TILE_BYTES) ++share;
+  while (share < MOST_SHARE && (a.n_rows << (share + 1)) <= 2 * device_attribute<cudaDevAttrMultiProcessorCount>(dev)) ++share;
+  return launched(launch_k(logit_rules_kernel<T>, dim3(a.n_rows, 1 << share), dim3(THR), staged ? most() * chunk_bytes<T> : 0, st, a, share, (int)most()));
 }
 
 }  // namespace
 
-cudaError_t launch_logit_rules(const LogitArgs& a, cudaStream_t st) {
-  // one row: as many CTAs as share it out over the chip; many: stretches that read a row's lists less often
-  const bool few = (long long)a.n_rows * a.vocab < 148ll * 4096;
-  if (a.f32) return few ? launch_g<float, 256, 1>(a, st) : launch_g<float, 512, 4>(a, st);
-  return few ? launch_g<bf16, 128, 1>(a, st) : launch_g<bf16, 512, 2>(a, st);
-}
+cudaError_t launch_logit_rules(const LogitArgs& a, cudaStream_t st) { return a.f32 ? launch_t<float>(a, st) : launch_t<bf16>(a, st); }
 
 }  // namespace qie
