@@ -6,7 +6,8 @@
 // An item is a kv head of a request and a block of its tokens: the rows of a tile are (token, query head of the group), so keys and values are read once
 // for the whole group and a decode row costs the tiles of its context alone.  The tiles of all items, one after the other, are cut into equal stretches,
 // one a CTA (two CTAs an SM; the host knows no lengths, so every CTA adds the requests up itself).  An item that is cut leaves its parts (rows of O, maximum,
-// sum, in fp32) in the work area, and a second kernel joins them.
+// sum, in fp32) in the work area, and a second kernel joins them, in their order.  (Joined by the CTA that comes last: no quicker for a single row, 10.4 us as with the
+// kernel, as what another SM wrote is as far away as the start of a kernel; and 10 us for 126 rows.)
 // Within a CTA:
 //   S = Q K^T  : tcgen05.mma, 128 x 64 fp32 in one of two TMEM buffers, issued two tiles ahead of its softmax, across items
 //   softmax    : warps 0-3, a thread a row (= TMEM lane).  The weights go back over the scores as bf16: the product's A operand (2^-8 of each weight; sums take
@@ -47,13 +48,13 @@ struct Smem {
   static constexpr int TOTAL = END > 76 * 1024 ? END : 76 * 1024;
   static_assert(512 / TMEM_COLS == 2 && 3 * (TOTAL + 1024) > 228 * 1024 && 2 * (TOTAL + 2048) <= 228 * 1024, "two CTAs an SM");
 };
-// a part of an item in the work area: O rows, then maxima and sums
+// The work area: of each CTA what there is to join of the item that begins there and goes on behind it; then two parts of each CTA, of the item that began before it and of
+// the one that goes on: O, four columns of all rows after four columns of all rows, so that threads with rows side by side write and read side by side, maxima, sums.
+struct JoinInfo {
+  int t0, tokens, kvh, parts;  // rows t0 .. t0 + tokens of Q; parts 0: nothing
+};
 template <int HD>
 constexpr int PART = TQ * HD + 2 * TQ;  // floats
-struct JoinInfo {
-  int t0, tokens, kvh, parts;  // rows t0 .. t0 + tokens of Q; parts 0: nothing to join
-};
-
 __device__ __forceinline__ void ld32(uint32_t taddr, uint32_t* r) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,"
@@ -116,14 +117,22 @@ __device__ __forceinline__ long long block_scan(long long v, long long* warp_sum
   return before + run - v;
 }
 
+// a / b of numbers that are not below 0, mostly of 32 bits
+__device__ __forceinline__ long long quotient(long long a, long long b) { return (a | b) >> 32 ? a / b : (long long)((unsigned)a / (unsigned)b); }
+
 template <int HD, bool TMA>
 __global__ void __launch_bounds__(NTHR, 2) attn_batch_kernel(BatchAttnArgs a, Shape sh, int box, const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap kvm) {
   using SM = Smem<HD>;
   constexpr int NB = SM::NB, ST = SM::ST;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
-  __shared__ long long s_sums[NTHR / 32], s_rest;
-  __shared__ int dead_s, s_req, s_kvh, s_block, s_skip, s_odd[2], s_edge[EDGES];  // s_odd, by the item's parity: there are values put aside; s_edge: first keys of the edge tiles
+  __shared__ long long s_sums[NTHR / 32];
+  __shared__ Walk s_walk;
+  __shared__ int dead_s, s_odd[2], s_edge[EDGES];  // s_odd, by the item's parity: there are values put aside; s_edge: first keys of the edge tiles
   volatile int* dead = &dead_s;
+  if (threadIdx.x == NTHR - 1) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&qm) : "memory");
+    if (TMA) asm volatile("prefetch.tensormap [%0];" ::"l"(&kvm) : "memory");
+  }
   pdl_wait();
   pdl_trigger();
   const uint32_t s0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -132,7 +141,7 @@ __global__ void __launch_bounds__(NTHR, 2) attn_batch_kernel(BatchAttnArgs a, Sh
                  free_k = bar_v + 8 * ST, free_v = free_k + 8 * ST, free_q = free_v + 8 * ST;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, tt = sh.tt, G = sh.g;
   if (tid == 0) {
-    dead_s = 0, s_odd[0] = s_odd[1] = 0, s_req = a.n_req;
+    dead_s = 0, s_odd[0] = s_odd[1] = 0, s_walk.left = 0;
     for (int i = 0; i < 2; ++i) mbar_init_tc(bar_s + 8 * i, 1), mbar_init_tc(bar_p + 8 * i, NSOFT), mbar_init_tc(bar_o + 8 * i, 1);
     mbar_init_tc(bar_q, 1), mbar_init_tc(free_q, 1);
     for (int i = 0; i < ST; ++i) mbar_init_tc(bar_k + 8 * i, 1), mbar_init_tc(bar_v + 8 * i, 1), mbar_init_tc(free_k + 8 * i, 1), mbar_init_tc(free_v + 8 * i, 1);
@@ -146,30 +155,33 @@ __global__ void __launch_bounds__(NTHR, 2) attn_batch_kernel(BatchAttnArgs a, Sh
   // ---- this CTA's stretch
   const int per = (a.n_req + NTHR - 1) / NTHR, r0 = min(a.n_req, tid * per), r1 = min(a.n_req, r0 + per);
   long long mine = 0, total;
+  Raw one;
   for (int i = r0; i < r1; ++i) {
-    const Raw w = request(a, i, tt);
-    mine += a.kv.n_kv * ab_cost(w.r, w.r.nb, tt, a.window);
+    one = request(a, i, tt);
+    mine += a.kv.n_kv * ab_cost(one.r, one.r.nb, tt, a.window);
   }
   const long long below = block_scan(mine, s_sums, total);
-  const long long share = (total + gridDim.x - 1) / gridDim.x, x0 = min(total, share * blockIdx.x), x1 = min(total, x0 + share);
-  if (x0 < x1 && below <= x0 && x0 < below + mine) {  // one thread: the request in which it begins
-    long long at = below;
-    for (int i = r0; i < r1; ++i) {
-      const Raw w = request(a, i, tt);
-      const long long c = a.kv.n_kv * ab_cost(w.r, w.r.nb, tt, a.window);
-      if (x0 < at + c) {
-        s_req = i, s_rest = x0 - at;
-        break;
+  const long long share = quotient(total + gridDim.x - 1, gridDim.x), x0 = min(total, share * blockIdx.x), x1 = min(total, x0 + share);
+  const bool own = x0 < x1 && below <= x0 && x0 < below + mine;
+  if (const unsigned owner = __ballot_sync(0xffffffffu, own)) {  // the warp of the thread that has the request in which it begins
+    int req = 0;
+    long long rest = 0;
+    if (own) {
+      rest = x0 - below;
+      for (req = r0; req < r1 - 1; ++req) {
+        one = request(a, req, tt);
+        const long long c = a.kv.n_kv * ab_cost(one.r, one.r.nb, tt, a.window);
+        if (rest < c) break;
+        rest -= c;
       }
-      at += c;
     }
-  }
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  __syncthreads();
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  if (warp == 0 && s_req < a.n_req) {  // the block in which it begins: the last one whose cost of blocks before is not above the rest, 32 at a time
-    const Raw w = request(a, s_req, tt);
-    const long long head = ab_cost(w.r, w.r.nb, tt, a.window), rest = s_rest % head;
+    const int from = __ffs(owner) - 1;
+    req = __shfl_sync(0xffffffffu, req, from), rest = __shfl_sync(0xffffffffu, rest, from);
+    const Raw w = request(a, req, tt);
+    const long long head = ab_cost(w.r, w.r.nb, tt, a.window);
+    const int kvh = (int)quotient(rest, head);
+    rest -= kvh * head;
+    // the block in which it begins: the last one whose cost of blocks before is not above the rest, 32 at a time
     int lo = 0, hi = w.r.nb;
     while (hi - lo > 1) {
       const int step = (hi - lo + 31) / 32, x = lo + lane * step;
@@ -177,18 +189,18 @@ __global__ void __launch_bounds__(NTHR, 2) attn_batch_kernel(BatchAttnArgs a, Sh
       const int k = 31 - __clz(in);  // (lane 0's is)
       hi = min(hi, lo + (k + 1) * step), lo += k * step;
     }
-    if (lane == 0) s_kvh = (int)(s_rest / head), s_block = lo, s_skip = (int)(rest - ab_cost(w.r, lo, tt, a.window));
+    if (lane == 0) s_walk = Walk{w, req, kvh, lo, (int)(rest - ab_cost(w.r, lo, tt, a.window)), x1 - x0};
   }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
-  Walk walk;
-  walk.req = s_req, walk.kvh = s_kvh, walk.block = s_block, walk.skip = s_skip, walk.left = s_req < a.n_req ? x1 - x0 : 0;
-  if (walk.left > 0) walk.w = request(a, walk.req, tt);
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  Walk walk = s_walk;
   uint32_t tmem;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(slot));
   const uint32_t t_o = tmem + 128;  // scores: columns 0 .. 63 and 64 .. 127, the weights over them
   JoinInfo* info = reinterpret_cast<JoinInfo*>(a.work);
   unsigned long long* odd_bits = reinterpret_cast<unsigned long long*>(smem_raw + (s0 - smem_u32(smem_raw)) + SM::ODD);  // [edge tile][column][2]
-  float* parts = reinterpret_cast<float*>(info + gridDim.x) + (size_t)blockIdx.x * 2 * PART<HD>;
+  float* parts = reinterpret_cast<float*>(info + gridDim.x);
 
   if (warp == NSOFT / 32 + 1) {
     // ---- copies
@@ -200,6 +212,9 @@ __global__ void __launch_bounds__(NTHR, 2) attn_batch_kernel(BatchAttnArgs a, Sh
     for (int item = 0; walk.next(a, tt, p); ++item) {
       const int* bt = a.block_table + (size_t)p.slot * a.max_pages;
       const int last_page = (p.limit - 1) / P;
+      const int c0 = p.key0 / box;  // chunks of `box` keys; a lane holds the page of chunk `held` + lane
+      int held = c0 + p.begin * chunks, page_of = 0;
+      if (TMA) page_of = bt[min((held + lane) * box / P, last_page)];  // chunks behind the last page repeat it (their keys are masked)
       if (item > 0) mbar_wait_tc(free_q, (uint32_t)((item - 1) & 1), dead);
       if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar_q), "r"(q_bytes) : "memory");
       __syncwarp();
@@ -208,15 +223,13 @@ __global__ void __launch_bounds__(NTHR, 2) attn_batch_kernel(BatchAttnArgs a, Sh
                      ::"r"(s0 + SM::Q + lane * QBLK), "l"(&qm), "r"(bar_q), "r"(lane * 64), "r"(p.kvh * G), "r"(p.t0)
                      : "memory");
       __syncwarp();
-      const int c0 = p.key0 / box;  // chunks of `box` keys; a lane holds the page of chunk `held` + lane
-      int held = -1000, page_of = 0;
       for (int i = p.begin; i < p.end; ++i, ++T) {
         const uint32_t st = (uint32_t)(T % ST);
         if constexpr (TMA) {
           const int ch = c0 + i * chunks;
-          if (ch < held || ch + chunks > held + 32) {
+          if (ch + chunks > held + 32) {
             held = ch;
-            page_of = bt[min((ch + lane) * box / P, last_page)];  // chunks behind the last page repeat it (their keys are masked)
+            page_of = bt[min((held + lane) * box / P, last_page)];
           }
           const int j = lane / NB, nb = lane % NB, page = __shfl_sync(0xffffffffu, page_of, (ch - held + j) & 31);
           const int at = min((ch + j) * box, last_page * P + P - box) % P;  // (positions end at 2^30)
@@ -435,7 +448,7 @@ __global__ void __launch_bounds__(NTHR, 2) attn_batch_kernel(BatchAttnArgs a, Sh
       if (some) {
         const float scale = *dead ? __int_as_float(0x7fc00000) : !whole ? 1.f : l_run > 0.f ? 1.f / l_run : l_run;
         bf16* dst = a.out + (size_t)(p.t0 + tok) * a.out_stride + (size_t)(p.kvh * G + g) * HD;
-        float* part = parts + (p.begin > 0 ? 0 : PART<HD>);
+        float* part = parts + ((size_t)blockIdx.x * 2 + (p.begin == 0)) * PART<HD>;
         if (!whole) part[TQ * HD + row] = m_ref, part[TQ * HD + TQ + row] = *dead ? __int_as_float(0x7fc00000) : l_run;
 #pragma unroll
         for (int c = 0; c < HD; c += 32) {
@@ -465,14 +478,12 @@ __global__ void __launch_bounds__(NTHR, 2) attn_batch_kernel(BatchAttnArgs a, Sh
             }
           } else {
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) *reinterpret_cast<uint4*>(part + row * HD + c + j) = make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
+            for (int j = 0; j < 32; j += 4) *reinterpret_cast<uint4*>(part + ((c + j) / 4 * TQ + row) * 4) = make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
           }
         }
       }
-      if (tid == 0 && !whole && p.begin == 0) {  // this CTA's last item goes on in the CTAs behind
-        const long long end = x0 + ((x1 - x0) - p.end) + p.tiles - 1;  // (the stretch ends with the piece) place of the item's last tile
-        info[blockIdx.x] = JoinInfo{p.t0, p.tokens, p.kvh, (int)(end / share) - (int)blockIdx.x + 1};
-      }
+      if (tid == 0 && !whole && p.begin == 0)  // goes on in the CTAs behind; the item's last tile is at x1 - left + tiles - 1
+        info[blockIdx.x] = JoinInfo{p.t0, p.tokens, p.kvh, (int)quotient(x1 - p.left + p.tiles - 1, share) - (int)blockIdx.x + 1};
       if (odd) {  // the same in every thread: arrivals at bar_p lie between the writes and this
         asm volatile("bar.sync 1, 128;" ::: "memory");
         for (int e = tid; e < EDGES * HD; e += NSOFT) odd_bits[2 * e] = odd_bits[2 * e + 1] = 0;
@@ -491,62 +502,108 @@ __global__ void __launch_bounds__(NTHR, 2) attn_batch_kernel(BatchAttnArgs a, Sh
   }
 }
 
-// The parts of an item that was cut: CTA k joins the one that CTA k of the kernel above began and did not end.  A group of warps a row, each with a share of
-// the parts; their sums meet in shared memory, in a fixed order.
-constexpr int JOIN_THR = 512, JOIN_WARPS = JOIN_THR / 32;
+// The parts of an item that was cut into the rows of its result: CTA k joins the item that CTA k of the kernel above began and did not end.  Sums are taken in a fixed
+// order.
+constexpr int JOIN_THR = 512;
+// 2^(m - top): a row sees nothing of some parts, and a sum that is no number counts whatever the maximum beside it
+__device__ __forceinline__ float weight(float m, float l, float top) { return l != l ? l : m > -INFINITY ? ex2_tc(m - top) : 0.f; }
+struct Sum4 {
+  float m = -INFINITY, l = 0.f;
+  float4 o = {0.f, 0.f, 0.f, 0.f};
+  __device__ __forceinline__ void add(float pm, float pl, const float4& x) {
+    const float top = fmaxf(m, pm), f = weight(m, l, top), pf = weight(pm, pl, top);
+    m = top;
+    l = l * f + pl * pf;
+    o.x *= f, o.y *= f, o.z *= f, o.w *= f;
+    if (pf != 0.f) o.x += x.x * pf, o.y += x.y * pf, o.z += x.z * pf, o.w += x.w * pf;
+  }
+};
 template <int HD>
-__global__ void __launch_bounds__(JOIN_THR) attn_batch_join_kernel(BatchAttnArgs a, int G, int n_cta) {
-  constexpr int E = HD / 32;
-  __shared__ float s_o[JOIN_WARPS][HD], s_m[JOIN_WARPS], s_l[JOIN_WARPS];
+__global__ void __launch_bounds__(JOIN_THR, 2) attn_batch_join_kernel(BatchAttnArgs a, int G, int n_cta) {
+  constexpr int C = HD / 4;  // groups of columns
+  __shared__ Sum4 sums[JOIN_THR];
   pdl_wait();
   pdl_trigger();
   const JoinInfo* info = reinterpret_cast<const JoinInfo*>(a.work);
   const JoinInfo in = info[blockIdx.x];
-  const float* base = reinterpret_cast<const float*>(info + n_cta);
-  const int rows = in.tokens * G, parts = in.parts, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int slice = blockIdx.y;  // of many rows' columns
+  const float* first = reinterpret_cast<const float*>(info + n_cta) + ((size_t)blockIdx.x * 2 + 1) * PART<HD>;
+  const int rows = in.tokens * G, n = in.parts, tid = threadIdx.x;
   // (a work area that two calls used at once must not lead outside)
-  if (parts <= 0 || parts > n_cta - (int)blockIdx.x || rows <= 0 || rows > TQ || in.t0 < 0 || in.t0 > a.n_tok - in.tokens || in.kvh < 0 || in.kvh >= a.kv.n_kv) return;
-  int wpr = 1;  // warps a row
-  while (wpr * 2 * rows <= JOIN_WARPS && wpr < parts) wpr *= 2;
-  const int groups = JOIN_WARPS / wpr, group = warp / wpr, sub = warp % wpr;
-  for (int r0 = 0; r0 < rows; r0 += groups) {
-    const int row = r0 + group;
-    float m = -INFINITY, l = 0.f, o[E];
-    for (int e = 0; e < E; ++e) o[e] = 0.f;
-    if (row < rows)
-      for (int q = sub; q < parts; q += wpr) {
-        const float* part = base + ((size_t)(blockIdx.x + q) * 2 + (q == 0)) * PART<HD>;
-        const float pm = part[TQ * HD + row], pl = part[TQ * HD + TQ + row];
-        float x[E];
-        for (int e = 0; e < E; ++e) x[e] = part[(size_t)row * HD + lane * E + e];
-        const float top = fmaxf(m, pm), f = m > -INFINITY ? ex2_tc(m - top) : 0.f, pf = pl != pl ? pl : pm > -INFINITY ? ex2_tc(pm - top) : 0.f;
-        m = top;
-        l = l * f + pl * pf;
-        for (int e = 0; e < E; ++e) o[e] = o[e] * f + (pf != 0.f ? x[e] * pf : 0.f);
+  if (n <= 1 || n > n_cta - (int)blockIdx.x || rows <= 0 || rows > TQ || in.t0 < 0 || in.t0 > a.n_tok - in.tokens || in.kvh < 0 || in.kvh >= a.kv.n_kv) return;
+  bf16* out = a.out + (size_t)in.t0 * a.out_stride + (size_t)in.kvh * G * HD;
+  auto store = [&](int row, int c, const float4& o, float f) {
+    *reinterpret_cast<uint2*>(out + (size_t)(row / G) * a.out_stride + (size_t)(row % G) * HD + c * 4) = make_uint2(pack2f(o.x * f, o.y * f), pack2f(o.z * f, o.w * f));
+  };
+  auto part_of = [&](int q) { return first + (q == 0 ? 0 : (size_t)(2 * q - 1) * PART<HD>); };  // the others are the first ones of the CTAs behind
+  const int all = rows * C;
+  if (all > JOIN_THR) {
+    // many rows: four threads a row with every fourth group of its columns; a part's weight is the row's
+    constexpr int MINE = C / (JOIN_THR / TQ);
+    const int row = tid % TQ, c0 = tid / TQ;
+    if (row >= rows) return;
+    float top = -INFINITY, sum = 0.f;
+    for (int q = 0; q < n; q += 4) {
+      float m[4], l[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float* part = part_of(min(q + u, n - 1)) + TQ * HD + row;
+        m[u] = q + u < n ? part[0] : -INFINITY, l[u] = q + u < n ? part[TQ] : 0.f;
       }
-    if (wpr > 1) {
-      __syncthreads();
-      for (int e = 0; e < E; ++e) s_o[warp][lane * E + e] = o[e];
-      if (lane == 0) s_m[warp] = m, s_l[warp] = l;
-      __syncthreads();
-      if (sub == 0) {
-        float top = m;
-        for (int w = 1; w < wpr; ++w) top = fmaxf(top, s_m[warp + w]);
-        float sum = 0.f;
-        for (int e = 0; e < E; ++e) o[e] = 0.f;
-        for (int w = 0; w < wpr; ++w) {
-          const float wl = s_l[warp + w], wm = s_m[warp + w], f = wl != wl ? wl : wm > -INFINITY ? ex2_tc(wm - top) : 0.f;
-          sum += wl * f;
-          for (int e = 0; e < E; ++e) o[e] += f != 0.f ? s_o[warp + w][lane * E + e] * f : 0.f;
-        }
-        l = sum;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float t = fmaxf(top, m[u]);
+        sum = sum * weight(top, sum, t) + l[u] * weight(m[u], l[u], t);
+        top = t;
       }
     }
-    if (row < rows && sub == 0) {
-      const float inv = l > 0.f ? 1.f / l : l;
-      bf16* dst = a.out + (size_t)(in.t0 + row / G) * a.out_stride + (size_t)(in.kvh * G + row % G) * HD + lane * E;
-      for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack2f(o[e] * inv, o[e + 1] * inv);
+    const float inv = sum > 0.f ? 1.f / sum : sum;
+#pragma unroll 1
+    for (int b = 4 * slice; b < min(MINE, 4 * slice + 4); b += 4) {
+      float4 o[4] = {};
+#pragma unroll 2
+      for (int q = 0; q < n; ++q) {
+        const float* part = part_of(q);
+        float4 x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = *reinterpret_cast<const float4*>(part + ((c0 + (b + e) * (JOIN_THR / TQ)) * TQ + row) * 4);
+        const float f = weight(part[TQ * HD + row], part[TQ * HD + TQ + row], top) * inv;
+        if (f != 0.f)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e].x += x[e].x * f, o[e].y += x[e].y * f, o[e].z += x[e].z * f, o[e].w += x[e].w * f;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) store(row, c0 + (b + e) * (JOIN_THR / TQ), o[e], 1.f);
     }
+    return;
+  }
+  if (slice) return;
+  // few rows: four columns of a row a thread, and the parts in turn with the threads that are left
+  constexpr int U = 4;
+  const int lanes = JOIN_THR / all, i = tid % all, q0 = tid / all, c = i / rows, row = i - c * rows;
+  Sum4 s;
+  if (q0 < lanes)
+    for (int q = q0; q < n; q += U * lanes) {
+      float m[U], l[U];
+      float4 x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int k = q + u * lanes;
+        m[u] = -INFINITY, l[u] = 0.f;
+        if (k >= n) continue;
+        const float* part = part_of(k);
+        m[u] = part[TQ * HD + row], l[u] = part[TQ * HD + TQ + row];
+        x[u] = *reinterpret_cast<const float4*>(part + (c * TQ + row) * 4);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (q + u * lanes < n) s.add(m[u], l[u], x[u]);
+    }
+  sums[tid] = s;
+  __syncthreads();
+  if (q0 == 0) {
+    for (int w = 1; w < min(lanes, n); ++w) s.add(sums[w * all + i].m, sums[w * all + i].l, sums[w * all + i].o);
+    store(row, c, s.o, s.l > 0.f ? 1.f / s.l : s.l);
   }
 }
 
@@ -562,7 +619,7 @@ cudaError_t launch_hd(const BatchAttnArgs& a, const TensorMap2D& qm, const Tenso
   const cudaError_t e = launched(launch_k(attn_batch_kernel<HD, TMA>, dim3(ctas), dim3(NTHR), Smem<HD>::TOTAL, st, a, Shape{G, TQ / G}, box,
                                           *reinterpret_cast<const CUtensorMap*>(&qm), *reinterpret_cast<const CUtensorMap*>(&kvm)));
   if (e != cudaSuccess) return e;
-  return launched(launch_k(attn_batch_join_kernel<HD>, dim3(ctas), dim3(JOIN_THR), 0, st, a, G, ctas));
+  return launched(launch_k(attn_batch_join_kernel<HD>, dim3(ctas, HD / 64), dim3(JOIN_THR), 0, st, a, G, ctas));
 }
 
 }  // namespace

@@ -66,6 +66,7 @@ __host__ __device__ __forceinline__ Raw request(const BatchAttnArgs& a, int i, i
 // a CTA's stretch of an item: tiles [begin, end) of its `tiles`, the first of which holds key `key0`
 struct Piece {
   int t0, tokens, kvh, slot, pos0, key0, begin, end, tiles, limit;  // limit: positions of the item's request
+  long long left;                                                    // of the CTA's stretch, with this piece
   __host__ __device__ int count() const { return end - begin; }
   __host__ __device__ bool whole() const { return begin == 0 && end == tiles; }
 };
@@ -89,6 +90,7 @@ struct Walk {
       const int tiles = last - first;
       const bool some = skip < tiles;
       if (some) {
+        p.left = left;
         p.begin = skip;
         p.end = skip + left < tiles ? (int)(skip + left) : tiles;
         p.tiles = tiles;
