@@ -12,7 +12,7 @@
 //   S = Q K^T  : tcgen05.mma, 128 x 64 fp32 in one of two TMEM buffers, issued two tiles ahead of its softmax, across items
 //   softmax    : warps 0-3, a thread a row (= TMEM lane).  The weights go back over the scores as bf16: the product's A operand (2^-8 of each weight; sums take
 //                them unrounded).  Warps without rows only pass the barriers on.
-//   O += P V   : accumulates in TMEM; rows scale it when their maximum grows
+//   O += P V   : accumulates in TMEM; rows scale it when their maximum grows by more than LAG
 //   warp 4     : the products.  warp 5: queries and 64-column boxes of the pages by TMA with the 128-byte swizzle, or, for pages of other than multiples of 16
 //                positions and pools of 2^31 rows, 16-byte copies to the same places.
 // Values of keys that some row of a tile does not see must not meet its zero weight when they are no numbers: tiles at the edges of what rows see are
@@ -37,6 +37,9 @@ constexpr int TQ = AB_TQ, TK = AB_TK;
 constexpr int QBLK = TQ * 128, KBLK = TK * 128;  // [rows][64 columns] bf16 in 8-row swizzle atoms
 constexpr int NSOFT = 128, NTHR = NSOFT + 64;
 constexpr uint32_t TMEM_COLS = 256;  // two tiles of scores, O
+// The weights' reference follows a row's maximum where it has fallen behind by more than this (powers of two): most tiles then leave O as it is, 7 % of a long prompt's
+// time.  Weights are as exact as before, 2^-8 of themselves, but the largest one is rounded too; sums are fp32.
+constexpr float LAG = 8.f;
 constexpr int EDGES = 6;             // tiles of an item at the edges of what its rows see: tokens span at most 128 positions, so three at either end
 
 template <int HD>
@@ -96,7 +99,7 @@ __device__ __forceinline__ unsigned long long twice(float x) {
 }
 
 struct Shape {
-  int g, tt;  // query heads of a group; tokens of a block
+  int g, tt, out32;  // query heads of a group; tokens of a block; rows of the result begin on 32-byte boundaries
 };
 // sum over the block of a 64-bit value a thread: what the threads below have, and all
 __device__ __forceinline__ long long block_scan(long long v, long long* warp_sums, long long& total) {
@@ -154,11 +157,11 @@ __global__ void __launch_bounds__(NTHR, 2) attn_batch_kernel(BatchAttnArgs a, Sh
   for (int i = tid; i < EDGES * HD; i += NTHR) asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(s0 + SM::ODD + i * 16), "r"(0u) : "memory");
   // ---- this CTA's stretch
   const int per = (a.n_req + NTHR - 1) / NTHR, r0 = min(a.n_req, tid * per), r1 = min(a.n_req, r0 + per);
-  long long mine = 0, total;
-  Raw one;
+  long long mine = 0, total, head = 0;  // head: a kv head's cost of the thread's last request
   for (int i = r0; i < r1; ++i) {
-    one = request(a, i, tt);
-    mine += a.kv.n_kv * ab_cost(one.r, one.r.nb, tt, a.window);
+    const Raw w = request(a, i, tt);
+    head = ab_cost(w.r, w.r.nb, tt, a.window);
+    mine += a.kv.n_kv * head;
   }
   const long long below = block_scan(mine, s_sums, total);
   const long long share = quotient(total + gridDim.x - 1, gridDim.x), x0 = min(total, share * blockIdx.x), x1 = min(total, x0 + share);
@@ -169,27 +172,31 @@ __global__ void __launch_bounds__(NTHR, 2) attn_batch_kernel(BatchAttnArgs a, Sh
     if (own) {
       rest = x0 - below;
       for (req = r0; req < r1 - 1; ++req) {
-        one = request(a, req, tt);
-        const long long c = a.kv.n_kv * ab_cost(one.r, one.r.nb, tt, a.window);
-        if (rest < c) break;
-        rest -= c;
+        const Raw w = request(a, req, tt);
+        const long long h = ab_cost(w.r, w.r.nb, tt, a.window);
+        if (rest < a.kv.n_kv * h) {
+          head = h;
+          break;
+        }
+        rest -= a.kv.n_kv * h;
       }
     }
     const int from = __ffs(owner) - 1;
-    req = __shfl_sync(0xffffffffu, req, from), rest = __shfl_sync(0xffffffffu, rest, from);
+    req = __shfl_sync(0xffffffffu, req, from), rest = __shfl_sync(0xffffffffu, rest, from), head = __shfl_sync(0xffffffffu, head, from);
     const Raw w = request(a, req, tt);
-    const long long head = ab_cost(w.r, w.r.nb, tt, a.window);
     const int kvh = (int)quotient(rest, head);
     rest -= kvh * head;
     // the block in which it begins: the last one whose cost of blocks before is not above the rest, 32 at a time
     int lo = 0, hi = w.r.nb;
+    long long before = 0;
     while (hi - lo > 1) {
       const int step = (hi - lo + 31) / 32, x = lo + lane * step;
-      const unsigned in = __ballot_sync(0xffffffffu, x < hi && ab_cost(w.r, x, tt, a.window) <= rest);
-      const int k = 31 - __clz(in);  // (lane 0's is)
+      const long long c = x < hi ? ab_cost(w.r, x, tt, a.window) : rest + 1;
+      const int k = 31 - __clz(__ballot_sync(0xffffffffu, c <= rest));  // (lane 0's is)
+      before = __shfl_sync(0xffffffffu, c, k);
       hi = min(hi, lo + (k + 1) * step), lo += k * step;
     }
-    if (lane == 0) s_walk = Walk{w, req, kvh, lo, (int)(rest - ab_cost(w.r, lo, tt, a.window)), x1 - x0};
+    if (lane == 0) s_walk = Walk{w, req, kvh, lo, (int)(rest - before), x1 - x0};
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
@@ -369,10 +376,10 @@ __global__ void __launch_bounds__(NTHR, 2) attn_batch_kernel(BatchAttnArgs a, Sh
 #pragma unroll
           for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(r[60 + e]));
           const float m_new = fmaxf(m_ref, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2);
-          const bool grow = __any_sync(0xffffffffu, m_new > m_ref);
-          const float f = m_new > -INFINITY ? ex2_tc(m_ref - m_new) : 1.f;
-          m_ref = m_new;
-          const unsigned long long s2 = twice(sl2), n2 = twice(m_new > -INFINITY ? -m_new : 0.f);
+          const bool grow = __any_sync(0xffffffffu, m_new > m_ref + LAG && tok < p.tokens);  // (rows behind the last token are anything)
+          const float f = grow && m_new > -INFINITY ? ex2_tc(m_ref - m_new) : 1.f;
+          if (grow) m_ref = m_new;
+          const unsigned long long s2 = twice(sl2), n2 = twice(m_ref > -INFINITY ? -m_ref : 0.f);
           float rs[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int c = 0; c < TK; c += 32) {
@@ -470,11 +477,17 @@ __global__ void __launch_bounds__(NTHR, 2) attn_batch_kernel(BatchAttnArgs a, Sh
           if (tok >= p.tokens) continue;
           if (whole) {
 #pragma unroll
-            for (int j = 0; j < 32; j += 8) {
-              uint32_t w[4];
+            for (int j = 0; j < 32; j += 16) {
+              uint32_t w[8];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) w[e] = pack2f(__uint_as_float(r[j + 2 * e]) * scale, __uint_as_float(r[j + 2 * e + 1]) * scale);
-              *reinterpret_cast<uint4*>(dst + c + j) = make_uint4(w[0], w[1], w[2], w[3]);
+              for (int e = 0; e < 8; ++e) w[e] = pack2f(__uint_as_float(r[j + 2 * e]) * scale, __uint_as_float(r[j + 2 * e + 1]) * scale);
+              if (sh.out32) {
+                asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + c + j), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                             : "memory");
+              } else {
+                *reinterpret_cast<uint4*>(dst + c + j) = make_uint4(w[0], w[1], w[2], w[3]);
+                *reinterpret_cast<uint4*>(dst + c + j + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+              }
             }
           } else {
 #pragma unroll
@@ -616,7 +629,7 @@ cudaError_t launch_hd(const BatchAttnArgs& a, const TensorMap2D& qm, const Tenso
     set.done();
   }
   const int G = a.n_q / a.kv.n_kv, ctas = 2 * a.num_sms;
-  const cudaError_t e = launched(launch_k(attn_batch_kernel<HD, TMA>, dim3(ctas), dim3(NTHR), Smem<HD>::TOTAL, st, a, Shape{G, TQ / G}, box,
+  const cudaError_t e = launched(launch_k(attn_batch_kernel<HD, TMA>, dim3(ctas), dim3(NTHR), Smem<HD>::TOTAL, st, a, Shape{G, TQ / G, (int)(reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && a.out_stride % 16 == 0)}, box,
                                           *reinterpret_cast<const CUtensorMap*>(&qm), *reinterpret_cast<const CUtensorMap*>(&kvm)));
   if (e != cudaSuccess) return e;
   return launched(launch_k(attn_batch_join_kernel<HD>, dim3(ctas, HD / 64), dim3(JOIN_THR), 0, st, a, G, ctas));
