@@ -466,7 +466,7 @@ static bool rope_ok(const qie_rope_plan* r, int head_dim) { return r && r->freq 
 int qie_rope_rows(const qie_bf16* x, size_t x_stride, qie_bf16* out, size_t out_stride, const qie_rope_plan* rope, const int* pos, int n_tok, int n_heads,
                   int head_dim, qie_stream st) {
   if (!rope_ok(rope, head_dim)) return fail(QIE_EINVAL, "rope_rows: need an even number of rotated elements, at most head_dim, and head_dim up to 1024");
-  if (n_tok < 0 || n_heads < 0 || (n_tok && n_heads && (!x || !out || !pos))) return fail(QIE_EINVAL, "rope_rows: bad argument");
+  if (n_tok < 0 || n_tok > 1 << 30 || n_heads < 0 || (n_tok && n_heads && (!x || !out || !pos))) return fail(QIE_EINVAL, "rope_rows: bad argument (at most 2^30 rows)");
   const size_t wide = (size_t)n_heads * head_dim;
   if (n_tok > 1 && (x_stride < wide || out_stride < wide)) return fail(QIE_EINVAL, "rope_rows: rows of %zu elements overlap", wide);
   if (n_tok > 1 && x == out && x_stride != out_stride) return fail(QIE_EINVAL, "rope_rows: in place with rows at other places");
@@ -485,7 +485,7 @@ int qie_rope_store(const qie_kv_view* kv, int layer, const qie_bf16* q, size_t q
       (long long)kv->n_pages * kv->page_size >= (1ll << 31))
     return fail(QIE_EINVAL, "rope_store: bad pool or layer");
   if (!rope_ok(rope, kv->head_dim)) return fail(QIE_EINVAL, "rope_store: need an even number of rotated elements, at most head_dim, and head_dim up to 1024");
-  if (n_tok < 0 || n_q_heads < 0 || (n_tok && (!k || !v || !pos || !row || (n_q_heads && (!q || !q_out))))) return fail(QIE_EINVAL, "rope_store: bad argument");
+  if (n_tok < 0 || n_tok > 1 << 30 || n_q_heads < 0 || (n_tok && (!k || !v || !pos || !row || (n_q_heads && (!q || !q_out))))) return fail(QIE_EINVAL, "rope_store: bad argument (at most 2^30 rows)");
   const size_t wide = (size_t)n_q_heads * kv->head_dim, kv_wide = (size_t)kv->n_kv_heads * kv->head_dim;
   if (n_tok > 1 && (k_stride < kv_wide || v_stride < kv_wide || (n_q_heads && (q_stride < wide || q_out_stride < wide))))
     return fail(QIE_EINVAL, "rope_store: rows overlap");

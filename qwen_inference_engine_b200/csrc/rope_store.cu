@@ -1,11 +1,14 @@
 // rope_store.cu -- rotary positions of q and k and the store of k and v into the cache pages, one launch (qie_rope_rows, qie_rope_store).
 //
 //   (a, b) -> (a c - b s, b c + a s),  c, s = factor * cos, sin(pos * freq[i]),  in fp32 with one rounding
-// The angle's turns pos * freq[i] / 2 pi are taken in 64 bits and only their fraction goes to 32: 2^31 positions leave it exact to 2^-20 of a turn.
+// A pair's turns a position, freq[i] / 2 pi, are kept as their fraction in 64-bit fixed point (of the nearest double); their product with the position modulo 2^64 is the
+// fraction of the turns at that position, off by at most 2^31 times half a unit of the double: 2^-23 of a turn.  Sine and cosine of that, in [-pi, pi], by the hardware's
+// functions: 2^-20.5 of one, where results are rounded to 2^-8 of themselves.  (In doubles, with the library's functions, the angles were a third of the kernel's
+// instructions.)
 //
-// Bound by memory: every element is read and written once.  A CTA takes a few tokens: their cosines and sines go to shared memory (once a token, not once a
-// head), then a thread takes the same place of the row in each token, V elements of a pair's first half and V of the second (or V / 2 neighbouring pairs),
-// with the loads of four tokens under way.
+// Bound by memory: every element is read and written once.  A thread has one place of the row (V elements of a pair's first half and V of the second, or V / 2
+// neighbouring pairs) and goes through groups of U tokens: the next group's loads are under way while it turns the one at hand, and the CTA's threads compute the next
+// group's cosines and sines, once a token, into the other half of shared memory.
 #include <algorithm>
 
 #include "common.cuh"
@@ -15,7 +18,7 @@
 namespace qie {
 namespace {
 
-constexpr int MOST_TOK = 8;  // tokens a CTA
+constexpr int MOST_THR = 512;
 
 template <int V>
 struct Vec {
@@ -45,38 +48,58 @@ __device__ __forceinline__ void store(bf16* p, const Vec<V>& r) {
   else *reinterpret_cast<uint16_t*>(p) = (uint16_t)r.w[0];
 }
 
+// two fp32 values at once
+struct Two {
+  unsigned long long v;
+  __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ explicit Two(uint32_t w) : Two(lo2f(w), hi2f(w)) {}
+  __device__ __forceinline__ uint32_t rounded() const {
+    float a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+    return pack2f(a, b);
+  }
+};
+__device__ __forceinline__ Two operator*(Two a, Two b) {
+  asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(a.v) : "l"(b.v));
+  return a;
+}
+__device__ __forceinline__ Two operator-(Two a, Two b) {
+  asm("sub.rn.f32x2 %0, %0, %1;" : "+l"(a.v) : "l"(b.v));
+  return a;
+}
+__device__ __forceinline__ Two fma(Two a, Two b, Two c) {
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c.v) : "l"(a.v), "l"(b.v));
+  return c;
+}
+
 // V elements at a time; NB: neighbours are pairs
-template <int V, bool NB>
-__global__ void rope_store_kernel(RopeArgs a, int n_tok) {
+template <int V, bool NB, int U>
+__global__ void __launch_bounds__(MOST_THR, 2) rope_store_kernel(RopeArgs a) {
   constexpr bool SPLIT = !NB || V == 1;  // a pair's elements are loaded one by one
-  extern __shared__ float2 cs[];  // [token][pair]
-  __shared__ int s_pos[MOST_TOK];
-  __shared__ long long s_at[MOST_TOK];  // offset of the token's cache row in the pool, below 0: none
+  constexpr int EACH = SPLIT ? V : V / 2;  // pairs of a place
+  constexpr int W = EACH > 1 ? 2 : 1;  // pairs together: their cosines, then their sines
+  extern __shared__ __align__(16) float cs[];  // [2][token][W pairs of the place][place]: threads at places side by side read side by side; then the pairs' turns
+  // of the groups at hand, next and behind that: positions, and offsets of the tokens' cache rows in the pool (below 0: none)
+  __shared__ int s_pos[4][U];
+  __shared__ long long s_at[4][U];
   pdl_wait();
   pdl_trigger();
-  const int t0 = blockIdx.x * n_tok, n = min(n_tok, a.n_tok - t0), hd = a.kv.hd, half = a.rotated / 2;
-  for (int i = threadIdx.x; i < n * half; i += blockDim.x) {
-    const int t = i / half;
-    const double turns = (double)a.pos[t0 + t] * a.freq[i - t * half] * 0.15915494309189533577;
-    float s, c;
-    sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
-    cs[i] = make_float2(c * a.factor, s * a.factor);
+  const int hd = a.kv.hd, half = a.rotated / 2, tid = threadIdx.x, thr = blockDim.x;
+  unsigned long long* turns_s = reinterpret_cast<unsigned long long*>(cs + (2 * U * a.rotated + 1) / 2 * 2);
+  for (int p = tid; p < half; p += thr) {
+    const double turns = a.freq[p] * 0.15915494309189533577;
+    turns_s[p] = (unsigned long long)((turns - floor(turns)) * 18446744073709551616.0);
   }
-  if (threadIdx.x < n) {
-    const int t = threadIdx.x;
-    s_pos[t] = a.pos[t0 + t];
-    s_at[t] = -1;
-    if (a.k) {
-      const int row = a.row[t0 + t];
-      if (row >= 0 && row < a.kv.n_pages * a.kv.page_size) s_at[t] = (long long)((size_t)(row / a.kv.page_size) * a.kv.page_stride() + (size_t)(row % a.kv.page_size) * hd);
-    }
-  }
-  __syncthreads();
   // places of a row: of each head of q and k the pairs, then what is not turned; the heads of v
-  const int other = NB ? 1 : half, pairs = SPLIT ? half / V : a.rotated / V, rest = (hd - a.rotated) / V, per = pairs + rest, n_kv = a.k ? a.kv.n_kv : 0;
-  const int turned = (a.n_q + n_kv) * per, all = turned + n_kv * (hd / V);
-  for (int u = threadIdx.x; u < all; u += blockDim.x) {
-    int head, place, kind;  // 0: q, 1: k, 2: v
+  const int other = NB ? 1 : half, pairs = half / EACH, rest = (hd - a.rotated) / V, per = pairs + rest, n_kv = a.k ? a.kv.n_kv : 0;
+  const int turned = (a.n_q + n_kv) * per, all = turned + n_kv * (hd / V), u = blockIdx.y * thr + tid;
+  int place = 0, kind = -1;  // 0: q, 1: k, 2: v, below 0: none
+  bool turn = false;
+  size_t stride = 0;
+  const bf16* src = nullptr;
+  bf16* dst = nullptr;
+  if (u < all) {
+    int head;
     if (u < turned) {
       head = u / per, place = u - head * per;
       kind = head >= a.n_q;
@@ -85,67 +108,132 @@ __global__ void rope_store_kernel(RopeArgs a, int n_tok) {
       head = (u - turned) / (hd / V), place = u - turned - head * (hd / V);
       kind = 2;
     }
-    const bool turn = kind < 2 && place < pairs;
+    turn = kind < 2 && place < pairs;
     const int at = turn ? place * (NB && SPLIT ? 2 : V) : kind == 2 ? place * V : a.rotated + (place - pairs) * V;
-    const size_t stride = kind == 0 ? a.q_stride : kind == 1 ? a.k_stride : a.v_stride;
-    const bf16* src = (kind == 0 ? a.q : kind == 1 ? a.k : a.v) + (size_t)t0 * stride + (size_t)head * hd + at;
-    bf16* dst = kind == 0 ? a.q_out + (size_t)t0 * a.q_out_stride + (size_t)head * hd + at : a.kv.chunk(0, a.layer, kind - 1, head) + at;
-    constexpr int U = 4;
-    for (int b = 0; b < n; b += U) {
-      Vec<V> x[U], y[U];
-#pragma unroll
-      for (int e = 0; e < U; ++e)
-        if (b + e < n) {
-          x[e] = load<V>(src + (size_t)(b + e) * stride);
-          if (SPLIT && turn) y[e] = load<V>(src + (size_t)(b + e) * stride + other);
-        }
-#pragma unroll
-      for (int e = 0; e < U; ++e) {
-        const int t = b + e;
-        if (t >= n || (kind == 0 ? s_pos[t] < 0 : s_at[t] < 0)) continue;
-        bf16* to = dst + (kind == 0 ? (size_t)t * a.q_out_stride : (size_t)s_at[t]);
-        if (turn) {
-          if constexpr (!SPLIT) {
-#pragma unroll
-            for (int i = 0; i < V / 2; ++i) {
-              const float2 c = cs[t * half + place * (V / 2) + i];
-              const float u0 = lo2f(x[e].w[i]), u1 = hi2f(x[e].w[i]);
-              x[e].w[i] = pack2f(u0 * c.x - u1 * c.y, u1 * c.x + u0 * c.y);
-            }
-          } else if constexpr (V == 1) {
-            const float2 c = cs[t * half + place];
-            const float u0 = lo2f(x[e].w[0]), u1 = lo2f(y[e].w[0]);
-            x[e].w[0] = pack2f(u0 * c.x - u1 * c.y, 0.f) & 0xffffu;
-            y[e].w[0] = pack2f(u1 * c.x + u0 * c.y, 0.f) & 0xffffu;
-          } else {
-#pragma unroll
-            for (int i = 0; i < V / 2; ++i) {
-              const float2 c0 = cs[t * half + place * V + 2 * i], c1 = cs[t * half + place * V + 2 * i + 1];
-              const float u0 = lo2f(x[e].w[i]), u1 = hi2f(x[e].w[i]), w0 = lo2f(y[e].w[i]), w1 = hi2f(y[e].w[i]);
-              x[e].w[i] = pack2f(u0 * c0.x - w0 * c0.y, u1 * c1.x - w1 * c1.y);
-              y[e].w[i] = pack2f(w0 * c0.x + u0 * c0.y, w1 * c1.x + u1 * c1.y);
-            }
-          }
-          if constexpr (SPLIT) store<V>(to + other, y[e]);
-        }
-        store<V>(to, x[e]);
-      }
-    }
+    stride = kind == 0 ? a.q_stride : kind == 1 ? a.k_stride : a.v_stride;
+    src = (kind == 0 ? a.q : kind == 1 ? a.k : a.v) + (size_t)head * hd + at;
+    dst = kind == 0 ? a.q_out + (size_t)head * hd + at : a.kv.chunk(0, a.layer, kind - 1, head) + at;
   }
+  struct Group {
+    Vec<V> x[U], y[U];
+  };
+  auto fetch = [&](int t0, Group& g) {
+#pragma unroll
+    for (int e = 0; e < U; ++e)
+      if (kind >= 0 && t0 + e < a.n_tok) {
+        const bf16* from = src + (size_t)(t0 + e) * stride;
+        g.x[e] = load<V>(from);
+        if (SPLIT && turn) g.y[e] = load<V>(from + other);
+      }
+  };
+  const int dt = thr / half, dp = thr - dt * half;
+  auto angles = [&](int t0, int k) {  // of the k-th group, whose positions are there
+    const int n = min(U, a.n_tok - t0);
+    float* c = cs + (k & 1) * U * a.rotated;
+    for (int t = tid / half, p = tid - t * half; t < n;) {
+      const int j = p % EACH;
+      const int turns = (int)((unsigned long long)(unsigned)s_pos[k & 3][t] * turns_s[p] >> 32);  // their fraction, in 2^-32 of a turn from -1/2 on
+      float sn, cn;
+      __sincosf((float)turns * 1.4629180792671596e-9f, &sn, &cn);  // (2 pi / 2^32)
+      float* at = c + t * a.rotated + ((j / W) * pairs + p / EACH) * 2 * W + j % W;
+      at[0] = cn * a.factor, at[W] = sn * a.factor;
+      t += dt, p += dp;
+      if (p >= half) p -= half, ++t;
+    }
+  };
+  int pos = -1, row = -1;
+  auto ask = [&](int t0) {  // a token's numbers, one of the first threads each
+    if (tid < U && t0 + tid < a.n_tok) pos = a.pos[t0 + tid], row = a.k ? a.row[t0 + tid] : -1;
+  };
+  auto note = [&](int k) {
+    if (tid >= U) return;
+    s_pos[k & 3][tid] = pos;
+    s_at[k & 3][tid] = row >= 0 && row < a.kv.n_pages * a.kv.page_size
+                           ? (long long)((size_t)(row / a.kv.page_size) * a.kv.page_stride() + (size_t)(row % a.kv.page_size) * hd) : -1;
+  };
+  auto put = [&](int t0, int k, Group& g) {
+    if (kind < 0) return;
+#pragma unroll
+    for (int e = 0; e < U; ++e) {
+      if (t0 + e >= a.n_tok) break;
+      const long long at = s_at[k & 3][e];
+      if (kind == 0 ? s_pos[k & 3][e] < 0 : at < 0) continue;
+      bf16* to = dst + (kind == 0 ? (size_t)(t0 + e) * a.q_out_stride : (size_t)at);
+      Vec<V> &x = g.x[e], &y = g.y[e];
+      if (turn) {
+        const float* mine = cs + ((k & 1) * U + e) * a.rotated + place * 2 * W;
+        if constexpr (!SPLIT && W == 2) {
+#pragma unroll
+          for (int i = 0; i < V / 2; i += 2) {
+            const float4 f = *reinterpret_cast<const float4*>(mine + i * pairs * 2);
+            const float u0 = lo2f(x.w[i]), u1 = hi2f(x.w[i]), u2 = lo2f(x.w[i + 1]), u3 = hi2f(x.w[i + 1]);
+            x.w[i] = pack2f(u0 * f.x - u1 * f.z, u1 * f.x + u0 * f.z);
+            x.w[i + 1] = pack2f(u2 * f.y - u3 * f.w, u3 * f.y + u2 * f.w);
+          }
+        } else if constexpr (!SPLIT) {
+          const float u0 = lo2f(x.w[0]), u1 = hi2f(x.w[0]);
+          x.w[0] = pack2f(u0 * mine[0] - u1 * mine[1], u1 * mine[0] + u0 * mine[1]);
+        } else if constexpr (V == 1) {
+          const float u0 = lo2f(x.w[0]), u1 = lo2f(y.w[0]);
+          x.w[0] = pack2f(u0 * mine[0] - u1 * mine[1], 0.f) & 0xffffu;
+          y.w[0] = pack2f(u1 * mine[0] + u0 * mine[1], 0.f) & 0xffffu;
+        } else {
+#pragma unroll
+          for (int i = 0; i < V / 2; ++i) {
+            const float4 f = *reinterpret_cast<const float4*>(mine + i * pairs * 4);
+            const Two c(f.x, f.y), s(f.z, f.w), v(x.w[i]), w(y.w[i]);
+            x.w[i] = (v * c - w * s).rounded();
+            y.w[i] = fma(v, s, w * c).rounded();
+          }
+        }
+        if constexpr (SPLIT) store<V>(to + other, y);
+      }
+      store<V>(to, x);
+    }
+  };
+  const int step = gridDim.x * U;
+  Group g;
+  int t = blockIdx.x * U, k = 0;
+  ask(t);
+  fetch(t, g);
+  note(0);
+  ask(t + step);
+  __syncthreads();
+  angles(t, 0);
+  note(1);
+  for (;; ++k) {
+    __syncthreads();
+    const int next = t + step;
+    if (next >= a.n_tok) break;
+    Group h;
+    ask(next + step);
+    fetch(next, h);
+    put(t, k, g);
+    angles(next, k + 1);
+    note(k + 2);
+    g = h;
+    t = next;
+  }
+  put(t, k, g);
 }
 
 template <int V, bool NB>
 cudaError_t launch_v(const RopeArgs& a, cudaStream_t st) {
+  constexpr int EACH = NB && V > 1 ? V / 2 : V;
   const int hd = a.kv.hd, n_kv = a.k ? a.kv.n_kv : 0;
-  const int per = (NB && V > 1 ? a.rotated : a.rotated / 2) / V + (hd - a.rotated) / V, all = (a.n_q + n_kv) * per + n_kv * (hd / V);
-  int sms = 0, dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
+  const int per = a.rotated / 2 / EACH + (hd - a.rotated) / V, all = (a.n_q + n_kv) * per + n_kv * (hd / V);
+  int dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  sms = device_attribute<cudaDevAttrMultiProcessorCount>(dev);
-  // as many tokens a CTA as leave four CTAs to an SM
-  const int n_tok = std::max(1, std::min({MOST_TOK, a.n_tok / (4 * std::max(1, sms)), 4096 / a.rotated}));
-  const int thr = std::min(256, (all + 31) / 32 * 32);
-  return launched(launch_k(rope_store_kernel<V, NB>, dim3((a.n_tok + n_tok - 1) / n_tok), dim3(thr), n_tok * (a.rotated / 2) * sizeof(float2), st, a, n_tok));
+  const int sms = std::max(1, device_attribute<cudaDevAttrMultiProcessorCount>(dev));
+  // a thread a place; CTAs that an SM has room for at once (at 64 registers a thread) go through the tokens
+  constexpr int U = NB ? 4 : 2;
+  const int ny = (all + MOST_THR - 1) / MOST_THR, thr = ((all + ny - 1) / ny + 31) / 32 * 32, most = std::max(1, 1024 / thr) * sms;
+  const int groups = (a.n_tok + U - 1) / U;
+  auto bytes = [&](int u) { return ((2 * u * a.rotated + 1) / 2 * 2 + a.rotated) * sizeof(float); };
+  if ((long long)groups * ny >= 2 * sms)
+    return launched(launch_k(rope_store_kernel<V, NB, U>, dim3(std::max(1, std::min(groups, most / ny)), ny), dim3(thr), bytes(U), st, a));
+  return launched(launch_k(rope_store_kernel<V, NB, 1>, dim3(a.n_tok, ny), dim3(thr), bytes(1), st, a));
 }
 
 }  // namespace

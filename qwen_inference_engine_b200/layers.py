@@ -84,7 +84,7 @@ class KvPool:
         self.pool = torch.zeros(n_pages, n_layers, 2, n_kv_heads, page_size, head_dim, dtype=torch.bfloat16,
                                 device="cuda")
         self.view = KvView(self.pool.data_ptr(), n_pages, page_size, n_layers, n_kv_heads, head_dim)
-        self.ref = C.byref(self.view)
+        self.ref, self.head_dim, self.kv_wide = C.byref(self.view), head_dim, n_kv_heads * head_dim
         self.max_pages = n_pages
         # identity-ish block table: sequence s owns pages s, s+max_seqs, ... (deliberately non-contiguous)
         bt = np.zeros((max_seqs, n_pages), np.int32)
@@ -101,7 +101,7 @@ class KvPool:
         self = cls.__new__(cls)
         self.pool, self.block_table = pool, block_table
         self.view = KvView(_p(pool), n_pages, page_size, n_layers, n_kv_heads, head_dim)
-        self.ref = C.byref(self.view)
+        self.ref, self.head_dim, self.kv_wide = C.byref(self.view), head_dim, n_kv_heads * head_dim
         self.max_pages = n_pages if block_table is None else block_table.shape[1]
         return self
 
@@ -197,7 +197,7 @@ class Batch:
         self.block_table, self.slots, self.cached, self.n_new, self.free_ring, self.ring_in = block_table, slots, cached, n_new, free_ring, ring_in
         self.ring_out, self.q_start, self.kv_len, self.status = ints(ring_out, 2), ints(q_start, n_req + 1), ints(kv_len, n_req), ints(status, 2)
         self.pos, self.slot, self.row = ints(pos, max_tokens), ints(slot, max_tokens), ints(row, max_tokens)
-        self.work = None
+        self.work, self.max_tokens = None, max_tokens
         b = self.view = BatchView(n_req=n_req, max_tokens=max_tokens, max_seqs=block_table.shape[0], max_pages=block_table.shape[1], n_pages=n_pages,
                                   page_size=page_size)
         for name, n in (("block_table", 0), ("slots", n_req), ("cached", n_req), ("n_new", n_req), ("free_ring", n_pages), ("ring_in", 2), ("ring_out", 2),
@@ -249,18 +249,22 @@ def launch_rope_rows(x, out, pos, rope, n_heads, head_dim):
 
 def launch_rope_store(q, k, v, q_out, pool, layer, pos, row, rope, n_q_heads):
     """q -> q_out, k and v -> the cache rows row[t] of the pool's layer"""
-    view, (n, wide) = pool.view, q.shape
-    kv = (n, view.n_kv_heads * view.head_dim)
+    (n, wide), (nk, kw), (nv, vw), (no, ow) = q.shape, k.shape, v.shape, q_out.shape
+    (qs, q1), (ks, k1), (vs, v1), (os, o1) = q.stride(), k.stride(), v.stride(), q_out.stride()
     assert q.dtype is k.dtype is v.dtype is q_out.dtype is torch.bfloat16, "bfloat16 rows expected"
-    assert q_out.shape == q.shape and k.shape == kv and v.shape == kv and wide == n_q_heads * view.head_dim, "rows of the heads of as many tokens expected"
+    assert n == nk == nv == no and wide == ow == n_q_heads * pool.head_dim and kw == vw == pool.kv_wide, "rows of the heads of as many tokens expected"
+    assert (q1 == o1 == 1 or wide <= 1) and (k1 == v1 == 1 or kw <= 1), "rows of contiguous elements expected"
+    assert q.get_device() == k.get_device() == v.get_device() == q_out.get_device(), "rows on one device expected"
     _here(q)
-    check(_lib.lib().qie_rope_store(pool.ref, layer, *_rows(q), *_rows(q_out), *_rows(k), *_rows(v), rope.ref, _ints(pos, n, "pos"), _ints(row, n, "row"), n,
-                                    n_q_heads, _st()))
+    if n == 1:
+        qs, os, ks, vs = wide, wide, kw, kw
+    check(_lib.lib().qie_rope_store(pool.ref, layer, q.data_ptr(), qs, q_out.data_ptr(), os, k.data_ptr(), ks, v.data_ptr(), vs, rope.ref, _ints(pos, n, "pos"),
+                                    _ints(row, n, "row"), n, n_q_heads, _st()))
 
 
 def launch_attn_batch(Q, out, pool, layer, batch, n_q_heads, window=0, scale=0.0):
     """attention of the batch's rows over the pool, ragged over its requests (fast numerics)"""
-    assert Q.dtype is out.dtype is torch.bfloat16 and Q.shape == out.shape == (batch.view.max_tokens, n_q_heads * pool.view.head_dim), "bfloat16 rows of the batch expected"
+    assert Q.dtype is out.dtype is torch.bfloat16 and Q.shape == out.shape == (batch.max_tokens, n_q_heads * pool.head_dim), "bfloat16 rows of the batch expected"
     if batch.work is None:
         batch.reserve(pool, n_q_heads)
     _here(Q)

@@ -46,7 +46,7 @@ def rope_rows(x=P, xs=256, out=P, outs=256, plan=None, pos=P, n=3, heads=2, hd=1
     return _lib.lib().qie_rope_rows(x, xs, out, outs, plan, pos, n, heads, hd, None)
 
 
-@pytest.mark.parametrize("over", [dict(x=0), dict(out=0), dict(pos=0), dict(n=-1), dict(heads=-1), dict(xs=255), dict(outs=255), dict(hd=1026, xs=4096, outs=4096), dict(hd=126),
+@pytest.mark.parametrize("over", [dict(x=0), dict(out=0), dict(pos=0), dict(n=-1), dict(n=2 ** 30 + 1), dict(heads=-1), dict(xs=255), dict(outs=255), dict(hd=1026, xs=4096, outs=4096), dict(hd=126),
                                   dict(outs=300), *(dict(plan=C.byref(RopePlan(f, r, 0, 1.0))) for f, r in ((0, 64), (P, 0), (P, 63), (P, 130), (P, -2)))])
 def test_rope_rows(over):
     refused(rope_rows(**over), "rope_rows")
@@ -62,7 +62,7 @@ def test_nothing_to_do_needs_no_device():
 
 @pytest.mark.parametrize("view,over", [(dict(pool=0), {}), (dict(n_pages=0), {}), (dict(page_size=0), {}), (dict(n_kv_heads=0), {}), (dict(n_pages=1 << 27), {}),
                                        (dict(head_dim=62), {}), ({}, dict(layer=2)), ({}, dict(layer=-1)), ({}, dict(q=0)), ({}, dict(k=0)), ({}, dict(v=0)), ({}, dict(pos=0)),
-                                       ({}, dict(row=0)), ({}, dict(ks=127)), ({}, dict(vs=127)), ({}, dict(qs=255)), ({}, dict(n=-1)), ({}, dict(q=2 * P, qs=384))])
+                                       ({}, dict(row=0)), ({}, dict(ks=127)), ({}, dict(vs=127)), ({}, dict(qs=255)), ({}, dict(n=-1)), ({}, dict(n=2 ** 30 + 1)), ({}, dict(q=2 * P, qs=384))])
 def test_rope_store(view, over):
     a = dict(layer=0, q=P, qs=256, k=P, ks=128, v=P, vs=128, pos=P, row=P, n=2, heads=4)
     a.update(over)
