@@ -14,7 +14,7 @@
 namespace qie {
 namespace {
 
-constexpr int MOST_THR = 512, MOST_CTA = 8, MOST_GRID = 256;
+constexpr int MOST_THR = 1024, MOST_CTA = 8, MOST_GRID = 256;
 
 struct Sums {
   long long tok, need, back;
@@ -189,12 +189,14 @@ cudaError_t launch_batch_layout(const BatchArgs& a, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     set.done();
   }
-  // A thread for four tokens and for a request.  Where the ring's state is updated in place the CTAs are one cluster (of eight at most): none may write it before all have read it.
-  const int thr = std::min(MOST_THR, std::max(128, (std::max((a.max_tokens + 3) / 4, a.n_req) + 31) / 32 * 32));
+  // A thread for four tokens and for a request.  Where the ring's state is updated in place the CTAs are one cluster (of eight at most): none may write it before all have
+  // read it.  More than a few thousand tokens: half of the CTAs for the pages given back, which else come ahead of the tokens (8192 tokens, 2600 pages given back: 7.5 us,
+  // so 6.0).  CTAs have 512 threads (with 1024 that case takes 8.4) but where a cluster of them is not enough (131072 tokens in place: 36 us, so 27; with a ring of its
+  // own behind the step 7.9).
   const bool in_place = a.ring_in == a.ring_out || a.ring_in + 1 == a.ring_out || a.ring_in == a.ring_out + 1;
-  const int want = std::max(1, (a.max_tokens / 4 + thr - 1) / thr), most = in_place ? MOST_CTA : MOST_GRID;
-  // more than a few thousand tokens: half of the CTAs for the pages given back, which else come ahead of the tokens (8192 tokens, 2600 pages given back: 7.5 us)
-  const int n_tok_cta = want > 1 ? std::min(want, most / 2) : 1, ctas = want > 1 ? 2 * n_tok_cta : 1;
+  const int quads = (a.max_tokens + 3) / 4, few = in_place && quads > MOST_CTA * 512 ? MOST_THR : 512;
+  const int thr = std::min(few, std::max(128, (std::max(quads, a.n_req) + 31) / 32 * 32)), want = (quads + thr - 1) / thr;
+  const int n_tok_cta = want > 1 ? std::min(want, (in_place ? MOST_CTA : MOST_GRID) / 2) : 1, ctas = want > 1 ? 2 * n_tok_cta : 1;
   const bool wide = ((reinterpret_cast<uintptr_t>(a.pos) | reinterpret_cast<uintptr_t>(a.slot) | reinterpret_cast<uintptr_t>(a.row)) & 15) == 0;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(ctas);
