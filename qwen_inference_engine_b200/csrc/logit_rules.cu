@@ -188,25 +188,31 @@ __global__ void __launch_bounds__(THR) logit_rules_kernel(LogitArgs a, int share
         before += __popc(have[i]);
       }
       __syncthreads();
-      for (int n = tid; n < n_used; n += THR) {
-        const int k = used[n], id = (int)key[k];
+      const int lane = tid & 31;
+      for (int first = tid - lane; first < n_used; first += THR) {
+        const bool some = first + lane < n_used;
+        const int k = used[some ? first + lane : first], id = (int)key[k], j = (int)entry[k];
         const uint32_t w = word[k], times = w & TIMES;
         T* at = staged ? reinterpret_cast<T*>(tile) + place_of(id) : out + id;
-        float v = load(at);
+        float v = load(at), sum = w & BIASED ? a.bias[bs.x + j] : 0.f;
+        // several biases of a token: the warp reads the list from its first one on together, and adds those of the token in their order
+        for (unsigned more = __ballot_sync(0xffffffffu, some && w & MORE); more; more &= more - 1) {
+          const int from = __ffs(more) - 1, of = __shfl_sync(0xffffffffu, id, from);
+          float all = 0.f;
+          for (int i = bs.x + __shfl_sync(0xffffffffu, j, from); i < bs.y; i += 32) {
+            const bool it = i + lane < bs.y && a.bias_ids[i + lane] == of;
+            const float b = it ? a.bias[i + lane] : 0.f;
+            for (unsigned its = __ballot_sync(0xffffffffu, it); its; its &= its - 1) all += __shfl_sync(0xffffffffu, b, __ffs(its) - 1);
+          }
+          if (lane == from) sum = all;
+        }
         if ((times || w & LISTED) && a.repetition) v = v > 0.f ? v / rep : v * rep;
         if (times) {
           v -= freq * (float)times;
           v -= pres;
         }
-        if (w & BIASED) {
-          const int j = (int)entry[k];
-          float sum = a.bias[bs.x + j];
-          if (w & MORE)
-            for (int i = bs.x + j + 1; i < bs.y; ++i)
-              if (a.bias_ids[i] == id) sum += a.bias[i];
-          v += sum;
-        }
-        store(at, v);
+        if (w & BIASED) v += sum;
+        if (some) store(at, v);
       }
       // the next class
       while (depth > share && (low >> (depth - 1) & 1)) --depth, low &= (1u << depth) - 1;
