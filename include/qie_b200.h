@@ -164,7 +164,8 @@ int qie_attention_prefill_tc(const qie_kv_view* kv, int layer, const qie_bf16* Q
  * The reference keeps one sequence's page list on the host (src/iengine.cu:25-96) and one state per call
  * (include/iengine.cuh:23-37); these operators take a step of many requests, decode rows beside ragged portions of
  * prompts, whose lengths are device data: one captured graph of them serves every step of up to max_tokens rows.
- * They are written one after another on a stream; arrays that one writes are what the next one reads.  Values in device
+ * They are launched one after another on a stream; arrays that one writes are what the next one reads, and of their own but where a
+ * comment says so.  Values in device
  * arrays that make no sense (lengths, offsets, page ids, rows outside their range) never lead outside the arrays named
  * here; what they say is then not defined, except where a function's comment does. */
 typedef struct {
@@ -436,7 +437,7 @@ int qie_forward_batch(qie_engine* e, int n_entries, const int* h_seqs, const int
 int qie_decode_step_device(qie_engine* e, const int* h_seqs, int n);
 int qie_sync(qie_engine* e);
 /* Kernels whose waits have a limit report one that ran out (their results are then not numbers): engine calls return QIE_ECUDA when they
- * wait for the stream, operators that use such kernels (qie_matmul, qie_matmul_fast, qie_attention, qie_attention_prefill_*) when the next one is called, or this call
+ * wait for the stream, operators that use such kernels (qie_matmul, qie_matmul_fast, qie_attention, qie_attention_prefill_*, qie_attention_batch) when the next one is called, or this call
  * does, behind the caller's own synchronisation.  A report is given once; the context stays usable.  qie_wait_selftest runs a wait that nothing
  * ends (about two seconds, in the first CTA of a pair, of which the other one reports) through the same path: on the engine (returns QIE_ECUDA), or with a null engine as an operator on `st`. */
 int qie_kernel_status(void);

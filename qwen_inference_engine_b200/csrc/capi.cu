@@ -422,6 +422,7 @@ int qie_batch_layout(const qie_batch* b, qie_stream st) {
   if (!b->free_ring || !b->ring_in || !b->ring_out || !b->q_start || !b->status || (b->n_req && (!b->cached || !b->n_new || !b->block_table || !b->kv_len)) ||
       (b->max_tokens && (!b->pos || !b->slot || !b->row)))
     return fail(QIE_EINVAL, "batch_layout: an array is missing");
+  if (b->n_req && (b->kv_len == b->cached || b->kv_len == b->n_new)) return fail(QIE_EINVAL, "batch_layout: kv_len must be an array of its own");
   if (!b->slots && b->n_req > b->max_seqs) return fail(QIE_EINVAL, "batch_layout: %d requests on %d rows of the block table", b->n_req, b->max_seqs);
   BatchArgs a{};
   a.n_req = b->n_req, a.max_tokens = b->max_tokens, a.max_seqs = b->max_seqs, a.max_pages = b->max_pages, a.n_pages = b->n_pages, a.page_size = b->page_size;
@@ -511,6 +512,7 @@ size_t qie_attention_batch_work(const qie_kv_view* kv, int n_q_heads) {
 int qie_attention_batch(const qie_kv_view* kv, int layer, const qie_batch* b, const qie_bf16* Q, size_t q_stride, qie_bf16* out, size_t out_stride, int n_q_heads,
                         int window, float scale, qie_stream st) {
   if (!kv || !kv->pool || layer < 0 || layer >= kv->n_layers || kv->n_pages <= 0 || kv->page_size <= 0) return fail(QIE_EINVAL, "attention_batch: bad pool or layer");
+  if ((unsigned long long)kv->n_pages * kv->n_layers * 2ull * kv->n_kv_heads * kv->page_size >= 1ull << 31) return fail(QIE_EINVAL, "attention_batch: a pool of 2^31 rows of a head");
   if (!batch_heads_ok(kv, n_q_heads)) return fail(QIE_EINVAL, "attention_batch: need n_q %% n_kv == 0, n_q / n_kv <= 128 and head_dim 64 or 128");
   if (!batch_sizes_ok(b) || b->page_size != kv->page_size || b->n_pages != kv->n_pages) return fail(QIE_EINVAL, "attention_batch: a batch of other pages, or of sizes out of range");
   if (!b->slots && b->n_req > b->max_seqs) return fail(QIE_EINVAL, "attention_batch: %d requests on %d rows of the block table", b->n_req, b->max_seqs);

@@ -96,7 +96,7 @@ class KvPool:
     @classmethod
     def over(cls, pool, block_table=None):
         """the same over a caller's pool [page][layer][k|v][kv_head][slot][head_dim] and, for the operators that take it from here, block table"""
-        assert pool.dim() == 6 and pool.shape[2] == 2 and pool.dtype == torch.bfloat16
+        assert pool.dim() == 6 and pool.shape[2] == 2 and pool.dtype == torch.bfloat16, "bfloat16 pool [page][layer][k|v][kv_head][slot][head_dim] expected"
         n_pages, n_layers, _, n_kv_heads, page_size, head_dim = pool.shape
         self = cls.__new__(cls)
         self.pool, self.block_table = pool, block_table
@@ -217,6 +217,7 @@ class Batch:
 
 
 def launch_batch_layout(batch):
+    _here(batch.block_table)
     check(_lib.lib().qie_batch_layout(batch.ref, _st()))
 
 
@@ -254,7 +255,7 @@ def launch_rope_store(q, k, v, q_out, pool, layer, pos, row, rope, n_q_heads):
     assert q.dtype is k.dtype is v.dtype is q_out.dtype is torch.bfloat16, "bfloat16 rows expected"
     assert n == nk == nv == no and wide == ow == n_q_heads * pool.head_dim and kw == vw == pool.kv_wide, "rows of the heads of as many tokens expected"
     assert (q1 == o1 == 1 or wide <= 1) and (k1 == v1 == 1 or kw <= 1), "rows of contiguous elements expected"
-    assert q.get_device() == k.get_device() == v.get_device() == q_out.get_device(), "rows on one device expected"
+    assert q.get_device() == k.get_device() == v.get_device() == q_out.get_device() == pool.pool.get_device(), "rows and pool on one device expected"
     _here(q)
     if n == 1:
         qs, os, ks, vs = wide, wide, kw, kw
@@ -267,6 +268,7 @@ def launch_attn_batch(Q, out, pool, layer, batch, n_q_heads, window=0, scale=0.0
     assert Q.dtype is out.dtype is torch.bfloat16 and Q.shape == out.shape == (batch.max_tokens, n_q_heads * pool.head_dim), "bfloat16 rows of the batch expected"
     if batch.work is None:
         batch.reserve(pool, n_q_heads)
+    assert Q.get_device() == out.get_device() == pool.pool.get_device() == batch.block_table.get_device(), "rows, pool and batch on one device expected"
     _here(Q)
     check(_lib.lib().qie_attention_batch(pool.ref, layer, batch.ref, *_rows(Q), *_rows(out), n_q_heads, window, scale, _st()))
 

@@ -13,7 +13,7 @@ ARRAYS = ("cached", "n_new", "slots", "block_table", "free_ring", "ring_in", "ri
 
 
 def batch(**over):
-    d = dict(n_req=4, max_tokens=8, max_seqs=4, max_pages=10, n_pages=40, page_size=16, work_bytes=1 << 30, **{a: P for a in ARRAYS})
+    d = dict(n_req=4, max_tokens=8, max_seqs=4, max_pages=10, n_pages=40, page_size=16, work_bytes=1 << 30, **{a: P * (i + 1) for i, a in enumerate(ARRAYS)})
     d.update(over)
     return C.byref(BatchView(**d))
 
@@ -31,7 +31,7 @@ def refused(rc, *words):
 
 
 @pytest.mark.parametrize("over", [dict(n_req=-1), dict(n_req=8193), dict(max_tokens=-1), dict(max_pages=0), dict(page_size=0), dict(n_pages=0), dict(max_seqs=0),
-                                  dict(max_seqs=-1), dict(max_pages=1 << 27), dict(n_pages=1 << 27), dict(slots=0, max_seqs=3),
+                                  dict(max_seqs=-1), dict(max_pages=1 << 27), dict(n_pages=1 << 27), dict(slots=0, max_seqs=3), dict(kv_len=2 * P, cached=2 * P), dict(kv_len=2 * P),
                                   *({a: 0} for a in ARRAYS if a not in ("slots", "work"))])
 def test_layout(over):
     refused(_lib.lib().qie_batch_layout(batch(**over), None), "batch_layout")
@@ -71,10 +71,10 @@ def test_rope_store(view, over):
 
 
 @pytest.mark.parametrize("view,over", [(dict(pool=0), {}), (dict(head_dim=96), {}), (dict(n_kv_heads=3), {}), (dict(n_kv_heads=1), dict(heads=129, qs=129 * 64, outs=129 * 64)),
-                                       (dict(page_size=8), {}), (dict(n_pages=41), {}), ({}, dict(layer=2)), ({}, dict(window=-1)), ({}, dict(scale=-1.0)),
+                                       (dict(page_size=8), {}), (dict(n_pages=41), {}), (dict(n_layers=1 << 25), {}), ({}, dict(layer=2)), ({}, dict(window=-1)), ({}, dict(scale=-1.0)),
                                        ({}, dict(scale=math.nan)), ({}, dict(scale=math.inf)), ({}, dict(qs=255)), ({}, dict(qs=260)), ({}, dict(outs=260)), ({}, dict(q=P + 8)),
                                        ({}, dict(out=P + 2)), ({}, dict(q=0)), ({}, dict(out=0)), ({}, dict(b=dict(q_start=0))), ({}, dict(b=dict(kv_len=0))),
-                                       ({}, dict(b=dict(block_table=0))), ({}, dict(b=dict(work=P + 4))), ({}, dict(b=dict(slots=0, max_seqs=2))), ({}, dict(b=dict(n_req=9000)))])
+                                       ({}, dict(b=dict(block_table=0))), ({}, dict(b=dict(work=P + 4))), ({}, dict(b=dict(max_tokens=1 << 24))), ({}, dict(b=dict(slots=0, max_seqs=2))), ({}, dict(b=dict(n_req=9000)))])
 def test_attention(view, over):
     a = dict(layer=0, q=P, qs=256, out=P, outs=256, heads=4, window=0, scale=0.0, b={})
     a.update(over)

@@ -430,6 +430,65 @@ def test_attention_nonsense_stays_inside(L):
     r.check(out)
 
 
+@pytest.mark.parametrize("ps", [16, 4])
+def test_offsets_beyond_32_bits(L, ps):
+    """a pool of more than 2^31 elements: store and attention at its end"""
+    pages = (2 ** 31 // (2 * ps * 128)) + 300
+    pool = torch.empty(pages, 1, 2, 1, ps, 128, dtype=torch.bfloat16, device="cuda")
+    n, g = 200, 4
+    mine = torch.arange(pages - 1, pages - 1 - (n + ps - 1) // ps, -1, dtype=torch.int32, device="cuda")
+    pos = torch.arange(n, dtype=torch.int32, device="cuda")
+    row = mine[(pos // ps).long()] * ps + pos % ps
+    qkv = rand(1, n, (g + 2) * 128).bfloat16()
+    q, k, v = qkv.split([g * 128, 128, 128], 1)
+    q_out, out, freq = torch.empty_like(q.contiguous()), torch.empty_like(q.contiguous()), torch.from_numpy(L.Rope.frequencies(128)[0]).cuda()
+    kv = L.KvPool.over(pool)
+    L.launch_rope_store(q, k, v, q_out, kv, 0, pos, row, L.Rope(freq), g)
+    batch = L.Batch(mine[None].contiguous(), ps, pages, 1, n, q_start=i32([0, n]), kv_len=i32([n]))
+    L.launch_attn_batch(q_out, out, kv, 0, batch, g)
+    turned = ref.rope(qkv.view(n, g + 2, 128), pos.long(), freq, 1.0, False)
+    near(q_out.view(n, g, 128), turned[:, :g], 2 * qkv.double().abs().max())
+    stored = pool[:, 0, 0, 0][mine.long()].reshape(-1, 128)[:n]
+    assert torch.equal(pool[:, 0, 1, 0][mine.long()].reshape(-1, 128)[:n], v)
+    want, size = ref.attention(q_out.view(n, g, 128), stored[:, None], v[:, None], 0)
+    assert ((out.view(n, g, 128).double() - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -9) * size).all()
+
+
+def test_attention_refuses_a_small_work_area(L):
+    from qwen_inference_engine_b200._lib import QieError
+    r = Requests(L, [(10, 1)], 2, 1, 64, 16)
+    r.batch.reserve(r.kv, 2)
+    n, r.batch.view.work_bytes = r.batch.view.work_bytes, r.batch.view.work_bytes - 1
+    with pytest.raises(QieError) as e:
+        L.launch_attn_batch(r.q, torch.empty_like(r.q), r.kv, r.layer, r.batch, 2)
+    assert e.value.code == -1 and "work area" in str(e.value)
+    r.batch.view.work_bytes = n
+    out = torch.empty_like(r.q)
+    L.launch_attn_batch(r.q, out, r.kv, r.layer, r.batch, 2)
+    r.check(out)
+
+
+def test_python_forms_refuse(L):
+    """types, shapes, strides and devices that the Python forms turn away"""
+    x, pos, freq = rand(1, 4, 128).bfloat16(), i32([0, 1, 2, 3]), torch.ones(32, dtype=torch.float64, device="cuda")
+    rope, pool = L.Rope(freq), L.KvPool.over(torch.zeros(3, 1, 2, 1, 16, 64, dtype=torch.bfloat16, device="cuda"))
+    table, k = i32([[0, 1, 2]]), rand(2, 4, 64).bfloat16()
+    batch = L.Batch(table, 16, 3, 1, 4, q_start=i32([0, 4]), kv_len=i32([4]))
+    for call in (lambda: L.launch_rope_rows(x.float(), x.float(), pos, rope, 2, 64), lambda: L.launch_rope_rows(x, x, pos[:3], rope, 2, 64),
+                 lambda: L.launch_rope_rows(x, x, pos, rope, 3, 64), lambda: L.launch_rope_rows(x.T.contiguous().T, x, pos, rope, 2, 64),
+                 lambda: L.launch_rope_rows(x.cpu(), x.cpu(), pos, rope, 2, 64), lambda: L.launch_rope_rows(x, x, pos.long(), rope, 2, 64),
+                 lambda: L.launch_rope_store(x, k, k[:3], x, pool, 0, pos, pos, rope, 2), lambda: L.launch_rope_store(x, k, k.cpu(), x, pool, 0, pos, pos, rope, 2),
+                 lambda: L.launch_rope_store(x, k, k, x, pool, 0, pos, pos.cpu(), rope, 2), lambda: L.launch_rope_store(x, x, k, x, pool, 0, pos, pos, rope, 2),
+                 lambda: L.launch_attn_batch(x[:3], x[:3].clone(), pool, 0, batch, 2), lambda: L.launch_attn_batch(x, x.float(), pool, 0, batch, 2),
+                 lambda: L.launch_attn_batch(x, x.cpu(), pool, 0, batch, 2), lambda: L.Rope(freq.float()), lambda: L.Batch(table.long(), 16, 3, 1, 4),
+                 lambda: L.Batch(table, 16, 3, 2, 4, kv_len=i32([1])), lambda: L.Batch(table, 16, 3, 1, 4, cached=i32([1]).cpu()), lambda: L.KvPool.over(k),
+                 lambda: L.launch_logits(x, x.float(), L.LogitRules()), lambda: L.launch_logits(x.half(), x.half(), L.LogitRules()),
+                 lambda: L.launch_logits(x, x, L.LogitRules(i32([0, 0]), pos)), lambda: L.LogitRules(i32([0, 1]).long(), pos), lambda: L.LogitRules(bias_start=i32([0, 1]), bias=freq.float()),
+                 lambda: L.LogitRules(mask=pos)):
+        with pytest.raises((AssertionError, ValueError)):
+            call()
+
+
 # ---------------------------------------------------------------- logits
 def ragged(rs, rows, most, vocab, wild=True):
     lens = rs.integers(0, most + 1, rows)
