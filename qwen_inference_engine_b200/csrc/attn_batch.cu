@@ -17,8 +17,8 @@
 //                positions, 16-byte copies to the same places.
 // Values of keys that some row of a tile does not see must not meet its zero weight when they are no numbers: tiles at the edges of what rows see are
 // looked over, such values are put aside, and rows that see them get them at the end.
-// What bounds it (B200).  Prompts: keys and values out of L2, 32 KB for 128 rows x 64 keys, 7.7 TB/s: 8192 rows of 28 heads of 128 on 4 take 500 us, 960 TFLOP/s (the
-// same without exponentials; one CTA an SM 940).  Decode rows: DRAM, 6.2 TB/s between the first tiles and the last: 64 rows at 1434 positions on average, 189 MB, take 43.6 us, of
+// What bounds it (B200).  Prompts: the chain of a tile (scores, softmax, product), of which an SM has two under way: tensor pipe 52 % busy, exponentials 53 %, issue 40 %, L2
+// 34 %; 8192 rows of 28 heads of 128 on 4 take 500 us, 960 TFLOP/s (without exponentials 486, with half of the keys' and values' bytes 447, one CTA an SM 940).  Decode rows: DRAM, 6.2 TB/s between the first tiles and the last: 64 rows at 1434 positions on average, 189 MB, take 41.8 us, of
 // which 7 us pass before the first scores and 6 behind the last tile.  One row behind 700 positions: 9.3 us, a chain of latencies (plan 1.3, pages and keys 2.4, a tile 0.8, its
 // product and results 1.2, the start of the second kernel 1.2, joining 2.0).
 // Every wait has a limit; when one runs out the CTA's results are not numbers and it reports it.
@@ -38,19 +38,23 @@ namespace qie {
 namespace {
 
 constexpr int TQ = AB_TQ, TK = AB_TK;
-constexpr int QBLK = TQ * 128, KBLK = TK * 128;  // [rows][64 columns] bf16 in 8-row swizzle atoms
+constexpr int KBLK = TK * 128;  // [rows][64 columns] bf16 in 8-row swizzle atoms
 constexpr int NSOFT = 128, NTHR = NSOFT + 64;
 constexpr uint32_t TMEM_COLS = 256;  // two tiles of scores, O
 // The weights' reference follows a row's maximum where it has fallen behind by more than this (powers of two): most tiles then leave O as it is, 7 % of a long prompt's
 // time.  Weights are as exact as before, 2^-8 of themselves, but the largest one is rounded too; sums are fp32.
 constexpr float LAG = 8.f;
-constexpr int EDGES = 6;             // tiles of an item at the edges of what its rows see: tokens span at most 128 positions, so three at either end
 
-template <int HD>
+// FEW: blocks of at most 16 rows (decode rows).  The products read 128 all the same, what lies behind their queries, and nobody looks at what comes of it; the room that the other
+// queries would take is a third stage of keys and values (head size 64: a fifth and sixth): 64 rows at 2048 43.6 us, so 41.8.
+template <int HD, bool FEW>
 struct Smem {
-  static constexpr int NB = HD / 64, ST = HD == 64 ? 4 : 2;  // column blocks; stages of K and of V
+  static constexpr int ROWS = FEW ? 16 : TQ, QBLK = ROWS * 128;
+  // tiles of an item at the edges of what its rows see: tokens span at most 128 positions, so three at either end (16: two)
+  static constexpr int EDGES = FEW ? 4 : 6;
+  static constexpr int NB = HD / 64, ST = HD == 64 ? (FEW ? 6 : 4) : (FEW ? 3 : 2);  // column blocks; stages of K and of V
   static constexpr int TILE = NB * KBLK;
-  static constexpr int Q = 0, K = NB * QBLK, V = K + ST * TILE, ODD = V + ST * TILE, BAR = ODD + EDGES * HD * 16, END = BAR + 256 + 1024;
+  static constexpr int Q = 0, K = NB * QBLK, V = K + ST * TILE, ODD = V + ST * TILE, BAR = ODD + EDGES * HD * 16, END = BAR + 512 + 1024;
   // (three CTAs an SM would wait for TMEM columns: see attn_prompt_tc.cu)
   static constexpr int TOTAL = END > 76 * 1024 ? END : 76 * 1024;
   static_assert(512 / TMEM_COLS == 2 && 3 * (TOTAL + 1024) > 228 * 1024 && 2 * (TOTAL + 2048) <= 228 * 1024, "two CTAs an SM");
@@ -127,10 +131,10 @@ __device__ __forceinline__ long long block_scan(long long v, long long* warp_sum
 // a / b of numbers that are not below 0, mostly of 32 bits
 __device__ __forceinline__ long long quotient(long long a, long long b) { return (a | b) >> 32 ? a / b : (long long)((unsigned)a / (unsigned)b); }
 
-template <int HD, bool TMA>
+template <int HD, bool TMA, bool FEW>
 __global__ void __launch_bounds__(NTHR, 2) attn_batch_kernel(BatchAttnArgs a, Shape sh, int box, const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap kvm) {
-  using SM = Smem<HD>;
-  constexpr int NB = SM::NB, ST = SM::ST;
+  using SM = Smem<HD, FEW>;
+  constexpr int NB = SM::NB, ST = SM::ST, QBLK = SM::QBLK, EDGES = SM::EDGES;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   __shared__ long long s_sums[NTHR / 32];
   __shared__ Walk s_walk;
@@ -624,16 +628,16 @@ __global__ void __launch_bounds__(JOIN_THR, 2) attn_batch_join_kernel(BatchAttnA
   }
 }
 
-template <int HD, bool TMA>
-cudaError_t launch_hd(const BatchAttnArgs& a, const TensorMap2D& qm, const TensorMap2D& kvm, int box, cudaStream_t st) {
+template <int HD, bool TMA, bool FEW>
+cudaError_t launch_hd(const BatchAttnArgs& a, int tt, const TensorMap2D& qm, const TensorMap2D& kvm, int box, cudaStream_t st) {
   static PerDeviceOnce set;
   if (set.need()) {
-    const cudaError_t e = cudaFuncSetAttribute(attn_batch_kernel<HD, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<HD>::TOTAL);
+    const cudaError_t e = cudaFuncSetAttribute(attn_batch_kernel<HD, TMA, FEW>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<HD, FEW>::TOTAL);
     if (e != cudaSuccess) return e;
     set.done();
   }
   const int G = a.n_q / a.kv.n_kv, ctas = 2 * a.num_sms;
-  const cudaError_t e = launched(launch_k(attn_batch_kernel<HD, TMA>, dim3(ctas), dim3(NTHR), Smem<HD>::TOTAL, st, a, Shape{G, TQ / G, (int)(reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && a.out_stride % 16 == 0)}, box,
+  const cudaError_t e = launched(launch_k(attn_batch_kernel<HD, TMA, FEW>, dim3(ctas), dim3(NTHR), Smem<HD, FEW>::TOTAL, st, a, Shape{G, tt, (int)(reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && a.out_stride % 16 == 0)}, box,
                                           *reinterpret_cast<const CUtensorMap*>(&qm), *reinterpret_cast<const CUtensorMap*>(&kvm)));
   if (e != cudaSuccess) return e;
   return launched(launch_k(attn_batch_join_kernel<HD>, dim3(ctas, HD / 64), dim3(JOIN_THR), 0, st, a, G, ctas));
@@ -645,15 +649,20 @@ size_t attention_batch_work(int hd, int num_sms) { return (size_t)2 * num_sms * 
 
 cudaError_t launch_attention_batch(const BatchAttnArgs& a, cudaStream_t st) {
   const int G = a.n_q / a.kv.n_kv, P = a.kv.page_size;
-  TensorMap2D qm, kvm{};
-  cudaError_t e = make_tensor_map_heads(&qm, a.q, a.kv.hd, a.n_q, a.n_tok, a.q_stride, G, TQ / G);
-  if (e != cudaSuccess) return e;
   const unsigned long long rows = (unsigned long long)a.kv.n_pages * a.kv.n_layers * 2ull * a.kv.n_kv * P;
   const bool tma = P % 16 == 0;
+  // No more rows than requests: a decode step, or nearly one (a request with several rows has blocks of fewer of them, and reads its keys and values that much more often).
+  // Else blocks of as many rows as the products take: one portion of 8192 rows of 7 heads a group has 456 blocks instead of 4096.
+  const bool few = tma && G <= 16 && a.n_tok <= a.n_req;
+  const int tt = (few ? 16 : TQ) / G;
+  TensorMap2D qm, kvm{};
+  cudaError_t e = make_tensor_map_heads(&qm, a.q, a.kv.hd, a.n_q, a.n_tok, a.q_stride, G, tt);
+  if (e != cudaSuccess) return e;
   const int box = !tma ? TK : P % 64 == 0 ? 64 : P % 32 == 0 ? 32 : 16;  // the largest that divides a page and a tile
   if (tma && (e = make_tensor_map_kv(&kvm, a.kv.pool, rows, a.kv.hd, box)) != cudaSuccess) return e;
-  if (a.kv.hd == 64) return tma ? launch_hd<64, true>(a, qm, kvm, box, st) : launch_hd<64, false>(a, qm, kvm, box, st);
-  return tma ? launch_hd<128, true>(a, qm, kvm, box, st) : launch_hd<128, false>(a, qm, kvm, box, st);
+  if (a.kv.hd == 64)
+    return few ? launch_hd<64, true, true>(a, tt, qm, kvm, box, st) : tma ? launch_hd<64, true, false>(a, tt, qm, kvm, box, st) : launch_hd<64, false, false>(a, tt, qm, kvm, box, st);
+  return few ? launch_hd<128, true, true>(a, tt, qm, kvm, box, st) : tma ? launch_hd<128, true, false>(a, tt, qm, kvm, box, st) : launch_hd<128, false, false>(a, tt, qm, kvm, box, st);
 }
 
 }  // namespace qie

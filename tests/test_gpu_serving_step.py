@@ -294,6 +294,15 @@ def test_attention(L, nq, nkv, hd, lens):
     attend(L, lens, nq, nkv, hd, 16, extra=3, seed=len(lens))
 
 
+@pytest.mark.parametrize("nq,nkv,hd", HEADS + [(16, 1, 128), (17, 1, 64), (16, 16, 64), (5, 1, 128), (9, 3, 128)])
+@pytest.mark.parametrize("window", [0, 70])
+@pytest.mark.parametrize("lens", [[(i * 97 % 1500, 1) for i in range(64)], [(0, 1)] * 3, [(500, 1), (77, 0), (0, 1), (64, 0), (63, 1)], [(300, 5), (10, 0), (9, 0), (8, 0), (6, 0)],
+                                  [(4000, 3), (100, 0), (200, 0), (1, 1)], [(20000, 1)]])
+def test_attention_no_more_rows_than_requests(L, nq, nkv, hd, window, lens):
+    """decode steps, and steps with a few more rows for some requests and none for others"""
+    attend(L, lens, nq, nkv, hd, 16, window=window, seed=len(lens) + nq)
+
+
 @pytest.mark.parametrize("ps", [1, 2, 3, 4, 5, 8, 16, 24, 32, 48, 64, 100, 128, 256])
 @pytest.mark.parametrize("nq,nkv,hd", [(14, 2, 64), (4, 1, 128)])
 def test_attention_page_sizes(L, ps, nq, nkv, hd):
