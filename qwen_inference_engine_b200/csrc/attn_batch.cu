@@ -450,6 +450,7 @@ __global__ void __launch_bounds__(NTHR, 2) attn_batch_kernel(BatchAttnArgs a, Sh
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           ++edge;
+          __syncwarp();  // (the loop above ends per thread, and what follows wants the warp's threads together)
         }
         wait_st();
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -482,8 +483,7 @@ __global__ void __launch_bounds__(NTHR, 2) attn_batch_kernel(BatchAttnArgs a, Sh
                 if (bits[1] & sees) r[j] = __float_as_uint(__uint_as_float(r[j]) - INFINITY);
               }
             }
-          if (tok >= p.tokens) continue;
-          if (whole) {
+          if (tok < p.tokens && whole) {
 #pragma unroll
             for (int j = 0; j < 32; j += 16) {
               uint32_t w[8];
@@ -497,10 +497,11 @@ __global__ void __launch_bounds__(NTHR, 2) attn_batch_kernel(BatchAttnArgs a, Sh
                 *reinterpret_cast<uint4*>(dst + c + j + 8) = make_uint4(w[4], w[5], w[6], w[7]);
               }
             }
-          } else {
+          } else if (tok < p.tokens) {
 #pragma unroll
             for (int j = 0; j < 32; j += 4) *reinterpret_cast<uint4*>(part + ((c + j) / 4 * TQ + row) * 4) = make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
           }
+          __syncwarp();
         }
       }
       if (tid == 0 && !whole && p.begin == 0)  // goes on in the CTAs behind; the item's last tile is at x1 - left + tiles - 1
