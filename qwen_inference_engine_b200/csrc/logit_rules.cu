@@ -119,15 +119,16 @@ __global__ void __launch_bounds__(THR) logit_rules_kernel(LogitArgs a, int share
     }
     cp_async_commit();
   };
-  if (copy) read();
+  // (numbers that lists and masks hang on, ahead of the copies)
+  const int2 ts = a.tok_start ? span(a.tok_start, row, a.n_tokens) : make_int2(0, 0), bs = a.bias_start ? span(a.bias_start, row, a.n_bias) : make_int2(0, 0);
+  const int gen = (a.gen_start && a.tok_start ? a.gen_start[row] : ts.x) - ts.x;
+  const float rep = a.repetition ? a.repetition[row] : 1.f, pres = a.presence ? a.presence[row] : 0.f, freq = a.frequency ? a.frequency[row] : 0.f;
   const int m = a.mask ? (a.mask_row ? a.mask_row[row] : row) : -1;
+  if (copy) read();
   const uint32_t* mask = m >= 0 && m < a.n_masks ? a.mask + (size_t)m * a.mask_words : nullptr;
   const bool staged = copy || mask;
   if (!copy && mask) read();
   // ---- the lists
-  const int2 ts = a.tok_start ? span(a.tok_start, row, a.n_tokens) : make_int2(0, 0), bs = a.bias_start ? span(a.bias_start, row, a.n_bias) : make_int2(0, 0);
-  const int gen = (a.gen_start && a.tok_start ? a.gen_start[row] : ts.x) - ts.x;
-  const float rep = a.repetition ? a.repetition[row] : 1.f, pres = a.presence ? a.presence[row] : 0.f, freq = a.frequency ? a.frequency[row] : 0.f;
   constexpr int UT = 8, UB = 1;
   auto collect = [&](auto&& ready) {  // `ready` between the loads and their use
     Next<UT> t(a.tokens, ts, tid);
