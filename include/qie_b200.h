@@ -170,7 +170,7 @@ int qie_attention_prefill_tc(const qie_kv_view* kv, int layer, const qie_bf16* Q
  * here; what they say is then not defined, except where a function's comment does. */
 typedef struct {
   int n_req;              /* requests of the step, 0 .. QIE_BATCH_MAX_REQ */
-  int max_tokens;         /* rows of pos / slot / row; qie_attention_batch: rows of Q and out, less than 2^24 */
+  int max_tokens;         /* rows of pos / slot / row, at most 2^30; qie_attention_batch: rows of Q and out, less than 2^24 */
   int max_seqs, max_pages; /* block_table[max_seqs][max_pages] */
   int n_pages, page_size;  /* of the pool; n_pages * page_size < 2^31, max_pages * page_size <= 2^30 */
   const int* cached;      /* [n_req] positions of the request that are in the cache */

@@ -419,6 +419,7 @@ int qie_batch_layout(const qie_batch* b, qie_stream st) {
   static_assert(BATCH_MAX_REQ == QIE_BATCH_MAX_REQ, "one limit");
   if (!batch_sizes_ok(b) || b->n_pages <= 0 || (long long)b->n_pages * b->page_size >= (1ll << 31))
     return fail(QIE_EINVAL, "batch_layout: need 0 to %d requests, and n_pages and max_pages above 0 with less than 2^31 and at most 2^30 positions", QIE_BATCH_MAX_REQ);
+  if (b->max_tokens > 1 << 30) return fail(QIE_EINVAL, "batch_layout: at most 2^30 rows");  // (a thread's next row is an int)
   if (!b->free_ring || !b->ring_in || !b->ring_out || !b->q_start || !b->status || (b->n_req && (!b->cached || !b->n_new || !b->block_table || !b->kv_len)) ||
       (b->max_tokens && (!b->pos || !b->slot || !b->row)))
     return fail(QIE_EINVAL, "batch_layout: an array is missing");
