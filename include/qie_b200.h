@@ -247,7 +247,7 @@ typedef struct {
   const float* bias;
   const uint32_t* mask;
   const int* mask_row;
-  int n_tokens, n_bias;       /* elements of tokens and of bias_ids / bias */
+  int n_tokens, n_bias;       /* elements of tokens (less than 2^29) and of bias_ids / bias (at most 2^30) */
   int mask_words, n_masks;    /* mask[n_masks][mask_words] */
 } qie_logit_rules;
 /* dtype: QIE_DTYPE_BF16 or QIE_DTYPE_F32.  out may be logits. */

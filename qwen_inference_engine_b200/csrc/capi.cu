@@ -545,7 +545,8 @@ int qie_logits_process(const void* logits, size_t stride, void* out, size_t out_
   if (n_rows > 1 && logits == out && stride != out_stride) return fail(QIE_EINVAL, "logits_process: in place with rows at other places");
   if (!aligned(dtype == QIE_DTYPE_F32 ? 4 : 2, {logits, out})) return fail(QIE_EINVAL, "logits_process: logits off their type's boundary");
   const qie_logit_rules& r = *rules;
-  if (r.n_tokens < 0 || r.n_bias < 0 || r.n_tokens > 1 << 30 || r.n_bias > 1 << 30 || (r.gen_start && !r.tok_start) || (r.tok_start && !r.tokens && r.n_tokens) ||
+  if (r.n_tokens >= 1 << 29 || r.n_bias > 1 << 30) return fail(QIE_EINVAL, "logits_process: lists of less than 2^29 tokens and at most 2^30 biases");  // (a token is counted in 29 bits)
+  if (r.n_tokens < 0 || r.n_bias < 0 || (r.gen_start && !r.tok_start) || (r.tok_start && !r.tokens && r.n_tokens) ||
       (r.bias_start && r.n_bias && (!r.bias_ids || !r.bias)) || ((r.repetition || r.presence || r.frequency) && !r.tok_start) || (r.bias && !r.bias_start))
     return fail(QIE_EINVAL, "logits_process: a rule without its lists");
   if (r.mask && (r.n_masks < 0 || (long long)r.mask_words * 32 < vocab)) return fail(QIE_EINVAL, "logits_process: masks of %d words for %d tokens", r.mask_words, vocab);
