@@ -214,7 +214,8 @@ typedef struct {
 #define QIE_ROPE_PARTS 4   /* by the turns over `original` positions: more than b (4) kept, fewer than a (1) / scale, a ramp over the turns between */
 /* HOST only: h_freq[rotated / 2] and *h_factor.  scale >= 1; a, b: 0 for the numbers in brackets. */
 int qie_rope_frequencies(double* h_freq, float* h_factor, int rotated, double base, int kind, double scale, int original, double a, double b);
-/* x [n_tok, n_heads * head_dim] -> out, rows `stride` elements apart (may be the same array); rows whose pos is below 0 are left as they are. */
+/* x [n_tok, n_heads * head_dim] -> out, rows `stride` elements apart (may be the same array); rows whose pos is below 0 are left as they are.  At most
+ * 2^24 elements of a token (q, k and v together below). */
 int qie_rope_rows(const qie_bf16* x, size_t x_stride, qie_bf16* out, size_t out_stride, const qie_rope_plan* rope, const int* pos, int n_tok,
                   int n_heads, int head_dim, qie_stream st);
 /* The same for q, and in the same launch k (rotated) and v into the cache rows row[t] of `layer`; q, k and v are rows `stride` apart, so they may be

@@ -464,11 +464,13 @@ int qie_rope_frequencies(double* h_freq, float* h_factor, int rotated, double ba
   }
   return QIE_OK;
 }
+static constexpr long long ROPE_ROW = 1 << 24;  // elements of a token's heads: places are ints, 512 of them at least a CTA of the grid's second dimension
 static bool rope_ok(const qie_rope_plan* r, int head_dim) { return r && r->freq && r->rotated >= 2 && !(r->rotated & 1) && r->rotated <= head_dim && head_dim <= 1024; }
 int qie_rope_rows(const qie_bf16* x, size_t x_stride, qie_bf16* out, size_t out_stride, const qie_rope_plan* rope, const int* pos, int n_tok, int n_heads,
                   int head_dim, qie_stream st) {
   if (!rope_ok(rope, head_dim)) return fail(QIE_EINVAL, "rope_rows: need an even number of rotated elements, at most head_dim, and head_dim up to 1024");
   if (n_tok < 0 || n_tok > 1 << 30 || n_heads < 0 || (n_tok && n_heads && (!x || !out || !pos))) return fail(QIE_EINVAL, "rope_rows: bad argument (at most 2^30 rows)");
+  if ((long long)n_heads * head_dim > ROPE_ROW) return fail(QIE_EINVAL, "rope_rows: at most 2^24 elements a row");
   const size_t wide = (size_t)n_heads * head_dim;
   if (n_tok > 1 && (x_stride < wide || out_stride < wide)) return fail(QIE_EINVAL, "rope_rows: rows of %zu elements overlap", wide);
   if (n_tok > 1 && x == out && x_stride != out_stride) return fail(QIE_EINVAL, "rope_rows: in place with rows at other places");
@@ -488,6 +490,7 @@ int qie_rope_store(const qie_kv_view* kv, int layer, const qie_bf16* q, size_t q
     return fail(QIE_EINVAL, "rope_store: bad pool or layer");
   if (!rope_ok(rope, kv->head_dim)) return fail(QIE_EINVAL, "rope_store: need an even number of rotated elements, at most head_dim, and head_dim up to 1024");
   if (n_tok < 0 || n_tok > 1 << 30 || n_q_heads < 0 || (n_tok && (!k || !v || !pos || !row || (n_q_heads && (!q || !q_out))))) return fail(QIE_EINVAL, "rope_store: bad argument (at most 2^30 rows)");
+  if (((long long)n_q_heads + 2ll * kv->n_kv_heads) * kv->head_dim > ROPE_ROW) return fail(QIE_EINVAL, "rope_store: at most 2^24 elements of a token's q, k and v");
   const size_t wide = (size_t)n_q_heads * kv->head_dim, kv_wide = (size_t)kv->n_kv_heads * kv->head_dim;
   if (n_tok > 1 && (k_stride < kv_wide || v_stride < kv_wide || (n_q_heads && (q_stride < wide || q_out_stride < wide))))
     return fail(QIE_EINVAL, "rope_store: rows overlap");
