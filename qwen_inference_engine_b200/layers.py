@@ -228,7 +228,7 @@ class Rope:
     def __init__(self, freq, factor=1.0, neighbours=False):
         assert freq.dtype == torch.float64 and freq.dim() == 1
         _here(freq)
-        self.freq = freq
+        self.freq, self.device = freq, freq.get_device()
         self.plan = RopePlan(_p(freq), 2 * freq.numel(), int(neighbours), float(factor))
         self.ref = C.byref(self.plan)
 
@@ -244,6 +244,7 @@ def launch_rope_rows(x, out, pos, rope, n_heads, head_dim):
     """rows [n_tok, n_heads * head_dim] -> out (may be x), token t at position pos[t]"""
     n, wide = x.shape
     assert x.dtype is out.dtype is torch.bfloat16 and x.shape == out.shape and wide == n_heads * head_dim, "bfloat16 rows of n_heads * head_dim expected"
+    assert x.get_device() == out.get_device() == pos.get_device() == rope.device, "rows, positions and frequencies on one device expected"
     _here(x)
     check(_lib.lib().qie_rope_rows(*_rows(x), *_rows(out), rope.ref, _ints(pos, n, "pos"), n, n_heads, head_dim, _st()))
 
@@ -255,7 +256,8 @@ def launch_rope_store(q, k, v, q_out, pool, layer, pos, row, rope, n_q_heads):
     assert q.dtype is k.dtype is v.dtype is q_out.dtype is torch.bfloat16, "bfloat16 rows expected"
     assert n == nk == nv == no and wide == ow == n_q_heads * pool.head_dim and kw == vw == pool.kv_wide, "rows of the heads of as many tokens expected"
     assert (q1 == o1 == 1 or wide <= 1) and (k1 == v1 == 1 or kw <= 1), "rows of contiguous elements expected"
-    assert q.get_device() == k.get_device() == v.get_device() == q_out.get_device() == pool.pool.get_device(), "rows and pool on one device expected"
+    assert q.get_device() == k.get_device() == v.get_device() == q_out.get_device() == pool.pool.get_device() == pos.get_device() == row.get_device() == rope.device, \
+        "rows, pool, positions and frequencies on one device expected"
     _here(q)
     if n == 1:
         qs, os, ks, vs = wide, wide, kw, kw
@@ -280,12 +282,13 @@ class LogitRules:
                  mask=None, mask_row=None):
         self.held = dict(tok_start=tok_start, tokens=tokens, gen_start=gen_start, repetition=repetition, presence=presence, frequency=frequency,
                          bias_start=bias_start, bias_ids=bias_ids, bias=bias, mask=mask, mask_row=mask_row)
-        self.n_rows = None  # rows that every list has
+        self.n_rows = self.device = None  # rows that every list has, and where they are
         for name, t in self.held.items():
             if t is None:
                 continue
             assert t.dtype == (torch.float32 if name in ("repetition", "presence", "frequency", "bias") else torch.int32), f"{name}: {t.dtype}"
             _here(t)
+            self.device = t.get_device()
             n = {"tokens": None, "bias_ids": None, "bias": None, "tok_start": t.numel() - 1, "bias_start": t.numel() - 1,
                  "mask": t.shape[0] if mask_row is None else None}.get(name, t.numel())
             if n is not None:
@@ -303,5 +306,6 @@ def launch_logits(logits, out, rules):
     (n, vocab), kind = logits.shape, logits.dtype
     assert kind is out.dtype and out.shape == logits.shape and (kind is torch.bfloat16 or kind is torch.float32), "bfloat16 or float32 logits, and out like them"
     assert rules.n_rows is None or rules.n_rows >= n, "rules for fewer rows"
+    assert logits.get_device() == out.get_device() and (rules.device is None or rules.device == logits.get_device()), "logits and rules on one device expected"
     _here(logits)
     check(_lib.lib().qie_logits_process(*_rows(logits), *_rows(out), int(kind is torch.float32), n, vocab, rules.ref, _st()))
