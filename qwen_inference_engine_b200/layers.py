@@ -197,7 +197,7 @@ class Batch:
         self.block_table, self.slots, self.cached, self.n_new, self.free_ring, self.ring_in = block_table, slots, cached, n_new, free_ring, ring_in
         self.ring_out, self.q_start, self.kv_len, self.status = ints(ring_out, 2), ints(q_start, n_req + 1), ints(kv_len, n_req), ints(status, 2)
         self.pos, self.slot, self.row = ints(pos, max_tokens), ints(slot, max_tokens), ints(row, max_tokens)
-        self.work, self.max_tokens = None, max_tokens
+        self.work, self.heads, self.replaced, self.max_tokens = None, 0, [], max_tokens
         b = self.view = BatchView(n_req=n_req, max_tokens=max_tokens, max_seqs=block_table.shape[0], max_pages=block_table.shape[1], n_pages=n_pages,
                                   page_size=page_size)
         for name, n in (("block_table", 0), ("slots", n_req), ("cached", n_req), ("n_new", n_req), ("free_ring", n_pages), ("ring_in", 2), ("ring_out", 2),
@@ -209,11 +209,16 @@ class Batch:
         self.ref = C.byref(b)
 
     def reserve(self, pool, n_q_heads):
-        """the work area of launch_attn_batch; one call at a time uses it"""
+        """the work area of launch_attn_batch; one call at a time uses it.  A smaller one from before is kept beside it: captured graphs and launches under way may
+        have it."""
         n = _lib.lib().qie_attention_batch_work(C.byref(pool.view), n_q_heads)
+        if n == 0:  # a geometry that the operator refuses
+            return
         if self.work is None or self.work.numel() < n:
+            self.replaced.append(self.work)
             self.work = torch.empty(n, dtype=torch.uint8, device=self.block_table.device)
             self.view.work, self.view.work_bytes = self.work.data_ptr(), n
+        self.heads = max(self.heads, pool.head_dim)  # the area's size hangs on the head size alone
 
 
 def launch_batch_layout(batch):
@@ -268,7 +273,7 @@ def launch_rope_store(q, k, v, q_out, pool, layer, pos, row, rope, n_q_heads):
 def launch_attn_batch(Q, out, pool, layer, batch, n_q_heads, window=0, scale=0.0):
     """attention of the batch's rows over the pool, ragged over its requests (fast numerics)"""
     assert Q.dtype is out.dtype is torch.bfloat16 and Q.shape == out.shape == (batch.max_tokens, n_q_heads * pool.head_dim), "bfloat16 rows of the batch expected"
-    if batch.work is None:
+    if batch.heads < pool.head_dim:
         batch.reserve(pool, n_q_heads)
     assert Q.get_device() == out.get_device() == pool.pool.get_device() == batch.block_table.get_device(), "rows, pool and batch on one device expected"
     _here(Q)

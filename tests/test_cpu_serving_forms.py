@@ -95,3 +95,64 @@ def test_every_tensor_is_of_the_current_device(L, form, name):
 def test_rules_of_nothing_have_no_device(L):
     L.launch_logits(Told(3, 100), Told(3, 100), L.LogitRules())
     assert L.calls == ["qie_logits_process"]
+
+
+def batch_of(L, pages=3):
+    return L.Batch(Told(1, pages, dtype=i32), 16, pages, 1, 4, **{n: Told(5, dtype=i32) for n in ("ring_out", "q_start", "kv_len", "pos", "slot", "row", "status")})
+
+
+@pytest.fixture
+def areas(L, monkeypatch):
+    """work areas in bytes: heads of 64 take 1000, of 128 2000; a call of attention with less than its heads take is refused as by the library"""
+    import weakref
+    made = []
+
+    def empty(n, dtype, device):
+        t = Told(n, dtype=dtype)
+        made.append(weakref.ref(t))
+        return t
+
+    need = {64: 1000, 128: 2000}
+
+    class Lib:
+        def qie_attention_batch_work(self, view, n_q):
+            return need.get(view._obj.head_dim, 0)
+
+        def qie_attention_batch(self, view, layer, batch, *rest):
+            L.calls.append((view._obj.head_dim, batch._obj.work_bytes))
+            return 0
+
+    monkeypatch.setattr(torch, "empty", empty)
+    monkeypatch.setattr(L._lib, "lib", Lib)
+    return made
+
+
+def attend(L, batch, hd):
+    L.launch_attn_batch(Told(4, 2 * hd), Told(4, 2 * hd), L.KvPool.over(Told(3, 1, 2, 1, 16, hd)), 0, batch, 2)
+
+
+def test_work_area_grows_with_the_heads(L, areas):
+    """one batch over pools of both head sizes; an area that a captured graph may have is kept"""
+    batch = batch_of(L)
+    for hd in (64, 64, 128, 64, 128):
+        attend(L, batch, hd)
+    assert L.calls == [(64, 1000), (64, 1000), (128, 2000), (64, 2000), (128, 2000)]
+    assert len(areas) == 2 and all(a() is not None for a in areas)
+
+
+def test_reserved_work_area_is_taken(L, areas):
+    batch = batch_of(L)
+    for hd in (128, 64):
+        batch.reserve(L.KvPool.over(Told(3, 1, 2, 1, 16, hd)), 2)
+    attend(L, batch, 128)
+    batch.view.work_bytes -= 1  # the caller's word stands, and the library refuses it
+    attend(L, batch, 128)
+    assert L.calls == [(128, 2000), (128, 1999)] and len(areas) == 1
+
+
+def test_heads_without_a_work_area(L, areas):
+    """heads that the operator does not take get none, and the library says so; the batch serves others all the same"""
+    batch = batch_of(L)
+    attend(L, batch, 96)
+    attend(L, batch, 64)
+    assert L.calls == [(96, 0), (64, 1000)]
