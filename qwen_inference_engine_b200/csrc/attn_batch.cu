@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(NTHR, 2) attn_batch_kernel(BatchAttnArgs a, Sh
       for (int i = p.begin; i < p.end; ++i, ++T) {
         const uint32_t b = 8u * (uint32_t)(T & 1), ph = (uint32_t)((T >> 1) & 1), ts = tmem + la + (uint32_t)((T & 1) * TK), st = (uint32_t)(T % ST);
         const int key = p.key0 + i * TK, last = my_pos - key, low = my_low - key;  // the first key of the tile; the last and the first that the row sees
-        mbar_wait_tc(bar_s + b, ph, dead);
+        mbar_wait_warp_tc(bar_s + b, ph, dead);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (some) {
           uint32_t r[64];
@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(NTHR, 2) attn_batch_kernel(BatchAttnArgs a, Sh
           }
           l_run = l_run * f + ((rs[0] + rs[1]) + (rs[2] + rs[3]));
           if (grow && i > p.begin) {  // scale O by the new reference; behind the exponentials the product of the tile before is in
-            mbar_wait_tc(bar_o + (b ^ 8u), (uint32_t)(((T - 1) >> 1) & 1), dead);
+            mbar_wait_warp_tc(bar_o + (b ^ 8u), (uint32_t)(((T - 1) >> 1) & 1), dead);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
             for (int c = 0; c < HD; c += 64) {
@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(NTHR, 2) attn_batch_kernel(BatchAttnArgs a, Sh
         mbar_arrive_tc(bar_p + b);
       }
       // ---- the item's rows
-      mbar_wait_tc(bar_o + 8u * (uint32_t)((T - 1) & 1), (uint32_t)(((T - 1) >> 1) & 1), dead);
+      mbar_wait_warp_tc(bar_o + 8u * (uint32_t)((T - 1) & 1), (uint32_t)(((T - 1) >> 1) & 1), dead);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const bool whole = p.whole();
       const int odd = *(volatile int*)&s_odd[item & 1];  // (a thread may be in the next item already, none in the one behind it)
@@ -469,6 +469,7 @@ __global__ void __launch_bounds__(NTHR, 2) attn_batch_kernel(BatchAttnArgs a, Sh
 #pragma unroll
         for (int c = 0; c < HD; c += 32) {
           uint32_t r[32];
+          __syncwarp();  // (the columns before end per thread)
           ld32(t_o + la + c, r);
           wait_ld();
           if (odd)
@@ -501,7 +502,6 @@ __global__ void __launch_bounds__(NTHR, 2) attn_batch_kernel(BatchAttnArgs a, Sh
 #pragma unroll
             for (int j = 0; j < 32; j += 4) *reinterpret_cast<uint4*>(part + ((c + j) / 4 * TQ + row) * 4) = make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
           }
-          __syncwarp();
         }
       }
       if (tid == 0 && !whole && p.begin == 0)  // goes on in the CTAs behind; the item's last tile is at x1 - left + tiles - 1
@@ -519,6 +519,7 @@ __global__ void __launch_bounds__(NTHR, 2) attn_batch_kernel(BatchAttnArgs a, Sh
   if (warp == NSOFT / 32) {
     drain_tc(dead);
     if (lane == 0) report_tc(dead, a.status);
+    __syncwarp();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
   }

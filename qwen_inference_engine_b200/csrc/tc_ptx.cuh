@@ -35,6 +35,11 @@ __device__ __forceinline__ bool mbar_wait_tc(uint32_t bar, uint32_t parity, vola
   *dead = 1;
   return false;
 }
+// The same by all threads of a warp.  They leave the loop above one by one, and tcgen05.ld and .st (`.sync.aligned`) want them together.
+__device__ __forceinline__ void mbar_wait_warp_tc(uint32_t bar, uint32_t parity, volatile int* dead) {
+  mbar_wait_tc(bar, parity, dead);
+  __syncwarp();
+}
 __device__ __forceinline__ bool mbar_ready_tc(uint32_t bar, uint32_t parity) {  // without waiting
   uint32_t done;
   asm volatile(
