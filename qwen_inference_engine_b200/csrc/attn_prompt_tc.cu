@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(NTHR, 2) attn_prompt_tc_kernel(FastAttnArgs a,
       for (int t = 0; t < n_tiles; ++t) {
         const uint32_t b = 8u * (uint32_t)(t & 1), ph = (uint32_t)((t >> 1) & 1), ts = tmem + la + (uint32_t)((t & 1) * TK);
         const int last = my_pos - (first + t) * TK;  // the last key of the tile that the row sees
-        mbar_wait_tc(bar_s + b, ph, dead);
+        mbar_wait_warp_tc(bar_s + b, ph, dead);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         uint32_t r[64];
         ld32(ts, r);
@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(NTHR, 2) attn_prompt_tc_kernel(FastAttnArgs a,
         }
         l_run = l_run * f + ((rs[0] + rs[1]) + (rs[2] + rs[3]));
         if (grow && t > 0) {  // scale O by the new reference; behind the exponentials the product of the tile before is in
-          mbar_wait_tc(bar_o + (b ^ 8u), (uint32_t)(((t - 1) >> 1) & 1), dead);
+          mbar_wait_warp_tc(bar_o + (b ^ 8u), (uint32_t)(((t - 1) >> 1) & 1), dead);
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
           for (int c = 0; c < HD; c += 64) {
@@ -283,6 +283,7 @@ __global__ void __launch_bounds__(NTHR, 2) attn_prompt_tc_kernel(FastAttnArgs a,
             for (int i = 0; i < NB * 8; ++i)
               asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(s0 + SM::V + (t & 1) * SM::TILE + (i >> 3) * KBLK + row * 128 + (i & 7) * 16), "r"(0u) : "memory");
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
         }
         wait_st();
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -291,7 +292,7 @@ __global__ void __launch_bounds__(NTHR, 2) attn_prompt_tc_kernel(FastAttnArgs a,
     };
     if (two) tiles(std::true_type{});
     else tiles(std::false_type{});
-    if (n_tiles > 0) mbar_wait_tc(bar_o + 8u * (uint32_t)((n_tiles - 1) & 1), (uint32_t)(((n_tiles - 1) >> 1) & 1), dead);
+    if (n_tiles > 0) mbar_wait_warp_tc(bar_o + 8u * (uint32_t)((n_tiles - 1) & 1), (uint32_t)(((n_tiles - 1) >> 1) & 1), dead);
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     uint32_t r[32];
     if (parts == 1) {
@@ -299,6 +300,7 @@ __global__ void __launch_bounds__(NTHR, 2) attn_prompt_tc_kernel(FastAttnArgs a,
       bf16* dst = a.out + (size_t)(t0 + row) * Dq + (size_t)h * HD;
 #pragma unroll
       for (int c = 0; c < HD; c += 32) {
+        __syncwarp();  // (rows end per thread)
         ld32(t_o + la + c, r);
         wait_ld();
         if (row < n_rows) {
@@ -370,6 +372,7 @@ __global__ void __launch_bounds__(NTHR, 2) attn_prompt_tc_kernel(FastAttnArgs a,
   if (warp == NSOFT / 32) {
     drain_tc(dead);
     if (lane == 0) report_tc(dead, a.status);
+    __syncwarp();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
   }
