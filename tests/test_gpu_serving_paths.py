@@ -1,0 +1,105 @@
+"""Paths of a serving step's kernels (csrc/rope_store.cu, logit_rules.cu, attn_batch.cu) that only large or unusual calls take, against plain forms in 64 bits.
+
+Bounds: a rounding to bf16 is off by at most 2^-8 of the value, to fp32 by 2^-24.
+Rotary positions: a pair's turns a position are a double's fraction in 64-bit fixed point, off by 2^-52 of a sixth of a turn, so at positions up to 2^31 the fraction by 2^-23.6 of a turn, 2^-21
+of a radian; as fp32, in [-pi, pi], with a rounded factor of 2 pi / 2^32, by three roundings of 2^-22.3 more.  The hardware's sine and cosine are off by 2^-21.2 there, the fp32 operations by
+3 * 2^-24.  Together 2^-19.2 of factor (|a| + |b|); the reference's own angle by 2^-22: 2^-18 of it holds all."""
+import numpy as np
+import pytest
+import torch
+
+import step_util as ref
+from test_gpu_serving_step import L, Requests, i32, placed, rand  # noqa: F401 (L is a fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------- rotary positions of many tokens
+def turned(x, pos, freq, factor, neighbours):
+    """(the heads turned, factor (|a| + |b|) of each element's pair, 0 for what is not turned), in float64"""
+    h = len(freq)
+    y = ref.rope(x, pos, freq, factor, neighbours)
+    size = torch.zeros_like(y)
+    a, b = (x[..., 0:2 * h:2], x[..., 1:2 * h:2]) if neighbours else (x[..., :h], x[..., h:2 * h])
+    s = factor * (a.double().abs() + b.double().abs())
+    if neighbours:
+        size[..., 0:2 * h:2] = size[..., 1:2 * h:2] = s
+    else:
+        size[..., :h] = size[..., h:2 * h] = s
+    return y, size
+
+
+def within(got, want, size):
+    assert torch.isfinite(got).all()
+    d = (got.double() - want).abs() - 2.0 ** -8 * want.abs() - 2.0 ** -18 * size
+    assert (d <= 0).all(), float(d.max())
+
+
+# heads and rotated elements that take accesses of 8, 4, 2 and 1 elements, and rows that do (`more` elements between them, `off` behind a boundary)
+WIDTHS = [(6, 1, 128, 128, False, 0, 0), (6, 1, 128, 64, True, 8, 8), (6, 1, 128, 24, False, 0, 0), (6, 1, 128, 20, True, 0, 0), (6, 1, 128, 20, False, 0, 0),
+          (6, 1, 128, 10, True, 0, 0), (6, 1, 128, 10, False, 0, 0), (6, 1, 128, 128, True, 1, 0), (6, 1, 128, 128, False, 4, 4), (6, 1, 128, 128, True, 4, 0),
+          (6, 1, 128, 128, False, 2, 0), (6, 1, 128, 96, True, 2, 2), (14, 2, 64, 32, True, 0, 0), (12, 2, 128, 128, False, 8, 0), (40, 8, 128, 128, False, 0, 0)]
+
+
+@pytest.mark.parametrize("nq,nkv,hd,rot,neighbours,more,off", WIDTHS)
+@pytest.mark.parametrize("n,far", [(30001, 2 ** 31 - 1), (30002, 40000), (3001, 5000), (601, 900)])
+def test_rope_store_of_many_tokens(L, nq, nkv, hd, rot, neighbours, more, off, n, far):
+    """several groups of tokens a CTA: what is fetched ahead, the angles of two groups, the positions of four"""
+    if nq == 40 and n > 10000:
+        n = n // 4 + 1  # (a CTA of the widest rows still has three groups)
+    ps = 7
+    pages = (n + ps - 1) // ps + 3
+    w, factor = L.Rope.frequencies(rot, 10000.0, "yarn", 2.0, 4096)
+    freq = torch.from_numpy(w).cuda()
+    g = torch.Generator("cuda").manual_seed(n + rot)
+    pos = torch.randint(max(0, far - 60000), far, (n,), generator=g, device="cuda")
+    row = torch.randperm(pages * ps, generator=g, device="cuda")[:n]
+    no_q, no_kv = (torch.rand(n, generator=g, device="cuda") < 0.1 for _ in range(2))
+    told_pos, told_row = torch.where(no_q, -1 - pos % 5, pos), torch.where(no_kv, torch.where(pos % 2 == 0, -1, pages * ps), row)
+    x = rand(n + hd, n, (nq + 2 * nkv) * hd).bfloat16()
+    qkv, buf = placed(x, off, (nq + 2 * nkv) * hd + more)
+    q, k, v = qkv.split([nq * hd, nkv * hd, nkv * hd], 1)
+    out, out_buf = placed(torch.full((n, nq * hd), 5.0, dtype=torch.bfloat16, device="cuda"), off, nq * hd + more)
+    pool = torch.full((pages, 2, 2, nkv, ps, hd), 3.0, dtype=torch.bfloat16, device="cuda")
+    kept = buf.clone()
+    L.launch_rope_store(q, k, v, out, L.KvPool.over(pool), 1, told_pos.int(), told_row.int(), L.Rope(freq, factor, neighbours), nq)
+    assert torch.equal(buf, kept)
+    heads = x.view(n, -1, hd)
+    want, size = turned(heads[:, :nq + nkv], pos, freq, factor, neighbours)
+    got = out.reshape(n, nq, hd)
+    within(got[~no_q], want[~no_q, :nq], size[~no_q, :nq])
+    assert torch.equal(got[~no_q][..., rot:], heads[~no_q, :nq, rot:])
+    assert (got[no_q] == 5).all() and (out_buf == 77).sum() >= out_buf.numel() - out.numel()
+    sure = ~no_q & ~no_kv
+    keys, values = (pool[:, 1, i].transpose(1, 2).reshape(-1, nkv, hd) for i in (0, 1))
+    within(keys[row[sure]], want[sure, nq:], size[sure, nq:])
+    assert torch.equal(values[row[~no_kv]], heads[~no_kv, nq + nkv:])
+    left = torch.ones(pages * ps, dtype=torch.bool, device="cuda")
+    left[row[~no_kv]] = False
+    assert (keys[left] == 3).all() and (values[left] == 3).all() and (pool[:, 0] == 3).all()
+    del want, size, keys, values, got
+    # q where it is, as an engine's step has it
+    L.launch_rope_store(q, k, v, q, L.KvPool.over(pool), 1, told_pos.int(), told_row.int(), L.Rope(freq, factor, neighbours), nq)
+    assert torch.equal(q[~no_q], out[~no_q]) and torch.equal(q[no_q], x[no_q, :nq * hd]) and torch.equal(k, x[:, nq * hd:(nq + nkv) * hd])
+
+
+@pytest.mark.parametrize("heads,hd,rot", [(9, 128, 128), (12, 64, 16), (5, 256, 256), (70, 64, 64)])
+@pytest.mark.parametrize("neighbours", [False, True])
+@pytest.mark.parametrize("more", [0, 8, 4, 2, 1])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_rope_rows_of_many_tokens(L, heads, hd, rot, neighbours, more, in_place):
+    n = 20003 if heads < 20 else 5003
+    freq = torch.from_numpy(L.Rope.frequencies(rot, 5e5)[0]).cuda()
+    x = rand(heads + more, n, heads * hd).bfloat16()
+    y, buf = placed(x, 0, heads * hd + more)
+    out, out_buf = (y, buf) if in_place else placed(torch.zeros_like(x), 0, heads * hd + more)
+    pos = torch.arange(n, device="cuda") * 97
+    told = torch.where(pos % 11 == 0, -1, pos)
+    L.launch_rope_rows(y, out, told.int(), L.Rope(freq, 1.0, neighbours), heads, hd)
+    want, size = turned(x.view(n, heads, hd), pos, freq, 1.0, neighbours)
+    yes = told >= 0
+    within(out.reshape(n, heads, hd)[yes], want[yes], size[yes])
+    assert torch.equal(out[~yes], x[~yes] if in_place else torch.zeros_like(x[~yes]))
+    assert (out_buf == 77).sum() >= out_buf.numel() - out.numel()
+    if not in_place:
+        assert torch.equal(y, x)
