@@ -3,7 +3,9 @@
 Bounds: a rounding to bf16 is off by at most 2^-8 of the value, to fp32 by 2^-24.
 Rotary positions: a pair's turns a position are a double's fraction in 64-bit fixed point, off by 2^-52 of a sixth of a turn, so at positions up to 2^31 the fraction by 2^-23.6 of a turn, 2^-21
 of a radian; as fp32, in [-pi, pi], with a rounded factor of 2 pi / 2^32, by three roundings of 2^-22.3 more.  The hardware's sine and cosine are off by 2^-21.2 there, the fp32 operations by
-3 * 2^-24.  Together 2^-19.2 of factor (|a| + |b|); the reference's own angle by 2^-22: 2^-18 of it holds all."""
+3 * 2^-24.  Together 2^-19.2 of factor (|a| + |b|); the reference's own angle by 2^-22: 2^-18 of it holds all.
+Logits: a quotient or product, n times the frequency, two differences and the bias, and as many additions as biases of the token: 7 + biases roundings of 2^-24 of at most
+|x| r + f n + p + sum |b|."""
 import numpy as np
 import pytest
 import torch
@@ -103,3 +105,79 @@ def test_rope_rows_of_many_tokens(L, heads, hd, rot, neighbours, more, in_place)
     assert (out_buf == 77).sum() >= out_buf.numel() - out.numel()
     if not in_place:
         assert torch.equal(y, x)
+
+
+# ---------------------------------------------------------------- logit rules with long lists
+def ruled(x, tokens, gen, rep, pres, freq, ids, bias, allowed):
+    """one row in float64: (the row by the rules, size of what was added up in it, biases of each token)"""
+    n = x.numel()
+
+    def counts(t, w=None):
+        ok = (t >= 0) & (t < n)
+        return torch.zeros(n, dtype=torch.float64, device="cuda").index_add_(0, t[ok], torch.ones_like(t[ok], dtype=torch.float64) if w is None else w[ok].double())
+
+    y = x.double()
+    listed, times = counts(tokens) > 0, counts(tokens[gen:])
+    y = torch.where(listed, torch.where(y > 0, y / rep, y * rep), y)
+    y = torch.where(times > 0, y - freq * times - pres, y) + counts(ids, bias)
+    size = 1.6 * x.double().abs() + abs(freq) * times + abs(pres) + counts(ids, bias.abs())
+    if allowed is not None:
+        y = torch.where(allowed, y, float("-inf"))
+    return y, size, counts(ids)
+
+
+def far_lists(rng, rows, vocab, lens, distinct, spread):
+    """tokens of each row: `distinct` of them at most, of chunks whose number is a multiple of `spread`, some outside the vocabulary"""
+    chunks = torch.arange(0, vocab, 256 * spread, device="cuda")
+    every = (chunks[:, None] + torch.arange(256, device="cuda")).flatten()
+    every = every[every < vocab]
+    out = []
+    for i in range(rows):
+        some = every[torch.randperm(len(every), generator=rng, device="cuda")[:distinct]]
+        n = lens[i % len(lens)]
+        t = some[torch.randint(0, len(some), (n,), generator=rng, device="cuda")]
+        t[:min(n, len(some))] = some[:min(n, len(some))]
+        t = t[torch.randperm(n, generator=rng, device="cuda")]
+        t[::97] = torch.tensor([-1, vocab, 2 ** 31 - 1, -2 ** 31], device="cuda").repeat(n // 97 + 1)[:len(t[::97])]
+        out.append(t)
+    start = i32(np.concatenate([[0], np.cumsum([len(t) for t in out])]))
+    return out, start, torch.cat(out).int()
+
+
+# rows and vocabulary; in place and without masks a row of 150 or more has one CTA, and its table is full at some 2000 tokens
+@pytest.mark.parametrize("rows,vocab,lens,distinct,spread,n_bias", [
+    (300, 20000, (6000, 12000, 0, 100), 20000, 1, (700, 0)),      # several classes of tokens
+    (150, 70000, (20000, 513), 70000, 1, (2000, 512, 513)),       # ten levels of them
+    (150, 300000, (9000, 4096, 4097), 9000, 32, (2000, 1)),       # tokens whose places agree in five bits
+    (1, 300000, (40000,), 40000, 64, (5000,)),                    # and in six, of one row: all in one of its 64 CTAs
+    (1, 151936, (120000,), 120000, 1, (30000,)),
+    (64, 151936, (9000, 4096, 4097, 4095), 9000, 1, (511, 512, 513, 2000)),
+])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("in_place,masked", [(True, False), (False, False), (True, True)])
+def test_logits_of_long_lists(L, rows, vocab, lens, distinct, spread, n_bias, dtype, in_place, masked):
+    rng = torch.Generator("cuda").manual_seed(rows + vocab)
+    x = rand(vocab, rows, vocab, scale=4.0).to(dtype)
+    tokens, start, all_tokens = far_lists(rng, rows, vocab, lens, distinct, spread)
+    ids, bias_start, all_ids = far_lists(rng, rows, vocab, n_bias, max(1, max(n_bias) * 2 // 3), spread)  # a third of the biases are repeated ones
+    bias = torch.rand(len(all_ids), generator=rng, device="cuda") * 12 - 6
+    rep, pres, freq = (torch.rand(rows, generator=rng, device="cuda") * (hi - lo) + lo for lo, hi in ((0.7, 1.6), (-1, 1), (0, 0.5)))
+    gen = [int(len(t) * 0.4) for t in tokens]
+    allowed = torch.rand(3, vocab, generator=rng, device="cuda") < 0.5
+    k = {}
+    if masked:
+        bits = np.packbits(allowed.cpu().numpy(), axis=1, bitorder="little")
+        bits = np.concatenate([bits, np.zeros((3, -bits.shape[1] % 4), np.uint8)], 1).view(np.int32)
+        k = dict(mask=torch.from_numpy(bits).cuda(), mask_row=i32([i % 4 - 1 for i in range(rows)]))
+    out = x.clone() if in_place else torch.zeros_like(x)
+    L.launch_logits(out if in_place else x, out, L.LogitRules(start, all_tokens, gen_start=i32(start.cpu().numpy()[:-1] + gen), repetition=rep, presence=pres, frequency=freq,
+                                                             bias_start=bias_start, bias_ids=all_ids, bias=bias, **k))
+    eps = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24
+    s, b = start.tolist(), bias_start.tolist()
+    for i in range(rows):
+        m = i % 4 - 1
+        want, size, n = ruled(x[i], tokens[i].long(), gen[i], *(float(p[i]) for p in (rep, pres, freq)), ids[i].long(), bias[b[i]:b[i + 1]], allowed[m] if masked and m >= 0 else None)
+        got, fine = out[i].double(), torch.isfinite(want)
+        assert torch.equal(got[~fine], want[~fine]), i
+        d = (got - want).abs()[fine] - eps * want.abs()[fine] - ((7 + n) * 2.0 ** -24 * size)[fine]
+        assert (d <= 0).all(), (i, s[i], float(d.max()))
