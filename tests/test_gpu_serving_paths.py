@@ -5,7 +5,8 @@ Rotary positions: a pair's turns a position are a double's fraction in 64-bit fi
 of a radian; as fp32, in [-pi, pi], with a rounded factor of 2 pi / 2^32, by three roundings of 2^-22.3 more.  The hardware's sine and cosine are off by 2^-21.2 there, the fp32 operations by
 3 * 2^-24.  Together 2^-19.2 of factor (|a| + |b|); the reference's own angle by 2^-22: 2^-18 of it holds all.
 Logits: a quotient or product, n times the frequency, two differences and the bias, and as many additions as biases of the token: 7 + biases roundings of 2^-24 of at most
-|x| r + f n + p + sum |b|."""
+|x| r + f n + p + sum |b|.
+Attention: as in test_gpu_serving_step.py."""
 import numpy as np
 import pytest
 import torch
@@ -181,3 +182,78 @@ def test_logits_of_long_lists(L, rows, vocab, lens, distinct, spread, n_bias, dt
         assert torch.equal(got[~fine], want[~fine]), i
         d = (got - want).abs()[fine] - eps * want.abs()[fine] - ((7 + n) * 2.0 ** -24 * size)[fine]
         assert (d <= 0).all(), (i, s[i], float(d.max()))
+
+
+# ---------------------------------------------------------------- attention: what is no number
+def put_odd(r, seed, each, lo=0):
+    """infinities and NaN among the values of each request (`each` of them, at positions from lo on), in the pages too"""
+    rs = np.random.default_rng(seed)
+    table = r.batch.block_table.cpu().numpy()
+    slots = range(len(r.lens)) if r.batch.slots is None else r.batch.slots.tolist()
+    ps = r.pool.shape[4]
+    for i, (c, m) in enumerate(r.lens):
+        for _ in range(min(each, c + m)):
+            p, h, d = int(rs.integers(min(lo, c + m - 1), c + m)), int(rs.integers(r.v[i].shape[1])), int(rs.integers(r.hd))
+            x = [float("inf"), float("-inf"), float("nan")][int(rs.integers(3))]
+            r.v[i][p, h, d] = x
+            r.pool[int(table[slots[i], p // ps]), r.layer, 1, h, p % ps, d] = x
+
+
+def check_odd(r, out, window):
+    """a row has an infinity where it sees it, no number where it sees one or both infinities, and its bound everywhere else"""
+    for i, (c, m) in enumerate(r.lens):
+        if not m:
+            continue
+        s, v, g = slice(r.start[i], r.start[i + 1]), r.v[i], r.nq // r.v[i].shape[1]
+        p, j = torch.arange(c, c + m, device="cuda")[:, None], torch.arange(c + m, device="cuda")
+        seen = ((j <= p) & (j > p - (window or c + m + 1))).float()
+        hit = [((seen @ what.float().flatten(1)) > 0).view(m, -1, 1, r.hd).expand(-1, -1, g, -1).reshape(m, r.nq, r.hd)
+               for what in (torch.isposinf(v) | torch.isnan(v), torch.isneginf(v) | torch.isnan(v))]
+        want, size = ref.attention(r.q[s].view(m, r.nq, r.hd), r.k[i], torch.where(torch.isfinite(v), v, torch.zeros_like(v)), c, window)
+        got = out[s].reshape(m, r.nq, r.hd).double()
+        assert torch.equal(torch.isnan(got), hit[0] & hit[1]), (i, c, m)
+        assert torch.equal(torch.isposinf(got), hit[0] & ~hit[1]) and torch.equal(torch.isneginf(got), hit[1] & ~hit[0]), (i, c, m)
+        fine = ~hit[0] & ~hit[1]
+        d = ((got - want).abs() - 2.0 ** -8 * want.abs() - (2.0 ** -8 + 2.0 ** -9) * size)[fine]
+        assert (d <= 0).all(), (i, c, m, float(d.max()))
+
+
+ODD = [([(0, 100), (70, 1)], 0), ([(0, 130), (64, 64), (1, 1), (63, 2)], 0), ([(699, 1), (0, 1), (64, 1), (63, 1), (128, 1)], 0),  # rows, and no more rows than requests
+       ([(300, 40), (0, 200), (900, 1), (129, 70)], 70), ([(300, 1), (64, 1), (69, 1), (70, 1), (1000, 1)], 70), ([(500, 3), (9, 0), (63, 0), (200, 1)], 64),
+       ([(20000, 1)], 0), ([(0, 2500), (3000, 200)], 0), ([(9000, 300)], 1000),  # items that are cut
+       ([(i * 7 % 90, i % 4) for i in range(400)], 0), ([(i * 13 % 300, 1) for i in range(700)], 100)]  # several items a CTA, one after the other
+
+
+@pytest.mark.parametrize("lens,window", ODD)
+@pytest.mark.parametrize("nq,nkv,hd,ps", [(14, 2, 64, 16), (6, 2, 128, 64), (4, 1, 128, 4), (3, 3, 64, 16)])
+@pytest.mark.parametrize("last", [False, True])
+def test_attention_of_values_that_are_no_numbers(L, lens, window, nq, nkv, hd, ps, last):
+    r = Requests(L, lens, nq, nkv, hd, ps, seed=len(lens) + window)
+    # at the last positions, whose tiles hold keys that some rows do not see; or anywhere
+    put_odd(r, len(lens), 3 if len(lens) > 50 else 9, max(c + m for c, m in lens) - 70 if last else 0)
+    out = torch.full_like(r.q, 9.0)
+    L.launch_attn_batch(r.q, out, r.kv, r.layer, r.batch, nq, window=window)
+    check_odd(r, out, window)
+    again = torch.full_like(r.q, 9.0)
+    L.launch_attn_batch(r.q, again, r.kv, r.layer, r.batch, nq, window=window)
+    assert torch.equal(again.view(torch.int16), out.view(torch.int16))
+
+
+@pytest.mark.parametrize("lens,window,at", [([(0, 100), (40, 1)], 0, 50), ([(200, 1), (3, 1), (64, 1)], 0, 3), ([(100, 60)], 30, 120), ([(0, 1500)], 0, 700), ([(5000, 1)], 0, 4000)])
+@pytest.mark.parametrize("nq,nkv,hd,ps", [(14, 2, 64, 16), (6, 2, 128, 8)])
+def test_attention_of_a_key_that_is_no_number(L, lens, window, at, nq, nkv, hd, ps):
+    """rows that see it have no numbers, rows that do not are as without it"""
+    r = Requests(L, lens, nq, nkv, hd, ps, seed=at)
+    plain, out = torch.full_like(r.q, 9.0), torch.full_like(r.q, 9.0)
+    L.launch_attn_batch(r.q, plain, r.kv, r.layer, r.batch, nq, window=window)
+    r.check(plain, window)
+    page = int(r.batch.block_table[r.batch.slots[0], at // ps])
+    r.pool[page, r.layer, 0, 0, at % ps, 5] = float("nan")
+    L.launch_attn_batch(r.q, out, r.kv, r.layer, r.batch, nq, window=window)
+    c, m = lens[0]
+    p = torch.arange(c, c + m, device="cuda")
+    sees = ((p >= at) & (p < at + (window or c + m + 1)))[:, None].expand(-1, nq).clone()
+    sees[:, nq // nkv:] = False  # the other kv head's
+    sees = torch.cat([sees, torch.zeros(len(out) - m, nq, dtype=torch.bool, device="cuda")])
+    o = out.view(len(out), nq, hd)
+    assert torch.isnan(o[sees]).all() and torch.equal(o[~sees], plain.view(len(out), nq, hd)[~sees])
