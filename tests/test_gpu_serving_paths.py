@@ -257,3 +257,27 @@ def test_attention_of_a_key_that_is_no_number(L, lens, window, at, nq, nkv, hd, 
     sees = torch.cat([sees, torch.zeros(len(out) - m, nq, dtype=torch.bool, device="cuda")])
     o = out.view(len(out), nq, hd)
     assert torch.isnan(o[sees]).all() and torch.equal(o[~sees], plain.view(len(out), nq, hd)[~sees])
+
+
+def test_batch_of_pools_of_both_head_sizes(L):
+    """one batch's arrays over a pool of heads of 64 and one of 128, in that order, and a graph that was captured with the first work area"""
+    lens = [(300, 20), (2000, 1), (5, 3)]
+    small, large = (Requests(L, lens, 4, 2, hd, 16, seed=3) for hd in (64, 128))
+    batch = small.batch
+    assert torch.equal(batch.block_table, large.batch.block_table)
+    out = torch.full_like(small.q, 9.0)
+    L.launch_attn_batch(small.q, out, small.kv, small.layer, batch, 4)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        L.launch_attn_batch(small.q, out, small.kv, small.layer, batch, 4)
+    wide = torch.full_like(large.q, 9.0)
+    L.launch_attn_batch(large.q, wide, large.kv, large.layer, batch, 4)
+    large.check(wide)
+    other = [torch.full((1 << 22,), 3.0, device="cuda") for _ in range(3)]  # what the allocator would have given an area to that was let go
+    out.fill_(9.0)
+    graph.replay()
+    small.check(out)
+    assert all((t == 3).all() for t in other)
+    out.fill_(9.0)
+    L.launch_attn_batch(small.q, out, small.kv, small.layer, batch, 4)
+    small.check(out)
