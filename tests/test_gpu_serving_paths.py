@@ -184,6 +184,47 @@ def test_logits_of_long_lists(L, rows, vocab, lens, distinct, spread, n_bias, dt
         assert (d <= 0).all(), (i, s[i], float(d.max()))
 
 
+def repeated(rows, vocab, distinct, times, seed=0):
+    """(starts, ids, biases): `distinct` tokens of each row, each `times` times, in any order"""
+    rng = torch.Generator("cuda").manual_seed(seed)
+    ids = [torch.randperm(vocab, generator=rng, device="cuda")[:distinct].repeat(times)[torch.randperm(distinct * times, generator=rng, device="cuda")] for _ in range(rows)]
+    n = distinct * times
+    return i32(np.arange(rows + 1) * n), torch.cat(ids).int(), torch.rand(rows * n, generator=rng, device="cuda") * 1e3 - 5e2
+
+
+@pytest.mark.parametrize("rows,vocab,distinct,times", [(1, 151936, 300, 2), (3, 5000, 4000, 3), (160, 9000, 5000, 2), (2, 600, 1, 5000), (160, 40000, 7, 65), (64, 151936, 33, 2), (1, 70000, 60000, 2)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_logits_of_several_biases_a_token(L, rows, vocab, distinct, times, in_place):
+    """they add up in the list's order, to the last bit"""
+    start, ids, bias = repeated(rows, vocab, distinct, times)
+    x = rand(vocab, rows, vocab)
+    out = x.clone() if in_place else torch.empty_like(x)
+    L.launch_logits(out if in_place else x, out, L.LogitRules(bias_start=start, bias_ids=ids, bias=bias))
+    n, h, b, want = distinct * times, ids.cpu().numpy(), bias.cpu().numpy(), x.cpu().numpy()
+    for i in range(rows):
+        total = np.zeros(vocab, np.float32)
+        np.add.at(total, h[i * n:(i + 1) * n], b[i * n:(i + 1) * n])  # one after the other
+        assert np.array_equal(out[i].cpu().numpy(), want[i] + total), i
+
+
+def test_logits_of_several_biases_take_no_walk_a_token(L):
+    """each of 5000 tokens twice: the list is read for a warp's tokens together, not once for each (which took 274 times as long as without the repeats)"""
+    x = rand(1, 64, 151936).bfloat16()
+    out, best = torch.empty_like(x), []
+    for times in (1, 2):
+        start, ids, bias = repeated(64, 151936, 5000, times)
+        rules, t = L.LogitRules(bias_start=start, bias_ids=ids, bias=bias), []
+        for _ in range(6):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(5):
+                L.launch_logits(x, out, rules)
+            b.record()
+            torch.cuda.synchronize()
+            t.append(a.elapsed_time(b))
+        best.append(min(t))
+    assert best[1] < 70 * best[0], best
+
 # ---------------------------------------------------------------- attention: what is no number
 def put_odd(r, seed, each, lo=0):
     """infinities and NaN among the values of each request (`each` of them, at positions from lo on), in the pages too"""
