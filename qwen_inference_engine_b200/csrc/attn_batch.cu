@@ -41,9 +41,11 @@ constexpr int TQ = AB_TQ, TK = AB_TK;
 constexpr int KBLK = TK * 128;  // [rows][64 columns] bf16 in 8-row swizzle atoms
 constexpr int NSOFT = 128, NTHR = NSOFT + 64;
 constexpr uint32_t TMEM_COLS = 256;  // two tiles of scores, O
-// The weights' reference follows a row's maximum where it has fallen behind by more than this (powers of two): most tiles then leave O as it is, 7 % of a long prompt's
-// time.  Weights are as exact as before, 2^-8 of themselves, but the largest one is rounded too; sums are fp32.
-constexpr float LAG = 8.f;
+// The weights' reference follows a row's maximum where it has fallen behind by more than this (powers of two), so that most tiles leave O as it is.  It costs exactness: the largest
+// weight is then one no longer, and rounded like the others, by 2^-8 of itself at most (sums are fp32).  8192 rows, time beside that with 8 and error beside that of a result which is
+// only rounded at its end: no lag 1.09 and 1.20, by 1 1.07 and 1.22, by 3 1.01 and 1.27, by 8 1.32.  Blocks of one token have none: 64 decode rows 42.2 us instead of 41.9
+// and 1.23 instead of 1.38.
+constexpr float LAG = 3.f;
 
 // FEW: blocks of at most 16 rows (decode rows).  The products read 128 all the same, what lies behind their queries, and nobody looks at what comes of it; the room that the other
 // queries would take is a third stage of keys and values (head size 64: a fifth and sixth): 64 rows at 2048 43.6 us, so 41.8.
@@ -352,6 +354,7 @@ __global__ void __launch_bounds__(NTHR, 2) attn_batch_kernel(BatchAttnArgs a, Sh
       const bool some = warp * 32 < p.tokens * G;  // the warp has rows
       const int my_pos = p.pos0 + min(tok, p.tokens - 1), my_low = a.window > 0 ? max(0, my_pos - a.window + 1) : 0;
       const int low0 = a.window > 0 ? max(0, p.pos0 - a.window + 1) : 0, low1 = a.window > 0 ? max(0, p.pos0 + p.tokens - a.window) : 0;  // of the first and the last token
+      const float lag = p.tokens > 1 ? LAG : 0.f;
       float m_ref = -INFINITY, l_run = 0.f;
       int edge = 0;
       for (int i = p.begin; i < p.end; ++i, ++T) {
@@ -384,7 +387,7 @@ __global__ void __launch_bounds__(NTHR, 2) attn_batch_kernel(BatchAttnArgs a, Sh
 #pragma unroll
           for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(r[60 + e]));
           const float m_new = fmaxf(m_ref, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2);
-          const bool grow = __any_sync(0xffffffffu, m_new > m_ref + LAG && tok < p.tokens);  // (rows behind the last token are anything)
+          const bool grow = __any_sync(0xffffffffu, m_new > m_ref + lag && tok < p.tokens);  // (rows behind the last token are anything)
           const float f = grow && m_new > -INFINITY ? ex2_tc(m_ref - m_new) : 1.f;
           if (grow) m_ref = m_new;
           const unsigned long long s2 = twice(sl2), n2 = twice(m_ref > -INFINITY ? -m_ref : 0.f);
