@@ -51,45 +51,6 @@ struct PromptSmem {
   static constexpr int PITCH = (HD + 4) * 4;     // a part's O rows
   static_assert(TQ * PITCH <= BAR, "O rows fit over the operands");
 };
-__device__ __forceinline__ void ld32(uint32_t taddr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,"
-      "%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
-        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
-        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-}
-__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void st32(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
-      "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
-      ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
-      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
-      "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
-      : "memory");
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-// two scores at once: x * s + n, and a + b
-__device__ __forceinline__ void fma2(float& x, float& y, unsigned long long s, unsigned long long n) {
-  asm("{\n\t.reg .b64 v;\n\tmov.b64 v, {%0, %1};\n\tfma.rn.f32x2 v, v, %2, %3;\n\tmov.b64 {%0, %1}, v;\n\t}" : "+f"(x), "+f"(y) : "l"(s), "l"(n));
-}
-__device__ __forceinline__ void add2(float& a, float& b, float x, float y) {
-  asm("{\n\t.reg .b64 u, v;\n\tmov.b64 u, {%0, %1};\n\tmov.b64 v, {%2, %3};\n\tadd.rn.f32x2 u, u, v;\n\tmov.b64 {%0, %1}, u;\n\t}"
-      : "+f"(a), "+f"(b) : "f"(x), "f"(y));
-}
-__device__ __forceinline__ unsigned long long twice(float x) {
-  unsigned long long v;
-  asm("mov.b64 %0, {%1, %1};" : "=l"(v) : "f"(x));
-  return v;
-}
 template <int HD>
 __global__ void __launch_bounds__(NTHR, 2) attn_prompt_tc_kernel(FastAttnArgs a, int two_term, int parts_max, int alone, const __grid_constant__ CUtensorMap kvm) {
   using SM = PromptSmem<HD>;
@@ -222,9 +183,9 @@ __global__ void __launch_bounds__(NTHR, 2) attn_prompt_tc_kernel(FastAttnArgs a,
         mbar_wait_warp_tc(bar_s + b, ph, dead);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         uint32_t r[64];
-        ld32(ts, r);
-        ld32(ts + 32, r + 32);
-        wait_ld();
+        tmem_ld32_tc(ts, r);
+        tmem_ld32_tc(ts + 32, r + 32);
+        tmem_wait_ld_tc();
         if (last < TK - 1) {
 #pragma unroll
           for (int j = 0; j < TK; ++j)
@@ -232,18 +193,18 @@ __global__ void __launch_bounds__(NTHR, 2) attn_prompt_tc_kernel(FastAttnArgs a,
         }
         float mx[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mx[i] = max3(__uint_as_float(r[i]), __uint_as_float(r[i + 4]), __uint_as_float(r[i + 8]));
+        for (int i = 0; i < 4; ++i) mx[i] = max3_tc(__uint_as_float(r[i]), __uint_as_float(r[i + 4]), __uint_as_float(r[i + 8]));
 #pragma unroll
         for (int j = 12; j + 8 <= TK; j += 8)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) mx[i] = max3(mx[i], __uint_as_float(r[j + i]), __uint_as_float(r[j + 4 + i]));
+          for (int i = 0; i < 4; ++i) mx[i] = max3_tc(mx[i], __uint_as_float(r[j + i]), __uint_as_float(r[j + 4 + i]));
 #pragma unroll
         for (int i = 0; i < 4; ++i) mx[i] = fmaxf(mx[i], __uint_as_float(r[60 + i]));
         const float m_new = fmaxf(m_ref, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2);
         const bool grow = __any_sync(0xffffffffu, m_new > m_ref);
         const float f = m_new > -INFINITY ? ex2_tc(m_ref - m_new) : 1.f;
         m_ref = m_new;
-        const unsigned long long s2 = twice(sl2), n2 = twice(m_new > -INFINITY ? -m_new : 0.f);
+        const unsigned long long s2 = twice_tc(sl2), n2 = twice_tc(m_new > -INFINITY ? -m_new : 0.f);
         float rs[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < TK; c += 32) {
@@ -251,9 +212,9 @@ __global__ void __launch_bounds__(NTHR, 2) attn_prompt_tc_kernel(FastAttnArgs a,
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             float e0 = __uint_as_float(r[c + 2 * e]), e1 = __uint_as_float(r[c + 2 * e + 1]);
-            fma2(e0, e1, s2, n2);
+            fma2_tc(e0, e1, s2, n2);
             e0 = ex2_tc(e0), e1 = ex2_tc(e1);
-            add2(rs[2 * (e & 1)], rs[2 * (e & 1) + 1], e0, e1);
+            add2_tc(rs[2 * (e & 1)], rs[2 * (e & 1) + 1], e0, e1);
             hi[e] = pack2f(e0, e1);
             if constexpr (pairs.value) lo[e] = pack2f(e0 - lo2f(hi[e]), e1 - hi2f(hi[e]));
           }
@@ -267,13 +228,13 @@ __global__ void __launch_bounds__(NTHR, 2) attn_prompt_tc_kernel(FastAttnArgs a,
 #pragma unroll
           for (int c = 0; c < HD; c += 64) {
             uint32_t o[64];
-            ld32(t_o + la + c, o);
-            ld32(t_o + la + c + 32, o + 32);
-            wait_ld();
+            tmem_ld32_tc(t_o + la + c, o);
+            tmem_ld32_tc(t_o + la + c + 32, o + 32);
+            tmem_wait_ld_tc();
 #pragma unroll
             for (int j = 0; j < 64; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-            st32(t_o + la + c, o);
-            st32(t_o + la + c + 32, o + 32);
+            tmem_st32_tc(t_o + la + c, o);
+            tmem_st32_tc(t_o + la + c + 32, o + 32);
           }
         }
         if (first + t == all_tiles - 1 && kv_len % TK) {  // value rows behind the sequence: whatever the pool holds there must not meet a zero weight
@@ -285,7 +246,7 @@ __global__ void __launch_bounds__(NTHR, 2) attn_prompt_tc_kernel(FastAttnArgs a,
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
         }
-        wait_st();
+        tmem_wait_st_tc();
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         mbar_arrive_tc(bar_p + b);
       }
@@ -301,8 +262,8 @@ __global__ void __launch_bounds__(NTHR, 2) attn_prompt_tc_kernel(FastAttnArgs a,
 #pragma unroll
       for (int c = 0; c < HD; c += 32) {
         __syncwarp();  // (rows end per thread)
-        ld32(t_o + la + c, r);
-        wait_ld();
+        tmem_ld32_tc(t_o + la + c, r);
+        tmem_wait_ld_tc();
         if (row < n_rows) {
 #pragma unroll
           for (int j = 0; j < 32; j += 8) {
@@ -319,8 +280,8 @@ __global__ void __launch_bounds__(NTHR, 2) attn_prompt_tc_kernel(FastAttnArgs a,
         const uint32_t dst = s0 + (uint32_t)row * SM::PITCH;
 #pragma unroll
         for (int c = 0; c < HD; c += 32) {
-          ld32(t_o + la + c, r);
-          wait_ld();
+          tmem_ld32_tc(t_o + la + c, r);
+          tmem_wait_ld_tc();
 #pragma unroll
           for (int j = 0; j < 32; j += 4)
             asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + (uint32_t)(c + j) * 4u), "r"(r[j]), "r"(r[j + 1]), "r"(r[j + 2]), "r"(r[j + 3]) : "memory");
