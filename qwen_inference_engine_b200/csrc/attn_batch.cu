@@ -618,7 +618,10 @@ cudaError_t launch_attention_batch(const BatchAttnArgs& a, cudaStream_t st) {
   const unsigned long long rows = (unsigned long long)a.kv.n_pages * a.kv.n_layers * 2ull * a.kv.n_kv * P;
   const bool tma = P % 16 == 0;
   // No more rows than requests: a decode step, or nearly one (a request with several rows has blocks of fewer of them, and reads its keys and values that much more often).
-  // Else blocks of as many rows as the products take: one portion of 8192 rows of 7 heads a group has 456 blocks instead of 4096.
+  // Else blocks of as many rows as the products take: one portion of 8192 rows of 7 heads a group has 456 blocks instead of 4096.  Rows behind 2000 positions, groups of 7,
+  // room for as many rows as requests and for one more: 64 requests of a row 53.2 and 55.2 us (heads of 64: 23.9 both), 32 of two 33.1 and 34.4 (16.8, 16.9), 8 of eight 27.1 and
+  // 23.1 (17.1, 22.8), one of 64 27.5 and 31.5 (17.5, 37.1).  The room counts, not the step's rows, which the host does not know: a graph with room for more rows than requests takes
+  // large blocks in its decode steps too.
   const bool few = tma && G <= 16 && a.n_tok <= a.n_req;
   const int tt = (few ? 16 : TQ) / G;
   TensorMap2D qm, kvm{};
