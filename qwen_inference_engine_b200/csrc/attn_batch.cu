@@ -18,7 +18,7 @@
 // Values of keys that some row of a tile does not see must not meet its zero weight when they are no numbers: tiles at the edges of what rows see are
 // looked over, such values are put aside, and rows that see them get them at the end.
 // What bounds it (B200).  Prompts: the chain of a tile (scores, softmax, product), of which an SM has two under way: tensor pipe 52 % busy, exponentials 53 %, issue 40 %, L2
-// 34 %; 8192 rows of 28 heads of 128 on 4 take 500 us, 960 TFLOP/s (without exponentials 486, with half of the keys' and values' bytes 447, one CTA an SM 940).  Decode rows: DRAM, 6.2 TB/s between the first tiles and the last: 64 rows at 1434 positions on average, 189 MB, take 41.8 us, of
+// 34 %; 8192 rows of 28 heads of 128 on 4 take 486 us, 990 TFLOP/s, for 10 ms at 1.96 GHz, and 552 us under the power cap at 1.7 (beside 500 in a run of 0.1 s: without exponentials 486, with half of the keys' and values' bytes 447, one CTA an SM 940).  Decode rows: DRAM, 6.2 TB/s between the first tiles and the last: 64 rows at 1434 positions on average, 189 MB, take 42.2 us, of
 // which 7 us pass before the first scores and 6 behind the last tile.  One row behind 700 positions: 9.3 us, a chain of latencies (plan 1.3, pages and keys 2.4, a tile 0.8, its
 // product and results 1.2, the start of the second kernel 1.2, joining 2.0).
 // Every wait has a limit; when one runs out the CTA's results are not numbers and it reports it.

@@ -2,8 +2,8 @@
 (step_util.py), one by one and as a step in a captured graph whose lengths change.
 
 Bounds: a rounding to bf16 is off by at most 2^-8 of the value, to fp32 by 2^-24.
-Rotary positions: the turns, in 64 bits, are off by 2^-51 of themselves (2^31 positions: 2^-22 of a turn, 2^-19.3 of a radian), their fraction as fp32 by 2^-24 of a radian, sine
-and cosine by 2^-22, the three fp32 operations by 2^-23 of |a| + |b|: 2^-18 of |a| + |b| holds them together.
+Rotary positions: the turns' fraction, in 64-bit fixed point, is off by 2^-23.6 of a turn at 2^31 positions, 2^-21 of a radian; as fp32, in [-pi, pi], by three roundings of 2^-22.3 more; the
+hardware's sine and cosine by 2^-21.2, the three fp32 operations by 2^-23 of |a| + |b|: 2^-18 of |a| + |b| holds them together.
 Attention: weights are rounded to bf16 in the product with the values: 2^-8 of the mean of |v| under the weights.  Scores in fp32 are off by at most 128 * 2^-23 of
 sum |q k| / sqrt(hd), below 2^6 here, so weights by 2^-10 of themselves, exponentials and sums by less: 2^-9 of that mean for all of it.
 Logits: seven fp32 operations and as many additions as biases, each off by 2^-24 of at most |x| r + f n + p + sum |b|."""
