@@ -342,3 +342,77 @@ def test_batch_of_pools_of_both_head_sizes(L):
     out.fill_(9.0)
     L.launch_attn_batch(small.q, out, small.kv, small.layer, batch, 4)
     small.check(out)
+
+
+FIRST = """
+import sys
+sys.path[:0] = {paths!r}
+import torch
+import step_util as ref
+from qwen_inference_engine_b200 import layers as L
+
+def i32(a):
+    return torch.tensor(a, dtype=torch.int32, device="cuda")
+
+n, hd, nq, ps, vocab = 3, 64, 4, 16, 700
+batch = L.Batch(i32([[-1] * 8] * n), ps, 24, n, 40, cached=i32([0] * n), n_new=i32([20, 1, 15]), free_ring=i32(list(range(24))), ring_in=i32([5, 24]))
+pool = L.KvPool.over(torch.zeros(24, 1, 2, 1, ps, hd, dtype=torch.bfloat16, device="cuda"))
+freq = torch.from_numpy(L.Rope.frequencies(hd)[0]).cuda()
+rope = L.Rope(freq)
+qkv = torch.randn(40, (nq + 2) * hd, device="cuda").bfloat16()
+q, k, v = qkv.split([nq * hd, hd, hd], 1)
+q_out, logits, rules = torch.zeros(40, nq * hd, dtype=torch.bfloat16, device="cuda"), torch.randn(n, vocab, device="cuda"), L.LogitRules(i32([0, 2, 2, 3]), i32([5, 6, 7]), repetition=torch.full((n,), 2.0, device="cuda"))
+outs = [torch.full_like(q_out, 9.0) for _ in range(2)]
+ruled = torch.empty_like(logits)
+
+def step(out):
+    L.launch_batch_layout(batch)
+    L.launch_rope_store(q, k, v, q_out, pool, 0, batch.pos, batch.row, rope, nq)
+    L.launch_attn_batch(q_out, out, pool, 0, batch, nq)
+    L.launch_logits(logits, ruled, rules)
+
+graphs = [torch.cuda.CUDAGraph() for _ in outs]
+for g, out in zip(graphs, outs):  # the first calls of the process; the first one makes the work area that both have
+    with torch.cuda.graph(g):
+        step(out)
+for g in graphs * 2:
+    g.replay()
+torch.cuda.synchronize()
+
+def check(out):
+    at = 0
+    for m in (20, 1, 15):
+        heads = ref.rope(qkv[at:at + m].view(m, nq + 2, hd)[:, :nq + 1], torch.arange(m, device="cuda"), freq, 1.0, False).bfloat16()
+        want, size = ref.attention(heads[:, :nq], heads[:, nq:], v[at:at + m].reshape(m, 1, hd), 0)
+        d = (out[at:at + m].view(m, nq, hd).double() - want).abs() - 2.0 ** -8 * want.abs() - 2.0 ** -7 * size
+        assert (d <= 0).all(), float(d.max())
+        at += m
+    assert (out[at:] == 9).all()
+
+check(outs[0]), check(outs[1])
+want = logits.clone()
+for r, t in ((0, 5), (0, 6), (2, 7)):
+    want[r, t] = want[r, t] / 2 if want[r, t] > 0 else want[r, t] * 2
+assert torch.equal(ruled, want)
+# the graph that made the work area goes; the other one and calls of their own still have it
+graphs[0].reset()
+del g
+other = [torch.full((1 << 22,), 3.0, device="cuda") for _ in range(4)]
+outs[1].fill_(9.0)
+graphs[1].replay()
+check(outs[1])
+outs[0].fill_(9.0)
+step(outs[0])
+check(outs[0])
+assert all((t == 3).all() for t in other)
+print("fine")
+"""
+
+
+def test_first_calls_of_a_process_are_captured_ones():
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    out = subprocess.run([sys.executable, "-c", FIRST.format(paths=[here, os.path.dirname(here)])], capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and out.stdout.strip().endswith("fine"), out.stdout[-2000:] + out.stderr[-3000:]
