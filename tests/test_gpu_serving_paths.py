@@ -153,6 +153,8 @@ def far_lists(rng, rows, vocab, lens, distinct, spread):
     (1, 300000, (40000,), 40000, 64, (5000,)),                    # and in six, of one row: all in one of its 64 CTAs
     (1, 151936, (120000,), 120000, 1, (30000,)),
     (64, 151936, (9000, 4096, 4097, 4095), 9000, 1, (511, 512, 513, 2000)),
+    (2, 2 ** 24 + 77, (9000, 30), 9000, 512, (2000, 7)),          # more CTAs a row than lists ask for
+    (1, 2 ** 27, (9000,), 9000, 8192, (2000,)),                   # the largest vocabulary
 ])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("in_place,masked", [(True, False), (False, False), (True, True)])
@@ -343,6 +345,47 @@ def test_batch_of_pools_of_both_head_sizes(L):
     L.launch_attn_batch(small.q, out, small.kv, small.layer, batch, 4)
     small.check(out)
 
+
+def test_the_largest_step(L):
+    """2^24 - 1 tokens of 8192 requests: layout, store and attention, in place and against sums over whole arrays; attention in full for some of the requests"""
+    n, ps, hd, tokens = 8192, 16, 64, 2 ** 24 - 1
+    new = np.full(n, 2048)
+    new[-1] -= 1
+    pages = n * 128
+    ring = torch.randperm(pages, generator=torch.Generator("cuda").manual_seed(1), device="cuda").int()
+    state = i32([pages - 5, pages])
+    batch = L.Batch(torch.full((n, 130), -1, dtype=torch.int32, device="cuda"), ps, pages, n, tokens, cached=i32(np.zeros(n)), n_new=i32(new), free_ring=ring, ring_in=state, ring_out=state)
+    L.launch_batch_layout(batch)
+    t = torch.arange(tokens, device="cuda")
+    first = (t // 16 + pages - 5) % pages  # every request has whole pages
+    assert batch.status.tolist() == [0, 0] and state.tolist() == [pages - 5, 0]
+    assert torch.equal(batch.pos, (t % 2048).int()) and torch.equal(batch.slot, (t // 2048).int())
+    assert torch.equal(batch.row, ring[first] * 16 + (t % 16).int())
+    assert torch.equal(batch.q_start.long(), torch.arange(n + 1, device="cuda").mul(2048).clamp(max=tokens)) and torch.equal(batch.kv_len, i32(new))
+    qkv = torch.empty(tokens, 3 * hd, dtype=torch.bfloat16, device="cuda")
+    qkv.normal_(generator=torch.Generator("cuda").manual_seed(2))
+    kv = L.KvPool.over(torch.zeros(pages, 1, 2, 1, ps, hd, dtype=torch.bfloat16, device="cuda"))
+    q, k, v = qkv.split([hd, hd, hd], 1)
+    out = torch.full((tokens, hd), 9.0, dtype=torch.bfloat16, device="cuda")
+    L.launch_rope_store(q, k, v, out, kv, 0, batch.pos, batch.row, L.Rope(torch.zeros(1, dtype=torch.float64, device="cuda")), 1)  # frequencies of zero: nothing turns
+    assert torch.equal(out, q)
+    table = batch.block_table.long()
+    for i in (0, 1, 4095, n - 1):
+        s, m = slice(i * 2048, i * 2048 + int(new[i])), int(new[i])
+        rows = [kv.pool[table[i, :128], 0, j, 0].reshape(-1, hd)[:m] for j in (0, 1)]
+        assert torch.equal(rows[0], k[s]) and torch.equal(rows[1], v[s])
+    out.fill_(9.0)
+    L.launch_attn_batch(q, out, kv, 0, batch, 1)
+    for i in (0, 1, 2, 777, 4095, 4096, n - 2, n - 1):
+        s, m = slice(i * 2048, i * 2048 + int(new[i])), int(new[i])
+        want, size = ref.attention(q[s].reshape(m, 1, hd), k[s].reshape(m, 1, hd), v[s].reshape(m, 1, hd), 0)
+        d = (out[s].view(m, 1, hd).double() - want).abs() - 2.0 ** -8 * want.abs() - (2.0 ** -8 + 2.0 ** -9) * size
+        assert (d <= 0).all(), (i, float(d.max()))
+    # rows of each request by their own values alone: with values of one every row is one, nearly
+    kv.pool[:, 0, 1] = 1
+    out.fill_(9.0)
+    L.launch_attn_batch(q, out, kv, 0, batch, 1)
+    assert ((out.float() - 1).abs() <= 2.0 ** -7).all()
 
 FIRST = """
 import sys
