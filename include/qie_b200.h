@@ -233,6 +233,31 @@ int qie_attention_batch(const qie_kv_view* kv, int layer, const qie_batch* b, co
 /* bytes of qie_batch.work on the current device (0: a geometry that qie_attention_batch refuses) */
 size_t qie_attention_batch_work(const qie_kv_view* kv, int n_q_heads);
 
+/* The same cache held in 8 bits: of each token and kv head a vector of codes and one scale for its key, and the same for its value.
+ * code: QIE_KV8_E4M3 (8-bit floats of 4 bits of exponent and 3 of mantissa) or QIE_KV8_INT8.  scale: a byte b stands for 2^(b - 127), 0 for a vector of zeros, 255 for one of
+ * no numbers; element = code * scale.  The store takes the smallest power of two with which the vector's largest element is at most 448 (127) times it, and rounds to nearest even, so an
+ * element is off by at most 2^-4 of itself or 2^-10 scales (1/2 scale); a vector with an infinity or NaN becomes one of no numbers.  A token's vectors are written once and never
+ * revised, so pages can be shared and appended to.  head_dim 64 or 128; n_pages * page_size < 2^31, and less than 2^31 vectors in all; codes on a 16-byte boundary. */
+typedef struct {
+  void* codes;     /* [n_pages][n_layers][k|v][n_kv_heads][page_size][head_dim] bytes */
+  uint8_t* scale;  /* [n_pages][n_layers][k|v][n_kv_heads][page_size] */
+  int n_pages, page_size, n_layers, n_kv_heads, head_dim, code;
+} qie_kv8_view;
+#define QIE_KV8_E4M3 0
+#define QIE_KV8_INT8 1
+/* qie_rope_store into such a cache.  Keys are coded as they come out of the rotation, in fp32.  rope NULL: keys as they are (pos is not read); n_q_heads must be 0. */
+int qie_rope_store8(const qie_kv8_view* kv, int layer, const qie_bf16* q, size_t q_stride, qie_bf16* q_out, size_t q_out_stride, const qie_bf16* k,
+                    size_t k_stride, const qie_bf16* v, size_t v_stride, const qie_rope_plan* rope, const int* pos, const int* row, int n_tok,
+                    int n_q_heads, qie_stream st);
+/* The cache rows row[i] of `layer` as the values that they stand for -> rows k[i], v[i] of [n_kv_heads * head_dim], `stride` elements apart; either may be NULL.  Exact (where a value is
+ * below bf16's smallest ones, rounded).  A row outside the pool: k[i] and v[i] are left as they are. */
+int qie_kv8_read(const qie_kv8_view* kv, int layer, const int* row, int n_rows, qie_bf16* k, size_t k_stride, qie_bf16* v, size_t v_stride, qie_stream st);
+/* qie_attention_batch over such a cache; its work area is qie_attention_batch8_work() bytes (one area of the larger size serves both).  Codes of e4m3 that are no numbers make
+ * rows that see them no numbers, in that column at least, and no other row. */
+int qie_attention_batch8(const qie_kv8_view* kv, int layer, const qie_batch* b, const qie_bf16* Q, size_t q_stride, qie_bf16* out, size_t out_stride,
+                         int n_q_heads, int window, float scale, qie_stream st);
+size_t qie_attention_batch8_work(const qie_kv8_view* kv, int n_q_heads);
+
 /* Rules for rows of logits, in front of the sampler.  Row i has the tokens [tok_start[i], tok_start[i + 1]), of which those from gen_start[i] on
  * are generated ones.  In this order, in fp32 with one rounding at the end:
  *   a token of the row's list:      x = x > 0 ? x / repetition[i] : x * repetition[i]   (qie_repetition_penalty)

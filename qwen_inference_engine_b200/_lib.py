@@ -40,6 +40,11 @@ class KvView(C.Structure):
                 ("n_layers", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int)]
 
 
+class Kv8View(C.Structure):
+    _fields_ = [("codes", C.c_void_p), ("scale", C.c_void_p), ("n_pages", C.c_int), ("page_size", C.c_int),
+                ("n_layers", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int), ("code", C.c_int)]
+
+
 class BatchView(C.Structure):
     _fields_ = [(n, C.c_int) for n in ("n_req", "max_tokens", "max_seqs", "max_pages", "n_pages", "page_size")] + \
                [(n, C.c_void_p) for n in ("cached", "n_new", "slots", "block_table", "free_ring", "ring_in", "ring_out", "q_start", "kv_len",
@@ -106,6 +111,10 @@ def lib():
         "qie_rope_store": (i32, [vp, i32, vp, sz, vp, sz, vp, sz, vp, sz, vp, vp, vp, i32, i32, vp]),
         "qie_attention_batch": (i32, [vp, i32, vp, vp, sz, vp, sz, i32, i32, f32, vp]),
         "qie_attention_batch_work": (sz, [vp, i32]),
+        "qie_rope_store8": (i32, [vp, i32, vp, sz, vp, sz, vp, sz, vp, sz, vp, vp, vp, i32, i32, vp]),
+        "qie_kv8_read": (i32, [vp, i32, vp, i32, vp, sz, vp, sz, vp]),
+        "qie_attention_batch8": (i32, [vp, i32, vp, vp, sz, vp, sz, i32, i32, f32, vp]),
+        "qie_attention_batch8_work": (sz, [vp, i32]),
         "qie_logits_process": (i32, [vp, sz, vp, sz, i32, i32, i32, vp, vp]),
         "qie_engine_opts_default": (None, [C.POINTER(EngineOpts)]),
         "qie_synth_checkpoint_write": (i32, [C.POINTER(Config), u64, C.c_char_p, C.c_char_p]),

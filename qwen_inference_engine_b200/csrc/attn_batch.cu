@@ -27,7 +27,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "attn_batch_plan.cuh"
+#include "attn_batch_split.cuh"
 #include "common.cuh"
 #include "kernels.h"
 #include "launch.h"
@@ -61,39 +61,9 @@ struct Smem {
   static constexpr int TOTAL = END > 76 * 1024 ? END : 76 * 1024;
   static_assert(512 / TMEM_COLS == 2 && 3 * (TOTAL + 1024) > 228 * 1024 && 2 * (TOTAL + 2048) <= 228 * 1024, "two CTAs an SM");
 };
-// The work area: of each CTA what there is to join of the item that begins there and goes on behind it; then two parts of each CTA, of the item that began before it and of
-// the one that goes on: O, four columns of all rows after four columns of all rows, so that threads with rows side by side write and read side by side, maxima, sums.
-struct JoinInfo {
-  int t0, tokens, kvh, parts;  // rows t0 .. t0 + tokens of Q; parts 0: nothing
-};
-template <int HD>
-constexpr int PART = TQ * HD + 2 * TQ;  // floats
-
 struct Shape {
   int g, tt, out32;  // query heads of a group; tokens of a block; rows of the result begin on 32-byte boundaries
 };
-// sum over the block of a 64-bit value a thread: what the threads below have, and all
-__device__ __forceinline__ long long block_scan(long long v, long long* warp_sums, long long& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long run = v;
-  for (int d = 1; d < 32; d <<= 1) {
-    const long long o = __shfl_up_sync(0xffffffffu, run, d);
-    if (lane >= d) run += o;
-  }
-  if (lane == 31) warp_sums[warp] = run;
-  __syncthreads();
-  long long before = 0;
-  total = 0;
-  for (int w = 0; w < NTHR / 32; ++w) {
-    if (w == warp) before = total;
-    total += warp_sums[w];
-  }
-  return before + run - v;
-}
-
-// a / b of numbers that are not below 0, mostly of 32 bits
-__device__ __forceinline__ long long quotient(long long a, long long b) { return (a | b) >> 32 ? a / b : (long long)((unsigned)a / (unsigned)b); }
-
 template <int HD, bool TMA, bool FEW>
 __global__ void __launch_bounds__(NTHR, 2) attn_batch_kernel(BatchAttnArgs a, Shape sh, int box, const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap kvm) {
   using SM = Smem<HD, FEW>;
@@ -126,49 +96,7 @@ __global__ void __launch_bounds__(NTHR, 2) attn_batch_kernel(BatchAttnArgs a, Sh
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   for (int i = tid; i < EDGES * HD; i += NTHR) asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(s0 + SM::ODD + i * 16), "r"(0u) : "memory");
-  // ---- this CTA's stretch
-  const int per = (a.n_req + NTHR - 1) / NTHR, r0 = min(a.n_req, tid * per), r1 = min(a.n_req, r0 + per);
-  long long mine = 0, total, head = 0;  // head: a kv head's cost of the thread's last request
-  for (int i = r0; i < r1; ++i) {
-    const Raw w = request(a, i, tt);
-    head = ab_cost(w.r, w.r.nb, tt, a.window);
-    mine += a.kv.n_kv * head;
-  }
-  const long long below = block_scan(mine, s_sums, total);
-  const long long share = quotient(total + gridDim.x - 1, gridDim.x), x0 = min(total, share * blockIdx.x), x1 = min(total, x0 + share);
-  const bool own = x0 < x1 && below <= x0 && x0 < below + mine;
-  if (const unsigned owner = __ballot_sync(0xffffffffu, own)) {  // the warp of the thread that has the request in which it begins
-    int req = 0;
-    long long rest = 0;
-    if (own) {
-      rest = x0 - below;
-      for (req = r0; req < r1 - 1; ++req) {
-        const Raw w = request(a, req, tt);
-        const long long h = ab_cost(w.r, w.r.nb, tt, a.window);
-        if (rest < a.kv.n_kv * h) {
-          head = h;
-          break;
-        }
-        rest -= a.kv.n_kv * h;
-      }
-    }
-    const int from = __ffs(owner) - 1;
-    req = __shfl_sync(0xffffffffu, req, from), rest = __shfl_sync(0xffffffffu, rest, from), head = __shfl_sync(0xffffffffu, head, from);
-    const Raw w = request(a, req, tt);
-    const int kvh = (int)quotient(rest, head);
-    rest -= kvh * head;
-    // the block in which it begins: the last one whose cost of blocks before is not above the rest, 32 at a time
-    int lo = 0, hi = w.r.nb;
-    long long before = 0;
-    while (hi - lo > 1) {
-      const int step = (hi - lo + 31) / 32, x = lo + lane * step;
-      const long long c = x < hi ? ab_cost(w.r, x, tt, a.window) : rest + 1;
-      const int k = 31 - __clz(__ballot_sync(0xffffffffu, c <= rest));  // (lane 0's is)
-      before = __shfl_sync(0xffffffffu, c, k);
-      hi = min(hi, lo + (k + 1) * step), lo += k * step;
-    }
-    if (lane == 0) s_walk = Walk{w, req, kvh, lo, (int)(rest - before), x1 - x0};
-  }
+  const auto [share, x1] = find_stretch<NTHR>(a, tt, s_sums, &s_walk);
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -428,7 +356,7 @@ __global__ void __launch_bounds__(NTHR, 2) attn_batch_kernel(BatchAttnArgs a, Sh
       if (some) {
         const float scale = *dead ? __int_as_float(0x7fc00000) : !whole ? 1.f : l_run > 0.f ? 1.f / l_run : l_run;
         bf16* dst = a.out + (size_t)(p.t0 + tok) * a.out_stride + (size_t)(p.kvh * G + g) * HD;
-        float* part = parts + ((size_t)blockIdx.x * 2 + (p.begin == 0)) * PART<HD>;
+        float* part = parts + ((size_t)blockIdx.x * 2 + (p.begin == 0)) * PART<HD, TQ>;
         if (!whole) part[TQ * HD + row] = m_ref, part[TQ * HD + TQ + row] = *dead ? __int_as_float(0x7fc00000) : l_run;
 #pragma unroll
         for (int c = 0; c < HD; c += 32) {
@@ -489,111 +417,6 @@ __global__ void __launch_bounds__(NTHR, 2) attn_batch_kernel(BatchAttnArgs a, Sh
   }
 }
 
-// The parts of an item that was cut into the rows of its result: CTA k joins the item that CTA k of the kernel above began and did not end.  Sums are taken in a fixed
-// order.
-constexpr int JOIN_THR = 512;
-// 2^(m - top): a row sees nothing of some parts, and a sum that is no number counts whatever the maximum beside it
-__device__ __forceinline__ float weight(float m, float l, float top) { return l != l ? l : m > -INFINITY ? ex2_tc(m - top) : 0.f; }
-struct Sum4 {
-  float m = -INFINITY, l = 0.f;
-  float4 o = {0.f, 0.f, 0.f, 0.f};
-  __device__ __forceinline__ void add(float pm, float pl, const float4& x) {
-    const float top = fmaxf(m, pm), f = weight(m, l, top), pf = weight(pm, pl, top);
-    m = top;
-    l = l * f + pl * pf;
-    o.x *= f, o.y *= f, o.z *= f, o.w *= f;
-    if (pf != 0.f) o.x += x.x * pf, o.y += x.y * pf, o.z += x.z * pf, o.w += x.w * pf;
-  }
-};
-template <int HD>
-__global__ void __launch_bounds__(JOIN_THR, 2) attn_batch_join_kernel(BatchAttnArgs a, int G, int n_cta) {
-  constexpr int C = HD / 4;  // groups of columns
-  __shared__ Sum4 sums[JOIN_THR];
-  pdl_wait();
-  pdl_trigger();
-  const JoinInfo* info = reinterpret_cast<const JoinInfo*>(a.work);
-  const JoinInfo in = info[blockIdx.x];
-  const int slice = blockIdx.y;  // of many rows' columns
-  const float* first = reinterpret_cast<const float*>(info + n_cta) + ((size_t)blockIdx.x * 2 + 1) * PART<HD>;
-  const int rows = in.tokens * G, n = in.parts, tid = threadIdx.x;
-  // (a work area that two calls used at once must not lead outside)
-  if (n <= 1 || n > n_cta - (int)blockIdx.x || rows <= 0 || rows > TQ || in.t0 < 0 || in.t0 > a.n_tok - in.tokens || in.kvh < 0 || in.kvh >= a.kv.n_kv) return;
-  bf16* out = a.out + (size_t)in.t0 * a.out_stride + (size_t)in.kvh * G * HD;
-  auto store = [&](int row, int c, const float4& o, float f) {
-    *reinterpret_cast<uint2*>(out + (size_t)(row / G) * a.out_stride + (size_t)(row % G) * HD + c * 4) = make_uint2(pack2f(o.x * f, o.y * f), pack2f(o.z * f, o.w * f));
-  };
-  auto part_of = [&](int q) { return first + (q == 0 ? 0 : (size_t)(2 * q - 1) * PART<HD>); };  // the others are the first ones of the CTAs behind
-  const int all = rows * C;
-  if (all > JOIN_THR) {
-    // many rows: four threads a row with every fourth group of its columns; a part's weight is the row's
-    constexpr int MINE = C / (JOIN_THR / TQ);
-    const int row = tid % TQ, c0 = tid / TQ;
-    if (row >= rows) return;
-    float top = -INFINITY, sum = 0.f;
-    for (int q = 0; q < n; q += 4) {
-      float m[4], l[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const float* part = part_of(min(q + u, n - 1)) + TQ * HD + row;
-        m[u] = q + u < n ? part[0] : -INFINITY, l[u] = q + u < n ? part[TQ] : 0.f;
-      }
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const float t = fmaxf(top, m[u]);
-        sum = sum * weight(top, sum, t) + l[u] * weight(m[u], l[u], t);
-        top = t;
-      }
-    }
-    const float inv = sum > 0.f ? 1.f / sum : sum;
-#pragma unroll 1
-    for (int b = 4 * slice; b < min(MINE, 4 * slice + 4); b += 4) {
-      float4 o[4] = {};
-#pragma unroll 2
-      for (int q = 0; q < n; ++q) {
-        const float* part = part_of(q);
-        float4 x[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = *reinterpret_cast<const float4*>(part + ((c0 + (b + e) * (JOIN_THR / TQ)) * TQ + row) * 4);
-        const float f = weight(part[TQ * HD + row], part[TQ * HD + TQ + row], top) * inv;
-        if (f != 0.f)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[e].x += x[e].x * f, o[e].y += x[e].y * f, o[e].z += x[e].z * f, o[e].w += x[e].w * f;
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) store(row, c0 + (b + e) * (JOIN_THR / TQ), o[e], 1.f);
-    }
-    return;
-  }
-  if (slice) return;
-  // few rows: four columns of a row a thread, and the parts in turn with the threads that are left
-  constexpr int U = 4;
-  const int lanes = JOIN_THR / all, i = tid % all, q0 = tid / all, c = i / rows, row = i - c * rows;
-  Sum4 s;
-  if (q0 < lanes)
-    for (int q = q0; q < n; q += U * lanes) {
-      float m[U], l[U];
-      float4 x[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int k = q + u * lanes;
-        m[u] = -INFINITY, l[u] = 0.f;
-        if (k >= n) continue;
-        const float* part = part_of(k);
-        m[u] = part[TQ * HD + row], l[u] = part[TQ * HD + TQ + row];
-        x[u] = *reinterpret_cast<const float4*>(part + (c * TQ + row) * 4);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (q + u * lanes < n) s.add(m[u], l[u], x[u]);
-    }
-  sums[tid] = s;
-  __syncthreads();
-  if (q0 == 0) {
-    for (int w = 1; w < min(lanes, n); ++w) s.add(sums[w * all + i].m, sums[w * all + i].l, sums[w * all + i].o);
-    store(row, c, s.o, s.l > 0.f ? 1.f / s.l : s.l);
-  }
-}
-
 template <int HD, bool TMA, bool FEW>
 cudaError_t launch_hd(const BatchAttnArgs& a, int tt, const TensorMap2D& qm, const TensorMap2D& kvm, int box, cudaStream_t st) {
   static PerDeviceOnce set;
@@ -606,12 +429,12 @@ cudaError_t launch_hd(const BatchAttnArgs& a, int tt, const TensorMap2D& qm, con
   const cudaError_t e = launched(launch_k(attn_batch_kernel<HD, TMA, FEW>, dim3(ctas), dim3(NTHR), Smem<HD, FEW>::TOTAL, st, a, Shape{G, tt, (int)(reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && a.out_stride % 16 == 0)}, box,
                                           *reinterpret_cast<const CUtensorMap*>(&qm), *reinterpret_cast<const CUtensorMap*>(&kvm)));
   if (e != cudaSuccess) return e;
-  return launched(launch_k(attn_batch_join_kernel<HD>, dim3(ctas, HD / 64), dim3(JOIN_THR), 0, st, a, G, ctas));
+  return launch_join<HD, TQ>(a, JoinShape{G, G, 1}, ctas, st);
 }
 
 }  // namespace
 
-size_t attention_batch_work(int hd, int num_sms) { return (size_t)2 * num_sms * (sizeof(JoinInfo) + 2 * (hd == 64 ? PART<64> : PART<128>) * sizeof(float)); }
+size_t attention_batch_work(int hd, int num_sms) { return (size_t)2 * num_sms * (sizeof(JoinInfo) + 2 * (hd == 64 ? PART<64, TQ> : PART<128, TQ>) * sizeof(float)); }
 
 cudaError_t launch_attention_batch(const BatchAttnArgs& a, cudaStream_t st) {
   const int G = a.n_q / a.kv.n_kv, P = a.kv.page_size;

@@ -540,6 +540,88 @@ int qie_attention_batch(const qie_kv_view* kv, int layer, const qie_batch* b, co
   return QIE_OK;
 }
 
+// ---- a cache in 8 bits
+static bool kv8_ok(const qie_kv8_view* kv, int layer) {
+  return kv && kv->codes && kv->scale && layer >= 0 && layer < kv->n_layers && kv->n_pages > 0 && kv->page_size > 0 && kv->n_kv_heads > 0 &&
+         (kv->head_dim == 64 || kv->head_dim == 128) && (kv->code == QIE_KV8_E4M3 || kv->code == QIE_KV8_INT8) && aligned(16, {kv->codes});
+}
+static bool kv8_fits(const qie_kv8_view* kv) {  // vectors are counted in 31 bits
+  const unsigned long long places = (unsigned long long)kv->n_pages * kv->page_size, heads = 2ull * kv->n_layers * kv->n_kv_heads;
+  return places < 1ull << 31 && heads < 1ull << 31 && places * heads < 1ull << 31;
+}
+static Kv8Geom kv8_geom(const qie_kv8_view* v) {
+  return Kv8Geom{(uint8_t*)v->codes, v->scale, v->n_pages, v->page_size, v->n_layers, v->n_kv_heads, v->head_dim, v->code};
+}
+int qie_rope_store8(const qie_kv8_view* kv, int layer, const qie_bf16* q, size_t q_stride, qie_bf16* q_out, size_t q_out_stride, const qie_bf16* k,
+                    size_t k_stride, const qie_bf16* v, size_t v_stride, const qie_rope_plan* rope, const int* pos, const int* row, int n_tok, int n_q_heads,
+                    qie_stream st) {
+  static_assert(KV8_E4M3 == QIE_KV8_E4M3 && KV8_INT8 == QIE_KV8_INT8, "one name");
+  if (!kv8_ok(kv, layer)) return fail(QIE_EINVAL, "rope_store8: bad pool or layer (heads of 64 or 128 elements, a known code, codes on a 16-byte boundary)");
+  if (!kv8_fits(kv)) return fail(QIE_EINVAL, "rope_store8: a pool of 2^31 vectors");
+  if (rope && !rope_ok(rope, kv->head_dim)) return fail(QIE_EINVAL, "rope_store8: need an even number of rotated elements, at most head_dim");
+  if (!rope && n_q_heads) return fail(QIE_EINVAL, "rope_store8: queries without a rotation");
+  if (n_tok < 0 || n_tok > 1 << 30 || n_q_heads < 0 || (n_tok && (!k || !v || (rope && !pos) || !row || (n_q_heads && (!q || !q_out))))) return fail(QIE_EINVAL, "rope_store8: bad argument (at most 2^30 rows)");
+  if (((long long)n_q_heads + 2ll * kv->n_kv_heads) * kv->head_dim > ROPE_ROW) return fail(QIE_EINVAL, "rope_store8: at most 2^24 elements of a token's q, k and v");
+  const size_t wide = (size_t)n_q_heads * kv->head_dim, kv_wide = (size_t)kv->n_kv_heads * kv->head_dim;
+  if (n_tok > 1 && (k_stride < kv_wide || v_stride < kv_wide || (n_q_heads && (q_stride < wide || q_out_stride < wide)))) return fail(QIE_EINVAL, "rope_store8: rows overlap");
+  if (n_tok > 1 && n_q_heads && q == q_out && q_stride != q_out_stride) return fail(QIE_EINVAL, "rope_store8: in place with rows at other places");
+  if (n_tok == 0) return QIE_OK;
+  Rope8Args a{};
+  a.q = (const bf16*)q, a.q_out = (bf16*)q_out, a.q_stride = q_stride, a.q_out_stride = q_out_stride;
+  a.k = (const bf16*)k, a.v = (const bf16*)v, a.k_stride = k_stride, a.v_stride = v_stride;
+  if (rope) a.freq = rope->freq, a.rotated = rope->rotated, a.neighbours = rope->neighbours, a.factor = rope->factor;
+  a.pos = pos, a.row = row, a.n_tok = n_tok, a.n_q = n_q_heads, a.layer = layer, a.kv = kv8_geom(kv);
+  CU(launch_rope_store8(a, (cudaStream_t)st));
+  return QIE_OK;
+}
+int qie_kv8_read(const qie_kv8_view* kv, int layer, const int* row, int n_rows, qie_bf16* k, size_t k_stride, qie_bf16* v, size_t v_stride, qie_stream st) {
+  if (!kv8_ok(kv, layer)) return fail(QIE_EINVAL, "kv8_read: bad pool or layer (heads of 64 or 128 elements, a known code, codes on a 16-byte boundary)");
+  if (!kv8_fits(kv)) return fail(QIE_EINVAL, "kv8_read: a pool of 2^31 vectors");
+  if (n_rows < 0 || n_rows > 1 << 30 || (n_rows && !row)) return fail(QIE_EINVAL, "kv8_read: bad argument (at most 2^30 rows)");
+  const size_t wide = (size_t)kv->n_kv_heads * kv->head_dim;
+  if ((long long)wide > ROPE_ROW) return fail(QIE_EINVAL, "kv8_read: at most 2^24 elements a row");
+  if (n_rows > 1 && ((k && k_stride < wide) || (v && v_stride < wide))) return fail(QIE_EINVAL, "kv8_read: rows of %zu elements overlap", wide);
+  if (n_rows == 0 || (!k && !v)) return QIE_OK;
+  Kv8ReadArgs a{row, (bf16*)k, (bf16*)v, k_stride, v_stride, n_rows, layer, kv8_geom(kv)};
+  CU(launch_kv8_read(a, (cudaStream_t)st));
+  return QIE_OK;
+}
+static bool batch8_heads_ok(const qie_kv8_view* kv, int n_q) {
+  return kv && heads_ok(n_q, kv->n_kv_heads) && n_q / kv->n_kv_heads <= 128 && (kv->head_dim == 64 || kv->head_dim == 128);
+}
+size_t qie_attention_batch8_work(const qie_kv8_view* kv, int n_q_heads) {
+  int sms = 0;
+  if (!batch8_heads_ok(kv, n_q_heads) || sm_count(&sms) != cudaSuccess) return 0;
+  return attention_batch8_work(kv->head_dim, sms);
+}
+int qie_attention_batch8(const qie_kv8_view* kv, int layer, const qie_batch* b, const qie_bf16* Q, size_t q_stride, qie_bf16* out, size_t out_stride, int n_q_heads,
+                         int window, float scale, qie_stream st) {
+  if (!kv8_ok(kv, layer)) return fail(QIE_EINVAL, "attention_batch8: bad pool or layer (heads of 64 or 128 elements, a known code, codes on a 16-byte boundary)");
+  if (!kv8_fits(kv)) return fail(QIE_EINVAL, "attention_batch8: a pool of 2^31 vectors");
+  if (!batch8_heads_ok(kv, n_q_heads)) return fail(QIE_EINVAL, "attention_batch8: need n_q %% n_kv == 0 and n_q / n_kv <= 128");
+  if (!batch_sizes_ok(b) || b->page_size != kv->page_size || b->n_pages != kv->n_pages) return fail(QIE_EINVAL, "attention_batch8: a batch of other pages, or of sizes out of range");
+  if (!b->slots && b->n_req > b->max_seqs) return fail(QIE_EINVAL, "attention_batch8: %d requests on %d rows of the block table", b->n_req, b->max_seqs);
+  if (window < 0 || !(scale >= 0.f) || scale > 1e6f) return fail(QIE_EINVAL, "attention_batch8: window and scale must not be below 0");
+  if (b->n_req == 0 || b->max_tokens == 0) return QIE_OK;
+  if (b->max_tokens >= 1 << 24) return fail(QIE_EINVAL, "attention_batch8: at most 2^24 - 1 rows");
+  if (!b->q_start || !b->kv_len || !b->block_table || !Q || !out) return fail(QIE_EINVAL, "attention_batch8: an array is missing");
+  const size_t wide = (size_t)n_q_heads * kv->head_dim;
+  if (q_stride < wide || out_stride < wide || q_stride % 8 || out_stride % 8 || q_stride >= (1ull << 38)) return fail(QIE_EINVAL, "attention_batch8: rows of Q and out are multiples of 8 elements, %zu at least", wide);
+  if (!aligned(16, {Q, out, b->work})) return fail(QIE_EINVAL, "attention_batch8: Q, out and the work area must start on a 16-byte boundary");
+  OP_STATUS(status);
+  BatchAttnArgs a{};
+  CU(sm_count(&a.num_sms));
+  if (!b->work || b->work_bytes < attention_batch8_work(kv->head_dim, a.num_sms)) return fail(QIE_EINVAL, "attention_batch8: needs a work area of %zu bytes", attention_batch8_work(kv->head_dim, a.num_sms));
+  a.q = (const bf16*)Q, a.out = (bf16*)out, a.q_stride = q_stride, a.out_stride = out_stride;
+  a.q_start = b->q_start, a.kv_len = b->kv_len, a.slots = b->slots, a.block_table = b->block_table;
+  a.n_req = b->n_req, a.n_tok = b->max_tokens, a.max_seqs = b->max_seqs, a.max_pages = b->max_pages, a.n_q = n_q_heads, a.layer = layer, a.window = window;
+  a.scale_log2 = 1.4426950408889634f * (scale > 0.f ? scale : 1.f / sqrtf((float)kv->head_dim));
+  a.kv = KvGeom{nullptr, kv->n_pages, kv->page_size, kv->n_layers, kv->n_kv_heads, kv->head_dim};
+  a.work = b->work, a.status = status;
+  CU(launch_attention_batch8(a, kv8_geom(kv), (cudaStream_t)st));
+  return QIE_OK;
+}
+
 int qie_logits_process(const void* logits, size_t stride, void* out, size_t out_stride, int dtype, int n_rows, int vocab, const qie_logit_rules* rules, qie_stream st) {
   if (dtype != QIE_DTYPE_BF16 && dtype != QIE_DTYPE_F32) return fail(QIE_EINVAL, "logits_process: bf16 or fp32 logits");
   if (!rules || n_rows < 0 || n_rows > 65535 || vocab <= 0 || vocab > 1 << 27 || (n_rows && (!logits || !out)))

@@ -194,6 +194,38 @@ struct RopeArgs {
 };
 cudaError_t launch_rope_store(const RopeArgs& a, cudaStream_t st);
 
+// the same pool in 8 bits (kv8.cuh): codes[page][layer][k|v][kv_head][slot][head_dim], scale[page][layer][k|v][kv_head][slot]
+enum { KV8_E4M3 = 0, KV8_INT8 = 1 };
+struct Kv8Geom {
+  uint8_t *codes, *scale;
+  int n_pages, page_size, n_layers, n_kv, hd, code;
+  // a layer's vector of a head in cache row `row`: `kv` 0 its key, 1 its value
+  __host__ __device__ size_t vec(int layer, int kv, int head, int row) const {
+    const int page = row / page_size;
+    return ((((size_t)page * n_layers + layer) * 2 + kv) * n_kv + head) * page_size + (row - page * page_size);
+  }
+};
+struct Rope8Args {
+  const bf16 *q, *k, *v;
+  bf16* q_out;
+  size_t q_stride, q_out_stride, k_stride, v_stride;
+  const double* freq;  // null: nothing turns, and there are no queries
+  int rotated, neighbours;
+  float factor;
+  const int *pos, *row;
+  int n_tok, n_q, layer;
+  Kv8Geom kv;
+};
+cudaError_t launch_rope_store8(const Rope8Args& a, cudaStream_t st);
+struct Kv8ReadArgs {
+  const int* row;
+  bf16 *k, *v;  // either may be null
+  size_t k_stride, v_stride;
+  int n_rows, layer;
+  Kv8Geom kv;
+};
+cudaError_t launch_kv8_read(const Kv8ReadArgs& a, cudaStream_t st);
+
 struct BatchAttnArgs {
   const bf16* q;
   bf16* out;
@@ -208,6 +240,8 @@ struct BatchAttnArgs {
 };
 size_t attention_batch_work(int hd, int num_sms);
 cudaError_t launch_attention_batch(const BatchAttnArgs& a, cudaStream_t st);
+size_t attention_batch8_work(int hd, int num_sms);
+cudaError_t launch_attention_batch8(const BatchAttnArgs& a, const Kv8Geom& kv, cudaStream_t st);  // a.kv: sizes alone
 
 struct LogitArgs {
   const void* in;

@@ -13,7 +13,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import BatchView, KvView, LogitRulesView, RopePlan, check
+from ._lib import BatchView, Kv8View, KvView, LogitRulesView, RopePlan, check
 
 
 def _p(t):
@@ -197,7 +197,7 @@ class Batch:
         self.block_table, self.slots, self.cached, self.n_new, self.free_ring, self.ring_in = block_table, slots, cached, n_new, free_ring, ring_in
         self.ring_out, self.q_start, self.kv_len, self.status = ints(ring_out, 2), ints(q_start, n_req + 1), ints(kv_len, n_req), ints(status, 2)
         self.pos, self.slot, self.row = ints(pos, max_tokens), ints(slot, max_tokens), ints(row, max_tokens)
-        self.work, self.heads, self.replaced, self.max_tokens = None, 0, [], max_tokens
+        self.work, self.heads, self.heads8, self.replaced, self.max_tokens = None, 0, 0, [], max_tokens
         b = self.view = BatchView(n_req=n_req, max_tokens=max_tokens, max_seqs=block_table.shape[0], max_pages=block_table.shape[1], n_pages=n_pages,
                                   page_size=page_size)
         for name, n in (("block_table", 0), ("slots", n_req), ("cached", n_req), ("n_new", n_req), ("free_ring", n_pages), ("ring_in", 2), ("ring_out", 2),
@@ -209,16 +209,20 @@ class Batch:
         self.ref = C.byref(b)
 
     def reserve(self, pool, n_q_heads):
-        """the work area of launch_attn_batch; one call at a time uses it.  A smaller one from before is kept beside it: captured graphs and launches under way may
-        have it."""
-        n = _lib.lib().qie_attention_batch_work(C.byref(pool.view), n_q_heads)
+        """the work area of launch_attn_batch and launch_attn_batch8; one call at a time uses it.  A smaller one from before is kept beside it: captured graphs and launches
+        under way may have it."""
+        eight = isinstance(pool, KvPool8)
+        n = (_lib.lib().qie_attention_batch8_work if eight else _lib.lib().qie_attention_batch_work)(pool.ref, n_q_heads)
         if n == 0:  # a geometry that the operator refuses
             return
         if self.work is None or self.work.numel() < n:
             self.replaced.append(self.work)
             self.work = torch.empty(n, dtype=torch.uint8, device=self.block_table.device)
             self.view.work, self.view.work_bytes = self.work.data_ptr(), n
-        self.heads = max(self.heads, pool.head_dim)  # the area's size hangs on the head size alone
+        if eight:  # the area's size hangs on the head size alone
+            self.heads8 = max(self.heads8, pool.head_dim)
+        else:
+            self.heads = max(self.heads, pool.head_dim)
 
 
 def launch_batch_layout(batch):
@@ -278,6 +282,72 @@ def launch_attn_batch(Q, out, pool, layer, batch, n_q_heads, window=0, scale=0.0
     assert Q.get_device() == out.get_device() == pool.pool.get_device() == batch.block_table.get_device(), "rows, pool and batch on one device expected"
     _here(Q)
     check(_lib.lib().qie_attention_batch(pool.ref, layer, batch.ref, *_rows(Q), *_rows(out), n_q_heads, window, scale, _st()))
+
+
+class KvPool8:
+    """the same pool in 8 bits (qie_kv8_view): codes [page][layer][k|v][kv_head][slot][head_dim] of torch.float8_e4m3fn or torch.int8, and scale bytes of the same shape without the last"""
+    CODES = {torch.float8_e4m3fn: 0, torch.int8: 1}
+
+    def __init__(self, n_pages, page_size, n_layers, n_kv_heads, head_dim, dtype=torch.float8_e4m3fn):
+        shape = (n_pages, n_layers, 2, n_kv_heads, page_size)
+        self._over(torch.zeros(*shape, head_dim, dtype=torch.uint8, device="cuda").view(dtype), torch.zeros(shape, dtype=torch.uint8, device="cuda"))
+
+    @classmethod
+    def over(cls, codes, scale):
+        """the same over a caller's arrays"""
+        self = cls.__new__(cls)
+        self._over(codes, scale)
+        return self
+
+    def _over(self, codes, scale):
+        assert codes.dtype in KvPool8.CODES and codes.dim() == 6 and codes.shape[2] == 2, "codes [page][layer][k|v][kv_head][slot][head_dim] of float8_e4m3fn or int8 expected"
+        assert scale.dtype is torch.uint8 and scale.shape == codes.shape[:5] and scale.get_device() == codes.get_device(), "a uint8 scale for each vector, beside them, expected"
+        n_pages, n_layers, _, n_kv_heads, page_size, head_dim = codes.shape
+        _here(codes)
+        self.codes, self.scale, self.head_dim, self.kv_wide = codes, scale, head_dim, n_kv_heads * head_dim
+        self.view = Kv8View(_p(codes), _p(scale), n_pages, page_size, n_layers, n_kv_heads, head_dim, KvPool8.CODES[codes.dtype])
+        self.ref = C.byref(self.view)
+
+
+def launch_rope_store8(q, k, v, q_out, pool, layer, pos, row, rope, n_q_heads):
+    """q -> q_out, k and v -> codes and scales in the cache rows row[t] of the pool's layer.  rope None: k as it is; then q, q_out and pos are None and n_q_heads 0"""
+    (n, kw), (nv, vw) = k.shape, v.shape
+    assert k.dtype is v.dtype is torch.bfloat16 and n == nv and kw == vw == pool.kv_wide, "bfloat16 rows of the heads of as many tokens expected"
+    (kp, ks), (vp, vs), rp = _rows(k), _rows(v), _ints(row, n, "row")
+    assert k.get_device() == v.get_device() == pool.codes.get_device() == row.get_device(), "rows and pool on one device expected"
+    _here(k)
+    if rope is None:
+        assert q is None and q_out is None and pos is None and n_q_heads == 0, "queries and positions without a rotation"
+        check(_lib.lib().qie_rope_store8(pool.ref, layer, None, 0, None, 0, kp, ks, vp, vs, None, None, rp, n, 0, _st()))
+        return
+    assert q.dtype is q_out.dtype is torch.bfloat16 and q.shape == q_out.shape == (n, n_q_heads * pool.head_dim), "bfloat16 rows of the heads of as many tokens expected"
+    assert k.get_device() == q.get_device() == q_out.get_device() == pos.get_device() == rope.device, "rows, positions and frequencies on one device expected"
+    (qp, qs), (op, os) = _rows(q), _rows(q_out)
+    check(_lib.lib().qie_rope_store8(pool.ref, layer, qp, qs, op, os, kp, ks, vp, vs, rope.ref, _ints(pos, n, "pos"), rp, n, n_q_heads, _st()))
+
+
+def launch_kv8_read(pool, layer, row, k, v):
+    """cache rows row[i] of the pool's layer -> rows k[i], v[i] (either may be None) of the values that they stand for"""
+    n, out = row.numel(), []
+    for x in (k, v):
+        if x is None:
+            out += [None, 0]
+            continue
+        assert x.dtype is torch.bfloat16 and x.shape == (n, pool.kv_wide) and x.get_device() == row.get_device(), "bfloat16 rows of the pool's heads, one for each index, expected"
+        out += _rows(x)
+    assert row.get_device() == pool.codes.get_device(), "rows and pool on one device expected"
+    _here(row)
+    check(_lib.lib().qie_kv8_read(pool.ref, layer, _ints(row, n, "row"), n, *out, _st()))
+
+
+def launch_attn_batch8(Q, out, pool, layer, batch, n_q_heads, window=0, scale=0.0):
+    """launch_attn_batch over a pool in 8 bits"""
+    assert Q.dtype is out.dtype is torch.bfloat16 and Q.shape == out.shape == (batch.max_tokens, n_q_heads * pool.head_dim), "bfloat16 rows of the batch expected"
+    if batch.heads8 < pool.head_dim:
+        batch.reserve(pool, n_q_heads)
+    assert Q.get_device() == out.get_device() == pool.codes.get_device() == batch.block_table.get_device(), "rows, pool and batch on one device expected"
+    _here(Q)
+    check(_lib.lib().qie_attention_batch8(pool.ref, layer, batch.ref, *_rows(Q), *_rows(out), n_q_heads, window, scale, _st()))
 
 
 class LogitRules:
