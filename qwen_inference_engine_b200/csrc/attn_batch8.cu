@@ -4,8 +4,8 @@
 //   out_t = sum_j 2^(x_tj - m) 2^ev_j v_j / sum_j 2^(x_tj - m),  x_tj = s 2^ek_j (q_t . k_j) over the positions j that row t sees, m their running maximum, k_j and v_j codes
 //
 // Codes become fp16 exactly.  A row's query is brought to fp16 by a power of two of its own, which loses nothing either, so scores are those of the values that the cache stands for,
-// summed in fp32.  Weights are fp16 in the product with the values (2^-11 of themselves; 2^12 times themselves and times their value's scale, so that none of at least 2^-26 of the
-// largest gets fewer bits), their sums fp32.
+// summed in fp32.  Weights are fp16 in the product with the values (2^-11 of themselves; 2^7 times themselves and times their value's scale, so that none of at least 2^-21 of the
+// largest gets fewer bits, and none is off by more than 2^-32 of it), their sums fp32.
 //
 // An item is a kv head of a request and a block of its tokens, its rows (token, query head of the group); items are shared out over the CTAs as in attn_batch.cu.
 #include <cuda.h>
@@ -22,8 +22,9 @@
 namespace qie {
 namespace {
 
-constexpr float LAG = 3.f;  // weights are at most 2^LAG: with 2^12 below the largest fp16
-constexpr int P_EXP = 12;
+// The weights' reference follows a row's maximum where it has fallen behind by more than 2^8: weights by 2^7 are at most 2^15 then, below the largest fp16.
+constexpr float LAG = 8.f;
+constexpr int P_EXP = 7;
 
 // ---------------------------------------------------------------- blocks of at most 16 rows
 constexpr int ROWS_F = 16, THR_F = 256, WARPS_F = THR_F / 32;
@@ -255,7 +256,7 @@ __global__ void __launch_bounds__(THR_F, NB == 1 ? 2 : 1) attn_few8_kernel(Batch
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[nb][b][e] *= f;
       }
-      float pv[2];  // 2^12 times a value's scale beside the largest
+      float pv[2];  // 2^7 times a value's scale beside the largest
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int e = max(1, (int)(i ? vb1 : vb0)) - lr + 127 + P_EXP;
@@ -383,20 +384,49 @@ cudaError_t launch_few(const BatchAttnArgs& a, const Kv8Geom& kv, const JoinShap
 // On tcgen05 / TMEM, one CTA an SM.  Two tiles of 128 rows work on the same keys and values, so that a tile of 64 of those is brought to fp16 once for both; each is a chain of its own
 // (scores, softmax, product), and while one is in its softmax the other one has the tensor pipe.
 //   warps 0-3, 4-7 : the softmax of a row tile, a thread a row (= TMEM lane); queries into TMEM (the A operand of the scores, as the weights are of the products, so that shared memory
-//                    feeds keys and values alone), the rows of the result
-//   warps 8-11     : codes to fp16: of a tile the powers of two beside its largest, which is a factor of all scores (keys) and of all weights (values), by the multiplication
-//   warps 12, 13   : the products of a row tile
-//   warp 14        : codes and scales by TMA, or, for pages of other than multiples of 16 positions, by 16-byte copies to the same places
-constexpr int ROWS_P = 256, THR_P = 15 * 32, TK = AB_TK;
+//                    feeds keys and values alone; with heads of 128 there is no room for both in TMEM, and they lie in shared memory), the rows of the result
+//   warps 8-15     : codes to fp16 (keys, values): of a tile the powers of two beside its largest, which is a factor of all scores (keys) and of all weights (values), by the multiplication
+//   warps 16, 17   : the products of a row tile
+//   warp 18        : codes and scales by TMA, or, for pages of other than multiples of 16 positions, by 16-byte copies to the same places; warp 19 has nothing to do
+// Registers: 96 a thread at launch; 144, 64 and 64 behind the split, as many in all.
+constexpr int ROWS_P = 256, THR_P = 20 * 32, TK = AB_TK;
 constexpr int KBLK = TK * 128;  // [keys][64 columns] fp16 in 8-row swizzle atoms
-constexpr int SLOTS = 8;        // tiles' scales: the softmax is at most STAGES + 1 tiles behind
+constexpr int SLOTS = 8;        // tiles' scales: the softmax is at most STAGES + 3 tiles behind
 template <int HD>
 struct SmemP {
-  static constexpr int NB = HD / 64, RAW = 4, ST = 3;  // column blocks; stages of codes, and of keys and values
-  static constexpr int CODES = TK * HD, TILE = NB * KBLK;
-  static constexpr int C = 0, K = RAW * 2 * CODES, V = K + ST * TILE, SC = V + ST * TILE, BAR = SC + RAW * 2 * TK, TOTAL = BAR + 512 + 1024;
-  static_assert(TOTAL <= 226 * 1024 && ST + 2 <= SLOTS, "");
+  static constexpr bool Q_TMEM = HD == 64;
+  static constexpr int NB = HD / 64, RAW = HD == 64 ? 4 : 3, ST = 3;  // column blocks; stages of codes, and of keys and values
+  static constexpr int CODES = TK * HD, TILE = NB * KBLK, QBLK = 128 * 128, QTILE = NB * QBLK;
+  static constexpr int C = 0, K = RAW * 2 * CODES, V = K + ST * TILE, Q = V + ST * TILE, SC = Q + (Q_TMEM ? 0 : 2 * QTILE), BAR = SC + RAW * 2 * TK, TOTAL = BAR + 512 + 1024;
+  static_assert(TOTAL <= 226 * 1024 && ST + 4 <= SLOTS, "");
 };
+// mbar_wait_tc in few instructions: with the compiler's loop around a try the warps that wait had half of the SM's instructions.  2^26 tries are about two seconds.
+__device__ __forceinline__ void wait_short(uint32_t bar, uint32_t parity, volatile int* dead) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  if (done || *dead) return;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 i;\n\t"
+      "mov.u32 i, 0;\n"
+      "again:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "@p bra.uni out;\n\t"
+      "add.u32 i, i, 1;\n\t"
+      "setp.lt.u32 q, i, 67108864;\n\t"
+      "@q bra.uni again;\n"
+      "out:\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  if (!done) *dead = 1;
+}
 // D = F32, A = B = F16
 __device__ __forceinline__ uint32_t idesc_h(int m, int n, bool b_mn) { return idesc_tc(m, n, b_mn) & ~((1u << 7) | (1u << 10)); }
 __device__ __forceinline__ void cp_async_arrive(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
@@ -404,10 +434,10 @@ __device__ __forceinline__ uint32_t mul_h2(uint32_t a, uint32_t b) {
   asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(a) : "r"(b));
   return a;
 }
-// 2^-d twice as fp16
+// 2^-d twice as fp16, d >= 0 (or, where nobody looks at what comes of it, any)
 __device__ __forceinline__ uint32_t pow2_h2(int d) {
-  const uint32_t h = d < 0 ? 0x3c00u : d <= 14 ? (uint32_t)(15 - d) << 10 : d <= 24 ? 1u << (24 - d) : 0u;
-  return h | h << 16;
+  const float f = __uint_as_float((uint32_t)max(127 - d, 0) << 23);
+  return pack_h(f, f);
 }
 
 template <int HD, int CODE, bool TMA>
@@ -416,28 +446,29 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
   constexpr int ST = SM::ST, RAW = SM::RAW;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   __shared__ long long s_sums[THR_P / 32];
-  __shared__ Walk s_walk;
+  __shared__ Walk s_walk, s_walks[THR_P / 32];
   __shared__ int dead_s;
   __shared__ int s_kt[SLOTS], s_vt[SLOTS];  // the largest scales of a tile's keys and values, as bytes
   __shared__ unsigned long long s_bad[2];   // (edge tiles, by parity) keys whose values are no numbers
   volatile int* dead = &dead_s;
-  if (TMA && threadIdx.x == 14 * 32) asm volatile("prefetch.tensormap [%0];" ::"l"(&cm) : "memory");
+  if (TMA && threadIdx.x == 18 * 32) asm volatile("prefetch.tensormap [%0];" ::"l"(&cm) : "memory");
   pdl_wait();
   pdl_trigger();
   const uint32_t s0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* smem = smem_raw + (s0 - smem_u32(smem_raw));
-  // barriers: of a row tile queries, scores, weights and product; of the stages of codes, keys and values full and free
-  const uint32_t bar_q = s0 + SM::BAR, bar_s = bar_q + 16, bar_p = bar_s + 16, bar_o = bar_p + 16, slot = bar_o + 16, raw_full = slot + 16, raw_free = raw_full + 8 * RAW, k_full = raw_free + 8 * RAW,
+  // barriers: of a row tile queries, and by its tile's parity scores, weights and product; of the stages of codes, keys and values full and free
+  const uint32_t bar_q = s0 + SM::BAR, bar_s = bar_q + 16, bar_p = bar_s + 32, bar_o = bar_p + 32, slot = bar_o + 32, raw_full = slot + 16, raw_free = raw_full + 8 * RAW, k_full = raw_free + 8 * RAW,
                  k_free = k_full + 8 * ST, v_full = k_free + 8 * ST, v_free = v_full + 8 * ST;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     dead_s = 0, s_walk.left = 0, s_bad[0] = s_bad[1] = 0;
-    for (int i = 0; i < 2; ++i) mbar_init_tc(bar_q + 8 * i, 128), mbar_init_tc(bar_s + 8 * i, 1), mbar_init_tc(bar_p + 8 * i, 128), mbar_init_tc(bar_o + 8 * i, 1);
-    for (int i = 0; i < RAW; ++i) mbar_init_tc(raw_full + 8 * i, TMA ? 1 : 64), mbar_init_tc(raw_free + 8 * i, 4);
+    for (int i = 0; i < 2; ++i) mbar_init_tc(bar_q + 8 * i, 128);
+    for (int i = 0; i < 4; ++i) mbar_init_tc(bar_s + 8 * i, 1), mbar_init_tc(bar_p + 8 * i, 128), mbar_init_tc(bar_o + 8 * i, 1);
+    for (int i = 0; i < RAW; ++i) mbar_init_tc(raw_full + 8 * i, TMA ? 1 : 64), mbar_init_tc(raw_free + 8 * i, 8);
     for (int i = 0; i < ST; ++i) mbar_init_tc(k_full + 8 * i, 4), mbar_init_tc(k_free + 8 * i, 2), mbar_init_tc(v_full + 8 * i, 4), mbar_init_tc(v_free + 8 * i, 2);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 12) {
+  if (warp == 16) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -445,232 +476,261 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  Walk walk = s_walk;
   uint32_t tmem;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(slot));
-  // TMEM: scores of 64 columns (the weights over them), queries, O of each row tile
-  auto t_s = [&](int g) { return tmem + (uint32_t)(g * TK); };
-  auto t_q = [&](int g) { return tmem + 2 * TK + (uint32_t)(g * (HD / 2)); };
-  auto t_o = [&](int g) { return tmem + 256 + (uint32_t)(g * HD); };
+  // TMEM: scores of 64 columns (the weights over them) of a row tile's two tiles at hand, its O, its queries
+  auto t_s = [&](int g, int b) { return tmem + (uint32_t)((2 * g + b) * TK); };
+  auto t_o = [&](int g) { return tmem + 4 * TK + (uint32_t)(g * HD); };
+  auto t_q = [&](int g) { return tmem + 4 * TK + 2 * HD + (uint32_t)(g * (HD / 2)); };
   JoinInfo* info = reinterpret_cast<JoinInfo*>(a.work);
   float* parts = reinterpret_cast<float*>(info + gridDim.x);
+  // the pieces of the stretch, every warp for itself; between them in shared memory (in registers they cost the softmax spills)
+  if (lane == 0) s_walks[warp] = s_walk;
+  __syncwarp();
+  auto next_piece = [&](Piece& p) {
+    Walk walk = s_walks[warp];
+    const bool some = walk.next(a, tt, p);
+    __syncwarp();
+    if (lane == 0) s_walks[warp] = walk;
+    __syncwarp();
+    return some;
+  };
   Piece p;
   int T = 0;  // tiles so far
 
-  if (warp == 14) {
-    // ---- codes and scales
-    const int P = kv.page_size, v_off = kv.n_kv * P;
-    const int chunks = TMA ? TK / box : 1;  // of a tile
-    uint8_t wait_sc[4];                     // (not TMA) the scales of the tile before
-    int waits = -1;
-    auto put_scales = [&]() {
-      if (waits < 0) return;
+  if (warp >= 16) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");  // (a warpgroup together)
+    if (warp >= 18) {
+      // ---- codes and scales
+      const int P = kv.page_size, v_off = kv.n_kv * P;
+      const int chunks = TMA ? TK / box : 1;  // of a tile
+      uint8_t wait_sc[4];                     // (not TMA) the scales of the tile before
+      int waits = -1;
+      auto put_scales = [&]() {
+        if (waits < 0) return;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) smem[SM::SC + waits * 2 * TK + j * 32 + lane] = wait_sc[j];
-      mbar_arrive_tc(raw_full + 8u * (uint32_t)waits);
-    };
-    while (walk.next(a, tt, p)) {
-      const int* bt = a.block_table + (size_t)p.slot * a.max_pages;
-      const int last_page = (p.limit - 1) / P, c0 = TMA ? p.key0 / box : 0;
-      int held = c0 + p.begin * chunks, page_of = 0;  // a lane holds the page of chunk `held` + lane
-      if (TMA) page_of = bt[min((held + lane) * box / P, last_page)];
-      for (int i = p.begin; i < p.end; ++i, ++T) {
-        const int st = T % RAW;
-        if (T >= RAW) mbar_wait_tc(raw_free + 8u * st, (uint32_t)((T / RAW - 1) & 1), dead);
-        __syncwarp();
-        const uint32_t bar = raw_full + 8u * st, dst = s0 + SM::C + st * 2 * SM::CODES, sc = s0 + SM::SC + st * 2 * TK;
-        if constexpr (TMA) {
-          const int ch = c0 + i * chunks;
-          if (ch + chunks > held + 32) {
-            held = ch;
-            page_of = bt[min((held + lane) * box / P, last_page)];
-          }
-          const int j = lane % 4;  // a chunk; lanes 0 .. 3 keys, 4 .. 7 values, 8 .. 15 their scales
-          int page = __shfl_sync(0xffffffffu, page_of, (ch - held + j) & 31);
-          if (page < 0 || page >= kv.n_pages) page = 0;
-          const int at = min((ch + j) * box, last_page * P + P - box) % P;  // (chunks behind the last page repeat its end: their keys are masked)
-          const int is_v = lane >> 2 & 1, row = ((page * kv.n_layers + a.layer) * 2 * kv.n_kv + p.kvh) * P + at + is_v * v_off;
-          if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"((uint32_t)(2 * SM::CODES + 2 * TK)) : "memory");
+        for (int j = 0; j < 4; ++j) smem[SM::SC + waits * 2 * TK + j * 32 + lane] = wait_sc[j];
+        mbar_arrive_tc(raw_full + 8u * (uint32_t)waits);
+      };
+      while (warp == 18 && next_piece(p)) {
+        const int* bt = a.block_table + (size_t)p.slot * a.max_pages;
+        const int last_page = (p.limit - 1) / P, c0 = TMA ? p.key0 / box : 0;
+        int held = c0 + p.begin * chunks, page_of = 0;  // a lane holds the page of chunk `held` + lane
+        if (TMA) page_of = bt[min((held + lane) * box / P, last_page)];
+        for (int i = p.begin; i < p.end; ++i, ++T) {
+          const int st = T % RAW;
+          if (T >= RAW) wait_short(raw_free + 8u * st, (uint32_t)((T / RAW - 1) & 1), dead);
           __syncwarp();
-          if (j < chunks && lane < 8)
-            asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-                         ::"r"(dst + is_v * SM::CODES + j * box * HD), "l"(&cm), "r"(bar), "r"(0), "r"(row)
-                         : "memory");
-          if (j < chunks && lane >= 8 && lane < 16)
-            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                         ::"r"(sc + is_v * TK + j * box), "l"(kv.scale + row), "r"(box), "r"(bar)
-                         : "memory");
-          __syncwarp();
-        } else {
-          put_scales();
-          // the lane's keys, lane and 32 + lane of the tile: their vectors
-          int vec[2];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int key = min(p.key0 + i * TK + h * 32 + lane, p.limit - 1), pg = key / P;
-            int page = bt[pg];
+          const uint32_t bar = raw_full + 8u * st, dst = s0 + SM::C + st * 2 * SM::CODES, sc = s0 + SM::SC + st * 2 * TK;
+          if constexpr (TMA) {
+            const int ch = c0 + i * chunks;
+            if (ch + chunks > held + 32) {
+              held = ch;
+              page_of = bt[min((held + lane) * box / P, last_page)];
+            }
+            const int j = lane % 4;  // a chunk; lanes 0 .. 3 keys, 4 .. 7 values, 8 .. 15 their scales
+            int page = __shfl_sync(0xffffffffu, page_of, (ch - held + j) & 31);
             if (page < 0 || page >= kv.n_pages) page = 0;
-            vec[h] = ((page * kv.n_layers + a.layer) * 2 * kv.n_kv + p.kvh) * P + (key - pg * P);
-            wait_sc[h] = kv.scale[vec[h]], wait_sc[2 + h] = kv.scale[vec[h] + v_off];
-          }
-          waits = st;
-          constexpr int PIECES = HD / 16;
+            const int at = min((ch + j) * box, last_page * P + P - box) % P;  // (chunks behind the last page repeat its end: their keys are masked)
+            const int is_v = lane >> 2 & 1, row = ((page * kv.n_layers + a.layer) * 2 * kv.n_kv + p.kvh) * P + at + is_v * v_off;
+            if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"((uint32_t)(2 * SM::CODES + 2 * TK)) : "memory");
+            __syncwarp();
+            if (j < chunks && lane < 8)
+              asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                           ::"r"(dst + is_v * SM::CODES + j * box * HD), "l"(&cm), "r"(bar), "r"(0), "r"(row)
+                           : "memory");
+            if (j < chunks && lane >= 8 && lane < 16)
+              asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                           ::"r"(sc + is_v * TK + j * box), "l"(kv.scale + row), "r"(box), "r"(bar)
+                           : "memory");
+            __syncwarp();
+          } else {
+            put_scales();
+            // the lane's keys, lane and 32 + lane of the tile: their vectors
+            int vec[2];
 #pragma unroll
-          for (int e = 0; e < TK * PIECES / 32; ++e) {
-            const int row = (e * 32 + lane) / PIECES, piece = lane % PIECES;
-            const int r = __shfl_sync(0xffffffffu, e * 32 / PIECES < 32 ? vec[0] : vec[1], row & 31);
-            const uint8_t* src = kv.codes + (size_t)r * HD + piece * 16;
-            const uint32_t to = dst + row * HD + ((HD == 128 ? piece ^ (row & 7) : piece ^ ((row >> 1) & 3)) << 4);
-            cp_async16(to, src);
-            cp_async16(to + SM::CODES, src + (size_t)v_off * HD);
+            for (int h = 0; h < 2; ++h) {
+              const int key = min(p.key0 + i * TK + h * 32 + lane, p.limit - 1), pg = key / P;
+              int page = bt[pg];
+              if (page < 0 || page >= kv.n_pages) page = 0;
+              vec[h] = ((page * kv.n_layers + a.layer) * 2 * kv.n_kv + p.kvh) * P + (key - pg * P);
+              wait_sc[h] = kv.scale[vec[h]], wait_sc[2 + h] = kv.scale[vec[h] + v_off];
+            }
+            waits = st;
+            constexpr int PIECES = HD / 16;
+#pragma unroll
+            for (int e = 0; e < TK * PIECES / 32; ++e) {
+              const int row = (e * 32 + lane) / PIECES, piece = lane % PIECES;
+              const int r = __shfl_sync(0xffffffffu, e * 32 / PIECES < 32 ? vec[0] : vec[1], row & 31);
+              const uint8_t* src = kv.codes + (size_t)r * HD + piece * 16;
+              const uint32_t to = dst + row * HD + ((HD == 128 ? piece ^ (row & 7) : piece ^ ((row >> 1) & 3)) << 4);
+              cp_async16(to, src);
+              cp_async16(to + SM::CODES, src + (size_t)v_off * HD);
+            }
+            cp_async_arrive(bar);
           }
-          cp_async_arrive(bar);
         }
       }
-    }
-    if (!TMA) put_scales();
-  } else if (warp >= 12) {
-    // ---- the products of row tile g
-    const int g = warp - 12;
-    const uint32_t id_s = idesc_h(128, TK, false), id_o = idesc_h(128, HD, true);
-    const uint64_t dk = desc_k_tc(s0 + SM::K), dv = desc_mn_tc(s0 + SM::V, KBLK);  // (steps are sums: in units of 16 bytes)
-    int items = 0, tg = 0;  // items and tiles of this row tile
-    auto issue_s = [&](int at) {
-      mbar_wait_tc(k_full + 8u * (uint32_t)(at % ST), (uint32_t)((at / ST) & 1), dead);
-      __syncwarp();
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      if (elect_tc()) {
-        const uint64_t k = dk + (uint64_t)((at % ST) * (SM::TILE >> 4));
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk) umma_ts_tc(t_s(g), t_q(g) + (uint32_t)(kk * 8), k + (uint64_t)(((kk >> 2) * KBLK + (kk & 3) * 32) >> 4), id_s, kk != 0);
-        umma_commit_tc(bar_s + 8u * g);
-        umma_commit_tc(k_free + 8u * (uint32_t)(at % ST));
-      }
-      __syncwarp();
-    };
-    while (walk.next(a, tt, p)) {
-      const int n = p.count();
-      if (g * 128 >= p.tokens * G) {  // nothing to do but to let the stages go
-        for (int i = 0; i < n; ++i, ++T) {
-          const uint32_t st = (uint32_t)(T % ST), ph = (uint32_t)((T / ST) & 1);
-          mbar_wait_tc(k_full + 8u * st, ph, dead);
-          if (lane == 0) mbar_arrive_tc(k_free + 8u * st);
-          mbar_wait_tc(v_full + 8u * st, ph, dead);
-          if (lane == 0) mbar_arrive_tc(v_free + 8u * st);
-          __syncwarp();
-        }
-        continue;
-      }
-      mbar_wait_tc(bar_q + 8u * g, (uint32_t)(items & 1), dead);
-      ++items;
-      issue_s(T);
-      for (int i = 0; i < n; ++i, ++T, ++tg) {
-        const uint32_t st = (uint32_t)(T % ST), ph = (uint32_t)(tg & 1);
-        mbar_wait_tc(v_full + 8u * st, (uint32_t)((T / ST) & 1), dead);
-        mbar_wait_tc(bar_p + 8u * g, ph, dead);
+      if (!TMA && warp == 18) put_scales();
+    } else {
+      // ---- the products of row tile g
+      const int g = warp - 16;
+      const uint32_t id_s = idesc_h(128, TK, false), id_o = idesc_h(128, HD, true);
+      const uint64_t dk = desc_k_tc(s0 + SM::K), dv = desc_mn_tc(s0 + SM::V, KBLK), dq = desc_k_tc(s0 + SM::Q + g * SM::QTILE);  // (steps are sums: in units of 16 bytes)
+      int items = 0, tg = 0;  // items and tiles of this row tile
+      auto issue_s = [&](int ahead) {
+        const int at = T + ahead, b = (tg + ahead) & 1;
+        wait_short(k_full + 8u * (uint32_t)(at % ST), (uint32_t)((at / ST) & 1), dead);
         __syncwarp();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (elect_tc()) {
-          const uint64_t v = dv + (uint64_t)(st * (SM::TILE >> 4));
+          const uint64_t k = dk + (uint64_t)((at % ST) * (SM::TILE >> 4));
 #pragma unroll
-          for (int kk = 0; kk < TK / 16; ++kk) umma_ts_tc(t_o(g), t_s(g) + (uint32_t)(kk * 8), v + (uint64_t)(kk * 128), id_o, i > 0 || kk > 0);
-          umma_commit_tc(bar_o + 8u * g);
-          umma_commit_tc(v_free + 8u * st);
+          for (int kk = 0; kk < HD / 16; ++kk) {
+            const uint64_t kd = k + (uint64_t)(((kk >> 2) * KBLK + (kk & 3) * 32) >> 4);
+            if constexpr (SM::Q_TMEM) umma_ts_tc(t_s(g, b), t_q(g) + (uint32_t)(kk * 8), kd, id_s, kk != 0);
+            else umma_tc(t_s(g, b), dq + (uint64_t)(((kk >> 2) * SM::QBLK + (kk & 3) * 32) >> 4), kd, id_s, kk != 0);
+          }
+          umma_commit_tc(bar_s + 16u * g + 8u * b);
+          umma_commit_tc(k_free + 8u * (uint32_t)(at % ST));
         }
         __syncwarp();
-        if (i + 1 < n) {
-          mbar_wait_tc(bar_o + 8u * g, ph, dead);  // the next scores go over the weights that this product reads
-          issue_s(T + 1);
+      };
+      while (next_piece(p)) {
+        const int n = p.count();
+        if (g * 128 >= p.tokens * G) {  // nothing to do but to let the stages go
+          for (int i = 0; i < n; ++i, ++T) {
+            const uint32_t st = (uint32_t)(T % ST), ph = (uint32_t)((T / ST) & 1);
+            wait_short(k_full + 8u * st, ph, dead);
+            if (lane == 0) mbar_arrive_tc(k_free + 8u * st);
+            wait_short(v_full + 8u * st, ph, dead);
+            if (lane == 0) mbar_arrive_tc(v_free + 8u * st);
+            __syncwarp();
+          }
+          continue;
+        }
+        wait_short(bar_q + 8u * g, (uint32_t)(items & 1), dead);
+        ++items;
+        issue_s(0);
+        if (n > 1) issue_s(1);
+        for (int i = 0; i < n; ++i, ++T, ++tg) {
+          const uint32_t st = (uint32_t)(T % ST), ph = (uint32_t)((tg >> 1) & 1);
+          const int b = tg & 1;
+          wait_short(v_full + 8u * st, (uint32_t)((T / ST) & 1), dead);
+          wait_short(bar_p + 16u * g + 8u * b, ph, dead);
+          __syncwarp();
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          if (elect_tc()) {
+            const uint64_t v = dv + (uint64_t)(st * (SM::TILE >> 4));
+#pragma unroll
+            for (int kk = 0; kk < TK / 16; ++kk) umma_ts_tc(t_o(g), t_s(g, b) + (uint32_t)(kk * 8), v + (uint64_t)(kk * 128), id_o, i > 0 || kk > 0);
+            umma_commit_tc(bar_o + 16u * g + 8u * b);
+            umma_commit_tc(v_free + 8u * st);
+          }
+          __syncwarp();
+          if (i + 2 < n) {
+            wait_short(bar_o + 16u * g + 8u * b, ph, dead);  // the scores two tiles ahead go over the weights that this product reads
+            issue_s(2);
+          }
         }
       }
     }
   } else if (warp >= 8) {
-    // ---- codes to fp16
-    constexpr int UNITS = TK * (HD / 16) / 128;  // 16 codes each, of keys a thread; as many of values
-    const int w = warp - 8, r8 = lane & 7, cq = lane >> 3;
+    // ---- codes to fp16: keys by the first four warps, values by the others
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    constexpr int UNITS = TK * (HD / 16) / 128;  // 16 codes each, of a thread
+    const int is_v = warp >= 12, w = warp & 3, r8 = lane & 7, cq = lane >> 3;
     // eight lanes side by side take the same columns of eight rows
     auto row_of = [&](int e) { return (HD == 128 ? e * 2 + (w & 1) : e * 4 + w) * 8 + r8; };
-    const int piece = HD == 128 ? (w >> 1) * 4 + cq : cq, nb = piece / 4;
+    const int piece = HD == 128 ? (w >> 1) * 4 + cq : cq, nb = piece / 4, c16 = (2 * piece) & 7;
+    const uint32_t full = is_v ? v_full : k_full, free_ = is_v ? v_free : k_free;
     int edges = 0;
-    while (walk.next(a, tt, p)) {
+    while (next_piece(p)) {
       const int low0 = a.window > 0 ? max(0, p.pos0 - a.window + 1) : 0, low1 = a.window > 0 ? max(0, p.pos0 + p.tokens - a.window) : 0, end = p.pos0 + p.tokens;
+#pragma unroll 1
       for (int i = p.begin; i < p.end; ++i, ++T) {
         const int rs = T % RAW, st = T % ST, key = p.key0 + i * TK;
         const bool edge = key + TK > p.pos0 + 1 || key < low1;  // some row does not see some key of the tile
-        mbar_wait_tc(raw_full + 8u * (uint32_t)rs, (uint32_t)((T / RAW) & 1), dead);
-        const unsigned char *codes = smem + SM::C + rs * 2 * SM::CODES, *sc = smem + SM::SC + rs * 2 * TK;
+        wait_short(raw_full + 8u * (uint32_t)rs, (uint32_t)((T / RAW) & 1), dead);
+        const unsigned char *codes = smem + SM::C + (rs * 2 + is_v) * SM::CODES, *sc = smem + SM::SC + rs * 2 * TK;
         auto seen = [&](int row) { return key + row >= low0 && key + row < end; };  // by some row
-        // the largest scales
-        uint32_t kt = 0, vt = 0;
+        uint4 code[UNITS];
+#pragma unroll
+        for (int e = 0; e < UNITS; ++e) {
+          const int row = row_of(e);
+          code[e] = *reinterpret_cast<const uint4*>(codes + row * HD + ((HD == 128 ? piece ^ (row & 7) : piece ^ ((row >> 1) & 3)) << 4));
+        }
+        // the lane's two keys: scales, the largest of the tile, and the factors that bring codes beside that
+        uint32_t sb[2], vb[2], top = is_v, v_top = 1;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int row = h * 32 + lane;
-          const uint32_t kb = sc[row], vb = sc[TK + row];
-          const bool yes = !edge || seen(row);
-          if (yes && kb != 255) kt = max(kt, kb);
-          if (yes && vb != 255) vt = max(vt, vb);
+          sb[h] = sc[is_v * TK + row], vb[h] = sc[TK + row];
+          if ((!edge || seen(row)) && sb[h] != 255) top = max(top, sb[h]);
+          if ((!edge || seen(row)) && vb[h] != 255) v_top = max(v_top, vb[h]);
         }
-        kt = __reduce_max_sync(0xffffffffu, kt), vt = max(__reduce_max_sync(0xffffffffu, vt), 1u);
-        auto at = [&](int row, int is_v) { return codes + is_v * SM::CODES + row * HD + ((HD == 128 ? piece ^ (row & 7) : piece ^ ((row >> 1) & 3)) << 4); };
-        uint4 kc[UNITS], vc[UNITS];
-#pragma unroll
-        for (int e = 0; e < UNITS; ++e) kc[e] = *reinterpret_cast<const uint4*>(at(row_of(e), 0)), vc[e] = *reinterpret_cast<const uint4*>(at(row_of(e), 1));
+        top = __reduce_max_sync(0xffffffffu, top), v_top = __reduce_max_sync(0xffffffffu, v_top);
         unsigned long long bad = 0;  // keys whose values are no numbers, where these must not meet a zero weight: zero values and scores that are no numbers
         if (edge && CODE == KV8_E4M3) {
           unsigned long long mine = 0;
+          if (is_v)
 #pragma unroll
-          for (int e = 0; e < UNITS; ++e)
-            if (kv8_nans(vc[e].x) | kv8_nans(vc[e].y) | kv8_nans(vc[e].z) | kv8_nans(vc[e].w)) mine |= 1ull << row_of(e);
+            for (int e = 0; e < UNITS; ++e)
+              if (kv8_nans(code[e].x) | kv8_nans(code[e].y) | kv8_nans(code[e].z) | kv8_nans(code[e].w)) mine |= 1ull << row_of(e);
           if (mine) atomicOr(&s_bad[edges & 1], mine);
-          asm volatile("bar.sync 1, 128;" ::: "memory");
+          asm volatile("bar.sync 1, 256;" ::: "memory");
           bad = *(volatile unsigned long long*)&s_bad[edges & 1];
-          if (w == 0 && lane == 0) s_bad[(edges & 1) ^ 1] = 0;  // (all are past the one before)
-          asm volatile("bar.sync 1, 128;" ::: "memory");
+          if (warp == 8 && lane == 0) s_bad[(edges & 1) ^ 1] = 0;  // (all are past the one before)
+          asm volatile("bar.sync 1, 256;" ::: "memory");
           ++edges;
         }
-        if (w == 0 && lane == 0) s_kt[T % SLOTS] = (int)kt, s_vt[T % SLOTS] = (int)vt;
+        if (warp == 8 && lane == 0) s_kt[T % SLOTS] = (int)top, s_vt[T % SLOTS] = (int)v_top;  // (both ahead of the keys: the softmax asks for no more than scores)
+        uint32_t factor[2];
+        bool clear = false;  // some values are not for the product: those of keys that no row sees, and those that are no numbers
 #pragma unroll
-        for (int is_v = 0; is_v < 2; ++is_v) {
-          if (T >= ST) mbar_wait_tc((is_v ? v_free : k_free) + 8u * (uint32_t)st, (uint32_t)((T / ST - 1) & 1), dead);
-          const uint32_t to = s0 + (is_v ? SM::V : SM::K) + st * SM::TILE + nb * KBLK;
+        for (int h = 0; h < 2; ++h) factor[h] = sb[h] == 0 ? 0u : pow2_h2((int)(top - sb[h]));
+        if (edge || __any_sync(0xffffffffu, sb[0] == 255 || sb[1] == 255 || vb[0] == 255 || vb[1] == 255)) {
+          clear = true;
 #pragma unroll
-          for (int e = 0; e < UNITS; ++e) {
-            const int row = row_of(e);
-            const uint32_t kb = sc[row], vb = sc[TK + row];
-            const bool none = vb == 255 || (bad >> row & 1);
-            const uint4 c = is_v ? vc[e] : kc[e];
-            const uint32_t b = is_v ? vb : kb;
-            uint32_t f = b == 0 ? 0u : pow2_h2((int)(is_v ? vt : kt) - (int)b);
-            if (!is_v && (none || kb == 255)) f = 0x7e007e00u;
-            uint32_t h[8];
-            kv8_unpack<CODE>(c.x, h[0], h[1]), kv8_unpack<CODE>(c.y, h[2], h[3]), kv8_unpack<CODE>(c.z, h[4], h[5]), kv8_unpack<CODE>(c.w, h[6], h[7]);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) h[j] = mul_h2(h[j], f);
-            if (is_v && (none || (edge && !seen(row)))) {
-#pragma unroll
-              for (int j = 0; j < 8; ++j) h[j] = 0;
-            }
-            const uint32_t line = to + row * 128;
-            const int c16 = (2 * piece) & 7;
-            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(line + ((c16 ^ r8) << 4)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
-            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(line + (((c16 + 1) ^ r8) << 4)), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7]) : "memory");
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive_tc((is_v ? v_full : k_full) + 8u * (uint32_t)st);
-            if (is_v) mbar_arrive_tc(raw_free + 8u * (uint32_t)rs);
+          for (int h = 0; h < 2; ++h) {
+            const int row = h * 32 + lane;
+            const bool none = vb[h] == 255 || (bad >> row & 1);
+            if (is_v ? none || !seen(row) : none || sb[h] == 255) factor[h] = is_v ? 0xffffffffu : 0x7e007e00u;
           }
         }
+        if (T >= ST) wait_short(free_ + 8u * (uint32_t)st, (uint32_t)((T / ST - 1) & 1), dead);
+        __syncwarp();
+        const uint32_t to = s0 + (is_v ? SM::V : SM::K) + st * SM::TILE + nb * KBLK;
+#pragma unroll
+        for (int e = 0; e < UNITS; ++e) {
+          const int row = row_of(e);
+          const uint32_t f = __shfl_sync(0xffffffffu, factor[HD == 128 ? e / 2 : e], row & 31);
+          const uint4 c = code[e];
+          uint32_t h[8];
+          kv8_unpack<CODE>(c.x, h[0], h[1]), kv8_unpack<CODE>(c.y, h[2], h[3]), kv8_unpack<CODE>(c.z, h[4], h[5]), kv8_unpack<CODE>(c.w, h[6], h[7]);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) h[j] = mul_h2(h[j], f);
+          if (clear) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) h[j] = f == 0xffffffffu ? 0u : h[j];
+          }
+          const uint32_t line = to + row * 128;
+          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(line + ((c16 ^ r8) << 4)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(line + (((c16 + 1) ^ r8) << 4)), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7]) : "memory");
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive_tc(full + 8u * (uint32_t)st), mbar_arrive_tc(raw_free + 8u * (uint32_t)rs);
       }
     }
   } else {
     // ---- softmax: this thread's row
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
     const int g = warp >> 2, row = g * 128 + (tid & 127), tok = row / G, gh = row - tok * G;
     const uint32_t la = (uint32_t)((warp & 3) * 32) << 16;
     int tg = 0;  // tiles of this row tile
     if (tid == 0) info[blockIdx.x].parts = 0;
-    while (walk.next(a, tt, p)) {
+    while (next_piece(p)) {
       const int rows = p.tokens * G;
       if (tid == 0 && !p.whole() && p.begin == 0)  // goes on in the CTAs behind; the item's last tile is at x1 - left + tiles - 1
         info[blockIdx.x] = JoinInfo{p.t0, p.tokens, p.kvh, (int)quotient(x1 - p.left + p.tiles - 1, share) - (int)blockIdx.x + 1};
@@ -682,41 +742,60 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
       // ---- the row's query
       float sl2;
       {
-        uint32_t x[HD / 2];
         const uint4* src = reinterpret_cast<const uint4*>(a.q + (size_t)(p.t0 + (mine ? tok : 0)) * a.q_stride + (size_t)(p.kvh * G + (mine ? gh : 0)) * HD);
+        auto words = [&](int at, uint32_t (&x)[32]) {
 #pragma unroll
-        for (int j = 0; j < HD / 8; ++j) {
-          const uint4 v = mine ? src[j] : make_uint4(0, 0, 0, 0);
-          x[4 * j] = v.x, x[4 * j + 1] = v.y, x[4 * j + 2] = v.z, x[4 * j + 3] = v.w;
+          for (int j = 0; j < 8; ++j) {
+            const uint4 v = mine ? src[at + j] : make_uint4(0, 0, 0, 0);
+            x[4 * j] = v.x, x[4 * j + 1] = v.y, x[4 * j + 2] = v.z, x[4 * j + 3] = v.w;
+          }
+        };
+        uint32_t x[32], most = 0;  // (64 elements at a time: the whole row would cost spills)
+#pragma unroll
+        for (int at = 0; at < HD / 8; at += 8) {
+          words(at, x);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) most = max(most, max(x[j] << 16 & 0x7fff0000u, x[j] & 0x7fff0000u));
         }
-        uint32_t most = 0;
-#pragma unroll
-        for (int j = 0; j < HD / 2; ++j) most = max(most, max(x[j] << 16 & 0x7fff0000u, x[j] & 0x7fff0000u));
         float there, back;
         query_scale(most, there, back);
         sl2 = a.scale_log2 * back;
 #pragma unroll
-        for (int j = 0; j < HD / 2; ++j) x[j] = pack_h(lo2f(x[j]) * there, hi2f(x[j]) * there);
-        __syncwarp();
+        for (int at = HD / 8 - 8; at >= 0; at -= 8) {
+          if (at < HD / 8 - 8) words(at, x);
 #pragma unroll
-        for (int j = 0; j < HD / 2; j += 32) tmem_st32_tc(t_q(g) + la + j, x + j);
-        tmem_wait_st_tc();
+          for (int j = 0; j < 32; ++j) x[j] = pack_h(lo2f(x[j]) * there, hi2f(x[j]) * there);
+          if constexpr (SM::Q_TMEM) {
+            __syncwarp();
+            tmem_st32_tc(t_q(g) + la + at * 4, x);
+          } else {
+            const uint32_t line = s0 + SM::Q + g * SM::QTILE + (at / 8) * SM::QBLK + (tid & 127) * 128;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(line + ((j ^ (tid & 7)) << 4)), "r"(x[4 * j]), "r"(x[4 * j + 1]), "r"(x[4 * j + 2]), "r"(x[4 * j + 3]) : "memory");
+          }
+        }
+        if constexpr (SM::Q_TMEM) tmem_wait_st_tc();
+        else asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         mbar_arrive_tc(bar_q + 8u * g);
       }
       const int my_pos = p.pos0 + min(tok, p.tokens - 1), my_low = a.window > 0 ? max(0, my_pos - a.window + 1) : 0;
       float m_ref = -INFINITY, l_run = 0.f;
       int lr = 1;  // the scale of the values that O is beside, as a byte
+#pragma unroll 1
       for (int i = p.begin; i < p.end; ++i, ++T, ++tg) {
-        const uint32_t ts = t_s(g) + la;
+        const int b = tg & 1;
+        const uint32_t ts = t_s(g, b) + la, ph = (uint32_t)((tg >> 1) & 1);
         const int key = p.key0 + i * TK, last = my_pos - key, low = my_low - key;  // the first key of the tile; the last and the first that the row sees
-        mbar_wait_warp_tc(bar_s + 8u * g, (uint32_t)(tg & 1), dead);
+        wait_short(bar_s + 16u * g + 8u * b, ph, dead);
+        __syncwarp();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const float s = fmaxf(sl2 * __uint_as_float((uint32_t)s_kt[T % SLOTS] << 23), 1e-37f);  // (zero must not meet minus infinity)
-        const int vt = s_vt[T % SLOTS];
-        uint32_t r[64];
+        uint32_t r[TK];
         tmem_ld32_tc(ts, r);
         tmem_ld32_tc(ts + 32, r + 32);
+        const float s = fmaxf(sl2 * __uint_as_float((uint32_t)s_kt[T % SLOTS] << 23), 1e-37f);  // (zero must not meet minus infinity)
+        const int vt = s_vt[T % SLOTS];
         tmem_wait_ld_tc();
         if (last < TK - 1) {
 #pragma unroll
@@ -743,13 +822,12 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
         if (grow) {
           if (m_new > -INFINITY) f = ex2_tc(m_ref - m_new);  // (nothing before: 0)
           m_ref = m_new;
+          l_run *= f;
+          if (vt > lr) f *= vt - lr < 127 ? __uint_as_float((uint32_t)(127 - (vt - lr)) << 23) : 0.f, lr = vt;
         }
-        l_run *= f;
-        if (vt > lr) f *= vt - lr < 127 ? __uint_as_float((uint32_t)(127 - (vt - lr)) << 23) : 0.f, lr = vt;
-        // weights by 2^12 and their values' scale beside the largest; 2^-64 of that is none in fp16, and one in the sum
+        // weights by 2^7 and their values' scale beside the largest; 2^-64 of that is none in fp16, and one in the sum
         const int d = max(vt - lr, -64) + P_EXP;
-        const float n = (m_ref > -INFINITY ? -m_ref : 0.f) + (float)d;
-        const unsigned long long s2 = twice_tc(s), n2 = twice_tc(n);
+        const unsigned long long s2 = twice_tc(s), n2 = twice_tc((m_ref > -INFINITY ? -m_ref : 0.f) + (float)d);
         float rs[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < TK; c += 32) {
@@ -765,23 +843,29 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
           tmem_st16_tc(ts + c / 2, wt);
         }
         l_run += ((rs[0] + rs[1]) + (rs[2] + rs[3])) * __uint_as_float((uint32_t)(127 - d) << 23);
-        if (grow && i > p.begin) {  // the product of the tile before is in: these scores were asked for behind it
-#pragma unroll
-          for (int c = 0; c < HD; c += 32) {
-            uint32_t o[32];
+        if (grow && i > p.begin) {  // O, behind the product of the tile before
+          wait_short(bar_o + 16u * g + 8u * (b ^ 1), (uint32_t)(((tg - 1) >> 1) & 1), dead);
+          __syncwarp();
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+          for (int c = 0; c < HD; c += 64) {
+            uint32_t o[64];
             tmem_ld32_tc(t_o(g) + la + c, o);
+            tmem_ld32_tc(t_o(g) + la + c + 32, o + 32);
             tmem_wait_ld_tc();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+            for (int j = 0; j < 64; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
             tmem_st32_tc(t_o(g) + la + c, o);
+            tmem_st32_tc(t_o(g) + la + c + 32, o + 32);
           }
         }
         tmem_wait_st_tc();
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        mbar_arrive_tc(bar_p + 8u * g);
+        mbar_arrive_tc(bar_p + 16u * g + 8u * b);
       }
       // ---- the row of the result
-      mbar_wait_warp_tc(bar_o + 8u * g, (uint32_t)((tg - 1) & 1), dead);
+      wait_short(bar_o + 16u * g + 8u * ((tg - 1) & 1), (uint32_t)(((tg - 1) >> 1) & 1), dead);
+        __syncwarp();
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const bool whole = p.whole();
       const float back = __uint_as_float((uint32_t)lr << 23) * (1.f / (1 << P_EXP)), nan = __int_as_float(0x7fc00000);
@@ -822,7 +906,7 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 16) {
     drain_tc(dead);
     if (lane == 0) report_tc(dead, a.status);
     __syncwarp();
