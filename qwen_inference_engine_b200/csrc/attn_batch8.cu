@@ -26,6 +26,39 @@ namespace {
 constexpr float LAG = 8.f;
 constexpr int P_EXP = 7;
 
+// mbar_wait_tc in few instructions: with the compiler's loop around a try the warps that wait had half of the SM's instructions.  2^26 tries are about two seconds.
+__device__ __forceinline__ void wait_short(uint32_t bar, uint32_t parity, volatile int* dead) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  if (done || *dead) return;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 i;\n\t"
+      "mov.u32 i, 0;\n"
+      "again:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "@p bra.uni out;\n\t"
+      "add.u32 i, i, 1;\n\t"
+      "setp.lt.u32 q, i, 67108864;\n\t"
+      "@q bra.uni again;\n"
+      "out:\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  if (!done) *dead = 1;
+}
+// a 16-byte piece of a row in shared memory: in the order that TMA gives with a swizzle over a row's bytes
+template <int HD>
+__device__ __forceinline__ int piece_at(int row, int piece) {
+  return row * HD + ((HD == 128 ? piece ^ (row & 7) : piece ^ (row >> 1 & 3)) << 4);
+}
+
 // ---------------------------------------------------------------- blocks of at most 16 rows
 constexpr int ROWS_F = 16, THR_F = 256, WARPS_F = THR_F / 32;
 
@@ -60,30 +93,37 @@ struct Ring {
   static constexpr int UNIT = 16 * HD, STAGES = HD == 128 ? 3 : 4, WARP = STAGES * 2 * UNIT;
 };
 template <int HD>
-constexpr int SMEM_F = WARPS_F * Ring<HD>::WARP;
+constexpr int SMEM_F = WARPS_F * Ring<HD>::WARP + 1024;
 
-// A warp takes every eighth unit of 16 keys of the CTA's stretch, by copies into a ring of its own: keys from there as the rows of a product K Q^T, the weights by a transposition of
+// A warp takes every eighth unit of 16 keys of the CTA's stretch, by copies into a ring of its own (TMA, or for pages of other than multiples of 16 positions 16 bytes a lane): keys from there as the rows of a product K Q^T, the weights by a transposition of
 // 8 x 8 into fragments of V^T P^T, values with neighbouring keys' bytes beside each other.  The columns of a row are numbered so that a lane's are 16 bytes together.  No barrier but the
 // warp's own; the warps' results are added up at the end of a piece.
-template <int HD, int CODE, int NB>
-__global__ void __launch_bounds__(THR_F, NB == 1 ? 2 : 1) attn_few8_kernel(BatchAttnArgs a, Kv8Geom kv, JoinShape sh, int tt) {
+template <int HD, int CODE, int NB, bool TMA>
+__global__ void __launch_bounds__(THR_F, NB == 1 ? 2 : 1) attn_few8_kernel(BatchAttnArgs a, Kv8Geom kv, JoinShape sh, int tt, const __grid_constant__ CUtensorMap cm) {
   constexpr int C = HD / 64, VW = HD / 32, MB = HD / 16;  // 16-byte pieces of a key row a lane; words of a value row a lane; blocks of 16 columns
   constexpr int UNIT = Ring<HD>::UNIT, ST = Ring<HD>::STAGES;
   static_assert(NB * 8 * HD * 4 <= Ring<HD>::WARP, "a warp's results take its ring's place");
-  extern __shared__ __align__(128) unsigned char s_ring[];  // [warp][stage][k|v][key][column], and in its place the warp's results [row][column]
+  extern __shared__ __align__(1024) unsigned char smem_raw[];  // [warp][stage][k|v][key][column], and in its place the warp's results [row][column]
   __shared__ long long s_sums[THR_F / 32];
   __shared__ Walk s_walk;
   __shared__ float s_m[WARPS_F][NB * 8], s_l[WARPS_F][NB * 8];
   __shared__ int s_r[WARPS_F];
-  __shared__ uint8_t s_scale[WARPS_F][ST][32];
+  __shared__ __align__(16) uint8_t s_scale[WARPS_F][ST][32];  // keys', values'
+  __shared__ unsigned long long s_bar[WARPS_F][ST];
+  __shared__ int dead_s;
+  volatile int* dead = &dead_s;
+  unsigned char* s_ring = smem_raw + ((smem_u32(smem_raw) + 1023u & ~1023u) - smem_u32(smem_raw));
   float* s_o = reinterpret_cast<float*>(s_ring);
+  if (TMA && threadIdx.x == 32) asm volatile("prefetch.tensormap [%0];" ::"l"(&cm) : "memory");
   pdl_wait();
   pdl_trigger();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const uint32_t ring = smem_u32(s_ring) + warp * Ring<HD>::WARP;
-  // 16-byte pieces of a row lie in an order of the row's, so that what lanes read together is in different banks
-  auto k_at = [](int row, int piece) { return HD == 128 ? row * 128 + ((piece ^ ((row & 1) << 2)) << 4) : row * 64 + (piece << 4); };
-  auto v_at = [](int row, int piece) { return HD == 128 ? row * 128 + ((piece ^ (row & 6)) << 4) : row * 64 + ((piece ^ ((row >> 1) & 3)) << 4); };
+  if (TMA && lane == 0) {
+    for (int i = 0; i < ST; ++i) mbar_init_tc(smem_u32(&s_bar[warp][i]), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (tid == 0) dead_s = 0;
   if (tid == 0) s_walk.left = 0;
   const auto [share, x1] = find_stretch<THR_F>(a, tt, s_sums, &s_walk);
   __syncthreads();
@@ -92,6 +132,7 @@ __global__ void __launch_bounds__(THR_F, NB == 1 ? 2 : 1) attn_few8_kernel(Batch
   float* parts = reinterpret_cast<float*>(info + gridDim.x);
   if (tid == 0) info[blockIdx.x].parts = 0;
   Piece p;
+  int J = 0;  // (TMA) units that the warp had in the pieces before
   while (walk.next(a, tt, p)) {
     const int sub = p.kvh % sh.subs, kvh = p.kvh / sh.subs, G = min(sh.g, sh.group - sub * sh.g), rows = p.tokens * G;
     const size_t head0 = (size_t)kvh * sh.group + sub * sh.g;
@@ -100,13 +141,30 @@ __global__ void __launch_bounds__(THR_F, NB == 1 ? 2 : 1) attn_few8_kernel(Batch
     const int units = (k_hi - k_lo + 15) / 16;
     const int* bt = a.block_table + (size_t)p.slot * a.max_pages;
     const int P = kv.page_size, v_off = kv.n_kv * P;
-    // the key of the unit that is the lane's (lanes 16 .. 31 the same again): its vector in the pool
-    auto vec_of = [&](int u) {
-      const int key = min(k_lo + u * 16 + (lane & 15), k_hi - 1), pg = key / P;
+    auto vec_at = [&](int key) {  // a key's vector in the pool
+      const int pg = key / P;
       int page = bt[pg];
       if (page < 0 || page >= kv.n_pages) page = 0;
       return ((page * kv.n_layers + a.layer) * 2 * kv.n_kv + kvh) * P + (key - pg * P);
     };
+    // TMA: unit j of the warp's, from the vector of its first key, which lane j % 32 holds
+    const int n_mine = units > warp ? (units - warp + WARPS_F - 1) / WARPS_F : 0;
+    int held = 0;
+    auto ask = [&](int j) {
+      if ((j & 31) == 0) held = vec_at(k_lo + min(warp + (j + lane) * WARPS_F, units - 1) * 16);
+      const int vec = __shfl_sync(0xffffffffu, held, j & 31);
+      const uint32_t stage = (uint32_t)((J + j) % ST), bar = smem_u32(&s_bar[warp][stage]), dst = ring + stage * 2 * UNIT, sc = smem_u32(s_scale[warp][stage]);
+      if (elect_tc()) {
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"((uint32_t)(2 * UNIT + 32)) : "memory");
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(&cm), "r"(bar), "r"(0), "r"(vec) : "memory");
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst + UNIT), "l"(&cm), "r"(bar), "r"(0), "r"(vec + v_off) : "memory");
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(sc), "l"(kv.scale + vec), "r"(16), "r"(bar) : "memory");
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(sc + 16), "l"(kv.scale + vec + v_off), "r"(16), "r"(bar) : "memory");
+      }
+      __syncwarp();
+    };
+    // 16 bytes a lane: the key of the unit that is the lane's (lanes 16 .. 31 the same again)
+    auto vec_of = [&](int u) { return vec_at(min(k_lo + u * 16 + (lane & 15), k_hi - 1)); };
     auto copy = [&](int vec, int stage) {
       constexpr int PIECES = HD / 16, EACH = 16 * PIECES / 32;
 #pragma unroll
@@ -114,8 +172,8 @@ __global__ void __launch_bounds__(THR_F, NB == 1 ? 2 : 1) attn_few8_kernel(Batch
         const int row = (i * 32 + lane) / PIECES, piece = lane % PIECES;
         const int r = __shfl_sync(0xffffffffu, vec, row);
         const uint8_t* src = kv.codes + (size_t)r * HD + piece * 16;
-        cp_async16(ring + stage * 2 * UNIT + k_at(row, piece), src);
-        cp_async16(ring + stage * 2 * UNIT + UNIT + v_at(row, piece), src + (size_t)v_off * HD);
+        cp_async16(ring + stage * 2 * UNIT + piece_at<HD>(row, piece), src);
+        cp_async16(ring + stage * 2 * UNIT + UNIT + piece_at<HD>(row, piece), src + (size_t)v_off * HD);
       }
     };
     auto scale_of = [&](int vec) { return kv.scale[vec + (lane >> 4) * v_off]; };  // lanes 0 .. 15: keys', 16 .. 31: values'
@@ -125,6 +183,10 @@ __global__ void __launch_bounds__(THR_F, NB == 1 ? 2 : 1) attn_few8_kernel(Batch
 #pragma unroll
     for (int s = 0; s < ST - 1; ++s) {
       const int u = warp + s * WARPS_F;
+      if constexpr (TMA) {
+        if (s < n_mine) ask(s);
+        continue;
+      }
       if (u < units) {
         const int vec = vec_of(u);
         copy(vec, s);
@@ -132,7 +194,7 @@ __global__ void __launch_bounds__(THR_F, NB == 1 ? 2 : 1) attn_few8_kernel(Batch
       }
       cp_async_commit();
     }
-    if (warp + (ST - 1) * WARPS_F < units) vec_next = vec_of(warp + (ST - 1) * WARPS_F);
+    if (!TMA && warp + (ST - 1) * WARPS_F < units) vec_next = vec_of(warp + (ST - 1) * WARPS_F);
     // ---- queries: the lane's columns of row g (and 8 + g)
     uint32_t q[NB][C][4][2];
     float qf[NB][2];
@@ -182,19 +244,26 @@ __global__ void __launch_bounds__(THR_F, NB == 1 ? 2 : 1) attn_few8_kernel(Batch
     for (int nb = 0; nb < NB; ++nb) m[nb][0] = m[nb][1] = -INFINITY, l[nb][0] = l[nb][1] = 0.f;
 #pragma unroll
     for (int s = 0; s < ST - 1; ++s)
-      if (warp + s * WARPS_F < units) s_scale[warp][s][lane] = first[s];
-    int stage = 0, into = ST - 1;  // of the unit at hand, and of the one that is asked for
-    for (int u = warp; u < units; u += WARPS_F) {
-      if (pend_at >= 0) s_scale[warp][pend_at][lane] = pend;  // (a step later than asked for)
-      cp_async_wait<ST - 2>();
-      __syncwarp();  // the unit is there, and nobody reads the one before any more
-      pend_at = -1;
-      if (u + (ST - 1) * WARPS_F < units) {
-        copy(vec_next, into);
-        pend = scale_of(vec_next), pend_at = into;
-        if (u + ST * WARPS_F < units) vec_next = vec_of(u + ST * WARPS_F);
+      if (!TMA && warp + s * WARPS_F < units) s_scale[warp][s][lane] = first[s];
+    int stage = TMA ? J % ST : 0, into = ST - 1, j = 0;  // of the unit at hand, and of the one that is asked for
+    for (int u = warp; u < units; u += WARPS_F, ++j) {
+      if constexpr (TMA) {
+        __syncwarp();  // nobody reads the unit before any more, and its stage is the next one's
+        if (j + ST - 1 < n_mine) ask(j + ST - 1);
+        wait_short(smem_u32(&s_bar[warp][stage]), (uint32_t)((J + j) / ST & 1), dead);
+        __syncwarp();
+      } else {
+        if (pend_at >= 0) s_scale[warp][pend_at][lane] = pend;  // (a step later than asked for)
+        cp_async_wait<ST - 2>();
+        __syncwarp();  // the unit is there, and nobody reads the one before any more
+        pend_at = -1;
+        if (u + (ST - 1) * WARPS_F < units) {
+          copy(vec_next, into);
+          pend = scale_of(vec_next), pend_at = into;
+          if (u + ST * WARPS_F < units) vec_next = vec_of(u + ST * WARPS_F);
+        }
+        cp_async_commit();
       }
-      cp_async_commit();
       const int key0 = k_lo + u * 16;
       const bool edge = key0 + 16 > p.pos0 + 1 || key0 < low1;  // some row does not see some key of the unit
       const uint32_t at = ring + stage * 2 * UNIT;
@@ -204,8 +273,8 @@ __global__ void __launch_bounds__(THR_F, NB == 1 ? 2 : 1) attn_few8_kernel(Batch
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         uint32_t k0[4], k1[4];
-        ld_shared_v4(at + k_at(g, c * 4 + t), k0);
-        ld_shared_v4(at + k_at(g + 8, c * 4 + t), k1);
+        ld_shared_v4(at + piece_at<HD>(g, c * 4 + t), k0);
+        ld_shared_v4(at + piece_at<HD>(g + 8, c * 4 + t), k1);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           uint32_t a0, a1, a2, a3;
@@ -219,11 +288,12 @@ __global__ void __launch_bounds__(THR_F, NB == 1 ? 2 : 1) attn_few8_kernel(Batch
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int row = 2 * t + (i & 1) + 8 * (i >> 1);
-        if constexpr (HD == 128) ld_shared_v4(at + UNIT + v_at(row, g), vr[i]);
-        else asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(vr[i][0]), "=r"(vr[i][1]) : "r"(at + UNIT + v_at(row, g >> 1) + (g & 1) * 8) : "memory");
+        if constexpr (HD == 128) ld_shared_v4(at + UNIT + piece_at<HD>(row, g), vr[i]);
+        else asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(vr[i][0]), "=r"(vr[i][1]) : "r"(at + UNIT + piece_at<HD>(row, g >> 1) + (g & 1) * 8) : "memory");
       }
       const uint32_t kb0 = sc[g], kb1 = sc[g + 8], vb0 = sc[g + 16], vb1 = sc[g + 24];
-      const int top = (int)__reduce_max_sync(0xffffffffu, lane < 16 || sc[lane] == 255 ? 0u : (uint32_t)sc[lane]);
+      const int key_l = key0 + (lane & 15);
+      const int top = (int)__reduce_max_sync(0xffffffffu, lane < 16 || sc[lane] == 255 || (edge && (key_l >= end || key_l < low0)) ? 0u : (uint32_t)sc[lane]);
       float ks[2] = {kv8_scale(vb0 == 255 ? 255u : kb0), kv8_scale(vb1 == 255 ? 255u : kb1)};
       if (edge && CODE == KV8_E4M3) {  // values that are no numbers must not meet a zero weight: they are zero, and their keys' scores no numbers
         uint32_t bad = 0;
@@ -315,7 +385,8 @@ __global__ void __launch_bounds__(THR_F, NB == 1 ? 2 : 1) attn_few8_kernel(Batch
       if (++stage == ST) stage = 0;
       if (++into == ST) into = 0;
     }
-    cp_async_wait<0>();
+    J += n_mine;
+    if (!TMA) cp_async_wait<0>();
     __syncwarp();
     // ---- the warps' results together
 #pragma unroll
@@ -350,33 +421,38 @@ __global__ void __launch_bounds__(THR_F, NB == 1 ? 2 : 1) attn_few8_kernel(Batch
       }
       const float back = __uint_as_float((uint32_t)r << 23) * (1.f / (1 << P_EXP));
       if (whole) {
-        const float f = sum > 0.f ? back / sum : sum;
+        const float f = *dead ? __int_as_float(0x7fc00000) : sum > 0.f ? back / sum : sum;
         const int tok = n / G;
         *reinterpret_cast<uint2*>(a.out + (size_t)(p.t0 + tok) * a.out_stride + (head0 + n - tok * G) * HD + c * 4) =
             make_uint2(pack2f(acc.x * f, acc.y * f), pack2f(acc.z * f, acc.w * f));
       } else {
         float* part = parts + ((size_t)blockIdx.x * 2 + (p.begin == 0)) * PART<HD, ROWS_F>;
-        if (c == 0) part[ROWS_F * HD + n] = top, part[ROWS_F * HD + ROWS_F + n] = sum;
+        if (c == 0) part[ROWS_F * HD + n] = top, part[ROWS_F * HD + ROWS_F + n] = *dead ? __int_as_float(0x7fc00000) : sum;
         *reinterpret_cast<float4*>(part + (c * ROWS_F + n) * 4) = make_float4(acc.x * back, acc.y * back, acc.z * back, acc.w * back);
       }
     }
     if (tid == 0 && !whole && p.begin == 0) info[blockIdx.x] = JoinInfo{p.t0, p.tokens, p.kvh, (int)quotient(x1 - p.left + p.tiles - 1, share) - (int)blockIdx.x + 1};
+    if (TMA) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (copies take the results' place)
     __syncthreads();
+  }
+  if (TMA && tid == 0) {
+    drain_tc(dead);
+    report_tc(dead, a.status);
   }
 }
 
-template <int HD, int CODE, int NB>
-cudaError_t launch_few(const BatchAttnArgs& a, const Kv8Geom& kv, const JoinShape& sh, int tt, cudaStream_t st) {
+template <int HD, int CODE, int NB, bool TMA>
+cudaError_t launch_few(const BatchAttnArgs& a, const Kv8Geom& kv, const JoinShape& sh, int tt, const TensorMap2D& cm, cudaStream_t st) {
   static PerDeviceOnce set;
   if (set.need()) {
-    const cudaError_t e = cudaFuncSetAttribute(attn_few8_kernel<HD, CODE, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_F<HD>);
+    const cudaError_t e = cudaFuncSetAttribute(attn_few8_kernel<HD, CODE, NB, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_F<HD>);
     if (e != cudaSuccess) return e;
     set.done();
   }
   const int ctas = 2 * a.num_sms;
   BatchAttnArgs b = a;
   b.kv.n_kv *= sh.subs;
-  const cudaError_t e = launched(launch_k(attn_few8_kernel<HD, CODE, NB>, dim3(ctas), dim3(THR_F), SMEM_F<HD>, st, b, kv, sh, tt));
+  const cudaError_t e = launched(launch_k(attn_few8_kernel<HD, CODE, NB, TMA>, dim3(ctas), dim3(THR_F), SMEM_F<HD>, st, b, kv, sh, tt, *reinterpret_cast<const CUtensorMap*>(&cm)));
   return e != cudaSuccess ? e : launch_join<HD, ROWS_F>(a, sh, ctas, st);
 }
 
@@ -400,33 +476,6 @@ struct SmemP {
   static constexpr int C = 0, K = RAW * 2 * CODES, V = K + ST * TILE, Q = V + ST * TILE, SC = Q + (Q_TMEM ? 0 : 2 * QTILE), BAR = SC + RAW * 2 * TK, TOTAL = BAR + 512 + 1024;
   static_assert(TOTAL <= 226 * 1024 && ST + 4 <= SLOTS, "");
 };
-// mbar_wait_tc in few instructions: with the compiler's loop around a try the warps that wait had half of the SM's instructions.  2^26 tries are about two seconds.
-__device__ __forceinline__ void wait_short(uint32_t bar, uint32_t parity, volatile int* dead) {
-  uint32_t done;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(done)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  if (done || *dead) return;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t.reg .u32 i;\n\t"
-      "mov.u32 i, 0;\n"
-      "again:\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "@p bra.uni out;\n\t"
-      "add.u32 i, i, 1;\n\t"
-      "setp.lt.u32 q, i, 67108864;\n\t"
-      "@q bra.uni again;\n"
-      "out:\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(done)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  if (!done) *dead = 1;
-}
 // D = F32, A = B = F16
 __device__ __forceinline__ uint32_t idesc_h(int m, int n, bool b_mn) { return idesc_tc(m, n, b_mn) & ~((1u << 7) | (1u << 10)); }
 __device__ __forceinline__ void cp_async_arrive(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
@@ -944,14 +993,15 @@ cudaError_t launch_attention_batch8(const BatchAttnArgs& a, const Kv8Geom& kv, c
   const bool tma = P % 16 == 0 && (reinterpret_cast<uintptr_t>(kv.scale) & 15) == 0;
   const int box = P % 64 == 0 ? 64 : P % 32 == 0 ? 32 : 16;  // the largest that divides a page and a tile
   TensorMap2D cm{};
-  if (!few && tma) {
-    const cudaError_t e = make_tensor_map_kv8(&cm, kv.codes, (unsigned long long)kv.n_pages * kv.n_layers * 2ull * kv.n_kv * P, kv.hd, box);
+  if (tma) {
+    const cudaError_t e = make_tensor_map_kv8(&cm, kv.codes, (unsigned long long)kv.n_pages * kv.n_layers * 2ull * kv.n_kv * P, kv.hd, few ? 16 : box);
     if (e != cudaSuccess) return e;
   }
   auto go = [&](auto hd, auto code) {
     constexpr int HD = decltype(hd)::value, CODE = decltype(code)::value;
     if (!few) return tma ? launch_prompt<HD, CODE, true>(a, kv, group, cm, box, st) : launch_prompt<HD, CODE, false>(a, kv, group, cm, box, st);
-    return group <= 8 ? launch_few<HD, CODE, 1>(a, kv, sh, 8 / g, st) : launch_few<HD, CODE, 2>(a, kv, sh, ROWS_F / g, st);
+    if (tma) return group <= 8 ? launch_few<HD, CODE, 1, true>(a, kv, sh, 8 / g, cm, st) : launch_few<HD, CODE, 2, true>(a, kv, sh, ROWS_F / g, cm, st);
+    return group <= 8 ? launch_few<HD, CODE, 1, false>(a, kv, sh, 8 / g, cm, st) : launch_few<HD, CODE, 2, false>(a, kv, sh, ROWS_F / g, cm, st);
   };
   using std::integral_constant;
   if (kv.hd == 64) return kv.code == KV8_E4M3 ? go(integral_constant<int, 64>(), integral_constant<int, KV8_E4M3>()) : go(integral_constant<int, 64>(), integral_constant<int, KV8_INT8>());
