@@ -60,7 +60,7 @@ __device__ __forceinline__ int piece_at(int row, int piece) {
 }
 
 // ---------------------------------------------------------------- blocks of at most 16 rows
-constexpr int ROWS_F = 16, THR_F = 256, WARPS_F = THR_F / 32;
+constexpr int ROWS_F = 16;
 
 // (volatile: instructions that a whole warp executes together stay where they are, between what brings its threads together)
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -87,28 +87,27 @@ __device__ __forceinline__ void query_scale(uint32_t amax, float& there, float& 
   if (e >= 255) there = back = __uint_as_float(0x7fc00000u);
 }
 
-// keys and values on their way to a warp: units of 16 keys
+// keys and values on their way to a warp, in units of 32 keys; two CTAs an SM
 template <int HD>
 struct Ring {
-  static constexpr int UNIT = 16 * HD, STAGES = HD == 128 ? 3 : 4, WARP = STAGES * 2 * UNIT;
+  static constexpr int WARPS = HD == 128 ? 6 : 8, THR = WARPS * 32;
+  static constexpr int UNIT = 32 * HD, STAGES = HD == 128 ? 2 : 3, WARP = STAGES * 2 * UNIT, SMEM = WARPS * WARP + 1024;
 };
-template <int HD>
-constexpr int SMEM_F = WARPS_F * Ring<HD>::WARP + 1024;
 
-// A warp takes every eighth unit of 16 keys of the CTA's stretch, by copies into a ring of its own (TMA, or for pages of other than multiples of 16 positions 16 bytes a lane): keys from there as the rows of a product K Q^T, the weights by a transposition of
-// 8 x 8 into fragments of V^T P^T, values with neighbouring keys' bytes beside each other.  The columns of a row are numbered so that a lane's are 16 bytes together.  No barrier but the
-// warp's own; the warps' results are added up at the end of a piece.
+// A warp takes units of 32 keys of the CTA's stretch, one of WARPS, by copies into a ring of its own (TMA boxes of as many rows as divide a page, or for pages of other than multiples of
+// four positions 16 bytes a lane): keys from there as the rows of a product K Q^T, the weights by a transposition of 8 x 8 into fragments of V^T P^T, values with neighbouring keys' bytes
+// beside each other.  The columns of a row are numbered so that a lane's are 16 bytes together.  No barrier but the warp's own; the warps' results are added up at the end of a piece.
 template <int HD, int CODE, int NB, bool TMA>
-__global__ void __launch_bounds__(THR_F, NB == 1 ? 2 : 1) attn_few8_kernel(BatchAttnArgs a, Kv8Geom kv, JoinShape sh, int tt, const __grid_constant__ CUtensorMap cm) {
+__global__ void __launch_bounds__(Ring<HD>::THR, NB == 1 ? 2 : 1) attn_few8_kernel(BatchAttnArgs a, Kv8Geom kv, JoinShape sh, int tt, int box, const __grid_constant__ CUtensorMap cm) {
   constexpr int C = HD / 64, VW = HD / 32, MB = HD / 16;  // 16-byte pieces of a key row a lane; words of a value row a lane; blocks of 16 columns
-  constexpr int UNIT = Ring<HD>::UNIT, ST = Ring<HD>::STAGES;
+  constexpr int UNIT = Ring<HD>::UNIT, ST = Ring<HD>::STAGES, WARPS_F = Ring<HD>::WARPS, THR_F = Ring<HD>::THR;
   static_assert(NB * 8 * HD * 4 <= Ring<HD>::WARP, "a warp's results take its ring's place");
   extern __shared__ __align__(1024) unsigned char smem_raw[];  // [warp][stage][k|v][key][column], and in its place the warp's results [row][column]
   __shared__ long long s_sums[THR_F / 32];
   __shared__ Walk s_walk;
   __shared__ float s_m[WARPS_F][NB * 8], s_l[WARPS_F][NB * 8];
   __shared__ int s_r[WARPS_F];
-  __shared__ __align__(16) uint8_t s_scale[WARPS_F][ST][32];  // keys', values'
+  __shared__ uint8_t s_scale[WARPS_F][ST][64];  // keys', values'
   __shared__ unsigned long long s_bar[WARPS_F][ST];
   __shared__ int dead_s;
   volatile int* dead = &dead_s;
@@ -137,77 +136,65 @@ __global__ void __launch_bounds__(THR_F, NB == 1 ? 2 : 1) attn_few8_kernel(Batch
     const int sub = p.kvh % sh.subs, kvh = p.kvh / sh.subs, G = min(sh.g, sh.group - sub * sh.g), rows = p.tokens * G;
     const size_t head0 = (size_t)kvh * sh.group + sub * sh.g;
     const int low0 = a.window > 0 ? max(0, p.pos0 - a.window + 1) : 0, low1 = a.window > 0 ? max(0, p.pos0 + p.tokens - a.window) : 0;  // of the first and the last token
-    const int end = p.pos0 + p.tokens, k_lo = max(p.key0 + p.begin * AB_TK, low0 & ~15), k_hi = min(p.key0 + p.end * AB_TK, end);
-    const int units = (k_hi - k_lo + 15) / 16;
+    const int end = p.pos0 + p.tokens, k_lo = max(p.key0 + p.begin * AB_TK, low0 & ~31), k_hi = min(p.key0 + p.end * AB_TK, end);
+    const int units = (k_hi - k_lo + 31) / 32, n = units > warp ? (units - warp + WARPS_F - 1) / WARPS_F : 0;  // the piece's, the warp's
     const int* bt = a.block_table + (size_t)p.slot * a.max_pages;
     const int P = kv.page_size, v_off = kv.n_kv * P;
-    auto vec_at = [&](int key) {  // a key's vector in the pool
-      const int pg = key / P;
+    auto vec_of = [&](int j) {  // of the lane's key of unit j: its vector in the pool
+      const int key = min(k_lo + (warp + j * WARPS_F) * 32 + lane, k_hi - 1), pg = key / P;
       int page = bt[pg];
       if (page < 0 || page >= kv.n_pages) page = 0;
       return ((page * kv.n_layers + a.layer) * 2 * kv.n_kv + kvh) * P + (key - pg * P);
     };
-    // TMA: unit j of the warp's, from the vector of its first key, which lane j % 32 holds
-    const int n_mine = units > warp ? (units - warp + WARPS_F - 1) / WARPS_F : 0;
-    int held = 0;
-    auto ask = [&](int j) {
-      if ((j & 31) == 0) held = vec_at(k_lo + min(warp + (j + lane) * WARPS_F, units - 1) * 16);
-      const int vec = __shfl_sync(0xffffffffu, held, j & 31);
-      const uint32_t stage = (uint32_t)((J + j) % ST), bar = smem_u32(&s_bar[warp][stage]), dst = ring + stage * 2 * UNIT, sc = smem_u32(s_scale[warp][stage]);
-      if (elect_tc()) {
-        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"((uint32_t)(2 * UNIT + 32)) : "memory");
-        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(&cm), "r"(bar), "r"(0), "r"(vec) : "memory");
-        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst + UNIT), "l"(&cm), "r"(bar), "r"(0), "r"(vec + v_off) : "memory");
-        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(sc), "l"(kv.scale + vec), "r"(16), "r"(bar) : "memory");
-        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(sc + 16), "l"(kv.scale + vec + v_off), "r"(16), "r"(bar) : "memory");
-      }
-      __syncwarp();
-    };
-    // 16 bytes a lane: the key of the unit that is the lane's (lanes 16 .. 31 the same again)
-    auto vec_of = [&](int u) { return vec_at(min(k_lo + u * 16 + (lane & 15), k_hi - 1)); };
     auto copy = [&](int vec, int stage) {
-      constexpr int PIECES = HD / 16, EACH = 16 * PIECES / 32;
+      const uint32_t dst = ring + stage * 2 * UNIT;
+      if constexpr (TMA) {
+        const uint32_t bar = smem_u32(&s_bar[warp][stage]);
+        if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"((uint32_t)(2 * UNIT)) : "memory");
+        __syncwarp();
+        if ((lane & (box - 1)) == 0) {  // (keys behind the last one: rows of the pool, or zeros behind it)
+          asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst + lane * HD), "l"(&cm), "r"(bar), "r"(0), "r"(vec) : "memory");
+          asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst + UNIT + lane * HD), "l"(&cm), "r"(bar), "r"(0), "r"(vec + v_off) : "memory");
+        }
+        __syncwarp();
+      } else {
+        constexpr int PIECES = HD / 16;
 #pragma unroll
-      for (int i = 0; i < EACH; ++i) {
-        const int row = (i * 32 + lane) / PIECES, piece = lane % PIECES;
-        const int r = __shfl_sync(0xffffffffu, vec, row);
-        const uint8_t* src = kv.codes + (size_t)r * HD + piece * 16;
-        cp_async16(ring + stage * 2 * UNIT + piece_at<HD>(row, piece), src);
-        cp_async16(ring + stage * 2 * UNIT + UNIT + piece_at<HD>(row, piece), src + (size_t)v_off * HD);
+        for (int i = 0; i < PIECES; ++i) {
+          const int row = (i * 32 + lane) / PIECES, piece = lane % PIECES, r = __shfl_sync(0xffffffffu, vec, row);
+          const uint8_t* src = kv.codes + (size_t)r * HD + piece * 16;
+          cp_async16(dst + piece_at<HD>(row, piece), src);
+          cp_async16(dst + UNIT + piece_at<HD>(row, piece), src + (size_t)v_off * HD);
+        }
+        cp_async_commit();
       }
     };
-    auto scale_of = [&](int vec) { return kv.scale[vec + (lane >> 4) * v_off]; };  // lanes 0 .. 15: keys', 16 .. 31: values'
     // ---- the first units on their way, and the vectors of the one behind them
-    uint8_t first[ST - 1], pend = 0;
-    int vec_next = 0, pend_at = -1;
+    uint8_t sk[ST - 1], sv[ST - 1];
+    int next = 0, pend_at = -1;
 #pragma unroll
-    for (int s = 0; s < ST - 1; ++s) {
-      const int u = warp + s * WARPS_F;
-      if constexpr (TMA) {
-        if (s < n_mine) ask(s);
-        continue;
+    for (int s = 0; s < ST - 1; ++s)
+      if (s < n) {
+        const int vec = vec_of(s);
+        copy(vec, (J + s) % ST);
+        sk[s] = kv.scale[vec], sv[s] = kv.scale[vec + v_off];
+      } else if (!TMA) {
+        cp_async_commit();
       }
-      if (u < units) {
-        const int vec = vec_of(u);
-        copy(vec, s);
-        first[s] = scale_of(vec);
-      }
-      cp_async_commit();
-    }
-    if (!TMA && warp + (ST - 1) * WARPS_F < units) vec_next = vec_of(warp + (ST - 1) * WARPS_F);
+    if (ST - 1 < n) next = vec_of(ST - 1);
     // ---- queries: the lane's columns of row g (and 8 + g)
     uint32_t q[NB][C][4][2];
     float qf[NB][2];
     int pos[NB][2];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      const int n = nb * 8 + g, tok = n / G;
+      const int r = nb * 8 + g, tok = r / G;
       uint4 x[C][2];
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         x[c][0] = x[c][1] = make_uint4(0, 0, 0, 0);
-        if (n < rows) {
-          const uint4* src = reinterpret_cast<const uint4*>(a.q + (size_t)(p.t0 + tok) * a.q_stride + (head0 + n - tok * G) * HD + c * 64 + t * 16);
+        if (r < rows) {
+          const uint4* src = reinterpret_cast<const uint4*>(a.q + (size_t)(p.t0 + tok) * a.q_stride + (head0 + r - tok * G) * HD + c * 64 + t * 16);
           x[c][0] = src[0], x[c][1] = src[1];
         }
       }
@@ -244,148 +231,150 @@ __global__ void __launch_bounds__(THR_F, NB == 1 ? 2 : 1) attn_few8_kernel(Batch
     for (int nb = 0; nb < NB; ++nb) m[nb][0] = m[nb][1] = -INFINITY, l[nb][0] = l[nb][1] = 0.f;
 #pragma unroll
     for (int s = 0; s < ST - 1; ++s)
-      if (!TMA && warp + s * WARPS_F < units) s_scale[warp][s][lane] = first[s];
-    int stage = TMA ? J % ST : 0, into = ST - 1, j = 0;  // of the unit at hand, and of the one that is asked for
-    for (int u = warp; u < units; u += WARPS_F, ++j) {
-      if constexpr (TMA) {
-        __syncwarp();  // nobody reads the unit before any more, and its stage is the next one's
-        if (j + ST - 1 < n_mine) ask(j + ST - 1);
-        wait_short(smem_u32(&s_bar[warp][stage]), (uint32_t)((J + j) / ST & 1), dead);
-        __syncwarp();
-      } else {
-        if (pend_at >= 0) s_scale[warp][pend_at][lane] = pend;  // (a step later than asked for)
-        cp_async_wait<ST - 2>();
-        __syncwarp();  // the unit is there, and nobody reads the one before any more
-        pend_at = -1;
-        if (u + (ST - 1) * WARPS_F < units) {
-          copy(vec_next, into);
-          pend = scale_of(vec_next), pend_at = into;
-          if (u + ST * WARPS_F < units) vec_next = vec_of(u + ST * WARPS_F);
-        }
+      if (s < n) s_scale[warp][(J + s) % ST][lane] = sk[s], s_scale[warp][(J + s) % ST][32 + lane] = sv[s];
+    int stage = J % ST;
+    for (int j = 0; j < n; ++j) {
+      if (pend_at >= 0) s_scale[warp][pend_at][lane] = sk[0], s_scale[warp][pend_at][32 + lane] = sv[0];  // (a step later than asked for)
+      if constexpr (TMA) wait_short(smem_u32(&s_bar[warp][stage]), (uint32_t)((J + j) / ST & 1), dead);
+      else cp_async_wait<ST - 2>();
+      __syncwarp();  // the unit is there, and nobody reads the one before any more
+      pend_at = -1;
+      if (j + ST - 1 < n) {
+        pend_at = stage == 0 ? ST - 1 : stage - 1;
+        copy(next, pend_at);
+        sk[0] = kv.scale[next], sv[0] = kv.scale[next + v_off];
+        if (j + ST < n) next = vec_of(j + ST);
+      } else if (!TMA) {
         cp_async_commit();
       }
-      const int key0 = k_lo + u * 16;
-      const bool edge = key0 + 16 > p.pos0 + 1 || key0 < low1;  // some row does not see some key of the unit
+      const int key0 = k_lo + (warp + j * WARPS_F) * 32;
+      const bool edge = key0 + 32 > p.pos0 + 1 || key0 < low1;  // some row does not see some key of the unit
       const uint32_t at = ring + stage * 2 * UNIT;
       const uint8_t* sc = s_scale[warp][stage];
-      // ---- scores: rows keys g and g + 8, columns rows 2t and 2t + 1
-      float x[NB][4] = {};
+      // ---- scores: rows keys g, g + 8, g + 16 and g + 24, columns rows 2t and 2t + 1; two sums each, of every other product (a chain of eight would be the unit's longest)
+      float x[NB][2][4];
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        uint32_t k0[4], k1[4];
-        ld_shared_v4(at + piece_at<HD>(g, c * 4 + t), k0);
-        ld_shared_v4(at + piece_at<HD>(g + 8, c * 4 + t), k1);
+      for (int kb = 0; kb < 2; ++kb) {
+        float y[NB][2][4] = {};
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          uint32_t a0, a1, a2, a3;
-          kv8_unpack<CODE>(k0[w], a0, a2);
-          kv8_unpack<CODE>(k1[w], a1, a3);
+        for (int c = 0; c < C; ++c) {
+          uint32_t k0[4], k1[4];
+          ld_shared_v4(at + piece_at<HD>(kb * 16 + g, c * 4 + t), k0);
+          ld_shared_v4(at + piece_at<HD>(kb * 16 + g + 8, c * 4 + t), k1);
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) mma_f16(x[nb], a0, a1, a2, a3, q[nb][c][w][0], q[nb][c][w][1]);
-        }
-      }
-      uint32_t vr[4][VW];
+          for (int w = 0; w < 4; ++w) {
+            uint32_t a0, a1, a2, a3;
+            kv8_unpack<CODE>(k0[w], a0, a2);
+            kv8_unpack<CODE>(k1[w], a1, a3);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = 2 * t + (i & 1) + 8 * (i >> 1);
-        if constexpr (HD == 128) ld_shared_v4(at + UNIT + piece_at<HD>(row, g), vr[i]);
-        else asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(vr[i][0]), "=r"(vr[i][1]) : "r"(at + UNIT + piece_at<HD>(row, g >> 1) + (g & 1) * 8) : "memory");
-      }
-      const uint32_t kb0 = sc[g], kb1 = sc[g + 8], vb0 = sc[g + 16], vb1 = sc[g + 24];
-      const int key_l = key0 + (lane & 15);
-      const int top = (int)__reduce_max_sync(0xffffffffu, lane < 16 || sc[lane] == 255 || (edge && (key_l >= end || key_l < low0)) ? 0u : (uint32_t)sc[lane]);
-      float ks[2] = {kv8_scale(vb0 == 255 ? 255u : kb0), kv8_scale(vb1 == 255 ? 255u : kb1)};
-      if (edge && CODE == KV8_E4M3) {  // values that are no numbers must not meet a zero weight: they are zero, and their keys' scores no numbers
-        uint32_t bad = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t any = 0;
-#pragma unroll
-          for (int w = 0; w < VW; ++w) any |= kv8_nans(vr[i][w]);
-          if (any) {
-            bad |= 1u << (2 * t + (i & 1) + 8 * (i >> 1));
-#pragma unroll
-            for (int w = 0; w < VW; ++w) vr[i][w] = 0;
+            for (int nb = 0; nb < NB; ++nb) mma_f16(y[nb][w & 1], a0, a1, a2, a3, q[nb][c][w][0], q[nb][c][w][1]);
           }
         }
-        bad = __reduce_or_sync(0xffffffffu, bad);
-        if (bad) {
-          // (the other lanes' columns of the key stay as they are: a row that sees it is no number by its score)
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            if (bad >> (g + 8 * i) & 1) ks[i] = __uint_as_float(0x7fc00000u);
-        }
-      }
-      if (top > lr) {  // the values' products so far, beside the new largest scale
-        const float f = top - lr < 127 ? __uint_as_float((uint32_t)(127 - (top - lr)) << 23) : 0.f;
-        lr = top;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-          for (int b = 0; b < MB; ++b)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[nb][b][e] *= f;
+          for (int e = 0; e < 4; ++e) x[nb][kb][e] = y[nb][0][e] + y[nb][1][e];
       }
-      float pv[2];  // 2^7 times a value's scale beside the largest
+      uint32_t kb_[4], vb_[4];  // scales of the keys g + 8 i
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int e = max(1, (int)(i ? vb1 : vb0)) - lr + 127 + P_EXP;
+      for (int i = 0; i < 4; ++i) kb_[i] = sc[g + 8 * i], vb_[i] = sc[32 + g + 8 * i];
+      const uint32_t mine = sc[32 + lane];
+      const int key_l = key0 + lane, top = (int)__reduce_max_sync(0xffffffffu, mine == 255 || (edge && (key_l >= end || key_l < low0)) ? 0u : mine);
+      uint32_t bad = 0;
+      if (edge && CODE == KV8_E4M3) {  // values that are no numbers must not meet a zero weight: they are zero, and their keys' scores no numbers
+#pragma unroll 1
+        for (int i = 0; i < HD / 16; ++i) {  // two keys a step; 16 or 8 bytes a lane
+          const int row = i * (512 / HD) + lane / (HD / 16), piece = lane % (HD / 16);
+          const uint32_t where = at + UNIT + piece_at<HD>(row, piece);
+          uint32_t c[4];
+          ld_shared_v4(where, c);
+          if (kv8_nans(c[0]) | kv8_nans(c[1]) | kv8_nans(c[2]) | kv8_nans(c[3])) {
+            bad |= 1u << row;
+            asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(where), "r"(0u) : "memory");
+          }
+        }
+        bad = __reduce_or_sync(0xffffffffu, bad);
+        if (TMA) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (a copy takes the place)
+        __syncwarp();
+      }
+      float pv[4];  // 2^7 times a value's scale beside the largest
+      const int lr_new = max(lr, top);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int e = max(1, (int)vb_[i]) - lr_new + 127 + P_EXP;
         pv[i] = e > 0 && e < 255 ? __uint_as_float((uint32_t)e << 23) : 0.f;
       }
-      bool grow = false;
+      bool grow = top > lr;
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[nb][e] *= ks[e >> 1] * qf[nb][e & 1];
-          if (edge) {
-            const int key = key0 + g + 8 * (e >> 1), at = pos[nb][e & 1];
-            if (key > at || (a.window > 0 && key <= at - a.window)) x[nb][e] = -INFINITY;
-          }
-          grow |= x[nb][e] > m[nb][e & 1] + LAG;
-        }
-      if (__any_sync(0xffffffffu, grow)) {
+      for (int i = 0; i < 4; ++i) {
+        const float ks = kv8_scale(vb_[i] == 255 || (bad >> (g + 8 * i) & 1) ? 255u : kb_[i]);
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float mx = fmaxf(x[nb][e], x[nb][e + 2]);
+            float& y = x[nb][i >> 1][(i & 1) * 2 + e];
+            y *= ks * qf[nb][e];
+            if (edge) {
+              const int key = key0 + g + 8 * i, pos_ = pos[nb][e];
+              if (key > pos_ || (a.window > 0 && key <= pos_ - a.window)) y = -INFINITY;
+            }
+            grow |= y > m[nb][e] + LAG;
+          }
+      }
+      if (__any_sync(0xffffffffu, grow)) {
+        // the values' products so far: beside the new largest scale, and the rows' new references
+        const float fs = lr_new - lr < 127 ? __uint_as_float((uint32_t)(127 - (lr_new - lr)) << 23) : 0.f;
+        lr = lr_new;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float mx = fmaxf(fmaxf(x[nb][0][e], x[nb][0][e + 2]), fmaxf(x[nb][1][e], x[nb][1][e + 2]));
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
             const float to = fmaxf(m[nb][e], mx), f = m[nb][e] > -INFINITY ? ex2_tc(m[nb][e] - to) : 1.f;
             m[nb][e] = to;
             l[nb][e] *= f;
 #pragma unroll
-            for (int b = 0; b < MB; ++b) o[nb][b][e] *= f, o[nb][b][e + 2] *= f;
+            for (int b = 0; b < MB; ++b) o[nb][b][e] *= f * fs, o[nb][b][e + 2] *= f * fs;
           }
       }
-      uint32_t pt[NB][2];
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        const float m0 = m[nb][0] > -INFINITY ? m[nb][0] : 0.f, m1 = m[nb][1] > -INFINITY ? m[nb][1] : 0.f;
-        const float w0 = ex2_tc(x[nb][0] - m0), w1 = ex2_tc(x[nb][1] - m1), w2 = ex2_tc(x[nb][2] - m0), w3 = ex2_tc(x[nb][3] - m1);
-        l[nb][0] += w0 + w2, l[nb][1] += w1 + w3;
-        pt[nb][0] = transpose_8x8(pack_h(w0 * pv[0], w1 * pv[0]));
-        pt[nb][1] = transpose_8x8(pack_h(w2 * pv[1], w3 * pv[1]));
-      }
+      for (int kb = 0; kb < 2; ++kb) {
+        uint32_t vr[4][VW];
 #pragma unroll
-      for (int w = 0; w < VW; ++w) {
-        uint32_t f[2][4];  // columns 4w .. 4w + 3 of two keys each
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          kv8_unpack<CODE>(__byte_perm(vr[2 * h][w], vr[2 * h + 1][w], 0x5140), f[h][0], f[h][1]);
-          kv8_unpack<CODE>(__byte_perm(vr[2 * h][w], vr[2 * h + 1][w], 0x7362), f[h][2], f[h][3]);
+        for (int i = 0; i < 4; ++i) {
+          const int row = kb * 16 + 2 * t + (i & 1) + 8 * (i >> 1);
+          if constexpr (HD == 128) ld_shared_v4(at + UNIT + piece_at<HD>(row, g), vr[i]);
+          else asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(vr[i][0]), "=r"(vr[i][1]) : "r"(at + UNIT + piece_at<HD>(row, g >> 1) + (g & 1) * 8) : "memory");
         }
+        uint32_t pt[NB][2];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-          mma_f16(o[nb][2 * w], f[0][0], f[0][1], f[1][0], f[1][1], pt[nb][0], pt[nb][1]);
-          mma_f16(o[nb][2 * w + 1], f[0][2], f[0][3], f[1][2], f[1][3], pt[nb][0], pt[nb][1]);
+          const float m0 = m[nb][0] > -INFINITY ? m[nb][0] : 0.f, m1 = m[nb][1] > -INFINITY ? m[nb][1] : 0.f;
+          const float w0 = ex2_tc(x[nb][kb][0] - m0), w1 = ex2_tc(x[nb][kb][1] - m1), w2 = ex2_tc(x[nb][kb][2] - m0), w3 = ex2_tc(x[nb][kb][3] - m1);
+          l[nb][0] += w0 + w2, l[nb][1] += w1 + w3;
+          pt[nb][0] = transpose_8x8(pack_h(w0 * pv[2 * kb], w1 * pv[2 * kb]));
+          pt[nb][1] = transpose_8x8(pack_h(w2 * pv[2 * kb + 1], w3 * pv[2 * kb + 1]));
+        }
+#pragma unroll
+        for (int w = 0; w < VW; ++w) {
+          uint32_t f[2][4];  // columns 4w .. 4w + 3 of two keys each
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            kv8_unpack<CODE>(__byte_perm(vr[2 * h][w], vr[2 * h + 1][w], 0x5140), f[h][0], f[h][1]);
+            kv8_unpack<CODE>(__byte_perm(vr[2 * h][w], vr[2 * h + 1][w], 0x7362), f[h][2], f[h][3]);
+          }
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            mma_f16(o[nb][2 * w], f[0][0], f[0][1], f[1][0], f[1][1], pt[nb][0], pt[nb][1]);
+            mma_f16(o[nb][2 * w + 1], f[0][2], f[0][3], f[1][2], f[1][3], pt[nb][0], pt[nb][1]);
+          }
         }
       }
       if (++stage == ST) stage = 0;
-      if (++into == ST) into = 0;
     }
-    J += n_mine;
+    J += n;
     if (!TMA) cp_async_wait<0>();
     __syncwarp();
     // ---- the warps' results together
@@ -395,9 +384,9 @@ __global__ void __launch_bounds__(THR_F, NB == 1 ? 2 : 1) attn_few8_kernel(Batch
       for (int e = 0; e < 2; ++e) {
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) l[nb][e] += __shfl_xor_sync(0xffffffffu, l[nb][e], d);
-        const int n = nb * 8 + 2 * t + e;
-        if (g == 0) s_m[warp][n] = m[nb][e], s_l[warp][n] = l[nb][e];
-        float* dst = s_o + warp * (Ring<HD>::WARP / 4) + n * HD + g * (HD / 8);
+        const int r = nb * 8 + 2 * t + e;
+        if (g == 0) s_m[warp][r] = m[nb][e], s_l[warp][r] = l[nb][e];
+        float* dst = s_o + warp * (Ring<HD>::WARP / 4) + r * HD + g * (HD / 8);
 #pragma unroll
         for (int b = 0; b < MB; ++b) *reinterpret_cast<float2*>(dst + 2 * b) = make_float2(o[nb][b][e], o[nb][b][e + 2]);
       }
@@ -405,7 +394,7 @@ __global__ void __launch_bounds__(THR_F, NB == 1 ? 2 : 1) attn_few8_kernel(Batch
     __syncthreads();
     const bool whole = p.whole();
     for (int i = tid; i < rows * (HD / 4); i += THR_F) {
-      const int n = i / (HD / 4), c = i - n * (HD / 4);
+      const int n = i / (HD / 4), c = i - n * (HD / 4);  // a row, four columns
       float top = -INFINITY, sum = 0.f;
       int r = 1;
 #pragma unroll
@@ -442,17 +431,17 @@ __global__ void __launch_bounds__(THR_F, NB == 1 ? 2 : 1) attn_few8_kernel(Batch
 }
 
 template <int HD, int CODE, int NB, bool TMA>
-cudaError_t launch_few(const BatchAttnArgs& a, const Kv8Geom& kv, const JoinShape& sh, int tt, const TensorMap2D& cm, cudaStream_t st) {
+cudaError_t launch_few(const BatchAttnArgs& a, const Kv8Geom& kv, const JoinShape& sh, int tt, int box, const TensorMap2D& cm, cudaStream_t st) {
   static PerDeviceOnce set;
   if (set.need()) {
-    const cudaError_t e = cudaFuncSetAttribute(attn_few8_kernel<HD, CODE, NB, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_F<HD>);
+    const cudaError_t e = cudaFuncSetAttribute(attn_few8_kernel<HD, CODE, NB, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<HD>::SMEM);
     if (e != cudaSuccess) return e;
     set.done();
   }
   const int ctas = 2 * a.num_sms;
   BatchAttnArgs b = a;
   b.kv.n_kv *= sh.subs;
-  const cudaError_t e = launched(launch_k(attn_few8_kernel<HD, CODE, NB, TMA>, dim3(ctas), dim3(THR_F), SMEM_F<HD>, st, b, kv, sh, tt, *reinterpret_cast<const CUtensorMap*>(&cm)));
+  const cudaError_t e = launched(launch_k(attn_few8_kernel<HD, CODE, NB, TMA>, dim3(ctas), dim3(Ring<HD>::THR), Ring<HD>::SMEM, st, b, kv, sh, tt, box, *reinterpret_cast<const CUtensorMap*>(&cm)));
   return e != cudaSuccess ? e : launch_join<HD, ROWS_F>(a, sh, ctas, st);
 }
 
@@ -990,18 +979,21 @@ cudaError_t launch_attention_batch8(const BatchAttnArgs& a, const Kv8Geom& kv, c
   const int group = a.n_q / kv.n_kv, g = std::min(group, ROWS_F), P = kv.page_size;
   const JoinShape sh{g, group, (group + g - 1) / g};
   const bool few = a.n_tok <= a.n_req;
-  const bool tma = P % 16 == 0 && (reinterpret_cast<uintptr_t>(kv.scale) & 15) == 0;
-  const int box = P % 64 == 0 ? 64 : P % 32 == 0 ? 32 : 16;  // the largest that divides a page and a tile
+  // boxes of the most rows, a power of two, that divide a page and a tile or unit; a tile's scales come by bulk copies of a multiple of 16 bytes
+  const int most = few ? 32 : 64;
+  int box = 1;
+  while (box < most && P % (2 * box) == 0) box *= 2;
+  const bool tma = few ? box >= 4 : box >= 16 && (reinterpret_cast<uintptr_t>(kv.scale) & 15) == 0;
   TensorMap2D cm{};
   if (tma) {
-    const cudaError_t e = make_tensor_map_kv8(&cm, kv.codes, (unsigned long long)kv.n_pages * kv.n_layers * 2ull * kv.n_kv * P, kv.hd, few ? 16 : box);
+    const cudaError_t e = make_tensor_map_kv8(&cm, kv.codes, (unsigned long long)kv.n_pages * kv.n_layers * 2ull * kv.n_kv * P, kv.hd, box);
     if (e != cudaSuccess) return e;
   }
   auto go = [&](auto hd, auto code) {
     constexpr int HD = decltype(hd)::value, CODE = decltype(code)::value;
     if (!few) return tma ? launch_prompt<HD, CODE, true>(a, kv, group, cm, box, st) : launch_prompt<HD, CODE, false>(a, kv, group, cm, box, st);
-    if (tma) return group <= 8 ? launch_few<HD, CODE, 1, true>(a, kv, sh, 8 / g, cm, st) : launch_few<HD, CODE, 2, true>(a, kv, sh, ROWS_F / g, cm, st);
-    return group <= 8 ? launch_few<HD, CODE, 1, false>(a, kv, sh, 8 / g, cm, st) : launch_few<HD, CODE, 2, false>(a, kv, sh, ROWS_F / g, cm, st);
+    if (tma) return group <= 8 ? launch_few<HD, CODE, 1, true>(a, kv, sh, 8 / g, box, cm, st) : launch_few<HD, CODE, 2, true>(a, kv, sh, ROWS_F / g, box, cm, st);
+    return group <= 8 ? launch_few<HD, CODE, 1, false>(a, kv, sh, 8 / g, box, cm, st) : launch_few<HD, CODE, 2, false>(a, kv, sh, ROWS_F / g, box, cm, st);
   };
   using std::integral_constant;
   if (kv.hd == 64) return kv.code == KV8_E4M3 ? go(integral_constant<int, 64>(), integral_constant<int, KV8_E4M3>()) : go(integral_constant<int, 64>(), integral_constant<int, KV8_INT8>());

@@ -120,21 +120,30 @@ __global__ void __launch_bounds__(JOIN_THR, 2) attn_batch_join_kernel(BatchAttnA
   __shared__ Sum4 sums[JOIN_THR];
   pdl_wait();
   pdl_trigger();
+  constexpr bool MANY = ROWS * C > JOIN_THR;  // rows enough for more than one step of a CTA's threads
   const JoinInfo* info = reinterpret_cast<const JoinInfo*>(a.work);
-  const JoinInfo in = info[blockIdx.x];
-  const int slice = blockIdx.y;  // of many rows' columns
-  const float* first = reinterpret_cast<const float*>(info + n_cta) + ((size_t)blockIdx.x * 2 + 1) * PART<HD, ROWS>;
+  JoinInfo in = info[blockIdx.x];
+  int slice = blockIdx.y, cta = blockIdx.x, slices = 1;  // of many rows' columns; of few rows' columns, where an item has many parts: the CTAs behind the first have none that begin there
+  if constexpr (!MANY) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const JoinInfo x = info[max((int)blockIdx.x - s, 0)];
+      const int share = x.parts >= 5 ? 4 : x.parts >= 3 ? 2 : 1;
+      if (x.parts > 1 && s < share && s <= (int)blockIdx.x) in = x, slice = s, cta = (int)blockIdx.x - s, slices = share;
+    }
+  }
+  const float* first = reinterpret_cast<const float*>(info + n_cta) + ((size_t)cta * 2 + 1) * PART<HD, ROWS>;
   const int sub = sh.subs > 1 ? in.kvh % sh.subs : 0, G = min(sh.g, sh.group - sub * sh.g), head0 = (sh.subs > 1 ? in.kvh / sh.subs : in.kvh) * sh.group + sub * sh.g;
   const int rows = in.tokens * G, n = in.parts, tid = threadIdx.x;
   // (a work area that two calls used at once must not lead outside)
-  if (n <= 1 || n > n_cta - (int)blockIdx.x || rows <= 0 || rows > ROWS || in.t0 < 0 || in.t0 > a.n_tok - in.tokens || in.kvh < 0 || in.kvh >= a.kv.n_kv * sh.subs) return;
+  if (n <= 1 || n > n_cta - cta || rows <= 0 || rows > ROWS || in.t0 < 0 || in.t0 > a.n_tok - in.tokens || in.kvh < 0 || in.kvh >= a.kv.n_kv * sh.subs) return;
   bf16* out = a.out + (size_t)in.t0 * a.out_stride + (size_t)head0 * HD;
   auto store = [&](int row, int c, const float4& o, float f) {
     *reinterpret_cast<uint2*>(out + (size_t)(row / G) * a.out_stride + (size_t)(row % G) * HD + c * 4) = make_uint2(pack2f(o.x * f, o.y * f), pack2f(o.z * f, o.w * f));
   };
   auto part_of = [&](int q) { return first + (q == 0 ? 0 : (size_t)(2 * q - 1) * PART<HD, ROWS>); };  // the others are the first ones of the CTAs behind
   const int all = rows * C;
-  if (ROWS * C > JOIN_THR && all > JOIN_THR) {
+  if (MANY && all > JOIN_THR) {
     // many rows: four threads a row with every fourth group of its columns; a part's weight is the row's
     constexpr int MINE = C / (JOIN_THR / ROWS) > 0 ? C / (JOIN_THR / ROWS) : 1;
     const int row = tid % ROWS, c0 = tid / ROWS;
@@ -174,10 +183,10 @@ __global__ void __launch_bounds__(JOIN_THR, 2) attn_batch_join_kernel(BatchAttnA
     }
     return;
   }
-  if (slice) return;
+  if (MANY && slice) return;
   // few rows: four columns of a row a thread, and the parts in turn with the threads that are left
   constexpr int U = 4;
-  const int lanes = JOIN_THR / all, i = tid % all, q0 = tid / all, c = i / rows, row = i - c * rows;
+  const int mine = all / slices, lanes = JOIN_THR / mine, i = tid % mine, q0 = tid / mine, c = i / rows + slice * (C / slices) * !MANY, row = i % rows;
   Sum4 s;
   if (q0 < lanes)
     for (int q = q0; q < n; q += U * lanes) {
@@ -199,7 +208,7 @@ __global__ void __launch_bounds__(JOIN_THR, 2) attn_batch_join_kernel(BatchAttnA
   sums[tid] = s;
   __syncthreads();
   if (q0 == 0) {
-    for (int w = 1; w < min(lanes, n); ++w) s.add(sums[w * all + i].m, sums[w * all + i].l, sums[w * all + i].o);
+    for (int w = 1; w < min(lanes, n); ++w) s.add(sums[w * mine + i].m, sums[w * mine + i].l, sums[w * mine + i].o);
     store(row, c, s.o, s.l > 0.f ? 1.f / s.l : s.l);
   }
 }
