@@ -98,7 +98,7 @@ struct Ring {
 // four positions 16 bytes a lane): keys from there as the rows of a product K Q^T, the weights by a transposition of 8 x 8 into fragments of V^T P^T, values with neighbouring keys' bytes
 // beside each other.  The columns of a row are numbered so that a lane's are 16 bytes together.  No barrier but the warp's own; the warps' results are added up at the end of a piece.
 template <int HD, int CODE, int NB, bool TMA>
-__global__ void __launch_bounds__(Ring<HD>::THR, NB == 1 ? 2 : 1) attn_few8_kernel(BatchAttnArgs a, Kv8Geom kv, JoinShape sh, int tt, int box, const __grid_constant__ CUtensorMap cm) {
+__global__ void __launch_bounds__(Ring<HD>::THR, NB == 1 ? 2 : 1) attn_few8_kernel(BatchAttnArgs a, Kv8Geom kv, JoinShape sh, int tt, int box, int behind, const __grid_constant__ CUtensorMap cm) {
   constexpr int C = HD / 64, VW = HD / 32, MB = HD / 16;  // 16-byte pieces of a key row a lane; words of a value row a lane; blocks of 16 columns
   constexpr int UNIT = Ring<HD>::UNIT, ST = Ring<HD>::STAGES, WARPS_F = Ring<HD>::WARPS, THR_F = Ring<HD>::THR;
   static_assert(NB * 8 * HD * 4 <= Ring<HD>::WARP, "a warp's results take its ring's place");
@@ -114,7 +114,9 @@ __global__ void __launch_bounds__(Ring<HD>::THR, NB == 1 ? 2 : 1) attn_few8_kern
   unsigned char* s_ring = smem_raw + ((smem_u32(smem_raw) + 1023u & ~1023u) - smem_u32(smem_raw));
   float* s_o = reinterpret_cast<float*>(s_ring);
   if (TMA && threadIdx.x == 32) asm volatile("prefetch.tensormap [%0];" ::"l"(&cm) : "memory");
-  pdl_wait();
+  // `behind` the kernel of larger blocks, whose results it has nothing to do with: that one let it in behind its own wait, so what both read is there, and it waits for it at the end, so that
+  // what follows follows both
+  if (!behind) pdl_wait();
   pdl_trigger();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const uint32_t ring = smem_u32(s_ring) + warp * Ring<HD>::WARP;
@@ -428,10 +430,11 @@ __global__ void __launch_bounds__(Ring<HD>::THR, NB == 1 ? 2 : 1) attn_few8_kern
     drain_tc(dead);
     report_tc(dead, a.status);
   }
+  if (behind) pdl_wait();
 }
 
 template <int HD, int CODE, int NB, bool TMA>
-cudaError_t launch_few(const BatchAttnArgs& a, const Kv8Geom& kv, const JoinShape& sh, int tt, int box, const TensorMap2D& cm, cudaStream_t st) {
+cudaError_t launch_few(const BatchAttnArgs& a, const Kv8Geom& kv, const JoinShape& sh, int tt, int box, bool behind, const TensorMap2D& cm, cudaStream_t st) {
   static PerDeviceOnce set;
   if (set.need()) {
     const cudaError_t e = cudaFuncSetAttribute(attn_few8_kernel<HD, CODE, NB, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<HD>::SMEM);
@@ -441,8 +444,8 @@ cudaError_t launch_few(const BatchAttnArgs& a, const Kv8Geom& kv, const JoinShap
   const int ctas = 2 * a.num_sms;
   BatchAttnArgs b = a;
   b.kv.n_kv *= sh.subs;
-  const cudaError_t e = launched(launch_k(attn_few8_kernel<HD, CODE, NB, TMA>, dim3(ctas), dim3(Ring<HD>::THR), Ring<HD>::SMEM, st, b, kv, sh, tt, box, *reinterpret_cast<const CUtensorMap*>(&cm)));
-  return e != cudaSuccess ? e : launch_join<HD, ROWS_F>(a, sh, ctas, st);
+  const cudaError_t e = launched(launch_k(attn_few8_kernel<HD, CODE, NB, TMA>, dim3(ctas), dim3(Ring<HD>::THR), Ring<HD>::SMEM, st, b, kv, sh, tt, box, (int)behind, *reinterpret_cast<const CUtensorMap*>(&cm)));
+  return e != cudaSuccess || behind ? e : launch_join<HD, ROWS_F>(a, sh, ctas, st);
 }
 
 // ---------------------------------------------------------------- blocks of up to 256 rows
@@ -962,38 +965,60 @@ cudaError_t launch_prompt(const BatchAttnArgs& a, const Kv8Geom& kv, int G, cons
     set.done();
   }
   const int out32 = reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && a.out_stride % 16 == 0;
-  const cudaError_t e = launched(launch_k(attn_prompt8_kernel<HD, CODE, TMA>, dim3(a.num_sms), dim3(THR_P), SmemP<HD>::TOTAL, st, a, kv, G, ROWS_P / G, out32, box,
+  BatchAttnArgs b = a;
+  b.rest = HD == 64 ? 5 : 8;  // (8192 rows, heads of 128, with 3: the CTAs that begin with a kv head's short items end at 680 us, the others at 555)
+  return launched(launch_k(attn_prompt8_kernel<HD, CODE, TMA>, dim3(a.num_sms), dim3(THR_P), SmemP<HD>::TOTAL, st, b, kv, G, ROWS_P / G, out32, box,
                                           *reinterpret_cast<const CUtensorMap*>(&cm)));
-  return e != cudaSuccess ? e : launch_join<HD, ROWS_P>(a, JoinShape{G, G, 1}, a.num_sms, st);
 }
+
+// the parts of both kernels' items
+template <int HD>
+__global__ void __launch_bounds__(JOIN_THR, 2) attn_both8_join_kernel(BatchAttnArgs large, BatchAttnArgs small, JoinShape sh_large, JoinShape sh_small, int n_large, int n_small) {
+  __shared__ Sum4 sums[JOIN_THR];
+  pdl_wait();
+  pdl_trigger();
+  if ((int)blockIdx.x < n_large) join_parts<HD, ROWS_P>(large, sh_large, n_large, blockIdx.x, sums);
+  else if (blockIdx.y == 0) join_parts<HD, ROWS_F>(small, sh_small, n_small, (int)blockIdx.x - n_large, sums);
+}
+size_t work_few(int hd, int num_sms) { return 2 * (size_t)num_sms * (sizeof(JoinInfo) + 2 * (hd == 64 ? PART<64, ROWS_F> : PART<128, ROWS_F>) * sizeof(float)); }
+size_t work_prompt(int hd, int num_sms) { return (size_t)num_sms * (sizeof(JoinInfo) + 2 * (hd == 64 ? PART<64, ROWS_P> : PART<128, ROWS_P>) * sizeof(float)); }
 
 }  // namespace
 
-size_t attention_batch8_work(int hd, int num_sms) {
-  const size_t few = 2 * (size_t)num_sms * (sizeof(JoinInfo) + 2 * (hd == 64 ? PART<64, ROWS_F> : PART<128, ROWS_F>) * sizeof(float));
-  const size_t prompt = (size_t)num_sms * (sizeof(JoinInfo) + 2 * (hd == 64 ? PART<64, ROWS_P> : PART<128, ROWS_P>) * sizeof(float));
-  return few > prompt ? few : prompt;
-}
+size_t attention_batch8_work(int hd, int num_sms) { return work_few(hd, num_sms) + work_prompt(hd, num_sms); }
 
 cudaError_t launch_attention_batch8(const BatchAttnArgs& a, const Kv8Geom& kv, cudaStream_t st) {
   const int group = a.n_q / kv.n_kv, g = std::min(group, ROWS_F), P = kv.page_size;
   const JoinShape sh{g, group, (group + g - 1) / g};
+  // Requests of so many rows that their keys and values are read once or twice by blocks of few rows are theirs, the others have blocks of up to 256 (a decode row in one of those costs
+  // what 256 rows do: 48 of them at 2800 positions on average beside four portions of a prompt TIME_MIXED_ALL us, by both kernels TIME_MIXED us).  Where the step has no more rows than requests, all of them
+  // are blocks of few rows (a request with many rows reads its keys and values that much more often); the room counts, which the host knows, and not the step's rows, which it does not.
   const bool few = a.n_tok <= a.n_req;
-  // boxes of the most rows, a power of two, that divide a page and a tile or unit; a tile's scales come by bulk copies of a multiple of 16 bytes
-  const int most = few ? 32 : 64;
+  // boxes of the most rows, a power of two, that divide a page and a unit or tile; a tile's scales come by bulk copies of a multiple of 16 bytes
   int box = 1;
-  while (box < most && P % (2 * box) == 0) box *= 2;
-  const bool tma = few ? box >= 4 : box >= 16 && (reinterpret_cast<uintptr_t>(kv.scale) & 15) == 0;
-  TensorMap2D cm{};
-  if (tma) {
-    const cudaError_t e = make_tensor_map_kv8(&cm, kv.codes, (unsigned long long)kv.n_pages * kv.n_layers * 2ull * kv.n_kv * P, kv.hd, box);
-    if (e != cudaSuccess) return e;
-  }
+  while (box < 64 && P % (2 * box) == 0) box *= 2;
+  const int box_f = std::min(box, 32);
+  const bool tma_f = box_f >= 4, tma_p = box >= 16 && (reinterpret_cast<uintptr_t>(kv.scale) & 15) == 0;
+  const unsigned long long rows = (unsigned long long)kv.n_pages * kv.n_layers * 2ull * kv.n_kv * P;
+  TensorMap2D cm_f{}, cm_p{};
+  cudaError_t e = tma_f ? make_tensor_map_kv8(&cm_f, kv.codes, rows, kv.hd, box_f) : cudaSuccess;
+  if (e == cudaSuccess && !few && tma_p) e = make_tensor_map_kv8(&cm_p, kv.codes, rows, kv.hd, box);
+  if (e != cudaSuccess) return e;
   auto go = [&](auto hd, auto code) {
     constexpr int HD = decltype(hd)::value, CODE = decltype(code)::value;
-    if (!few) return tma ? launch_prompt<HD, CODE, true>(a, kv, group, cm, box, st) : launch_prompt<HD, CODE, false>(a, kv, group, cm, box, st);
-    if (tma) return group <= 8 ? launch_few<HD, CODE, 1, true>(a, kv, sh, 8 / g, box, cm, st) : launch_few<HD, CODE, 2, true>(a, kv, sh, ROWS_F / g, box, cm, st);
-    return group <= 8 ? launch_few<HD, CODE, 1, false>(a, kv, sh, 8 / g, box, cm, st) : launch_few<HD, CODE, 2, false>(a, kv, sh, ROWS_F / g, box, cm, st);
+    BatchAttnArgs small = a, large = a;
+    if (!few) {
+      small.n_most = large.n_more = ROWS_F / g;
+      small.work = static_cast<char*>(a.work) + work_prompt(HD, a.num_sms);
+      const cudaError_t r = tma_p ? launch_prompt<HD, CODE, true>(large, kv, group, cm_p, box, st) : launch_prompt<HD, CODE, false>(large, kv, group, cm_p, box, st);
+      if (r != cudaSuccess) return r;
+    }
+    cudaError_t r;
+    if (tma_f) r = group <= 8 ? launch_few<HD, CODE, 1, true>(small, kv, sh, 8 / g, box_f, !few, cm_f, st) : launch_few<HD, CODE, 2, true>(small, kv, sh, ROWS_F / g, box_f, !few, cm_f, st);
+    else r = group <= 8 ? launch_few<HD, CODE, 1, false>(small, kv, sh, 8 / g, box_f, !few, cm_f, st) : launch_few<HD, CODE, 2, false>(small, kv, sh, ROWS_F / g, box_f, !few, cm_f, st);
+    if (few || r != cudaSuccess) return r;
+    constexpr int SLICES = HD / 4 / (JOIN_THR / ROWS_P) / 4;
+    return launched(launch_k(attn_both8_join_kernel<HD>, dim3(3 * a.num_sms, SLICES), dim3(JOIN_THR), 0, st, large, small, JoinShape{group, group, 1}, sh, a.num_sms, 2 * a.num_sms));
   };
   using std::integral_constant;
   if (kv.hd == 64) return kv.code == KV8_E4M3 ? go(integral_constant<int, 64>(), integral_constant<int, KV8_E4M3>()) : go(integral_constant<int, 64>(), integral_constant<int, KV8_INT8>());

@@ -35,10 +35,10 @@ __host__ __device__ __forceinline__ void ab_tiles(const AbRequest& r, int b, int
   last = (int)((r.c + row1 + AB_TK - 1) / AB_TK);
 }
 // cost of the first x blocks
-__host__ __device__ __forceinline__ long long ab_cost(const AbRequest& r, int x, int tt, int window) {
+__host__ __device__ __forceinline__ long long ab_cost(const AbRequest& r, int x, int tt, int window, int rest = AB_REST) {
   if (x <= 0) return 0;
   const int full = x < r.nb ? x : r.nb - 1;
-  long long sum = (long long)x * AB_REST;
+  long long sum = (long long)x * rest;
   if (full > 0) sum += floor_sum(full, tt, (unsigned)r.c + tt + AB_TK - 1);
   if (x == r.nb) sum += ((long long)r.c + r.n + AB_TK - 1) / AB_TK;
   if (window > 0) {
@@ -54,11 +54,12 @@ struct Raw {
   AbRequest r;
   int t0, slot;
 };
+__host__ __device__ __forceinline__ int ab_rest(const BatchAttnArgs& a) { return a.rest ? a.rest : AB_REST; }
 __host__ __device__ __forceinline__ Raw request(const BatchAttnArgs& a, int i, int tt) {
   Raw w;
   const int t0 = a.q_start[i], t1 = a.q_start[i + 1], len = a.kv_len[i];
   w.slot = a.slots ? a.slots[i] : i;
-  const bool ok = t0 >= 0 && t1 > t0 && t1 <= a.n_tok && len >= t1 - t0 && len <= (long long)a.max_pages * a.kv.page_size && w.slot >= 0 && w.slot < a.max_seqs;
+  const bool ok = t0 >= 0 && t1 > t0 && t1 <= a.n_tok && t1 - t0 > a.n_more && (a.n_most == 0 || t1 - t0 <= a.n_most) && len >= t1 - t0 && len <= (long long)a.max_pages * a.kv.page_size && w.slot >= 0 && w.slot < a.max_seqs;
   w.t0 = t0;
   w.r.n = ok ? t1 - t0 : 0;
   w.r.c = ok ? len - w.r.n : 0;
@@ -104,7 +105,7 @@ struct Walk {
         p.pos0 = w.r.c + block * tt;
         p.limit = w.r.c + w.r.n;
       }
-      left -= tiles + AB_REST - skip;
+      left -= tiles + ab_rest(a) - skip;
       skip = 0;
       ++block;
       if (some) return true;

@@ -44,7 +44,7 @@ __device__ __forceinline__ Stretch find_stretch(const BatchAttnArgs& a, int tt, 
   long long mine = 0, total, head = 0;  // head: a kv head's cost of the thread's last request
   for (int i = r0; i < r1; ++i) {
     const Raw w = request(a, i, tt);
-    head = ab_cost(w.r, w.r.nb, tt, a.window);
+    head = ab_cost(w.r, w.r.nb, tt, a.window, ab_rest(a));
     mine += a.kv.n_kv * head;
   }
   const long long below = block_scan<NTHR>(mine, s_sums, total);
@@ -57,7 +57,7 @@ __device__ __forceinline__ Stretch find_stretch(const BatchAttnArgs& a, int tt, 
       rest = x0 - below;
       for (req = r0; req < r1 - 1; ++req) {
         const Raw w = request(a, req, tt);
-        const long long h = ab_cost(w.r, w.r.nb, tt, a.window);
+        const long long h = ab_cost(w.r, w.r.nb, tt, a.window, ab_rest(a));
         if (rest < a.kv.n_kv * h) {
           head = h;
           break;
@@ -75,7 +75,7 @@ __device__ __forceinline__ Stretch find_stretch(const BatchAttnArgs& a, int tt, 
     long long before = 0;
     while (hi - lo > 1) {
       const int step = (hi - lo + 31) / 32, x = lo + lane * step;
-      const long long c = x < hi ? ab_cost(w.r, x, tt, a.window) : rest + 1;
+      const long long c = x < hi ? ab_cost(w.r, x, tt, a.window, ab_rest(a)) : rest + 1;
       const int k = 31 - __clz(__ballot_sync(0xffffffffu, c <= rest));  // (lane 0's is)
       before = __shfl_sync(0xffffffffu, c, k);
       hi = min(hi, lo + (k + 1) * step), lo += k * step;
@@ -115,21 +115,18 @@ struct JoinShape {
   int g, group, subs;
 };
 template <int HD, int ROWS>
-__global__ void __launch_bounds__(JOIN_THR, 2) attn_batch_join_kernel(BatchAttnArgs a, JoinShape sh, int n_cta) {
+__device__ __forceinline__ void join_parts(const BatchAttnArgs& a, const JoinShape& sh, int n_cta, int of, Sum4* sums) {  // of: the CTA of the kernel above
   constexpr int C = HD / 4;  // groups of columns
-  __shared__ Sum4 sums[JOIN_THR];
-  pdl_wait();
-  pdl_trigger();
   constexpr bool MANY = ROWS * C > JOIN_THR;  // rows enough for more than one step of a CTA's threads
   const JoinInfo* info = reinterpret_cast<const JoinInfo*>(a.work);
-  JoinInfo in = info[blockIdx.x];
-  int slice = blockIdx.y, cta = blockIdx.x, slices = 1;  // of many rows' columns; of few rows' columns, where an item has many parts: the CTAs behind the first have none that begin there
+  JoinInfo in = info[of];
+  int slice = blockIdx.y, cta = of, slices = 1;  // of many rows' columns; of few rows' columns, where an item has many parts: the CTAs behind the first have none that begin there
   if constexpr (!MANY) {
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      const JoinInfo x = info[max((int)blockIdx.x - s, 0)];
+      const JoinInfo x = info[max(of - s, 0)];
       const int share = x.parts >= 5 ? 4 : x.parts >= 3 ? 2 : 1;
-      if (x.parts > 1 && s < share && s <= (int)blockIdx.x) in = x, slice = s, cta = (int)blockIdx.x - s, slices = share;
+      if (x.parts > 1 && s < share && s <= of) in = x, slice = s, cta = of - s, slices = share;
     }
   }
   const float* first = reinterpret_cast<const float*>(info + n_cta) + ((size_t)cta * 2 + 1) * PART<HD, ROWS>;
@@ -214,6 +211,13 @@ __global__ void __launch_bounds__(JOIN_THR, 2) attn_batch_join_kernel(BatchAttnA
 }
 
 
+template <int HD, int ROWS>
+__global__ void __launch_bounds__(JOIN_THR, 2) attn_batch_join_kernel(BatchAttnArgs a, JoinShape sh, int n_cta) {
+  __shared__ Sum4 sums[JOIN_THR];
+  pdl_wait();
+  pdl_trigger();
+  join_parts<HD, ROWS>(a, sh, n_cta, blockIdx.x, sums);
+}
 template <int HD, int ROWS>
 inline cudaError_t launch_join(const BatchAttnArgs& a, const JoinShape& sh, int ctas, cudaStream_t st) {
   constexpr int SLICES = ROWS * (HD / 4) > JOIN_THR ? HD / 4 / (JOIN_THR / ROWS) / 4 : 1;

@@ -237,6 +237,8 @@ struct BatchAttnArgs {
   void* work;
   int num_sms;
   int* status;  // see FastAttnArgs
+  int n_more, n_most;  // requests of more than n_more rows and, where n_most is not 0, of at most n_most
+  int rest;            // what an item costs beside its tiles, in tiles; 0: AB_REST
 };
 size_t attention_batch_work(int hd, int num_sms);
 cudaError_t launch_attention_batch(const BatchAttnArgs& a, cudaStream_t st);
