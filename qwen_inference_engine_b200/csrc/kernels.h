@@ -199,11 +199,6 @@ enum { KV8_E4M3 = 0, KV8_INT8 = 1 };
 struct Kv8Geom {
   uint8_t *codes, *scale;
   int n_pages, page_size, n_layers, n_kv, hd, code;
-  // a layer's vector of a head in cache row `row`: `kv` 0 its key, 1 its value
-  __host__ __device__ size_t vec(int layer, int kv, int head, int row) const {
-    const int page = row / page_size;
-    return ((((size_t)page * n_layers + layer) * 2 + kv) * n_kv + head) * page_size + (row - page * page_size);
-  }
 };
 struct Rope8Args {
   const bf16 *q, *k, *v;

@@ -304,7 +304,7 @@ class KvPool8:
         assert scale.dtype is torch.uint8 and scale.shape == codes.shape[:5] and scale.get_device() == codes.get_device(), "a uint8 scale for each vector, beside them, expected"
         n_pages, n_layers, _, n_kv_heads, page_size, head_dim = codes.shape
         _here(codes)
-        self.codes, self.scale, self.head_dim, self.kv_wide = codes, scale, head_dim, n_kv_heads * head_dim
+        self.codes, self.scale, self.head_dim, self.kv_wide, self.device = codes, scale, head_dim, n_kv_heads * head_dim, codes.get_device()
         self.view = Kv8View(_p(codes), _p(scale), n_pages, page_size, n_layers, n_kv_heads, head_dim, KvPool8.CODES[codes.dtype])
         self.ref = C.byref(self.view)
 
@@ -312,18 +312,26 @@ class KvPool8:
 def launch_rope_store8(q, k, v, q_out, pool, layer, pos, row, rope, n_q_heads):
     """q -> q_out, k and v -> codes and scales in the cache rows row[t] of the pool's layer.  rope None: k as it is; then q, q_out and pos are None and n_q_heads 0"""
     (n, kw), (nv, vw) = k.shape, v.shape
-    assert k.dtype is v.dtype is torch.bfloat16 and n == nv and kw == vw == pool.kv_wide, "bfloat16 rows of the heads of as many tokens expected"
-    (kp, ks), (vp, vs), rp = _rows(k), _rows(v), _ints(row, n, "row")
-    assert k.get_device() == v.get_device() == pool.codes.get_device() == row.get_device(), "rows and pool on one device expected"
+    (ks, k1), (vs, v1) = k.stride(), v.stride()
+    assert k.dtype is v.dtype is torch.bfloat16 and n == nv and kw == vw == pool.kv_wide and k1 == v1 == 1, "bfloat16 rows of the heads of as many tokens expected"
+    dev = pool.device
+    assert k.get_device() == v.get_device() == row.get_device() == dev, "rows and pool on one device expected"
     _here(k)
+    if n == 1:
+        ks, vs = kw, kw
     if rope is None:
         assert q is None and q_out is None and pos is None and n_q_heads == 0, "queries and positions without a rotation"
-        check(_lib.lib().qie_rope_store8(pool.ref, layer, None, 0, None, 0, kp, ks, vp, vs, None, None, rp, n, 0, _st()))
+        check(_lib.lib().qie_rope_store8(pool.ref, layer, None, 0, None, 0, k.data_ptr(), ks, v.data_ptr(), vs, None, None, _ints(row, n, "row"), n, 0, _st()))
         return
-    assert q.dtype is q_out.dtype is torch.bfloat16 and q.shape == q_out.shape == (n, n_q_heads * pool.head_dim), "bfloat16 rows of the heads of as many tokens expected"
-    assert k.get_device() == q.get_device() == q_out.get_device() == pos.get_device() == rope.device, "rows, positions and frequencies on one device expected"
-    (qp, qs), (op, os) = _rows(q), _rows(q_out)
-    check(_lib.lib().qie_rope_store8(pool.ref, layer, qp, qs, op, os, kp, ks, vp, vs, rope.ref, _ints(pos, n, "pos"), rp, n, n_q_heads, _st()))
+    (nq, wide), (no, ow) = q.shape, q_out.shape
+    (qs, q1), (os, o1) = q.stride(), q_out.stride()
+    assert q.dtype is q_out.dtype is torch.bfloat16 and nq == no == n and wide == ow == n_q_heads * pool.head_dim, "bfloat16 rows of the heads of as many tokens expected"
+    assert q1 == o1 == 1 or wide <= 1, "rows of contiguous elements expected"
+    assert q.get_device() == q_out.get_device() == pos.get_device() == rope.device == dev, "rows, positions and frequencies on one device expected"
+    if n == 1:
+        qs, os = wide, wide
+    check(_lib.lib().qie_rope_store8(pool.ref, layer, q.data_ptr(), qs, q_out.data_ptr(), os, k.data_ptr(), ks, v.data_ptr(), vs, rope.ref, _ints(pos, n, "pos"),
+                                     _ints(row, n, "row"), n, n_q_heads, _st()))
 
 
 def launch_kv8_read(pool, layer, row, k, v):
@@ -333,9 +341,11 @@ def launch_kv8_read(pool, layer, row, k, v):
         if x is None:
             out += [None, 0]
             continue
-        assert x.dtype is torch.bfloat16 and x.shape == (n, pool.kv_wide) and x.get_device() == row.get_device(), "bfloat16 rows of the pool's heads, one for each index, expected"
-        out += _rows(x)
-    assert row.get_device() == pool.codes.get_device(), "rows and pool on one device expected"
+        (m, wide), (stride, one) = x.shape, x.stride()
+        assert x.dtype is torch.bfloat16 and m == n and wide == pool.kv_wide and one == 1 and x.get_device() == pool.device, \
+            "bfloat16 rows of the pool's heads, one for each index, beside it expected"
+        out += [x.data_ptr(), stride if n > 1 else wide]
+    assert row.get_device() == pool.device, "rows and pool on one device expected"
     _here(row)
     check(_lib.lib().qie_kv8_read(pool.ref, layer, _ints(row, n, "row"), n, *out, _st()))
 
@@ -345,7 +355,7 @@ def launch_attn_batch8(Q, out, pool, layer, batch, n_q_heads, window=0, scale=0.
     assert Q.dtype is out.dtype is torch.bfloat16 and Q.shape == out.shape == (batch.max_tokens, n_q_heads * pool.head_dim), "bfloat16 rows of the batch expected"
     if batch.heads8 < pool.head_dim:
         batch.reserve(pool, n_q_heads)
-    assert Q.get_device() == out.get_device() == pool.codes.get_device() == batch.block_table.get_device(), "rows, pool and batch on one device expected"
+    assert Q.get_device() == out.get_device() == pool.device == batch.block_table.get_device(), "rows, pool and batch on one device expected"
     _here(Q)
     check(_lib.lib().qie_attention_batch8(pool.ref, layer, batch.ref, *_rows(Q), *_rows(out), n_q_heads, window, scale, _st()))
 
