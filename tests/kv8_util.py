@@ -91,7 +91,7 @@ class Requests8:
             if m:
                 s = slice(self.start[i], self.start[i + 1])
                 want, size = ref.attention(self.q[s].view(m, self.nq, self.hd), self.k[i], self.v[i], c, window, scale)
-                tiny = 2.0 ** -36 * (c + m) * self.v[i].abs().max()
+                tiny = 2.0 ** -31 * (c + m) * self.v[i].abs().max()
                 d = (out[s].reshape(m, self.nq, self.hd).double() - want).abs() - 2.0 ** -8 * want.abs() - (2.0 ** -11 + 2.0 ** -9 + more) * size - tiny
                 assert (d <= 0).all(), (i, c, m, float((d / size).max()))
         if left is not None:

@@ -2,8 +2,8 @@
 
 Bounds.  Read back: exact.  Values stored: exact codes.  Keys: the rotation in fp32 is off by 2^-18 of |a| + |b| (derived in test_gpu_serving_step.py), and rounding a number that is off by d
 gives one that is off by d and half a step of the code: 2^-4 of itself or half of 2^-9 scales for e4m3, half a scale for int8; 2^-24 more of each for the comparison's own arithmetic.
-Attention: weights are rounded to fp16 in the product with the values, 2^-11 of the mean of |v| under the weights, and below 2^-14 of 2^-12 times the largest by 2^-25 of that:
-2^-37 of the largest |v| for each key (2^-36 with the factor 2^3 by which the largest weight may be below the one that the reference is for ... at most 2^-36 in all).
+Attention: weights are rounded to fp16 in the product with the values, 2^-11 of the mean of |v| under the weights.  They are there by 2^7, so one below 2^-14 of fp16's is off by 2^-25 of 2^7
+of a row's reference, which the largest weight is not below: 2^-32 of it, for each key, times the largest |v|; 2^-31 with what the values' powers of two add.
 Codes and queries are exact in fp16; scores in fp32 are off by at most 128 * 2^-23 of sum |q k| / sqrt(hd), below 2^6 here, so weights by 2^-10 of themselves, exponentials and sums by
 less: 2^-9 of that mean for all of it."""
 import numpy as np
@@ -273,3 +273,264 @@ def test_attention_same_bits_again(L):
         for _ in range(3):
             r.batch.work.random_(0, 255)  # whatever an earlier call left in the work area
             assert torch.equal(r.attend(L), out)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("lens", [[(300, 70), (900, 1)], [(300, 1), (900, 1)]])
+def test_attention_values_behind_the_weights(L, kind, lens):
+    """large scores: the largest weight is one and the others vanish; and rows whose keys are all alike"""
+    r = Requests8(L, lens, 4, 2, 128, 16, kind, seed=5)
+    r.q.mul_(30)
+    # scores are 30 times as large and their fp32 errors with them: weights off by 2^-5 of themselves, the mean of |v| by the bound's 2^-9 plus that
+    r.check(r.attend(L), more=2.0 ** -4)
+    r.q.zero_()
+    r.check(r.attend(L))
+
+
+@pytest.mark.parametrize("lens", [[(500, 200), (3, 1), (1000, 1)], [(500, 1), (3, 1), (3000, 1)]])
+@pytest.mark.parametrize("nq,nkv,hd", [(7, 1, 128), (14, 2, 64), (16, 1, 128)])
+def test_attention_scales_far_apart(L, lens, nq, nkv, hd):
+    """Keys and values whose scales differ by up to 2^40: what a key or a value beside a far larger one loses is 2^-24 of the larger one's smallest unit's, which its part of the result does not
+    show: weights are those of the exact scores, and the result is off by the bound's share of the mean of |v|."""
+    r = Requests8(L, lens, nq, nkv, hd, 16, "e4m3", seed=6, spread=5.0)
+    r.q.mul_(2.0 ** -18)  # (scores stay below 2^6)
+    r.check(r.attend(L), more=2.0 ** -9)
+
+
+def put(r, i, pos, j, codes=None, scale=None):
+    """bytes into position pos of request i's keys (j 0) or values (1), of the first kv head"""
+    pg, at = int(r.kv_at[i][0][pos]), int(r.kv_at[i][1][pos])
+    if codes is not None:
+        r.codes[pg, r.layer, j, 0, at] = codes
+    if scale is not None:
+        r.scale[pg, r.layer, j, 0, at] = scale
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("j", [0, 1])
+@pytest.mark.parametrize("lens,at", [([(0, 100), (70, 1)], 50), ([(300, 300), (9, 2)], 300), ([(64, 1), (40, 1), (33, 1)], 3), ([(200, 3), (0, 0), (5, 1), (6, 0)], 201)])
+def test_attention_vectors_of_no_numbers(L, kind, j, lens, at):
+    """a key's or value's scale of 255: no number in every column of the rows that see it, and nothing in the others"""
+    r = Requests8(L, lens, 4, 2, 64, 16, kind, seed=6)
+    before = r.attend(L)
+    put(r, 0, at, j, scale=255)
+    out = r.attend(L).view(-1, 4, 64)
+    c, m = lens[0]
+    sees = torch.zeros(len(out), dtype=torch.bool, device="cuda")
+    sees[max(0, at - c):m] = True
+    assert out[sees][:, :2].isnan().all()
+    assert torch.equal(out[~sees], before.view(-1, 4, 64)[~sees]) and torch.equal(out[:, 2:], before.view(-1, 4, 64)[:, 2:])
+
+
+@pytest.mark.parametrize("lens,at", [([(0, 100), (70, 1)], 50), ([(300, 300), (9, 2)], 300), ([(200, 3), (0, 0), (5, 1), (6, 0)], 201)])
+def test_attention_codes_of_no_number(L, lens, at):
+    """e4m3's code for no number among the values: in that column at least of the rows that see it, and in no other row"""
+    r = Requests8(L, lens, 4, 2, 64, 16, "e4m3", seed=6)
+    before = r.attend(L).view(-1, 4, 64)
+    for code in (0x7f, 0xff):
+        bytes_ = r.codes[int(r.kv_at[0][0][at]), r.layer, 1, 0, int(r.kv_at[0][1][at])].clone()
+        bytes_[7] = code
+        put(r, 0, at, 1, codes=bytes_)
+        out = r.attend(L).view(-1, 4, 64)
+        c, m = lens[0]
+        sees = torch.zeros(len(out), dtype=torch.bool, device="cuda")
+        sees[max(0, at - c):m] = True
+        assert out[sees][:, :2, 7].isnan().all() and torch.equal(out[~sees], before[~sees]) and torch.equal(out[:, 2:], before[:, 2:])
+
+
+def test_attention_queries_of_no_numbers(L):
+    for lens in ([(50, 20), (300, 2)], [(50, 1), (300, 1)]):
+        r = Requests8(L, lens, 4, 2, 128, 16, "int8", seed=7)
+        before = r.attend(L).view(-1, 4, 128)
+        r.q.view(-1, 4, 128)[0, 1, 5], r.q.view(-1, 4, 128)[1, 2, 0] = float("inf"), float("nan")
+        out = r.attend(L).view(-1, 4, 128)
+        assert out[0, 1].isnan().all() and out[1, 2].isnan().all()
+        out[0, 1], out[1, 2] = before[0, 1], before[1, 2]
+        assert torch.equal(out, before)
+
+
+@pytest.mark.parametrize("lens", [[(500, 90), (0, 1), (64, 2)], [(500, 1), (0, 1), (64, 1)]])
+def test_attention_of_zeros(L, lens):
+    """keys of zeros: the mean of the values; values of zeros: zeros; a pool as it is made"""
+    r = Requests8(L, lens, 14, 2, 64, 16, "e4m3", seed=7)
+    for x in r.k:
+        x.zero_()
+    r.codes[:, r.layer, 0], r.scale[:, r.layer, 0] = 0, 0
+    r.check(r.attend(L))
+    r.codes.zero_(), r.scale.zero_()
+    assert (r.attend(L)[:r.start[-1]] == 0).all()
+
+
+@pytest.mark.parametrize("lens", [[(1500, 1), (0, 400), (33, 2)], [(1500, 1), (40, 1), (33, 1)]])
+def test_attention_two_streams(L, lens):
+    """two calls at once, each with a work area of its own"""
+    a = [Requests8(L, lens, 14, 2, 64, 16, "int8", seed=20 + i) for i in range(2)]
+    outs, streams = [torch.full_like(r.q, 9.0) for r in a], [torch.cuda.Stream() for _ in a]
+    for r in a:
+        r.batch.reserve(r.kv, 14)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for r, o, s in zip(a, outs, streams):
+            with torch.cuda.stream(s):
+                L.launch_attn_batch8(r.q, o, r.kv, r.layer, r.batch, 14)
+    torch.cuda.synchronize()
+    for r, o in zip(a, outs):
+        r.check(o)
+
+
+@pytest.mark.parametrize("lens", [[(100, 10), (50, 20), (300, 1), (7, 5)], [(100, 1), (50, 1), (300, 1), (7, 1)]])
+@pytest.mark.parametrize("ps", [16, 4, 5])
+def test_attention_nonsense_stays_inside(L, lens, ps):
+    """offsets, lengths, slots and pages that make no sense: nothing is read or written outside, and requests beside them keep their results"""
+    r = Requests8(L, lens, 14, 2, 64, ps, "e4m3", seed=11)
+    s, n = r.start, int(r.start[-1])
+    kv_len, slots, table = r.batch.kv_len.clone(), r.batch.slots.clone(), r.batch.block_table.clone()
+    want = r.attend(L)
+    r.check(want)
+    r.batch.kv_len[1] = 2 ** 31 - 1
+    r.batch.block_table[slots[1]] = i32([-5])
+    r.batch.block_table[slots[1], 1] = 2 ** 31 - 1
+    out = r.attend(L)
+    good = torch.ones(n, dtype=torch.bool, device="cuda")
+    good[s[1]:s[2]] = False
+    # the split over the positions may fall elsewhere: two results within their bounds
+    assert ((out[good].double() - want[good].double()).abs() <= 2.0 ** -6 * 20).all()
+    r.batch.kv_len.copy_(kv_len)
+    r.attend(L)  # pages that are none
+    r.batch.block_table.copy_(table)
+    for bad in (-1, 10 ** 6, -2 ** 31):
+        r.batch.slots[1] = bad
+        out = r.attend(L)
+        assert (out[s[1]:s[2]] == 9).all() and torch.isfinite(out).all()
+    r.batch.slots.copy_(slots)
+    for start in ([0, 10, 30, 31, 2 ** 31 - 1], [0, -50, 30, 31, 36], [36, 31, 30, 10, 0], [2 ** 31 - 1] * 5, [-2 ** 31, 2 ** 31 - 1, 0, 0, 0]):
+        r.batch.q_start.copy_(i32(start))
+        r.attend(L)
+    for k in (-2 ** 31, -1, 0):
+        r.batch.q_start.copy_(i32(r.start))
+        r.batch.kv_len.fill_(k)
+        r.attend(L)
+    r.batch.kv_len.copy_(kv_len)
+    r.check(r.attend(L))
+
+
+@pytest.mark.parametrize("ps", [16, 5])
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n,room", [(200, 200), (1, 1)])
+def test_offsets_beyond_32_bits(L, ps, kind, n, room):
+    """a pool of more than 2^32 bytes: store, read and attention at its end"""
+    pages, g, cached = 2 ** 32 // (2 * ps * 128) + 300, 4, 199 if n == 1 else 0
+    codes = torch.empty(pages, 1, 2, 1, ps, 128, dtype=torch.uint8, device="cuda").view(DTYPES[kind])
+    scale = torch.empty(pages, 1, 2, 1, ps, dtype=torch.uint8, device="cuda")
+    total = cached + n
+    mine = torch.arange(pages - 1, pages - 1 - (total + ps - 1) // ps, -1, dtype=torch.int32, device="cuda")
+    pos = torch.arange(total, dtype=torch.int32, device="cuda")
+    row = mine[(pos // ps).long()] * ps + pos % ps
+    x = rand(1, total, (g + 2) * 128).bfloat16()
+    q, k, v = x.split([g * 128, 128, 128], 1)
+    q_out, freq = torch.empty_like(q.contiguous()), torch.from_numpy(L.Rope.frequencies(128)[0]).cuda()
+    kv = L.KvPool8.over(codes, scale)
+    L.launch_rope_store8(q, k, v, q_out, kv, 0, pos, row, L.Rope(freq), g)
+    kb, vb = torch.empty_like(k.contiguous()), torch.empty_like(v.contiguous())
+    L.launch_kv8_read(kv, 0, row, kb, vb)
+    c, b = coded(v.view(total, 1, 128), kind)
+    assert torch.equal(vb.double(), (c * torch.exp2(b.double() - 127)[..., None]).flatten(1))
+    batch = L.Batch(mine[None].contiguous(), ps, pages, 1, n, q_start=i32([0, n]), kv_len=i32([total]))
+    rows = q_out[cached:].contiguous()
+    out = torch.empty_like(rows)
+    L.launch_attn_batch8(rows, out, kv, 0, batch, g)
+    want, size = ref.attention(rows.view(n, g, 128), kb[:, None], vb[:, None], cached)
+    assert ((out.view(n, g, 128).double() - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -11 + 2.0 ** -9) * size + 2.0 ** -20).all()
+
+
+def test_attention_refuses_a_small_work_area(L):
+    from qwen_inference_engine_b200._lib import QieError
+    r = Requests8(L, [(10, 1)], 2, 1, 64, 16, "e4m3")
+    r.batch.reserve(r.kv, 2)
+    n, r.batch.view.work_bytes = r.batch.view.work_bytes, r.batch.view.work_bytes - 1
+    with pytest.raises(QieError, match="work area"):
+        r.attend(L)
+    r.batch.view.work_bytes = n
+    r.check(r.attend(L))
+
+
+def test_one_batch_over_both_pools(L):
+    """a batch whose work area serves the pool in bfloat16 and the one in 8 bits, and a graph from before it grew"""
+    lens = [(100, 30), (0, 1), (64, 65)]
+    r = Requests8(L, lens, 4, 2, 64, 16, "int8", seed=3)
+    out8, out16 = torch.zeros_like(r.q), torch.zeros_like(r.q)
+    pool = torch.zeros(r.codes.shape, dtype=torch.bfloat16, device="cuda")
+    for i in range(len(lens)):
+        pg, at = r.kv_at[i]
+        pool[pg, r.layer, 0, :, at], pool[pg, r.layer, 1, :, at] = r.k[i].bfloat16(), r.v[i].bfloat16()
+    kv = L.KvPool.over(pool)
+    L.launch_attn_batch(r.q, out16, kv, r.layer, r.batch, 4)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        L.launch_attn_batch(r.q, out16, kv, r.layer, r.batch, 4)
+    L.launch_attn_batch8(r.q, out8, r.kv, r.layer, r.batch, 4)
+    out16.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    r.check(out8)
+    r.check(out16, more=2.0 ** -8)  # (weights in bf16)
+
+
+# ---------------------------------------------------------------- a step
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("room", [0, 60])
+def test_step_in_a_graph(L, kind, room):
+    """a layer's part of serving steps, captured once: layout, rotary positions with the store, attention, over lengths that change between replays; every row against its request's own
+    history, as the cache stands for it"""
+    n, nq, nkv, hd, ps, pages = 5, 6, 2, 64, 16, 120
+    most = n + room
+    rope = L.Rope(torch.from_numpy(L.Rope.frequencies(hd)[0]).cuda())
+    kv = L.KvPool8(pages, ps, 1, nkv, hd, dtype=DTYPES[kind])
+    table, ring = torch.zeros(n, 40, dtype=torch.int32, device="cuda"), torch.randperm(pages, generator=torch.Generator("cuda").manual_seed(1), device="cuda").int()
+    cached, new, at = (torch.zeros(n, dtype=torch.int32, device="cuda") for _ in range(3))
+    ring_in = i32([0, pages])
+    b = L.Batch(table, ps, pages, n, most, cached=cached, n_new=new, free_ring=ring, ring_in=ring_in)
+    b.ring_out, b.view.ring_out = ring_in, ring_in.data_ptr()
+    qkv = torch.zeros(most, (nq + 2 * nkv) * hd, dtype=torch.bfloat16, device="cuda")
+    q, k, v = qkv.split([nq * hd, nkv * hd, nkv * hd], 1)
+    q_out, out = torch.zeros(most, nq * hd, dtype=torch.bfloat16, device="cuda"), torch.zeros(most, nq * hd, dtype=torch.bfloat16, device="cuda")
+
+    def step():
+        L.launch_batch_layout(b)
+        L.launch_rope_store8(q, k, v, q_out, kv, 0, b.pos, b.row, rope, nq)
+        L.launch_attn_batch8(q_out, out, kv, 0, b, nq)
+
+    b.reserve(kv, nq)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step()
+    rs, have = np.random.default_rng(2), np.zeros(n, int)
+    for turn in range(6):
+        m = rs.integers(0, 2, n) if room == 0 else rs.integers(0, 14, n) * (rs.random(n) < 0.8)
+        cached.copy_(i32(have)), new.copy_(i32(m))
+        qkv.copy_(rand(turn, *qkv.shape).bfloat16())
+        out.fill_(9.0)
+        g.replay()
+        torch.cuda.synchronize()
+        assert (b.status == 0).all()
+        start = np.concatenate([[0], np.cumsum(m)])
+        for i in range(n):
+            if m[i]:
+                p = torch.arange(have[i] + m[i], device="cuda")
+                row = table[i, p // ps] * ps + (p % ps).int()
+                kb, vb = (torch.empty(len(p), nkv * hd, dtype=torch.bfloat16, device="cuda") for _ in (0, 1))
+                L.launch_kv8_read(kv, 0, row.int(), kb, vb)
+                s = slice(start[i], start[i + 1])
+                want, size = ref.attention(q_out[s].view(-1, nq, hd), kb.view(-1, nkv, hd), vb.view(-1, nkv, hd), have[i])
+                assert ((out[s].view(-1, nq, hd).double() - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -11 + 2.0 ** -9) * size + 2.0 ** -20).all()
+                turned = ref.rope(k[s].reshape(-1, nkv, hd), p[have[i]:], rope.freq, 1.0, False)
+                near = 2.0 ** -3 if kind == "e4m3" else 2.0 ** -6  # (half a step of the largest element's, twice)
+                assert ((kb.view(-1, nkv, hd)[have[i]:].double() - turned).abs() <= near * turned.abs().amax(-1, keepdim=True)).all()
+        assert (out[start[-1]:] == 9).all()
+        have += m
+
+
+def test_no_wait_ran_out(L):
+    """in the kernels of the tests above"""
+    from qwen_inference_engine_b200 import _lib
+    assert _lib.lib().qie_kernel_status() == 0
