@@ -768,7 +768,7 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
     // ---- softmax: this thread's row
     asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
     const int g = warp >> 2, row = g * 128 + (tid & 127), tok = row / G, gh = row - tok * G;
-    const uint32_t la = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t la = (uint32_t)((warp & 3) * 32) << 16, mine_turn = 2u + 2u * (uint32_t)(warp & 3) + (uint32_t)g;  // the barrier of this warp's turns, beside that of the other row tile's
     int tg = 0;  // tiles of this row tile
     if (tid == 0) info[blockIdx.x].parts = 0;
     while (next_piece(p)) {
@@ -824,6 +824,9 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
       const int my_pos = p.pos0 + min(tok, p.tokens - 1), my_low = a.window > 0 ? max(0, my_pos - a.window + 1) : 0;
       float m_ref = -INFINITY, l_run = 0.f;
       int lr = 1;  // the scale of the values that O is beside, as a byte
+      // The two warps of an SM quarter take turns at its exponentials, a tile each: side by side they would both be slow at these, and then leave the unit idle together.
+      const bool turns = 128 < rows;  // (both row tiles have rows)
+      if (turns && g == 1) asm volatile("bar.arrive %0, 64;" ::"r"(mine_turn ^ 1u) : "memory");
 #pragma unroll 1
       for (int i = p.begin; i < p.end; ++i, ++T, ++tg) {
         const int b = tg & 1;
@@ -869,6 +872,7 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
         // weights by 2^7 and their values' scale beside the largest; 2^-64 of that is none in fp16, and one in the sum
         const int d = max(vt - lr, -64) + P_EXP;
         const unsigned long long s2 = twice_tc(s), n2 = twice_tc((m_ref > -INFINITY ? -m_ref : 0.f) + (float)d);
+        if (turns) asm volatile("bar.sync %0, 64;" ::"r"(mine_turn) : "memory");
         float rs[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < TK; c += 32) {
@@ -883,6 +887,7 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
           }
           tmem_st16_tc(ts + c / 2, wt);
         }
+        if (turns && (g == 0 || i + 1 < p.end)) asm volatile("bar.arrive %0, 64;" ::"r"(mine_turn ^ 1u) : "memory");
         l_run += ((rs[0] + rs[1]) + (rs[2] + rs[3])) * __uint_as_float((uint32_t)(127 - d) << 23);
         if (grow && i > p.begin) {  // O, behind the product of the tile before
           wait_short(bar_o + 16u * g + 8u * (b ^ 1), (uint32_t)(((tg - 1) >> 1) & 1), dead);
