@@ -444,6 +444,7 @@ cudaError_t launch_few(const BatchAttnArgs& a, const Kv8Geom& kv, const JoinShap
   const int ctas = 2 * a.num_sms;
   BatchAttnArgs b = a;
   b.kv.n_kv *= sh.subs;
+  b.rest = 7;  // (64 rows, heads of 128, with 3: CTAs with one piece end at 18 us, with two at 21)
   const cudaError_t e = launched(launch_k(attn_few8_kernel<HD, CODE, NB, TMA>, dim3(ctas), dim3(Ring<HD>::THR), Ring<HD>::SMEM, st, b, kv, sh, tt, box, (int)behind, *reinterpret_cast<const CUtensorMap*>(&cm)));
   return e != cudaSuccess || behind ? e : launch_join<HD, ROWS_F>(a, sh, ctas, st);
 }
