@@ -234,8 +234,8 @@ int qie_attention_batch(const qie_kv_view* kv, int layer, const qie_batch* b, co
 size_t qie_attention_batch_work(const qie_kv_view* kv, int n_q_heads);
 
 /* The same cache held in 8 bits: of each token and kv head a vector of codes and one scale for its key, and the same for its value.
- * code: QIE_KV8_E4M3 (8-bit floats of 4 bits of exponent and 3 of mantissa) or QIE_KV8_INT8.  scale: a byte b stands for 2^(b - 127), 0 for a vector of zeros, 255 for one of
- * no numbers; element = code * scale.  The store takes the smallest power of two with which the vector's largest element is at most 448 (127) times it, and rounds to nearest even, so an
+ * code: QIE_KV8_E4M3 (8-bit floats of 4 bits of exponent and 3 of mantissa) or QIE_KV8_INT8.  scale: a byte b stands for 2^(b - 127), 0 for a vector of zeros (whatever its codes,
+ * if they are numbers), 255 for one of no numbers; element = code * scale.  The store takes the smallest power of two with which the vector's largest element is at most 448 (127) times it, and rounds to nearest even, so an
  * element is off by at most 2^-4 of itself or 2^-10 scales (1/2 scale); a vector with an infinity or NaN becomes one of no numbers.  A token's vectors are written once and never
  * revised, so pages can be shared and appended to.  head_dim 64 or 128; n_pages * page_size < 2^31, and less than 2^31 vectors in all; codes on a 16-byte boundary. */
 typedef struct {
@@ -245,14 +245,16 @@ typedef struct {
 } qie_kv8_view;
 #define QIE_KV8_E4M3 0
 #define QIE_KV8_INT8 1
-/* qie_rope_store into such a cache.  Keys are coded as they come out of the rotation, in fp32.  rope NULL: keys as they are (pos is not read); n_q_heads must be 0. */
+/* qie_rope_store into such a cache.  Keys are coded as they come out of the rotation, in fp32; cosines and sines are rounded from 64 bits.  Each cache row at most once in a call (what two tokens
+ * leave in one row may be codes of one beside a scale of the other).  rope NULL: keys as they are (pos is not read); n_q_heads must be 0. */
 int qie_rope_store8(const qie_kv8_view* kv, int layer, const qie_bf16* q, size_t q_stride, qie_bf16* q_out, size_t q_out_stride, const qie_bf16* k,
                     size_t k_stride, const qie_bf16* v, size_t v_stride, const qie_rope_plan* rope, const int* pos, const int* row, int n_tok,
                     int n_q_heads, qie_stream st);
 /* The cache rows row[i] of `layer` as the values that they stand for -> rows k[i], v[i] of [n_kv_heads * head_dim], `stride` elements apart; either may be NULL.  Exact (where a value is
- * below bf16's smallest ones, rounded).  A row outside the pool: k[i] and v[i] are left as they are. */
+ * below bf16's smallest ones, rounded; above its largest, an infinity).  A row outside the pool: k[i] and v[i] are left as they are. */
 int qie_kv8_read(const qie_kv8_view* kv, int layer, const int* row, int n_rows, qie_bf16* k, size_t k_stride, qie_bf16* v, size_t v_stride, qie_stream st);
-/* qie_attention_batch over such a cache; its work area is qie_attention_batch8_work() bytes (one area of the larger size serves both).  Codes of e4m3 that are no numbers make
+/* qie_attention_batch over such a cache; its work area is qie_attention_batch8_work() bytes (one area of the larger size serves both).  Weights are fp16 in the product with the values,
+ * 2^7 times themselves beside the largest: none is off by more than 2^-11 of itself or 2^-32 of the largest.  Codes of e4m3 that are no numbers make
  * rows that see them no numbers, in that column at least, and no other row. */
 int qie_attention_batch8(const qie_kv8_view* kv, int layer, const qie_batch* b, const qie_bf16* Q, size_t q_stride, qie_bf16* out, size_t out_stride,
                          int n_q_heads, int window, float scale, qie_stream st);

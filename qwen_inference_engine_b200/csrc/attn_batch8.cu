@@ -7,7 +7,17 @@
 // summed in fp32.  Weights are fp16 in the product with the values (2^-11 of themselves; 2^7 times themselves and times their value's scale, so that none of at least 2^-21 of the
 // largest gets fewer bits, and none is off by more than 2^-32 of it), their sums fp32.
 //
-// An item is a kv head of a request and a block of its tokens, its rows (token, query head of the group); items are shared out over the CTAs as in attn_batch.cu.
+// An item is a kv head of a request and a block of its tokens, its rows (token, query head of the group); items are shared out over the CTAs as in attn_batch.cu.  There are two kernels: for blocks
+// of at most 16 rows (decode), which memory bounds, one that keeps a unit of keys and values in registers between loads and products, and for larger blocks one on tcgen05 / TMEM.
+//
+// What bounds them (B200, in a graph; the cache as it is read, with its scales).
+//   Few rows.  64 at 1434 positions on average, 28 heads of 128 on 4, e4m3, 96 MB: 29.6 us (over a bf16 cache 42.8).  2.3 us pass before the first copies (the requests' numbers, the search for a
+//   CTA's stretch), then units come at 4.9 TB/s until the median CTA ends at 21 us and the last one at 25, and the kernel that joins takes the rest.  4 at 70000 positions, 12 heads on 2, int8,
+//   144 MB: 38.0 (62.3).  One at 700, 14 heads of 64 on 2: 8.8 (9.4), the plan, one tile's latency and the join.
+//   Larger blocks.  8192 rows of 28 heads of 128 on 4: e4m3 586 us, 821 TFLOP/s, int8 554 (over a bf16 cache 491, which has nothing to convert).  A tile of 64 keys of 256 rows has 1024 cycles
+//   of exponentials and 1280 of products and takes 2600.  Without the exponentials' instructions it would take 6 % less, without the conversion's arithmetic 13 % (e4m3 comes by the unit that the
+//   exponentials use), without maxima 6 %, with an eighth of Q K^T 11 %: several chains of a tile (scores, softmax, product; copy, conversion) are about as long as each other.  An item's
+//   beginning and end, at which both row tiles drain, cost 7 us.
 #include <cuda.h>
 
 #include <algorithm>
@@ -26,7 +36,8 @@ namespace {
 constexpr float LAG = 8.f;
 constexpr int P_EXP = 7;
 
-// mbar_wait_tc in few instructions: with the compiler's loop around a try the warps that wait had half of the SM's instructions.  2^26 tries are about two seconds.
+// mbar_wait_tc in few instructions: the loops of a CTA's roles are to stay in the instruction caches together (where they did not, 8192 rows took
+// 943 us instead of 786).  2^26 tries are about two seconds.
 __device__ __forceinline__ void wait_short(uint32_t bar, uint32_t parity, volatile int* dead) {
   uint32_t done;
   asm volatile(
@@ -303,8 +314,8 @@ __global__ void __launch_bounds__(Ring<HD>::THR, NB == 1 ? 2 : 1) attn_few8_kern
       const int lr_new = max(lr, top);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int e = max(1, (int)vb_[i]) - lr_new + 127 + P_EXP;
-        pv[i] = e > 0 && e < 255 ? __uint_as_float((uint32_t)e << 23) : 0.f;
+        const int e = (int)vb_[i] - lr_new + 127 + P_EXP;
+        pv[i] = vb_[i] != 0 && e > 0 && e < 255 ? __uint_as_float((uint32_t)e << 23) : 0.f;
       }
       bool grow = top > lr;
 #pragma unroll
@@ -460,7 +471,7 @@ cudaError_t launch_few(const BatchAttnArgs& a, const Kv8Geom& kv, const JoinShap
 // Registers: 96 a thread at launch; 144, 64 and 64 behind the split, as many in all.
 constexpr int ROWS_P = 256, THR_P = 20 * 32, TK = AB_TK;
 constexpr int KBLK = TK * 128;  // [keys][64 columns] fp16 in 8-row swizzle atoms
-constexpr int SLOTS = 8;        // tiles' scales: the softmax is at most STAGES + 3 tiles behind
+constexpr int SLOTS = 8;        // tiles' scales: the softmax is at most ST + 3 tiles behind
 template <int HD>
 struct SmemP {
   static constexpr bool Q_TMEM = HD == 64;
@@ -700,7 +711,7 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
 #pragma unroll
         for (int e = 0; e < UNITS; ++e) {
           const int row = row_of(e);
-          code[e] = *reinterpret_cast<const uint4*>(codes + row * HD + ((HD == 128 ? piece ^ (row & 7) : piece ^ ((row >> 1) & 3)) << 4));
+          code[e] = *reinterpret_cast<const uint4*>(codes + piece_at<HD>(row, piece));
         }
         // the lane's two keys: scales, the largest of the tile, and the factors that bring codes beside that
         uint32_t sb[2], vb[2], top = is_v, v_top = 1;
@@ -825,7 +836,8 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
       const int my_pos = p.pos0 + min(tok, p.tokens - 1), my_low = a.window > 0 ? max(0, my_pos - a.window + 1) : 0;
       float m_ref = -INFINITY, l_run = 0.f;
       int lr = 1;  // the scale of the values that O is beside, as a byte
-      // The two warps of an SM quarter take turns at its exponentials, a tile each: side by side they would both be slow at these, and then leave the unit idle together.
+      // The two warps of an SM quarter take turns at its exponentials, a tile each: side by side they would both be slow at these, and then leave the unit idle together (8192 rows 596 and
+      // 591 us).
       const bool turns = 128 < rows;  // (both row tiles have rows)
       if (turns && g == 1) asm volatile("bar.arrive %0, 64;" ::"r"(mine_turn ^ 1u) : "memory");
 #pragma unroll 1
@@ -912,7 +924,7 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
       }
       // ---- the row of the result
       wait_short(bar_o + 16u * g + 8u * ((tg - 1) & 1), (uint32_t)(((tg - 1) >> 1) & 1), dead);
-        __syncwarp();
+      __syncwarp();
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const bool whole = p.whole();
       const float back = __uint_as_float((uint32_t)lr << 23) * (1.f / (1 << P_EXP)), nan = __int_as_float(0x7fc00000);
@@ -997,7 +1009,7 @@ cudaError_t launch_attention_batch8(const BatchAttnArgs& a, const Kv8Geom& kv, c
   const int group = a.n_q / kv.n_kv, g = std::min(group, ROWS_F), P = kv.page_size;
   const JoinShape sh{g, group, (group + g - 1) / g};
   // Requests of so many rows that their keys and values are read once or twice by blocks of few rows are theirs, the others have blocks of up to 256 (a decode row in one of those costs
-  // what 256 rows do: 48 of them at 2800 positions on average beside four portions of a prompt TIME_MIXED_ALL us, by both kernels TIME_MIXED us).  Where the step has no more rows than requests, all of them
+  // what 256 rows do: 48 of them at 2800 positions on average beside four portions of a prompt 105 us, by both kernels 84; 16 portions without decode rows 104 and 107).  Where the step has no more rows than requests, all of them
   // are blocks of few rows (a request with many rows reads its keys and values that much more often); the room counts, which the host knows, and not the step's rows, which it does not.
   const bool few = a.n_tok <= a.n_req;
   // boxes of the most rows, a power of two, that divide a page and a unit or tile; a tile's scales come by bulk copies of a multiple of 16 bytes

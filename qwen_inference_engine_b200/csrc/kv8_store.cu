@@ -4,8 +4,10 @@
 // of a border between two codes, cosines and sines are rounded from 64 bits (with the hardware's functions, 2^-20.5, the codes' error beside the exact rotation's was twice that of a rotation
 // in fp32 from exact cosines).
 // A warp takes a token and some of its heads, eight elements a lane, so that a head is 8 or 16 lanes: cosines and sines are computed once for all of them, a lane's share each, a pair's other
-// half is a shuffle away, and so is the largest element.   Queries are loaded four groups at a time.
-// Bound by memory: every element is read and written once.
+// half is a shuffle away, and so is the largest element.  Queries are loaded four groups at a time (two 16.5 us and three 15.9 for the first call below with the hardware's cosines, four 16.6; for
+// the second 25.9, 26.3 and 24.5), the first groups before the token's position and row are there; four CTAs an SM (three 17.3 and 24.6, five, of fewer registers, 20.7 and 28.6).
+// Every element is read and written once.  B200, in a graph: 8192 tokens of 12 + 2 x 2 heads of 128, 63 MB, 17.0 us (3.7 TB/s; the store of bf16 keys and values 15.5: a wave and a half of
+// CTAs, and the shuffles and conversions of their instructions); 20011 of 14 + 2 x 2 of 64 in int8, half of each rotated, stored and read back 26.7; 64 of 28 + 2 x 4 of 128 3.0, a launch.
 #include <algorithm>
 
 #include "common.cuh"
@@ -221,7 +223,8 @@ cudaError_t launch_code(const Rope8Args& a, bool wide, cudaStream_t st) {
   return a.rotated % 16 == 0 ? launch_turn<HD, CODE, TURN_LANES>(a, wide, st) : launch_turn<HD, CODE, TURN_ANY>(a, wide, st);
 }
 
-// Sixteen elements a thread, which has one place of a row (k or v, head, piece) and goes through rows U at a time: their indexes, then scales and codes, then results.
+// Sixteen elements a thread, which has one place of a row (k or v, head, piece) and goes through rows U at a time: their indexes, then scales and codes, then results.  Bound by memory: 32768
+// rows of 4 x 2 heads of 128, 101 MB, 18.6 us, 5.4 TB/s; 701 of 2 x 2 of 64 1.7, a launch.  With a place a thread found by divisions, a row at a time, and results of 16 bytes 24.1.
 template <int CODE, int W>  // W: elements of a result's access, 16, 8 or 1
 __global__ void __launch_bounds__(THR) kv8_read_kernel(Kv8ReadArgs a, PageDiv div, int wide, int deep) {  // wide x deep threads: places of a row, rows
   constexpr int U = 4;

@@ -534,3 +534,52 @@ def test_no_wait_ran_out(L):
     """in the kernels of the tests above"""
     from qwen_inference_engine_b200 import _lib
     assert _lib.lib().qie_kernel_status() == 0
+
+
+@pytest.mark.parametrize("lens", [[(100, 200), (0, 1), (64, 65)], [(100, 1), (0, 1), (64, 1)]])
+@pytest.mark.parametrize("ps", [16, 64])
+def test_attention_scales_off_a_boundary(L, lens, ps):
+    """scale bytes that begin anywhere: bulk copies of them would need 16-byte boundaries"""
+    r = Requests8(L, lens, 14, 2, 64, ps, "e4m3", seed=3)
+    want = r.attend(L)
+    for off in (1, 8):
+        buf = torch.empty(r.scale.numel() + 16, dtype=torch.uint8, device="cuda")
+        s = buf[off:off + r.scale.numel()].view(r.scale.shape)
+        s.copy_(r.scale)
+        r.kv = L.KvPool8.over(r.codes.view(DTYPES["e4m3"]), s)
+        out = r.attend(L)
+        r.check(out)
+        assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("lens", [[(100, 200), (64, 65)], [(100, 1), (64, 1)]])
+@pytest.mark.parametrize("kind", KINDS)
+def test_attention_scale_of_zero(L, lens, kind):
+    """a scale byte of 0 stands for zeros, whatever the codes beside it"""
+    r = Requests8(L, lens, 4, 2, 64, 16, kind, seed=4)
+    for i in range(len(lens)):
+        pg, at = r.kv_at[i]
+        for p in range(0, lens[i][0], 3):
+            r.scale[pg[p], r.layer, 1, :, at[p]] = 0
+            r.v[i][p] = 0
+        r.scale[pg[1], r.layer, 0, :, at[1]] = 0
+        r.k[i][1] = 0
+    r.check(r.attend(L))
+
+
+def test_calls_that_do_not_fit(L):
+    """what the Python forms refuse"""
+    r = Requests8(L, [(10, 3)], 2, 1, 64, 16, "e4m3")
+    kv, row = r.kv, i32([0, 1, 2])
+    k, v = (torch.zeros(3, 64, dtype=torch.bfloat16, device="cuda") for _ in (0, 1))
+    rope = L.Rope(torch.from_numpy(L.Rope.frequencies(64)[0]).cuda())
+    q = torch.zeros(3, 128, dtype=torch.bfloat16, device="cuda")
+    for bad in (lambda: L.KvPool8.over(r.codes, r.scale), lambda: L.KvPool8.over(r.codes.view(torch.int8), r.scale[:-1]), lambda: L.KvPool8.over(r.codes.view(torch.int8), r.scale.int()),
+                lambda: L.KvPool8.over(r.codes.view(torch.int8).cpu(), r.scale.cpu()), lambda: L.launch_kv8_read(kv, 1, row, k[:2], v), lambda: L.launch_kv8_read(kv, 1, row.long(), k, v),
+                lambda: L.launch_kv8_read(kv, 1, row, k.float(), v), lambda: L.launch_kv8_read(kv, 1, row, k, v.cpu()), lambda: L.launch_rope_store8(None, k, v[:2], None, kv, 1, None, row, None, 0),
+                lambda: L.launch_rope_store8(q, k, v, q, kv, 1, row, row, None, 2), lambda: L.launch_rope_store8(q[:, :64], k, v, q, kv, 1, row, row, rope, 2),
+                lambda: L.launch_rope_store8(q, k, v, q, kv, 1, row[:2], row, rope, 2), lambda: L.launch_rope_store8(q, k.T.contiguous().T, v, q, kv, 1, row, row, rope, 2),
+                lambda: L.launch_attn_batch8(r.q[:2], r.q[:2], kv, 1, r.batch, 2), lambda: L.launch_attn_batch8(r.q.float(), r.q.float(), kv, 1, r.batch, 2)):
+        with pytest.raises(AssertionError):
+            bad()
+    torch.cuda.synchronize()
