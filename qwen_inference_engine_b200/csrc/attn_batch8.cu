@@ -14,10 +14,10 @@
 //   Few rows.  64 at 1434 positions on average, 28 heads of 128 on 4, e4m3, 96 MB: 29.6 us (over a bf16 cache 42.8).  2.3 us pass before the first copies (the requests' numbers, the search for a
 //   CTA's stretch), then units come at 4.9 TB/s until the median CTA ends at 21 us and the last one at 25, and the kernel that joins takes the rest.  4 at 70000 positions, 12 heads on 2, int8,
 //   144 MB: 38.0 (62.3).  One at 700, 14 heads of 64 on 2: 8.8 (9.4), the plan, one tile's latency and the join.
-//   Larger blocks.  8192 rows of 28 heads of 128 on 4: e4m3 586 us, 821 TFLOP/s, int8 554 (over a bf16 cache 491, which has nothing to convert).  A tile of 64 keys of 256 rows has 1024 cycles
-//   of exponentials and 1280 of products and takes 2600.  Without the exponentials' instructions it would take 6 % less, without the conversion's arithmetic 13 % (e4m3 comes by the unit that the
-//   exponentials use), without maxima 6 %, with an eighth of Q K^T 11 %: several chains of a tile (scores, softmax, product; copy, conversion) are about as long as each other.  An item's
-//   beginning and end, at which both row tiles drain, cost 7 us.
+//   Larger blocks.  8192 rows of 28 heads of 128 on 4: e4m3 564 us, 853 TFLOP/s, int8 553 (over a bf16 cache 491, which has nothing to convert).  A tile of 64 keys of 256 rows has 1024 cycles
+//   of exponentials, 1280 of products and 1500 of shared memory's bandwidth (its products' operands, codes and fp16 in and out) and takes 2600.  At 586 us it was 6 % less without the exponentials'
+//   instructions, 13 % without the conversion's arithmetic, 6 % without maxima, 11 % with an eighth of Q K^T: several chains of a tile (scores, softmax, product; copy, conversion) are about as
+//   long as each other.  An item's beginning and end, at which both row tiles drain, cost 7 us.
 #include <cuda.h>
 
 #include <algorithm>
@@ -783,12 +783,14 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
     const uint32_t la = (uint32_t)((warp & 3) * 32) << 16, mine_turn = 2u + 2u * (uint32_t)(warp & 3) + (uint32_t)g;  // the barrier of this warp's turns, beside that of the other row tile's
     int tg = 0;  // tiles of this row tile
     if (tid == 0) info[blockIdx.x].parts = 0;
-    while (next_piece(p)) {
+    bool more = next_piece(p);
+    while (more) {
       const int rows = p.tokens * G;
       if (tid == 0 && !p.whole() && p.begin == 0)  // goes on in the CTAs behind; the item's last tile is at x1 - left + tiles - 1
         info[blockIdx.x] = JoinInfo{p.t0, p.tokens, p.kvh, (int)quotient(x1 - p.left + p.tiles - 1, share) - (int)blockIdx.x + 1};
       if (g * 128 >= rows) {
         T += p.count();
+        more = next_piece(p);
         continue;
       }
       const bool mine = row < rows;
@@ -922,15 +924,16 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         mbar_arrive_tc(bar_p + 16u * g + 8u * b);
       }
-      // ---- the row of the result
+      // ---- the row of the result, and (heads of 128) the next piece while the last product is under way: 8192 rows 586 -> 562 us; with heads of 64 16 portions 107 -> 108
+      const bool whole = p.whole();
+      bf16* dst = a.out + (size_t)(p.t0 + tok) * a.out_stride + (size_t)(p.kvh * G + gh) * HD;
+      float* part = parts + ((size_t)blockIdx.x * 2 + (p.begin == 0)) * PART<HD, ROWS_P>;
+      if (HD == 128) more = next_piece(p);
       wait_short(bar_o + 16u * g + 8u * ((tg - 1) & 1), (uint32_t)(((tg - 1) >> 1) & 1), dead);
       __syncwarp();
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const bool whole = p.whole();
       const float back = __uint_as_float((uint32_t)lr << 23) * (1.f / (1 << P_EXP)), nan = __int_as_float(0x7fc00000);
       const float scale = *dead ? nan : !whole ? back : l_run > 0.f ? back / l_run : l_run;
-      bf16* dst = a.out + (size_t)(p.t0 + tok) * a.out_stride + (size_t)(p.kvh * G + gh) * HD;
-      float* part = parts + ((size_t)blockIdx.x * 2 + (p.begin == 0)) * PART<HD, ROWS_P>;
       if (!whole) part[ROWS_P * HD + row] = m_ref, part[ROWS_P * HD + ROWS_P + row] = *dead ? nan : l_run;
 #pragma unroll
       for (int c = 0; c < HD; c += 32) {
@@ -961,6 +964,7 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
       }
       __syncwarp();
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");  // (the next queries and weights let the products on)
+      if (HD == 64) more = next_piece(p);
     }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
