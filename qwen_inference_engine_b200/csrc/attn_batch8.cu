@@ -505,8 +505,6 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
   __shared__ unsigned long long s_bad[2];   // (edge tiles, by parity) keys whose values are no numbers
   volatile int* dead = &dead_s;
   if (TMA && threadIdx.x == 18 * 32) asm volatile("prefetch.tensormap [%0];" ::"l"(&cm) : "memory");
-  pdl_wait();
-  pdl_trigger();
   const uint32_t s0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* smem = smem_raw + (s0 - smem_u32(smem_raw));
   // barriers: of a row tile queries, and by its tile's parity scores, weights and product; of the stages of codes, keys and values full and free
@@ -525,6 +523,8 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  pdl_wait();
+  pdl_trigger();
   const auto [share, x1] = find_stretch<THR_P>(a, tt, s_sums, &s_walk);
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
@@ -994,13 +994,14 @@ cudaError_t launch_prompt(const BatchAttnArgs& a, const Kv8Geom& kv, int G, cons
 }
 
 // the parts of both kernels' items
-template <int HD>
+template <int HD, int SLICES>
 __global__ void __launch_bounds__(JOIN_THR, 2) attn_both8_join_kernel(BatchAttnArgs large, BatchAttnArgs small, JoinShape sh_large, JoinShape sh_small, int n_large, int n_small) {
   __shared__ Sum4 sums[JOIN_THR];
   pdl_wait();
   pdl_trigger();
-  if ((int)blockIdx.x < n_large) join_parts<HD, ROWS_P>(large, sh_large, n_large, blockIdx.x, sums);
-  else if (blockIdx.y == 0) join_parts<HD, ROWS_F>(small, sh_small, n_small, (int)blockIdx.x - n_large, sums);
+  const int k = blockIdx.x;  // (of large items' columns parts side by side, and behind them small items)
+  if (k < n_large * SLICES) join_parts<HD, ROWS_P>(large, sh_large, n_large, k / SLICES, k % SLICES, sums);
+  else join_parts<HD, ROWS_F>(small, sh_small, n_small, k - n_large * SLICES, 0, sums);
 }
 size_t work_few(int hd, int num_sms) { return 2 * (size_t)num_sms * (sizeof(JoinInfo) + 2 * (hd == 64 ? PART<64, ROWS_F> : PART<128, ROWS_F>) * sizeof(float)); }
 size_t work_prompt(int hd, int num_sms) { return (size_t)num_sms * (sizeof(JoinInfo) + 2 * (hd == 64 ? PART<64, ROWS_P> : PART<128, ROWS_P>) * sizeof(float)); }
@@ -1040,7 +1041,7 @@ cudaError_t launch_attention_batch8(const BatchAttnArgs& a, const Kv8Geom& kv, c
     else r = group <= 8 ? launch_few<HD, CODE, 1, false>(small, kv, sh, 8 / g, box_f, !few, cm_f, st) : launch_few<HD, CODE, 2, false>(small, kv, sh, ROWS_F / g, box_f, !few, cm_f, st);
     if (few || r != cudaSuccess) return r;
     constexpr int SLICES = HD / 4 / (JOIN_THR / ROWS_P) / 4;
-    return launched(launch_k(attn_both8_join_kernel<HD>, dim3(3 * a.num_sms, SLICES), dim3(JOIN_THR), 0, st, large, small, JoinShape{group, group, 1}, sh, a.num_sms, 2 * a.num_sms));
+    return launched(launch_k(attn_both8_join_kernel<HD, SLICES>, dim3((SLICES + 2) * a.num_sms), dim3(JOIN_THR), 0, st, large, small, JoinShape{group, group, 1}, sh, a.num_sms, 2 * a.num_sms));
   };
   using std::integral_constant;
   if (kv.hd == 64) return kv.code == KV8_E4M3 ? go(integral_constant<int, 64>(), integral_constant<int, KV8_E4M3>()) : go(integral_constant<int, 64>(), integral_constant<int, KV8_INT8>());

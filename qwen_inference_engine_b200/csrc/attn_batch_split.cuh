@@ -115,12 +115,12 @@ struct JoinShape {
   int g, group, subs;
 };
 template <int HD, int ROWS>
-__device__ __forceinline__ void join_parts(const BatchAttnArgs& a, const JoinShape& sh, int n_cta, int of, Sum4* sums) {  // of: the CTA of the kernel above
+__device__ __forceinline__ void join_parts(const BatchAttnArgs& a, const JoinShape& sh, int n_cta, int of, int part_of_rows, Sum4* sums) {  // of: the CTA of the kernel above; of many rows' columns the part
   constexpr int C = HD / 4;  // groups of columns
   constexpr bool MANY = ROWS * C > JOIN_THR;  // rows enough for more than one step of a CTA's threads
   const JoinInfo* info = reinterpret_cast<const JoinInfo*>(a.work);
   JoinInfo in = info[of];
-  int slice = blockIdx.y, cta = of, slices = 1;  // of many rows' columns; of few rows' columns, where an item has many parts: the CTAs behind the first have none that begin there
+  int slice = part_of_rows, cta = of, slices = 1;  // of many rows' columns; of few rows' columns, where an item has many parts: the CTAs behind the first have none that begin there
   if constexpr (!MANY) {
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(JOIN_THR, 2) attn_batch_join_kernel(BatchAttnA
   __shared__ Sum4 sums[JOIN_THR];
   pdl_wait();
   pdl_trigger();
-  join_parts<HD, ROWS>(a, sh, n_cta, blockIdx.x, sums);
+  join_parts<HD, ROWS>(a, sh, n_cta, blockIdx.x, blockIdx.y, sums);
 }
 template <int HD, int ROWS>
 inline cudaError_t launch_join(const BatchAttnArgs& a, const JoinShape& sh, int ctas, cudaStream_t st) {
