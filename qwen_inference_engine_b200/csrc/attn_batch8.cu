@@ -1014,7 +1014,7 @@ cudaError_t launch_attention_batch8(const BatchAttnArgs& a, const Kv8Geom& kv, c
   const int group = a.n_q / kv.n_kv, g = std::min(group, ROWS_F), P = kv.page_size;
   const JoinShape sh{g, group, (group + g - 1) / g};
   // Requests of so many rows that their keys and values are read once or twice by blocks of few rows are theirs, the others have blocks of up to 256 (a decode row in one of those costs
-  // what 256 rows do: 48 of them at 2800 positions on average beside four portions of a prompt 105 us, by both kernels 84; 16 portions without decode rows 104 and 107).  Where the step has no more rows than requests, all of them
+  // what 256 rows do: 48 of them at 2800 positions on average beside four portions of a prompt 105 us, by both kernels 82; 16 portions without decode rows 104 and 105).  Where the step has no more rows than requests, all of them
   // are blocks of few rows (a request with many rows reads its keys and values that much more often); the room counts, which the host knows, and not the step's rows, which it does not.
   const bool few = a.n_tok <= a.n_req;
   // boxes of the most rows, a power of two, that divide a page and a unit or tile; a tile's scales come by bulk copies of a multiple of 16 bytes
