@@ -519,7 +519,7 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
     for (int i = 0; i < ST; ++i) mbar_init_tc(k_full + 8 * i, 4), mbar_init_tc(k_free + 8 * i, 2), mbar_init_tc(v_full + 8 * i, 4), mbar_init_tc(v_free + 8 * i, 2);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 16) {
+  if (warp == 16) {  // (ahead of the kernel before: 61440 of an SM's registers are this CTA's, so none of that kernel's that still wants TMEM columns is on the SM)
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
