@@ -109,7 +109,7 @@ struct Ring {
 // four positions 16 bytes a lane): keys from there as the rows of a product K Q^T, the weights by a transposition of 8 x 8 into fragments of V^T P^T, values with neighbouring keys' bytes
 // beside each other.  The columns of a row are numbered so that a lane's are 16 bytes together.  No barrier but the warp's own; the warps' results are added up at the end of a piece.
 template <int HD, int CODE, int NB, bool TMA>
-__global__ void __launch_bounds__(Ring<HD>::THR, NB == 1 ? 2 : 1) attn_few8_kernel(BatchAttnArgs a, Kv8Geom kv, JoinShape sh, int tt, int box, int behind, const __grid_constant__ CUtensorMap cm) {
+__global__ void __launch_bounds__(Ring<HD>::THR, NB == 1 ? 2 : 1) attn_few8_kernel(BatchAttnArgs a, Kv8Geom kv, JoinShape sh, int tt, int box, const __grid_constant__ CUtensorMap cm) {
   constexpr int C = HD / 64, VW = HD / 32, MB = HD / 16;  // 16-byte pieces of a key row a lane; words of a value row a lane; blocks of 16 columns
   constexpr int UNIT = Ring<HD>::UNIT, ST = Ring<HD>::STAGES, WARPS_F = Ring<HD>::WARPS, THR_F = Ring<HD>::THR;
   static_assert(NB * 8 * HD * 4 <= Ring<HD>::WARP, "a warp's results take its ring's place");
@@ -125,9 +125,7 @@ __global__ void __launch_bounds__(Ring<HD>::THR, NB == 1 ? 2 : 1) attn_few8_kern
   unsigned char* s_ring = smem_raw + ((smem_u32(smem_raw) + 1023u & ~1023u) - smem_u32(smem_raw));
   float* s_o = reinterpret_cast<float*>(s_ring);
   if (TMA && threadIdx.x == 32) asm volatile("prefetch.tensormap [%0];" ::"l"(&cm) : "memory");
-  // `behind` the kernel of larger blocks, whose results it has nothing to do with: that one let it in behind its own wait, so what both read is there, and it waits for it at the end, so that
-  // what follows follows both
-  if (!behind) pdl_wait();
+  pdl_wait();  // (behind the kernel of larger blocks too, with which it shares nothing: what that one waited for is there for this one's loads behind a wait of its own)
   pdl_trigger();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const uint32_t ring = smem_u32(s_ring) + warp * Ring<HD>::WARP;
@@ -441,7 +439,6 @@ __global__ void __launch_bounds__(Ring<HD>::THR, NB == 1 ? 2 : 1) attn_few8_kern
     drain_tc(dead);
     report_tc(dead, a.status);
   }
-  if (behind) pdl_wait();
 }
 
 template <int HD, int CODE, int NB, bool TMA>
@@ -456,7 +453,7 @@ cudaError_t launch_few(const BatchAttnArgs& a, const Kv8Geom& kv, const JoinShap
   BatchAttnArgs b = a;
   b.kv.n_kv *= sh.subs;
   b.rest = 7;  // (64 rows, heads of 128, with 3: CTAs with one piece end at 18 us, with two at 21)
-  const cudaError_t e = launched(launch_k(attn_few8_kernel<HD, CODE, NB, TMA>, dim3(ctas), dim3(Ring<HD>::THR), Ring<HD>::SMEM, st, b, kv, sh, tt, box, (int)behind, *reinterpret_cast<const CUtensorMap*>(&cm)));
+  const cudaError_t e = launched(launch_k(attn_few8_kernel<HD, CODE, NB, TMA>, dim3(ctas), dim3(Ring<HD>::THR), Ring<HD>::SMEM, st, b, kv, sh, tt, box, *reinterpret_cast<const CUtensorMap*>(&cm)));
   return e != cudaSuccess || behind ? e : launch_join<HD, ROWS_F>(a, sh, ctas, st);
 }
 
