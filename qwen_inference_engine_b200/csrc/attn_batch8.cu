@@ -36,34 +36,6 @@ namespace {
 constexpr float LAG = 8.f;
 constexpr int P_EXP = 7;
 
-// mbar_wait_tc in few instructions: the loops of a CTA's roles are to stay in the instruction caches together (where they did not, 8192 rows took
-// 943 us instead of 786).  2^26 tries are about two seconds.
-__device__ __forceinline__ void wait_short(uint32_t bar, uint32_t parity, volatile int* dead) {
-  uint32_t done;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(done)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  if (done || *dead) return;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t.reg .u32 i;\n\t"
-      "mov.u32 i, 0;\n"
-      "again:\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "@p bra.uni out;\n\t"
-      "add.u32 i, i, 1;\n\t"
-      "setp.lt.u32 q, i, 67108864;\n\t"
-      "@q bra.uni again;\n"
-      "out:\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(done)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  if (!done) *dead = 1;
-}
 // a 16-byte piece of a row in shared memory: in the order that TMA gives with a swizzle over a row's bytes
 template <int HD>
 __device__ __forceinline__ int piece_at(int row, int piece) {
@@ -246,7 +218,7 @@ __global__ void __launch_bounds__(Ring<HD>::THR, NB == 1 ? 2 : 1) attn_few8_kern
     int stage = J % ST;
     for (int j = 0; j < n; ++j) {
       if (pend_at >= 0) s_scale[warp][pend_at][lane] = sk[0], s_scale[warp][pend_at][32 + lane] = sv[0];  // (a step later than asked for)
-      if constexpr (TMA) wait_short(smem_u32(&s_bar[warp][stage]), (uint32_t)((J + j) / ST & 1), dead);
+      if constexpr (TMA) mbar_wait_short_tc(smem_u32(&s_bar[warp][stage]), (uint32_t)((J + j) / ST & 1), dead);
       else cp_async_wait<ST - 2>();
       __syncwarp();  // the unit is there, and nobody reads the one before any more
       pend_at = -1;
@@ -569,7 +541,7 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
         if (TMA) page_of = bt[min((held + lane) * box / P, last_page)];
         for (int i = p.begin; i < p.end; ++i, ++T) {
           const int st = T % RAW;
-          if (T >= RAW) wait_short(raw_free + 8u * st, (uint32_t)((T / RAW - 1) & 1), dead);
+          if (T >= RAW) mbar_wait_short_tc(raw_free + 8u * st, (uint32_t)((T / RAW - 1) & 1), dead);
           __syncwarp();
           const uint32_t bar = raw_full + 8u * st, dst = s0 + SM::C + st * 2 * SM::CODES, sc = s0 + SM::SC + st * 2 * TK;
           if constexpr (TMA) {
@@ -630,7 +602,7 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
       int items = 0, tg = 0;  // items and tiles of this row tile
       auto issue_s = [&](int ahead) {
         const int at = T + ahead, b = (tg + ahead) & 1;
-        wait_short(k_full + 8u * (uint32_t)(at % ST), (uint32_t)((at / ST) & 1), dead);
+        mbar_wait_short_tc(k_full + 8u * (uint32_t)(at % ST), (uint32_t)((at / ST) & 1), dead);
         __syncwarp();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (elect_tc()) {
@@ -651,23 +623,23 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
         if (g * 128 >= p.tokens * G) {  // nothing to do but to let the stages go
           for (int i = 0; i < n; ++i, ++T) {
             const uint32_t st = (uint32_t)(T % ST), ph = (uint32_t)((T / ST) & 1);
-            wait_short(k_full + 8u * st, ph, dead);
+            mbar_wait_short_tc(k_full + 8u * st, ph, dead);
             if (lane == 0) mbar_arrive_tc(k_free + 8u * st);
-            wait_short(v_full + 8u * st, ph, dead);
+            mbar_wait_short_tc(v_full + 8u * st, ph, dead);
             if (lane == 0) mbar_arrive_tc(v_free + 8u * st);
             __syncwarp();
           }
           continue;
         }
-        wait_short(bar_q + 8u * g, (uint32_t)(items & 1), dead);
+        mbar_wait_short_tc(bar_q + 8u * g, (uint32_t)(items & 1), dead);
         ++items;
         issue_s(0);
         if (n > 1) issue_s(1);
         for (int i = 0; i < n; ++i, ++T, ++tg) {
           const uint32_t st = (uint32_t)(T % ST), ph = (uint32_t)((tg >> 1) & 1);
           const int b = tg & 1;
-          wait_short(v_full + 8u * st, (uint32_t)((T / ST) & 1), dead);
-          wait_short(bar_p + 16u * g + 8u * b, ph, dead);
+          mbar_wait_short_tc(v_full + 8u * st, (uint32_t)((T / ST) & 1), dead);
+          mbar_wait_short_tc(bar_p + 16u * g + 8u * b, ph, dead);
           __syncwarp();
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           if (elect_tc()) {
@@ -679,7 +651,7 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
           }
           __syncwarp();
           if (i + 2 < n) {
-            wait_short(bar_o + 16u * g + 8u * b, ph, dead);  // the scores two tiles ahead go over the weights that this product reads
+            mbar_wait_short_tc(bar_o + 16u * g + 8u * b, ph, dead);  // the scores two tiles ahead go over the weights that this product reads
             issue_s(2);
           }
         }
@@ -701,7 +673,7 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
       for (int i = p.begin; i < p.end; ++i, ++T) {
         const int rs = T % RAW, st = T % ST, key = p.key0 + i * TK;
         const bool edge = key + TK > p.pos0 + 1 || key < low1;  // some row does not see some key of the tile
-        wait_short(raw_full + 8u * (uint32_t)rs, (uint32_t)((T / RAW) & 1), dead);
+        mbar_wait_short_tc(raw_full + 8u * (uint32_t)rs, (uint32_t)((T / RAW) & 1), dead);
         const unsigned char *codes = smem + SM::C + (rs * 2 + is_v) * SM::CODES, *sc = smem + SM::SC + rs * 2 * TK;
         auto seen = [&](int row) { return key + row >= low0 && key + row < end; };  // by some row
         uint4 code[UNITS];
@@ -748,7 +720,7 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
             if (is_v ? none || !seen(row) : none || sb[h] == 255) factor[h] = is_v ? 0xffffffffu : 0x7e007e00u;
           }
         }
-        if (T >= ST) wait_short(free_ + 8u * (uint32_t)st, (uint32_t)((T / ST - 1) & 1), dead);
+        if (T >= ST) mbar_wait_short_tc(free_ + 8u * (uint32_t)st, (uint32_t)((T / ST - 1) & 1), dead);
         __syncwarp();
         const uint32_t to = s0 + (is_v ? SM::V : SM::K) + st * SM::TILE + nb * KBLK;
 #pragma unroll
@@ -844,7 +816,7 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
         const int b = tg & 1;
         const uint32_t ts = t_s(g, b) + la, ph = (uint32_t)((tg >> 1) & 1);
         const int key = p.key0 + i * TK, last = my_pos - key, low = my_low - key;  // the first key of the tile; the last and the first that the row sees
-        wait_short(bar_s + 16u * g + 8u * b, ph, dead);
+        mbar_wait_short_tc(bar_s + 16u * g + 8u * b, ph, dead);
         __syncwarp();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         uint32_t r[TK];
@@ -902,7 +874,7 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
         if (turns && (g == 0 || i + 1 < p.end)) asm volatile("bar.arrive %0, 64;" ::"r"(mine_turn ^ 1u) : "memory");
         l_run += ((rs[0] + rs[1]) + (rs[2] + rs[3])) * __uint_as_float((uint32_t)(127 - d) << 23);
         if (grow && i > p.begin) {  // O, behind the product of the tile before
-          wait_short(bar_o + 16u * g + 8u * (b ^ 1), (uint32_t)(((tg - 1) >> 1) & 1), dead);
+          mbar_wait_short_tc(bar_o + 16u * g + 8u * (b ^ 1), (uint32_t)(((tg - 1) >> 1) & 1), dead);
           __syncwarp();
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
@@ -926,7 +898,7 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
       bf16* dst = a.out + (size_t)(p.t0 + tok) * a.out_stride + (size_t)(p.kvh * G + gh) * HD;
       float* part = parts + ((size_t)blockIdx.x * 2 + (p.begin == 0)) * PART<HD, ROWS_P>;
       if (HD == 128) more = next_piece(p);
-      wait_short(bar_o + 16u * g + 8u * ((tg - 1) & 1), (uint32_t)(((tg - 1) >> 1) & 1), dead);
+      mbar_wait_short_tc(bar_o + 16u * g + 8u * ((tg - 1) & 1), (uint32_t)(((tg - 1) >> 1) & 1), dead);
       __syncwarp();
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const float back = __uint_as_float((uint32_t)lr << 23) * (1.f / (1 << P_EXP)), nan = __int_as_float(0x7fc00000);

@@ -395,19 +395,20 @@ cudaError_t launch_hd(const FastAttnArgs& a, int two_term, const TensorMap2D& kv
   return cudaLaunchKernelEx(&cfg, attn_prompt_tc_kernel<HD>, a, two_term, parts, alone, *reinterpret_cast<const CUtensorMap*>(&kvm));
 }
 
-// a pair of CTAs: the wait is the first one's, the report the other one's
+// a pair of CTAs: the wait is the first one's, the report the other one's, where a short wait of a whole warp of its own has run out too
 __global__ void __cluster_dims__(2) wait_selftest_kernel(int* status) {
   __shared__ __align__(8) unsigned long long bar;
-  __shared__ int dead_s;
+  __shared__ int dead_s, short_s;
   const bool one = threadIdx.x == 0;
-  if (one) dead_s = 0, mbar_init_tc(smem_u32(&bar), 1);
+  if (one) dead_s = short_s = 0, mbar_init_tc(smem_u32(&bar), 1);
   cluster_sync_all();
+  if (blockIdx.x == 1) mbar_wait_short_tc(smem_u32(&bar), 0, &short_s);
   if (blockIdx.x == 0 && one) {
     mbar_wait_tc(smem_u32(&bar), 0, &dead_s);
     tell_other_tc(&dead_s);
   }
   cluster_sync_all();
-  if (blockIdx.x == 1 && one) report_tc(&dead_s, status);
+  if (blockIdx.x == 1 && one && short_s) report_tc(&dead_s, status);
 }
 
 }  // namespace

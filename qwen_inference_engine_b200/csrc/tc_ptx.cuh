@@ -14,18 +14,21 @@ __device__ __forceinline__ void mbar_arrive_tc(uint32_t bar) {
 // Waits for the phase of this parity.  After about two seconds it sets *dead, and from then on no wait of the CTA waits: its kernel stores values
 // that are not numbers, lets copies in flight land (drain_tc), reports (report_tc) and returns.  The clock is read only where a wait is long.
 constexpr long long WAIT_CYCLES_TC = 4000000000ll;
+__device__ __forceinline__ bool mbar_try_tc(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
 __device__ __forceinline__ bool mbar_wait_tc(uint32_t bar, uint32_t parity, volatile int* dead) {
   long long t0 = 0;
   for (int i = 0;; ++i) {
-    uint32_t done = 0;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    if (done) return true;
+    if (mbar_try_tc(bar, parity)) return true;
     if ((i & 31) == 31) {
       if (*dead) return false;
       if (i == 31) t0 = clock64();
@@ -35,7 +38,18 @@ __device__ __forceinline__ bool mbar_wait_tc(uint32_t bar, uint32_t parity, vola
   *dead = 1;
   return false;
 }
-// The same by all threads of a warp.  They leave the loop above one by one, and tcgen05.ld and .st (`.sync.aligned`) want them together.
+// The same in fewer instructions, for kernels whose roles' loops only just share the instruction caches (8192 rows of attention over a cache in 8 bits with the loop above 943 us, with a short one
+// 786): the clock at every try of a wait that is not over at once, each of which the hardware may stretch as it likes.
+__device__ __forceinline__ void mbar_wait_short_tc(uint32_t bar, uint32_t parity, volatile int* dead) {
+  if (mbar_try_tc(bar, parity) || *dead) return;
+  const long long t0 = clock64();
+#pragma unroll 1
+  do {
+    if (mbar_try_tc(bar, parity) || *dead) return;
+  } while (clock64() - t0 <= WAIT_CYCLES_TC);
+  *dead = 1;
+}
+// The first one by all threads of a warp.  They leave the loop above one by one, and tcgen05.ld and .st (`.sync.aligned`) want them together.
 __device__ __forceinline__ void mbar_wait_warp_tc(uint32_t bar, uint32_t parity, volatile int* dead) {
   mbar_wait_tc(bar, parity, dead);
   __syncwarp();

@@ -1,6 +1,8 @@
 """A wait inside a kernel that runs out (csrc/tc_ptx.cuh) is an error of the call that learns of it, once, and the context stays usable.  The
 self-test's wait is on a barrier that nothing completes, through the limit and the report that the tcgen05 kernels use.  It is a pair of CTAs as the GEMM's are: the
 first one waits and the other one, which waits for nothing, reports what it was told (tell_other_tc)."""
+import time
+
 import numpy as np
 import pytest
 import torch
@@ -50,3 +52,15 @@ def test_an_engine_learns_of_its_own(lib):
         assert e.prefill(s, ids) == want
         assert np.asarray(e.decode_step([s], [want])).size == 1
         e.close()
+
+
+def test_both_kinds_of_waits_end_in_time(lib):
+    """the self-test has the long loop and the short one (mbar_wait_short_tc, of attention over a cache in 8 bits) run out side by side, and reports where both did"""
+    L = lib.lib()
+    for _ in range(2):
+        torch.cuda.synchronize()
+        t0 = time.monotonic()
+        assert L.qie_wait_selftest(None, None) == 0
+        torch.cuda.synchronize()
+        assert 1.0 < time.monotonic() - t0 < 8.0  # 4e9 cycles at 0.5 to 2 GHz, and no second limit behind the first
+        assert L.qie_kernel_status() < 0 and L.qie_kernel_status() == 0
