@@ -51,7 +51,7 @@ template <int HD, int CODE, int TURN, bool WIDE>
 __global__ void __launch_bounds__(THR, 4) rope_store8_kernel(Rope8Args a, PageDiv div, int chunks, int per) {
   constexpr int LH = HD / 8, HW = 32 / LH;                                             // lanes of a head, heads of a warp at a time: a group
   constexpr int NP = TURN == TURN_NEIGHBOURS ? 4 : TURN == TURN_NONE ? 1 : 8, U = 4;  // pairs that the lane has a part of; groups ahead
-  __shared__ bf16 s_row[TURN == TURN_ANY ? WARPS * HW * HD : 1];
+  __shared__ uint4 s_row[TURN == TURN_ANY ? WARPS * HW * LH : 1];  // (a type with the alignment of its accesses)
   __shared__ unsigned long long s_turns[HD / 2];          // of the pairs a position, their fraction in 2^-64
   __shared__ __align__(16) float2 s_cs[WARPS][HD / 2];  // of a warp's token
   pdl_wait();
@@ -136,9 +136,10 @@ __global__ void __launch_bounds__(THR, 4) rope_store8_kernel(Rope8Args a, PageDi
 #pragma unroll
         for (int j = 0; j < 4; ++j) y[2 * j] = lo2f(x[j]), y[2 * j + 1] = hi2f(x[j]);
         if constexpr (TURN == TURN_ANY) {
-          bf16* mine = s_row + (warp * HW + sub) * HD;
+          uint4* head = s_row + (warp * HW + sub) * LH;
+          const bf16* mine = reinterpret_cast<const bf16*>(head);
           __syncwarp();
-          *reinterpret_cast<uint4*>(mine + e0) = make_uint4(x[0], x[1], x[2], x[3]);
+          head[p] = make_uint4(x[0], x[1], x[2], x[3]);
           __syncwarp();
 #pragma unroll
           for (int j = 0; j < 8; ++j) {

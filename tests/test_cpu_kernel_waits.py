@@ -24,3 +24,14 @@ def test_waits_whatever_the_call(name, n):
         assert lines.index("  pdl_trigger();") > at, kernel
         early = "\n".join(lines[:at])
         assert not re.search(r"\ba\.(q|out|work|status|q_start|kv_len|slots|block_table|pos|row|k|v|freq)\b|\bkv\.(codes|scale)\b|find_stretch|join_parts", early), kernel
+
+
+def test_shared_arrays_have_the_alignment_of_their_accesses():
+    """no __shared__ array of elements below 16 bytes, without an alignment of its own, that the file goes through 16 bytes at a time"""
+    for name in ("attn_batch8.cu", "attn_batch_split.cuh", "kv8_store.cu"):
+        src = re.sub(r" *//[^\n]*", "", open(os.path.join(CSRC, name)).read())
+        small = re.findall(r"__shared__ (?:bf16|float|int|uint8_t|uint32_t|long long|unsigned long long) (\w+)\[", src)
+        for a in small:
+            names = {a} | set(re.findall(r"\* *(\w+) = (?:reinterpret_cast<[^>]*>\()?%s\b" % a, src))
+            for n in names:
+                assert not re.search(r"reinterpret_cast<(?:const )?(?:uint4|float4|int4|uint2|float2)\*>\(&?%s\b" % n, src), (name, a)
