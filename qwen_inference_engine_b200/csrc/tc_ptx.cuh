@@ -39,15 +39,27 @@ __device__ __forceinline__ bool mbar_wait_tc(uint32_t bar, uint32_t parity, vola
   return false;
 }
 // The same in fewer instructions, for kernels whose roles' loops only just share the instruction caches (8192 rows of attention over a cache in 8 bits with the loop above 943 us, with a short one
-// 786): the clock at every try of a wait that is not over at once, each of which the hardware may stretch as it likes.
+// 786; written as a loop of C++ with a look at `dead` at every try 631 where this one is 546).  The clock is read at every try, each of which the hardware may stretch as it likes; threads leave
+// one by one.
 __device__ __forceinline__ void mbar_wait_short_tc(uint32_t bar, uint32_t parity, volatile int* dead) {
   if (mbar_try_tc(bar, parity) || *dead) return;
-  const long long t0 = clock64();
-#pragma unroll 1
-  do {
-    if (mbar_try_tc(bar, parity) || *dead) return;
-  } while (clock64() - t0 <= WAIT_CYCLES_TC);
-  *dead = 1;
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .s64 t0, t;\n\t"
+      "mov.u64 t0, %%clock64;\n"
+      "again:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "@p bra out;\n\t"
+      "mov.u64 t, %%clock64;\n\t"
+      "sub.s64 t, t, t0;\n\t"
+      "setp.le.s64 q, t, %3;\n\t"
+      "@q bra again;\n"
+      "out:\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity), "n"(WAIT_CYCLES_TC)
+      : "memory");
+  if (!done) *dead = 1;
 }
 // The first one by all threads of a warp.  They leave the loop above one by one, and tcgen05.ld and .st (`.sync.aligned`) want them together.
 __device__ __forceinline__ void mbar_wait_warp_tc(uint32_t bar, uint32_t parity, volatile int* dead) {
