@@ -3,9 +3,9 @@
 //
 //   out_t = sum_j 2^(x_tj - m) 2^ev_j v_j / sum_j 2^(x_tj - m),  x_tj = s 2^ek_j (q_t . k_j) over the positions j that row t sees, m their running maximum, k_j and v_j codes
 //
-// Codes become fp16 exactly.  A row's query is brought to fp16 by a power of two of its own, which loses nothing either, so scores are those of the values that the cache stands for,
-// summed in fp32.  Weights are fp16 in the product with the values (2^-11 of themselves; 2^7 times themselves and times their value's scale, so that none of at least 2^-21 of the
-// largest gets fewer bits, and none is off by more than 2^-32 of it), their sums fp32.
+// Codes become fp16 exactly (larger blocks: beside their tile's largest scale).  A row's query is brought to fp16 by a power of two of its own, which loses nothing, and scores are summed in
+// fp32.  Weights are fp16 in the product with the values, 2^-11 of themselves; they are there by 2^7 and their value's scale, in blocks of few rows beside the largest such product that the row
+// itself has seen, so that none is off by more than 2^-31 of that, whatever lies beside it; their sums are fp32.
 //
 // An item is a kv head of a request and a block of its tokens, its rows (token, query head of the group); items are shared out over the CTAs as in attn_batch.cu.  There are two kernels: for blocks
 // of at most 16 rows (decode), which memory bounds, one that keeps a unit of keys and values in registers between loads and products, and for larger blocks one on tcgen05 / TMEM.
@@ -33,8 +33,11 @@ namespace qie {
 namespace {
 
 // The weights' reference follows a row's maximum where it has fallen behind by more than 2^8: weights by 2^7 are at most 2^15 then, below the largest fp16.
-constexpr float LAG = 8.f;
-constexpr int P_EXP = 7;
+constexpr int LAG_EXP = 8, P_EXP = 7;
+constexpr float LAG = LAG_EXP;
+// from sums beside the reference `ref` of weights times scales (2^P_EXP times themselves) to sums of weights beside `m`, but for 2^LAG_EXP: weights' sums are at most so much more than they
+// would be beside their maximum, and the factor must not leave the range ahead of them.  A row that has seen no value but zeros: 0
+__device__ __forceinline__ float result_scale(float ref, float m) { return ref > -INFINITY ? ex2_tc(ref - m - (float)(P_EXP + LAG_EXP)) : 0.f; }
 
 // a 16-byte piece of a row in shared memory: in the order that TMA gives with a swizzle over a row's bytes
 template <int HD>
@@ -88,8 +91,7 @@ __global__ void __launch_bounds__(Ring<HD>::THR, NB == 1 ? 2 : 1) attn_few8_kern
   extern __shared__ __align__(1024) unsigned char smem_raw[];  // [warp][stage][k|v][key][column], and in its place the warp's results [row][column]
   __shared__ long long s_sums[THR_F / 32];
   __shared__ Walk s_walk;
-  __shared__ float s_m[WARPS_F][NB * 8], s_l[WARPS_F][NB * 8];
-  __shared__ int s_r[WARPS_F];
+  __shared__ float s_m[WARPS_F][NB * 8], s_l[WARPS_F][NB * 8], s_ref[WARPS_F][NB * 8];
   __shared__ uint8_t s_scale[WARPS_F][ST][64];  // keys', values'
   __shared__ unsigned long long s_bar[WARPS_F][ST];
   __shared__ int dead_s;
@@ -208,10 +210,10 @@ __global__ void __launch_bounds__(Ring<HD>::THR, NB == 1 ? 2 : 1) attn_few8_kern
         pos[nb][e] = p.pos0 + min((nb * 8 + 2 * t + e) / G, p.tokens - 1);
       }
     }
-    float o[NB][MB][4] = {}, m[NB][2], l[NB][2];
-    int lr = 1;  // the largest scale of a value so far, as its byte
+    // a row's references: of its weights (l), and of its weights times their values' scales (o), a whole number; both are the row's own, of keys that it sees
+    float o[NB][MB][4] = {}, m[NB][2], l[NB][2], ref[NB][2];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) m[nb][0] = m[nb][1] = -INFINITY, l[nb][0] = l[nb][1] = 0.f;
+    for (int nb = 0; nb < NB; ++nb) m[nb][0] = m[nb][1] = ref[nb][0] = ref[nb][1] = -INFINITY, l[nb][0] = l[nb][1] = 0.f;
 #pragma unroll
     for (int s = 0; s < ST - 1; ++s)
       if (s < n) s_scale[warp][(J + s) % ST][lane] = sk[s], s_scale[warp][(J + s) % ST][32 + lane] = sv[s];
@@ -261,8 +263,6 @@ __global__ void __launch_bounds__(Ring<HD>::THR, NB == 1 ? 2 : 1) attn_few8_kern
       uint32_t kb_[4], vb_[4];  // scales of the keys g + 8 i
 #pragma unroll
       for (int i = 0; i < 4; ++i) kb_[i] = sc[g + 8 * i], vb_[i] = sc[32 + g + 8 * i];
-      const uint32_t mine = sc[32 + lane];
-      const int key_l = key0 + lane, top = (int)__reduce_max_sync(0xffffffffu, mine == 255 || (edge && (key_l >= end || key_l < low0)) ? 0u : mine);
       uint32_t bad = 0;
       if (edge && CODE == KV8_E4M3) {  // values that are no numbers must not meet a zero weight: they are zero, and their keys' scores no numbers
 #pragma unroll 1
@@ -280,14 +280,10 @@ __global__ void __launch_bounds__(Ring<HD>::THR, NB == 1 ? 2 : 1) attn_few8_kern
         if (TMA) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (a copy takes the place)
         __syncwarp();
       }
-      float pv[4];  // 2^7 times a value's scale beside the largest
-      const int lr_new = max(lr, top);
+      float ve[4];  // the values' scales, as exponents (of zeros: minus infinity)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int e = (int)vb_[i] - lr_new + 127 + P_EXP;
-        pv[i] = vb_[i] != 0 && e > 0 && e < 255 ? __uint_as_float((uint32_t)e << 23) : 0.f;
-      }
-      bool grow = top > lr;
+      for (int i = 0; i < 4; ++i) ve[i] = vb_[i] == 0 ? -INFINITY : (float)((int)vb_[i] - 127);
+      bool grow = false;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float ks = kv8_scale(vb_[i] == 255 || (bad >> (g + 8 * i) & 1) ? 255u : kb_[i]);
@@ -301,25 +297,24 @@ __global__ void __launch_bounds__(Ring<HD>::THR, NB == 1 ? 2 : 1) attn_few8_kern
               const int key = key0 + g + 8 * i, pos_ = pos[nb][e];
               if (key > pos_ || (a.window > 0 && key <= pos_ - a.window)) y = -INFINITY;
             }
-            grow |= y > m[nb][e] + LAG;
+            grow |= y > m[nb][e] + LAG || y + ve[i] > ref[nb][e] + LAG;
           }
       }
       if (__any_sync(0xffffffffu, grow)) {
-        // the values' products so far: beside the new largest scale, and the rows' new references
-        const float fs = lr_new - lr < 127 ? __uint_as_float((uint32_t)(127 - (lr_new - lr)) << 23) : 0.f;
-        lr = lr_new;
+        // the rows' new references, and what there is so far beside them
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             float mx = fmaxf(fmaxf(x[nb][0][e], x[nb][0][e + 2]), fmaxf(x[nb][1][e], x[nb][1][e + 2]));
+            float rx = fmaxf(fmaxf(x[nb][0][e] + ve[0], x[nb][0][e + 2] + ve[1]), fmaxf(x[nb][1][e] + ve[2], x[nb][1][e + 2] + ve[3]));
 #pragma unroll
-            for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-            const float to = fmaxf(m[nb][e], mx), f = m[nb][e] > -INFINITY ? ex2_tc(m[nb][e] - to) : 1.f;
-            m[nb][e] = to;
-            l[nb][e] *= f;
+            for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d)), rx = fmaxf(rx, __shfl_xor_sync(0xffffffffu, rx, d));
+            const float to = fmaxf(m[nb][e], mx), rto = fmaxf(ref[nb][e], ceilf(rx)), f = ref[nb][e] > -INFINITY ? ex2_tc(ref[nb][e] - rto) : 1.f;
+            if (m[nb][e] > -INFINITY) l[nb][e] *= ex2_tc(m[nb][e] - to);
+            m[nb][e] = to, ref[nb][e] = rto;
 #pragma unroll
-            for (int b = 0; b < MB; ++b) o[nb][b][e] *= f * fs, o[nb][b][e + 2] *= f * fs;
+            for (int b = 0; b < MB; ++b) o[nb][b][e] *= f, o[nb][b][e + 2] *= f;
           }
       }
 #pragma unroll
@@ -335,10 +330,12 @@ __global__ void __launch_bounds__(Ring<HD>::THR, NB == 1 ? 2 : 1) attn_few8_kern
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
           const float m0 = m[nb][0] > -INFINITY ? m[nb][0] : 0.f, m1 = m[nb][1] > -INFINITY ? m[nb][1] : 0.f;
-          const float w0 = ex2_tc(x[nb][kb][0] - m0), w1 = ex2_tc(x[nb][kb][1] - m1), w2 = ex2_tc(x[nb][kb][2] - m0), w3 = ex2_tc(x[nb][kb][3] - m1);
-          l[nb][0] += w0 + w2, l[nb][1] += w1 + w3;
-          pt[nb][0] = transpose_8x8(pack_h(w0 * pv[2 * kb], w1 * pv[2 * kb]));
-          pt[nb][1] = transpose_8x8(pack_h(w2 * pv[2 * kb + 1], w3 * pv[2 * kb + 1]));
+          const float x0 = x[nb][kb][0], x1_ = x[nb][kb][1], x2 = x[nb][kb][2], x3 = x[nb][kb][3];
+          l[nb][0] += ex2_tc(x0 - m0) + ex2_tc(x2 - m0), l[nb][1] += ex2_tc(x1_ - m1) + ex2_tc(x3 - m1);
+          // for the product 2^7 times themselves and their values' scales, beside the row's reference of those
+          const float r0 = P_EXP - (ref[nb][0] > -INFINITY ? ref[nb][0] : 0.f), r1 = P_EXP - (ref[nb][1] > -INFINITY ? ref[nb][1] : 0.f), v0 = ve[2 * kb], v1 = ve[2 * kb + 1];
+          pt[nb][0] = transpose_8x8(pack_h(ex2_tc(x0 + (v0 + r0)), ex2_tc(x1_ + (v0 + r1))));
+          pt[nb][1] = transpose_8x8(pack_h(ex2_tc(x2 + (v1 + r0)), ex2_tc(x3 + (v1 + r1))));
         }
 #pragma unroll
         for (int w = 0; w < VW; ++w) {
@@ -368,39 +365,37 @@ __global__ void __launch_bounds__(Ring<HD>::THR, NB == 1 ? 2 : 1) attn_few8_kern
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) l[nb][e] += __shfl_xor_sync(0xffffffffu, l[nb][e], d);
         const int r = nb * 8 + 2 * t + e;
-        if (g == 0) s_m[warp][r] = m[nb][e], s_l[warp][r] = l[nb][e];
+        if (g == 0) s_m[warp][r] = m[nb][e], s_l[warp][r] = l[nb][e], s_ref[warp][r] = ref[nb][e];
         float* dst = s_o + warp * (Ring<HD>::WARP / 4) + r * HD + g * (HD / 8);
 #pragma unroll
         for (int b = 0; b < MB; ++b) *reinterpret_cast<float2*>(dst + 2 * b) = make_float2(o[nb][b][e], o[nb][b][e + 2]);
       }
-    if (lane == 0) s_r[warp] = lr;
     __syncthreads();
     const bool whole = p.whole();
     for (int i = tid; i < rows * (HD / 4); i += THR_F) {
       const int n = i / (HD / 4), c = i - n * (HD / 4);  // a row, four columns
-      float top = -INFINITY, sum = 0.f;
-      int r = 1;
+      float top = -INFINITY, sum = 0.f, r = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < WARPS_F; ++w) top = fmaxf(top, s_m[w][n]), r = max(r, s_r[w]);
+      for (int w = 0; w < WARPS_F; ++w) top = fmaxf(top, s_m[w][n]), r = fmaxf(r, s_ref[w][n]);
       float4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < WARPS_F; ++w) {
-        const float f = weight(s_m[w][n], s_l[w][n], top);
-        sum += s_l[w][n] * f;
-        const float fo = f * (r - s_r[w] < 127 ? __uint_as_float((uint32_t)(127 - (r - s_r[w])) << 23) : 0.f);
+        sum += s_l[w][n] * weight(s_m[w][n], s_l[w][n], top);
+        const float fo = s_ref[w][n] > -INFINITY ? ex2_tc(s_ref[w][n] - r) : 0.f;
         const float4 x = *reinterpret_cast<const float4*>(s_o + w * (Ring<HD>::WARP / 4) + n * HD + c * 4);
         if (fo != 0.f) acc.x += x.x * fo, acc.y += x.y * fo, acc.z += x.z * fo, acc.w += x.w * fo;
       }
-      const float back = __uint_as_float((uint32_t)r << 23) * (1.f / (1 << P_EXP));
+      const float back = result_scale(r, top);
       if (whole) {
-        const float f = *dead ? __int_as_float(0x7fc00000) : sum > 0.f ? back / sum : sum;
+        const float f = *dead ? __int_as_float(0x7fc00000) : sum > 0.f ? back * ((1 << LAG_EXP) / sum) : sum;
         const int tok = n / G;
         *reinterpret_cast<uint2*>(a.out + (size_t)(p.t0 + tok) * a.out_stride + (head0 + n - tok * G) * HD + c * 4) =
             make_uint2(pack2f(acc.x * f, acc.y * f), pack2f(acc.z * f, acc.w * f));
       } else {
         float* part = parts + ((size_t)blockIdx.x * 2 + (p.begin == 0)) * PART<HD, ROWS_F>;
+        const float all = back * (1 << LAG_EXP);
         if (c == 0) part[ROWS_F * HD + n] = top, part[ROWS_F * HD + ROWS_F + n] = *dead ? __int_as_float(0x7fc00000) : sum;
-        *reinterpret_cast<float4*>(part + (c * ROWS_F + n) * 4) = make_float4(acc.x * back, acc.y * back, acc.z * back, acc.w * back);
+        *reinterpret_cast<float4*>(part + (c * ROWS_F + n) * 4) = make_float4(acc.x * all, acc.y * all, acc.z * all, acc.w * all);
       }
     }
     if (tid == 0 && !whole && p.begin == 0) info[blockIdx.x] = JoinInfo{p.t0, p.tokens, p.kvh, (int)quotient(x1 - p.left + p.tiles - 1, share) - (int)blockIdx.x + 1};
