@@ -35,10 +35,9 @@ namespace {
 // The weights' reference follows a row's maximum where it has fallen behind by more than 2^8: weights by 2^7 are at most 2^15 then, below the largest fp16.
 constexpr int LAG_EXP = 8, P_EXP = 7;
 constexpr float LAG = LAG_EXP;
-// from sums beside the reference `ref` of weights times scales (2^P_EXP times themselves) to sums of weights beside `m`, but for 2^LAG_EXP: weights' sums are at most so much more than they
-// would be beside their maximum, and the factor must not leave the range ahead of them.  A row that has seen no value but zeros: 0
-__device__ __forceinline__ float result_scale(float ref, float m) { return ref > -INFINITY ? ex2_tc(ref - m - (float)(P_EXP + LAG_EXP)) : 0.f; }
-
+// from sums beside the reference of products, 2^rel times the one of weights (2^P_EXP times themselves), to sums beside that one, but for 2^LAG_EXP: weights' sums are at most so much more than
+// they would be beside their maximum, and the factor must not leave the range ahead of them.  A row that has seen no value but zeros: 0
+__device__ __forceinline__ float result_scale(float rel) { return rel > -INFINITY ? ex2_tc(rel - (float)(P_EXP + LAG_EXP)) : 0.f; }
 // a 16-byte piece of a row in shared memory: in the order that TMA gives with a swizzle over a row's bytes
 template <int HD>
 __device__ __forceinline__ int piece_at(int row, int piece) {
@@ -91,7 +90,7 @@ __global__ void __launch_bounds__(Ring<HD>::THR, NB == 1 ? 2 : 1) attn_few8_kern
   extern __shared__ __align__(1024) unsigned char smem_raw[];  // [warp][stage][k|v][key][column], and in its place the warp's results [row][column]
   __shared__ long long s_sums[THR_F / 32];
   __shared__ Walk s_walk;
-  __shared__ float s_m[WARPS_F][NB * 8], s_l[WARPS_F][NB * 8], s_ref[WARPS_F][NB * 8];
+  __shared__ float s_m[WARPS_F][NB * 8], s_l[WARPS_F][NB * 8], s_rel[WARPS_F][NB * 8];
   __shared__ uint8_t s_scale[WARPS_F][ST][64];  // keys', values'
   __shared__ unsigned long long s_bar[WARPS_F][ST];
   __shared__ int dead_s;
@@ -210,10 +209,10 @@ __global__ void __launch_bounds__(Ring<HD>::THR, NB == 1 ? 2 : 1) attn_few8_kern
         pos[nb][e] = p.pos0 + min((nb * 8 + 2 * t + e) / G, p.tokens - 1);
       }
     }
-    // a row's references: of its weights (l), and of its weights times their values' scales (o), a whole number; both are the row's own, of keys that it sees
-    float o[NB][MB][4] = {}, m[NB][2], l[NB][2], ref[NB][2];
+    // a row's references: m of its weights (l), and rel beside m of its weights times their values' scales (o); both are the row's own, of keys that it sees
+    float o[NB][MB][4] = {}, m[NB][2], l[NB][2], rel[NB][2];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) m[nb][0] = m[nb][1] = ref[nb][0] = ref[nb][1] = -INFINITY, l[nb][0] = l[nb][1] = 0.f;
+    for (int nb = 0; nb < NB; ++nb) m[nb][0] = m[nb][1] = rel[nb][0] = rel[nb][1] = -INFINITY, l[nb][0] = l[nb][1] = 0.f;
 #pragma unroll
     for (int s = 0; s < ST - 1; ++s)
       if (s < n) s_scale[warp][(J + s) % ST][lane] = sk[s], s_scale[warp][(J + s) % ST][32 + lane] = sv[s];
@@ -292,12 +291,12 @@ __global__ void __launch_bounds__(Ring<HD>::THR, NB == 1 ? 2 : 1) attn_few8_kern
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             float& y = x[nb][i >> 1][(i & 1) * 2 + e];
-            y *= ks * qf[nb][e];
+            y = __fmul_rn(y, ks * qf[nb][e]);  // (rounded here: its difference from the largest is that of rounded scores)
             if (edge) {
               const int key = key0 + g + 8 * i, pos_ = pos[nb][e];
               if (key > pos_ || (a.window > 0 && key <= pos_ - a.window)) y = -INFINITY;
             }
-            grow |= y > m[nb][e] + LAG || y + ve[i] > ref[nb][e] + LAG;
+            grow |= y > m[nb][e] + LAG || (y - m[nb][e]) + ve[i] > rel[nb][e] + LAG;
           }
       }
       if (__any_sync(0xffffffffu, grow)) {
@@ -307,12 +306,19 @@ __global__ void __launch_bounds__(Ring<HD>::THR, NB == 1 ? 2 : 1) attn_few8_kern
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             float mx = fmaxf(fmaxf(x[nb][0][e], x[nb][0][e + 2]), fmaxf(x[nb][1][e], x[nb][1][e + 2]));
-            float rx = fmaxf(fmaxf(x[nb][0][e] + ve[0], x[nb][0][e + 2] + ve[1]), fmaxf(x[nb][1][e] + ve[2], x[nb][1][e + 2] + ve[3]));
 #pragma unroll
-            for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d)), rx = fmaxf(rx, __shfl_xor_sync(0xffffffffu, rx, d));
-            const float to = fmaxf(m[nb][e], mx), rto = fmaxf(ref[nb][e], ceilf(rx)), f = ref[nb][e] > -INFINITY ? ex2_tc(ref[nb][e] - rto) : 1.f;
-            if (m[nb][e] > -INFINITY) l[nb][e] *= ex2_tc(m[nb][e] - to);
-            m[nb][e] = to, ref[nb][e] = rto;
+            for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+            const float to = fmaxf(m[nb][e], mx), t0 = to > -INFINITY ? to : 0.f;
+            float rx = fmaxf(fmaxf((x[nb][0][e] - t0) + ve[0], (x[nb][0][e + 2] - t0) + ve[1]), fmaxf((x[nb][1][e] - t0) + ve[2], (x[nb][1][e + 2] - t0) + ve[3]));
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) rx = fmaxf(rx, __shfl_xor_sync(0xffffffffu, rx, d));
+            float f = 1.f;
+            if (m[nb][e] > -INFINITY) {
+              const float before = rel[nb][e] + (m[nb][e] - to);
+              rx = fmaxf(rx, before), l[nb][e] *= ex2_tc(m[nb][e] - to);
+              if (before > -INFINITY) f = ex2_tc(before - rx);
+            }
+            m[nb][e] = to, rel[nb][e] = rx;
 #pragma unroll
             for (int b = 0; b < MB; ++b) o[nb][b][e] *= f, o[nb][b][e + 2] *= f;
           }
@@ -330,10 +336,10 @@ __global__ void __launch_bounds__(Ring<HD>::THR, NB == 1 ? 2 : 1) attn_few8_kern
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
           const float m0 = m[nb][0] > -INFINITY ? m[nb][0] : 0.f, m1 = m[nb][1] > -INFINITY ? m[nb][1] : 0.f;
-          const float x0 = x[nb][kb][0], x1_ = x[nb][kb][1], x2 = x[nb][kb][2], x3 = x[nb][kb][3];
-          l[nb][0] += ex2_tc(x0 - m0) + ex2_tc(x2 - m0), l[nb][1] += ex2_tc(x1_ - m1) + ex2_tc(x3 - m1);
+          const float x0 = x[nb][kb][0] - m0, x1_ = x[nb][kb][1] - m1, x2 = x[nb][kb][2] - m0, x3 = x[nb][kb][3] - m1;
+          l[nb][0] += ex2_tc(x0) + ex2_tc(x2), l[nb][1] += ex2_tc(x1_) + ex2_tc(x3);
           // for the product 2^7 times themselves and their values' scales, beside the row's reference of those
-          const float r0 = P_EXP - (ref[nb][0] > -INFINITY ? ref[nb][0] : 0.f), r1 = P_EXP - (ref[nb][1] > -INFINITY ? ref[nb][1] : 0.f), v0 = ve[2 * kb], v1 = ve[2 * kb + 1];
+          const float r0 = P_EXP - (rel[nb][0] > -INFINITY ? rel[nb][0] : 0.f), r1 = P_EXP - (rel[nb][1] > -INFINITY ? rel[nb][1] : 0.f), v0 = ve[2 * kb], v1 = ve[2 * kb + 1];
           pt[nb][0] = transpose_8x8(pack_h(ex2_tc(x0 + (v0 + r0)), ex2_tc(x1_ + (v0 + r1))));
           pt[nb][1] = transpose_8x8(pack_h(ex2_tc(x2 + (v1 + r0)), ex2_tc(x3 + (v1 + r1))));
         }
@@ -365,7 +371,7 @@ __global__ void __launch_bounds__(Ring<HD>::THR, NB == 1 ? 2 : 1) attn_few8_kern
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) l[nb][e] += __shfl_xor_sync(0xffffffffu, l[nb][e], d);
         const int r = nb * 8 + 2 * t + e;
-        if (g == 0) s_m[warp][r] = m[nb][e], s_l[warp][r] = l[nb][e], s_ref[warp][r] = ref[nb][e];
+        if (g == 0) s_m[warp][r] = m[nb][e], s_l[warp][r] = l[nb][e], s_rel[warp][r] = rel[nb][e];
         float* dst = s_o + warp * (Ring<HD>::WARP / 4) + r * HD + g * (HD / 8);
 #pragma unroll
         for (int b = 0; b < MB; ++b) *reinterpret_cast<float2*>(dst + 2 * b) = make_float2(o[nb][b][e], o[nb][b][e + 2]);
@@ -376,16 +382,19 @@ __global__ void __launch_bounds__(Ring<HD>::THR, NB == 1 ? 2 : 1) attn_few8_kern
       const int n = i / (HD / 4), c = i - n * (HD / 4);  // a row, four columns
       float top = -INFINITY, sum = 0.f, r = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < WARPS_F; ++w) top = fmaxf(top, s_m[w][n]), r = fmaxf(r, s_ref[w][n]);
+      for (int w = 0; w < WARPS_F; ++w) top = fmaxf(top, s_m[w][n]);
+      auto beside = [&](int w) { return s_m[w][n] > -INFINITY ? s_rel[w][n] + (s_m[w][n] - top) : -INFINITY; };  // the warp's reference of products, beside the row's maximum
+#pragma unroll
+      for (int w = 0; w < WARPS_F; ++w) r = fmaxf(r, beside(w));
       float4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < WARPS_F; ++w) {
         sum += s_l[w][n] * weight(s_m[w][n], s_l[w][n], top);
-        const float fo = s_ref[w][n] > -INFINITY ? ex2_tc(s_ref[w][n] - r) : 0.f;
+        const float at = beside(w), fo = at > -INFINITY ? ex2_tc(at - r) : 0.f;
         const float4 x = *reinterpret_cast<const float4*>(s_o + w * (Ring<HD>::WARP / 4) + n * HD + c * 4);
         if (fo != 0.f) acc.x += x.x * fo, acc.y += x.y * fo, acc.z += x.z * fo, acc.w += x.w * fo;
       }
-      const float back = result_scale(r, top);
+      const float back = result_scale(r);
       if (whole) {
         const float f = *dead ? __int_as_float(0x7fc00000) : sum > 0.f ? back * ((1 << LAG_EXP) / sum) : sum;
         const int tok = n / G;

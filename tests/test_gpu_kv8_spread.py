@@ -150,6 +150,29 @@ def test_keys_beside_a_far_larger_one(L, kind, hd, d, few, case):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("d", [12, 18, 20, 24, 40, 60])
+@pytest.mark.parametrize("few,case", [(True, c) for c in FEW])
+def test_scores_beyond_their_differences(L, kind, hd, d, few, case):
+    """two keys alike, far above the others, with scores of 2^d and more, and values 2^3 apart: their mean, however few bits a score has behind its point"""
+    lens, nq, nkv = case
+    r = requests(L, lens, nq, nkv, hd, kind, seed=d + 4)
+    r.q.view(-1, nq, hd)[..., 0] = 4.0
+    codes = torch.zeros(hd, device="cuda")
+    codes[0] = 112.0
+    at = (5, lens[0][0] - 2)
+    for a in at:
+        pg, slot = int(r.kv_at[0][0][a]), int(r.kv_at[0][1][a])
+        r.codes[pg, r.layer, 0, :, slot] = codes.to(DTYPES[kind]).view(torch.uint8)
+        scaled(r, 0, a, 0, torch.full((nkv,), 127 + d))
+    raised(r, 0, at[1], 1, 3)
+    out = r.attend(L)[:lens[0][1]].view(-1, nq, hd).double()
+    v = [r.v[0][a].repeat_interleave(nq // nkv, 0) for a in at]
+    want, size = (v[0] + v[1]) / 2, (v[0].abs() + v[1].abs()) / 2
+    assert ((out - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -11 + 2.0 ** -9) * size).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("hd,ps", [(64, 16), (128, 24), (128, 16)])
 @pytest.mark.parametrize("few,case", [(True, c) for c in FEW])
 @pytest.mark.parametrize("window", [0, 90])
