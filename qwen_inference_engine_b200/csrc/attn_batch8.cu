@@ -35,6 +35,7 @@ namespace {
 // The weights' reference follows a row's maximum where it has fallen behind by more than 2^8: weights by 2^7 are at most 2^15 then, below the largest fp16.
 constexpr int LAG_EXP = 8, P_EXP = 7;
 constexpr float LAG = LAG_EXP;
+constexpr float NOTHING = -3.4e38f;  // the reference of a row that has seen nothing: below every score, and a number
 // from sums beside the reference of products, 2^rel times the one of weights (2^P_EXP times themselves), to sums beside that one, but for 2^LAG_EXP: weights' sums are at most so much more than
 // they would be beside their maximum, and the factor must not leave the range ahead of them.  A row that has seen no value but zeros: 0
 __device__ __forceinline__ float result_scale(float rel) { return rel > -INFINITY ? ex2_tc(rel - (float)(P_EXP + LAG_EXP)) : 0.f; }
@@ -212,7 +213,7 @@ __global__ void __launch_bounds__(Ring<HD>::THR, NB == 1 ? 2 : 1) attn_few8_kern
     // a row's references: m of its weights (l), and rel beside m of its weights times their values' scales (o); both are the row's own, of keys that it sees
     float o[NB][MB][4] = {}, m[NB][2], l[NB][2], rel[NB][2];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) m[nb][0] = m[nb][1] = rel[nb][0] = rel[nb][1] = -INFINITY, l[nb][0] = l[nb][1] = 0.f;
+    for (int nb = 0; nb < NB; ++nb) m[nb][0] = m[nb][1] = rel[nb][0] = rel[nb][1] = NOTHING, l[nb][0] = l[nb][1] = 0.f;
 #pragma unroll
     for (int s = 0; s < ST - 1; ++s)
       if (s < n) s_scale[warp][(J + s) % ST][lane] = sk[s], s_scale[warp][(J + s) % ST][32 + lane] = sv[s];
@@ -282,7 +283,6 @@ __global__ void __launch_bounds__(Ring<HD>::THR, NB == 1 ? 2 : 1) attn_few8_kern
       float ve[4];  // the values' scales, as exponents (of zeros: minus infinity)
 #pragma unroll
       for (int i = 0; i < 4; ++i) ve[i] = vb_[i] == 0 ? -INFINITY : (float)((int)vb_[i] - 127);
-      bool grow = false;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float ks = kv8_scale(vb_[i] == 255 || (bad >> (g + 8 * i) & 1) ? 255u : kb_[i]);
@@ -296,9 +296,26 @@ __global__ void __launch_bounds__(Ring<HD>::THR, NB == 1 ? 2 : 1) attn_few8_kern
               const int key = key0 + g + 8 * i, pos_ = pos[nb][e];
               if (key > pos_ || (a.window > 0 && key <= pos_ - a.window)) y = -INFINITY;
             }
-            grow |= y > m[nb][e] + LAG || (y - m[nb][e]) + ve[i] > rel[nb][e] + LAG;
           }
       }
+      // exponents of weights beside their reference, and for the product 2^7 times themselves and their values' scales, beside the reference of those
+      float p[NB][2][4];
+      bool grow = false;
+      auto exponents = [&](int nb, int i, int e) {
+        const int at = (i & 1) * 2 + e;
+        const float d = x[nb][i >> 1][at] - m[nb][e];
+        p[nb][i >> 1][at] = d + (ve[i] + (P_EXP - rel[nb][e]));
+        return d;
+      };
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float d = exponents(nb, i, e);
+            grow |= d > LAG || p[nb][i >> 1][(i & 1) * 2 + e] > LAG + P_EXP;
+          }
       if (__any_sync(0xffffffffu, grow)) {
         // the rows' new references, and what there is so far beside them
 #pragma unroll
@@ -308,19 +325,17 @@ __global__ void __launch_bounds__(Ring<HD>::THR, NB == 1 ? 2 : 1) attn_few8_kern
             float mx = fmaxf(fmaxf(x[nb][0][e], x[nb][0][e + 2]), fmaxf(x[nb][1][e], x[nb][1][e + 2]));
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-            const float to = fmaxf(m[nb][e], mx), t0 = to > -INFINITY ? to : 0.f;
-            float rx = fmaxf(fmaxf((x[nb][0][e] - t0) + ve[0], (x[nb][0][e + 2] - t0) + ve[1]), fmaxf((x[nb][1][e] - t0) + ve[2], (x[nb][1][e + 2] - t0) + ve[3]));
+            const float to = fmaxf(m[nb][e], mx);
+            float rx = fmaxf(fmaxf((x[nb][0][e] - to) + ve[0], (x[nb][0][e + 2] - to) + ve[1]), fmaxf((x[nb][1][e] - to) + ve[2], (x[nb][1][e + 2] - to) + ve[3]));
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) rx = fmaxf(rx, __shfl_xor_sync(0xffffffffu, rx, d));
-            float f = 1.f;
-            if (m[nb][e] > -INFINITY) {
-              const float before = rel[nb][e] + (m[nb][e] - to);
-              rx = fmaxf(rx, before), l[nb][e] *= ex2_tc(m[nb][e] - to);
-              if (before > -INFINITY) f = ex2_tc(before - rx);
-            }
-            m[nb][e] = to, rel[nb][e] = rx;
+            const float before = rel[nb][e] + (m[nb][e] - to), f = ex2_tc(before - fmaxf(before, rx));  // (nothing before: 0, of zeros)
+            l[nb][e] *= ex2_tc(m[nb][e] - to);
+            m[nb][e] = to, rel[nb][e] = fmaxf(before, rx);
 #pragma unroll
             for (int b = 0; b < MB; ++b) o[nb][b][e] *= f, o[nb][b][e + 2] *= f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) exponents(nb, i, e);
           }
       }
 #pragma unroll
@@ -335,13 +350,9 @@ __global__ void __launch_bounds__(Ring<HD>::THR, NB == 1 ? 2 : 1) attn_few8_kern
         uint32_t pt[NB][2];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-          const float m0 = m[nb][0] > -INFINITY ? m[nb][0] : 0.f, m1 = m[nb][1] > -INFINITY ? m[nb][1] : 0.f;
-          const float x0 = x[nb][kb][0] - m0, x1_ = x[nb][kb][1] - m1, x2 = x[nb][kb][2] - m0, x3 = x[nb][kb][3] - m1;
-          l[nb][0] += ex2_tc(x0) + ex2_tc(x2), l[nb][1] += ex2_tc(x1_) + ex2_tc(x3);
-          // for the product 2^7 times themselves and their values' scales, beside the row's reference of those
-          const float r0 = P_EXP - (rel[nb][0] > -INFINITY ? rel[nb][0] : 0.f), r1 = P_EXP - (rel[nb][1] > -INFINITY ? rel[nb][1] : 0.f), v0 = ve[2 * kb], v1 = ve[2 * kb + 1];
-          pt[nb][0] = transpose_8x8(pack_h(ex2_tc(x0 + (v0 + r0)), ex2_tc(x1_ + (v0 + r1))));
-          pt[nb][1] = transpose_8x8(pack_h(ex2_tc(x2 + (v1 + r0)), ex2_tc(x3 + (v1 + r1))));
+          l[nb][0] += ex2_tc(x[nb][kb][0] - m[nb][0]) + ex2_tc(x[nb][kb][2] - m[nb][0]), l[nb][1] += ex2_tc(x[nb][kb][1] - m[nb][1]) + ex2_tc(x[nb][kb][3] - m[nb][1]);
+          pt[nb][0] = transpose_8x8(pack_h(ex2_tc(p[nb][kb][0]), ex2_tc(p[nb][kb][1])));
+          pt[nb][1] = transpose_8x8(pack_h(ex2_tc(p[nb][kb][2]), ex2_tc(p[nb][kb][3])));
         }
 #pragma unroll
         for (int w = 0; w < VW; ++w) {
@@ -371,7 +382,7 @@ __global__ void __launch_bounds__(Ring<HD>::THR, NB == 1 ? 2 : 1) attn_few8_kern
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) l[nb][e] += __shfl_xor_sync(0xffffffffu, l[nb][e], d);
         const int r = nb * 8 + 2 * t + e;
-        if (g == 0) s_m[warp][r] = m[nb][e], s_l[warp][r] = l[nb][e], s_rel[warp][r] = rel[nb][e];
+        if (g == 0) s_m[warp][r] = m[nb][e] > NOTHING ? m[nb][e] : -INFINITY, s_l[warp][r] = l[nb][e], s_rel[warp][r] = rel[nb][e];
         float* dst = s_o + warp * (Ring<HD>::WARP / 4) + r * HD + g * (HD / 8);
 #pragma unroll
         for (int b = 0; b < MB; ++b) *reinterpret_cast<float2*>(dst + 2 * b) = make_float2(o[nb][b][e], o[nb][b][e + 2]);
