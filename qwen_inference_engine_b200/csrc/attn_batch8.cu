@@ -3,9 +3,10 @@
 //
 //   out_t = sum_j 2^(x_tj - m) 2^ev_j v_j / sum_j 2^(x_tj - m),  x_tj = s 2^ek_j (q_t . k_j) over the positions j that row t sees, m their running maximum, k_j and v_j codes
 //
-// Codes become fp16 exactly (larger blocks: beside their tile's largest scale).  A row's query is brought to fp16 by a power of two of its own, which loses nothing, and scores are summed in
-// fp32.  Weights are fp16 in the product with the values, 2^-11 of themselves; they are there by 2^7 and their value's scale, in blocks of few rows beside the largest such product that the row
-// itself has seen, so that none is off by more than 2^-31 of that, whatever lies beside it; their sums are fp32.
+// Codes become fp16 exactly, in larger blocks with a power of two beside them that a tile's keys, or values, have in common.  A row's query is brought to fp16 by a power of two of its own, which
+// loses nothing, and scores are summed in fp32.  A row goes by what it sees and by nothing beside it: m is its own running maximum, and its weights, which are fp16 in the product with the values
+// (2^-11 of themselves), stand there times their values' scales beside the largest such product that the row itself has met (a reference of their own), so that none is off by more than 2^-31 of that,
+// in larger blocks 2^-23, where a tile has one scale for values that are at most 2^8 apart.  Weights' sums are fp32.
 //
 // An item is a kv head of a request and a block of its tokens, its rows (token, query head of the group); items are shared out over the CTAs as in attn_batch.cu.  There are two kernels: for blocks
 // of at most 16 rows (decode), which memory bounds, one that keeps a unit of keys and values in registers between loads and products, and for larger blocks one on tcgen05 / TMEM.
@@ -451,18 +452,29 @@ cudaError_t launch_few(const BatchAttnArgs& a, const Kv8Geom& kv, const JoinShap
 //                    feeds keys and values alone; with heads of 128 there is no room for both in TMEM, and they lie in shared memory), the rows of the result
 //   warps 8-15     : codes to fp16 (keys, values): of a tile the powers of two beside its largest, which is a factor of all scores (keys) and of all weights (values), by the multiplication
 //   warps 16, 17   : the products of a row tile
-//   warp 18        : codes and scales by TMA, or, for pages of other than multiples of 16 positions, by 16-byte copies to the same places; warp 19 has nothing to do
+//   warp 18        : codes and scales by TMA, or, for pages of other than multiples of 16 positions, by 16-byte copies to the same places
+//   warp 19        : of a tile the largest scales, which keys go by them, and every key's and value's factor
 // Registers: 96 a thread at launch; 144, 64 and 64 behind the split, as many in all.
 constexpr int ROWS_P = 256, THR_P = 20 * 32, TK = AB_TK;
 constexpr int KBLK = TK * 128;  // [keys][64 columns] fp16 in 8-row swizzle atoms
-constexpr int SLOTS = 8;        // tiles' scales: the softmax is at most ST + 3 tiles behind
+constexpr int PLANS = 4, SLOTS = 16;  // tiles' factors; tiles' scales: warp 19 is at most PLANS tiles ahead of the conversion, and the softmax ST + 3 behind that
+// A tile is brought to fp16 beside its largest scales, so keys far below those would lose bits and values would lie far from what the rows that see them go by.  Where keys' scales are more than
+// KEYS_APART powers of two apart (a code's smallest step is fp16's smallest number then) or values' more than VALUES_APART, the tile is gone through again for those: scores, softmax and product
+// of some of its keys at a time (TILE_PART), until all have been there (TILE_AGAIN: not yet).
+// A word of a tile: its values' largest scale in the lowest byte, its keys' where a float has its exponent, and these.  TILE_CLEAR: some values are not for the product.
+constexpr int TILE_AGAIN = 1 << 8, TILE_PART = 1 << 9, TILE_CLEAR = 1 << 10;
+template <int CODE>
+constexpr uint32_t KEYS_APART = CODE == KV8_E4M3 ? 15 : 24;
+constexpr uint32_t VALUES_APART = 8;
+constexpr uint32_t NONE_H2 = 0x7e007e00u, CLEAR_H2 = 0xffffffffu;  // factors: no numbers; (of values) zeros, whatever the codes
+__device__ __forceinline__ bool far_below(uint32_t byte, uint32_t top, uint32_t apart) { return byte != 0 && byte + apart < top; }  // (zeros: at any scale; no numbers: above all)
 template <int HD>
 struct SmemP {
   static constexpr bool Q_TMEM = HD == 64;
   static constexpr int NB = HD / 64, RAW = HD == 64 ? 4 : 3, ST = 3;  // column blocks; stages of codes, and of keys and values
   static constexpr int CODES = TK * HD, TILE = NB * KBLK, QBLK = 128 * 128, QTILE = NB * QBLK;
   static constexpr int C = 0, K = RAW * 2 * CODES, V = K + ST * TILE, Q = V + ST * TILE, SC = Q + (Q_TMEM ? 0 : 2 * QTILE), BAR = SC + RAW * 2 * TK, TOTAL = BAR + 512 + 1024;
-  static_assert(TOTAL <= 226 * 1024 && ST + 4 <= SLOTS, "");
+  static_assert(TOTAL <= 226 * 1024 && ST + PLANS + 3 <= SLOTS, "");
 };
 // D = F32, A = B = F16
 __device__ __forceinline__ uint32_t idesc_h(int m, int n, bool b_mn) { return idesc_tc(m, n, b_mn) & ~((1u << 7) | (1u << 10)); }
@@ -485,20 +497,23 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
   __shared__ long long s_sums[THR_P / 32];
   __shared__ Walk s_walk, s_walks[THR_P / 32];
   __shared__ int dead_s;
-  __shared__ int s_kt[SLOTS], s_vt[SLOTS];  // the largest scales of a tile's keys and values, as bytes
-  __shared__ unsigned long long s_bad[2];   // (edge tiles, by parity) keys whose values are no numbers
+  __shared__ int s_tile[2][SLOTS];               // of a row tile's tiles the words
+  __shared__ unsigned long long s_in[2][SLOTS];  // TILE_PART: which keys
+  __shared__ int s_plan[PLANS];                  // the words of the tiles that are to be brought to fp16, and of those each key's and value's factor, twice as fp16
+  __shared__ uint32_t s_factor[PLANS][2][TK];
   volatile int* dead = &dead_s;
   if (TMA && threadIdx.x == 18 * 32) asm volatile("prefetch.tensormap [%0];" ::"l"(&cm) : "memory");
   const uint32_t s0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* smem = smem_raw + (s0 - smem_u32(smem_raw));
-  // barriers: of a row tile queries, and by its tile's parity scores, weights and product; of the stages of codes, keys and values full and free
+  // barriers: of a row tile queries, and by its tile's parity scores, weights and product; of the stages of codes, keys and values full and free; of the tiles' factors full and free
   const uint32_t bar_q = s0 + SM::BAR, bar_s = bar_q + 16, bar_p = bar_s + 32, bar_o = bar_p + 32, slot = bar_o + 32, raw_full = slot + 16, raw_free = raw_full + 8 * RAW, k_full = raw_free + 8 * RAW,
-                 k_free = k_full + 8 * ST, v_full = k_free + 8 * ST, v_free = v_full + 8 * ST;
+                 k_free = k_full + 8 * ST, v_full = k_free + 8 * ST, v_free = v_full + 8 * ST, plan_full = v_free + 8 * ST, plan_free = plan_full + 8 * PLANS;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
-    dead_s = 0, s_walk.left = 0, s_bad[0] = s_bad[1] = 0;
+    dead_s = 0, s_walk.left = 0;
     for (int i = 0; i < 2; ++i) mbar_init_tc(bar_q + 8 * i, 128);
     for (int i = 0; i < 4; ++i) mbar_init_tc(bar_s + 8 * i, 1), mbar_init_tc(bar_p + 8 * i, 128), mbar_init_tc(bar_o + 8 * i, 1);
+    for (int i = 0; i < PLANS; ++i) mbar_init_tc(plan_full + 8 * i, 1), mbar_init_tc(plan_free + 8 * i, 8);
     for (int i = 0; i < RAW; ++i) mbar_init_tc(raw_full + 8 * i, TMA ? 1 : 64), mbar_init_tc(raw_free + 8 * i, 8);
     for (int i = 0; i < ST; ++i) mbar_init_tc(k_full + 8 * i, 4), mbar_init_tc(k_free + 8 * i, 2), mbar_init_tc(v_full + 8 * i, 4), mbar_init_tc(v_free + 8 * i, 2);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -532,6 +547,8 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
     __syncwarp();
     return some;
   };
+  // the warp's tile again?  (Behind a wait that ran out words may be any; the warp goes on together.)
+  auto once_more = [&](int word) { return __any_sync(0xffffffffu, word & TILE_AGAIN) && !__any_sync(0xffffffffu, *dead); };
   Piece p;
   int T = 0;  // tiles so far
 
@@ -609,16 +626,98 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
         }
       }
       if (!TMA && warp == 18) put_scales();
+      // ---- the tiles' largest scales and factors, of the lane's keys, lane and 32 + lane
+      int T1 = 0, tiles = 0;  // tiles of the second row tile; tiles as they are copied
+      while (warp == 19 && next_piece(p)) {
+        const int low0 = a.window > 0 ? max(0, p.pos0 - a.window + 1) : 0, low1 = a.window > 0 ? max(0, p.pos0 + p.tokens - a.window) : 0, end = p.pos0 + p.tokens;
+        const bool both = p.tokens * G > 128;  // (row tiles with rows)
+        int R = p.begin;
+#pragma unroll 1
+        for (; R < p.end; ++R) {
+          const int at = tiles + R - p.begin, rs = at % RAW, key = p.key0 + R * TK;
+          const bool edge = key + TK > p.pos0 + 1 || key < low1;  // some row does not see some key of the tile
+          mbar_wait_short_tc(raw_full + 8u * (uint32_t)rs, (uint32_t)((at / RAW) & 1), dead);
+          __syncwarp();
+          const unsigned char *vc = smem + SM::C + (rs * 2 + 1) * SM::CODES, *sc = smem + SM::SC + rs * 2 * TK;
+          unsigned long long bad = 0;  // keys whose values are no numbers, where these must not meet a zero weight: zero values and scores that are no numbers
+          if (edge && CODE == KV8_E4M3) {
+#pragma unroll 4
+            for (int e = 0; e < TK * HD / 512; ++e) {
+              const uint4 c = *reinterpret_cast<const uint4*>(vc + (e * 32 + lane) * 16);
+              if (kv8_nans(c.x) | kv8_nans(c.y) | kv8_nans(c.z) | kv8_nans(c.w)) bad |= 1ull << ((e * 32 + lane) * 16 / HD);
+            }
+            bad = __reduce_or_sync(0xffffffffu, (uint32_t)bad) | (unsigned long long)__reduce_or_sync(0xffffffffu, (uint32_t)(bad >> 32)) << 32;
+          }
+          uint32_t kb[2], vb[2];
+          bool in[2];  // whether it is still to come
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int row = h * 32 + lane;
+            kb[h] = sc[row], vb[h] = sc[TK + row], in[h] = !edge || (key + row >= low0 && key + row < end);
+          }
+          int word;
+#pragma unroll 1
+          do {
+            uint32_t kt = 0, vt = 1;
+            bool now[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              now[h] = in[h];
+              if (in[h] && kb[h] != 255) kt = max(kt, kb[h]);
+              if (in[h] && vb[h] != 255) vt = max(vt, vb[h]);
+            }
+            kt = __reduce_max_sync(0xffffffffu, kt), vt = __reduce_max_sync(0xffffffffu, vt);
+            auto far = [&](int h) { return in[h] && (far_below(kb[h], kt, KEYS_APART<CODE>) || far_below(vb[h], vt, VALUES_APART)); };
+            word = 0;
+            if (__any_sync(0xffffffffu, far(0) || far(1))) {  // of the keys near the largest those whose values are near the largest of theirs; the others another time
+              vt = 1;
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                now[h] = in[h] && !far_below(kb[h], kt, KEYS_APART<CODE>);
+                if (now[h] && vb[h] != 255) vt = max(vt, vb[h]);
+              }
+              vt = __reduce_max_sync(0xffffffffu, vt);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) now[h] = now[h] && !far_below(vb[h], vt, VALUES_APART);
+              word = TILE_AGAIN;
+            }
+            const unsigned long long mask = __ballot_sync(0xffffffffu, now[0]) | (unsigned long long)__ballot_sync(0xffffffffu, now[1]) << 32;
+            const bool none[2] = {vb[0] == 255 || (bad >> lane & 1), vb[1] == 255 || (bad >> 32 >> lane & 1)};
+            if (edge || ~mask || __any_sync(0xffffffffu, none[0] || none[1])) word |= TILE_CLEAR;
+            if (~mask) word |= TILE_PART;
+            word |= (int)(kt << 23 | vt);
+            const int pl = T % PLANS;
+            if (T >= PLANS) mbar_wait_short_tc(plan_free + 8u * (uint32_t)pl, (uint32_t)((T / PLANS - 1) & 1), dead);
+            __syncwarp();
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              s_factor[pl][0][h * 32 + lane] = none[h] || kb[h] == 255 ? NONE_H2 : kb[h] == 0 ? 0u : pow2_h2((int)(kt - kb[h]));
+              s_factor[pl][1][h * 32 + lane] = none[h] || !now[h] ? CLEAR_H2 : vb[h] == 0 ? 0u : pow2_h2((int)(vt - vb[h]));
+              in[h] = in[h] && !now[h];
+            }
+            if (lane == 0) {  // (ahead of the keys: the softmax asks for no more than scores)
+              s_plan[pl] = s_tile[0][T % SLOTS] = word, s_in[0][T % SLOTS] = mask;
+              if (both) s_tile[1][T1 % SLOTS] = word, s_in[1][T1 % SLOTS] = mask;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive_tc(plan_full + 8u * (uint32_t)pl);
+            ++T, T1 += both;
+          } while (once_more(word));
+        }
+        tiles += p.count();
+      }
     } else {
       // ---- the products of row tile g
       const int g = warp - 16;
       const uint32_t id_s = idesc_h(128, TK, false), id_o = idesc_h(128, HD, true);
       const uint64_t dk = desc_k_tc(s0 + SM::K), dv = desc_mn_tc(s0 + SM::V, KBLK), dq = desc_k_tc(s0 + SM::Q + g * SM::QTILE);  // (steps are sums: in units of 16 bytes)
       int items = 0, tg = 0;  // items and tiles of this row tile
-      auto issue_s = [&](int ahead) {
+      int left = 0, ahead = 0;  // tiles of the piece of which scores are to be asked for; scores that are ahead of their product
+      auto issue_s = [&]() {
         const int at = T + ahead, b = (tg + ahead) & 1;
         mbar_wait_short_tc(k_full + 8u * (uint32_t)(at % ST), (uint32_t)((at / ST) & 1), dead);
         __syncwarp();
+        const int word = *(volatile int*)&s_tile[g][(tg + ahead) % SLOTS];  // (there when it is asked for, behind the instructions)
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (elect_tc()) {
           const uint64_t k = dk + (uint64_t)((at % ST) * (SM::TILE >> 4));
@@ -632,13 +731,17 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
           umma_commit_tc(k_free + 8u * (uint32_t)(at % ST));
         }
         __syncwarp();
+        if (!once_more(word)) --left;
+        ++ahead;
       };
       while (next_piece(p)) {
-        const int n = p.count();
+        left = p.count();
         if (g * 128 >= p.tokens * G) {  // nothing to do but to let the stages go
-          for (int i = 0; i < n; ++i, ++T) {
+          for (; left > 0; ++T) {
             const uint32_t st = (uint32_t)(T % ST), ph = (uint32_t)((T / ST) & 1);
             mbar_wait_short_tc(k_full + 8u * st, ph, dead);
+            __syncwarp();
+            if (!once_more(*(volatile int*)&s_tile[0][T % SLOTS])) --left;
             if (lane == 0) mbar_arrive_tc(k_free + 8u * st);
             mbar_wait_short_tc(v_full + 8u * st, ph, dead);
             if (lane == 0) mbar_arrive_tc(v_free + 8u * st);
@@ -648,9 +751,9 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
         }
         mbar_wait_short_tc(bar_q + 8u * g, (uint32_t)(items & 1), dead);
         ++items;
-        issue_s(0);
-        if (n > 1) issue_s(1);
-        for (int i = 0; i < n; ++i, ++T, ++tg) {
+        issue_s();
+        if (left > 0) issue_s();
+        for (bool first = true; ahead > 0; first = false, --ahead, ++T, ++tg) {
           const uint32_t st = (uint32_t)(T % ST), ph = (uint32_t)((tg >> 1) & 1);
           const int b = tg & 1;
           mbar_wait_short_tc(v_full + 8u * st, (uint32_t)((T / ST) & 1), dead);
@@ -660,14 +763,14 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
           if (elect_tc()) {
             const uint64_t v = dv + (uint64_t)(st * (SM::TILE >> 4));
 #pragma unroll
-            for (int kk = 0; kk < TK / 16; ++kk) umma_ts_tc(t_o(g), t_s(g, b) + (uint32_t)(kk * 8), v + (uint64_t)(kk * 128), id_o, i > 0 || kk > 0);
+            for (int kk = 0; kk < TK / 16; ++kk) umma_ts_tc(t_o(g), t_s(g, b) + (uint32_t)(kk * 8), v + (uint64_t)(kk * 128), id_o, !first || kk > 0);
             umma_commit_tc(bar_o + 16u * g + 8u * b);
             umma_commit_tc(v_free + 8u * st);
           }
           __syncwarp();
-          if (i + 2 < n) {
+          if (left > 0) {
             mbar_wait_short_tc(bar_o + 16u * g + 8u * b, ph, dead);  // the scores two tiles ahead go over the weights that this product reads
-            issue_s(2);
+            issue_s();
           }
         }
       }
@@ -681,75 +784,39 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
     auto row_of = [&](int e) { return (HD == 128 ? e * 2 + (w & 1) : e * 4 + w) * 8 + r8; };
     const int piece = HD == 128 ? (w >> 1) * 4 + cq : cq, nb = piece / 4, c16 = (2 * piece) & 7;
     const uint32_t full = is_v ? v_full : k_full, free_ = is_v ? v_free : k_free;
-    int edges = 0;
+    int R = 0;  // tiles as they are copied
     while (next_piece(p)) {
-      const int low0 = a.window > 0 ? max(0, p.pos0 - a.window + 1) : 0, low1 = a.window > 0 ? max(0, p.pos0 + p.tokens - a.window) : 0, end = p.pos0 + p.tokens;
 #pragma unroll 1
-      for (int i = p.begin; i < p.end; ++i, ++T) {
-        const int rs = T % RAW, st = T % ST, key = p.key0 + i * TK;
-        const bool edge = key + TK > p.pos0 + 1 || key < low1;  // some row does not see some key of the tile
-        mbar_wait_short_tc(raw_full + 8u * (uint32_t)rs, (uint32_t)((T / RAW) & 1), dead);
-        const unsigned char *codes = smem + SM::C + (rs * 2 + is_v) * SM::CODES, *sc = smem + SM::SC + rs * 2 * TK;
-        auto seen = [&](int row) { return key + row >= low0 && key + row < end; };  // by some row
+      for (int left = p.count(); left > 0; ++T) {
+        const int rs = R % RAW, st = T % ST, pl = T % PLANS;
+        mbar_wait_short_tc(raw_full + 8u * (uint32_t)rs, (uint32_t)((R / RAW) & 1), dead);
+        const unsigned char* codes = smem + SM::C + (rs * 2 + is_v) * SM::CODES;
         uint4 code[UNITS];
 #pragma unroll
         for (int e = 0; e < UNITS; ++e) {
           const int row = row_of(e);
           code[e] = *reinterpret_cast<const uint4*>(codes + piece_at<HD>(row, piece));
         }
-        // the lane's two keys: scales, the largest of the tile, and the factors that bring codes beside that
-        uint32_t sb[2], vb[2], top = is_v, v_top = 1;
+        mbar_wait_short_tc(plan_full + 8u * (uint32_t)pl, (uint32_t)((T / PLANS) & 1), dead);
+        const int word = *(volatile int*)&s_plan[pl];
+        uint32_t factor[UNITS];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int row = h * 32 + lane;
-          sb[h] = sc[is_v * TK + row], vb[h] = sc[TK + row];
-          if ((!edge || seen(row)) && sb[h] != 255) top = max(top, sb[h]);
-          if ((!edge || seen(row)) && vb[h] != 255) v_top = max(v_top, vb[h]);
-        }
-        top = __reduce_max_sync(0xffffffffu, top), v_top = __reduce_max_sync(0xffffffffu, v_top);
-        unsigned long long bad = 0;  // keys whose values are no numbers, where these must not meet a zero weight: zero values and scores that are no numbers
-        if (edge && CODE == KV8_E4M3) {
-          unsigned long long mine = 0;
-          if (is_v)
-#pragma unroll
-            for (int e = 0; e < UNITS; ++e)
-              if (kv8_nans(code[e].x) | kv8_nans(code[e].y) | kv8_nans(code[e].z) | kv8_nans(code[e].w)) mine |= 1ull << row_of(e);
-          if (mine) atomicOr(&s_bad[edges & 1], mine);
-          asm volatile("bar.sync 1, 256;" ::: "memory");
-          bad = *(volatile unsigned long long*)&s_bad[edges & 1];
-          if (warp == 8 && lane == 0) s_bad[(edges & 1) ^ 1] = 0;  // (all are past the one before)
-          asm volatile("bar.sync 1, 256;" ::: "memory");
-          ++edges;
-        }
-        if (warp == 8 && lane == 0) s_kt[T % SLOTS] = (int)top, s_vt[T % SLOTS] = (int)v_top;  // (both ahead of the keys: the softmax asks for no more than scores)
-        uint32_t factor[2];
-        bool clear = false;  // some values are not for the product: those of keys that no row sees, and those that are no numbers
-#pragma unroll
-        for (int h = 0; h < 2; ++h) factor[h] = sb[h] == 0 ? 0u : pow2_h2((int)(top - sb[h]));
-        if (edge || __any_sync(0xffffffffu, sb[0] == 255 || sb[1] == 255 || vb[0] == 255 || vb[1] == 255)) {
-          clear = true;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int row = h * 32 + lane;
-            const bool none = vb[h] == 255 || (bad >> row & 1);
-            if (is_v ? none || !seen(row) : none || sb[h] == 255) factor[h] = is_v ? 0xffffffffu : 0x7e007e00u;
-          }
-        }
+        for (int e = 0; e < UNITS; ++e) factor[e] = *(volatile uint32_t*)&s_factor[pl][is_v][row_of(e)];
         if (T >= ST) mbar_wait_short_tc(free_ + 8u * (uint32_t)st, (uint32_t)((T / ST - 1) & 1), dead);
         __syncwarp();
         const uint32_t to = s0 + (is_v ? SM::V : SM::K) + st * SM::TILE + nb * KBLK;
 #pragma unroll
         for (int e = 0; e < UNITS; ++e) {
           const int row = row_of(e);
-          const uint32_t f = __shfl_sync(0xffffffffu, factor[HD == 128 ? e / 2 : e], row & 31);
+          const uint32_t f = factor[e];
           const uint4 c = code[e];
           uint32_t h[8];
           kv8_unpack<CODE>(c.x, h[0], h[1]), kv8_unpack<CODE>(c.y, h[2], h[3]), kv8_unpack<CODE>(c.z, h[4], h[5]), kv8_unpack<CODE>(c.w, h[6], h[7]);
 #pragma unroll
           for (int j = 0; j < 8; ++j) h[j] = mul_h2(h[j], f);
-          if (clear) {
+          if (word & TILE_CLEAR) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) h[j] = f == 0xffffffffu ? 0u : h[j];
+            for (int j = 0; j < 8; ++j) h[j] = f == CLEAR_H2 ? 0u : h[j];
           }
           const uint32_t line = to + row * 128;
           asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(line + ((c16 ^ r8) << 4)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
@@ -757,14 +824,19 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        if (lane == 0) mbar_arrive_tc(full + 8u * (uint32_t)st), mbar_arrive_tc(raw_free + 8u * (uint32_t)rs);
+        const bool again = once_more(word);
+        if (lane == 0) {
+          mbar_arrive_tc(full + 8u * (uint32_t)st), mbar_arrive_tc(plan_free + 8u * (uint32_t)pl);
+          if (!again) mbar_arrive_tc(raw_free + 8u * (uint32_t)rs);
+        }
+        if (!again) ++R, --left;
       }
     }
   } else {
     // ---- softmax: this thread's row
     asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
     const int g = warp >> 2, row = g * 128 + (tid & 127), tok = row / G, gh = row - tok * G;
-    const uint32_t la = (uint32_t)((warp & 3) * 32) << 16, mine_turn = 2u + 2u * (uint32_t)(warp & 3) + (uint32_t)g;  // the barrier of this warp's turns, beside that of the other row tile's
+    const uint32_t la = (uint32_t)((warp & 3) * 32) << 16;
     int tg = 0;  // tiles of this row tile
     if (tid == 0) info[blockIdx.x].parts = 0;
     bool more = next_piece(p);
@@ -773,7 +845,6 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
       if (tid == 0 && !p.whole() && p.begin == 0)  // goes on in the CTAs behind; the item's last tile is at x1 - left + tiles - 1
         info[blockIdx.x] = JoinInfo{p.t0, p.tokens, p.kvh, (int)quotient(x1 - p.left + p.tiles - 1, share) - (int)blockIdx.x + 1};
       if (g * 128 >= rows) {
-        T += p.count();
         more = next_piece(p);
         continue;
       }
@@ -820,14 +891,12 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
         mbar_arrive_tc(bar_q + 8u * g);
       }
       const int my_pos = p.pos0 + min(tok, p.tokens - 1), my_low = a.window > 0 ? max(0, my_pos - a.window + 1) : 0;
-      float m_ref = -INFINITY, l_run = 0.f;
-      int lr = 1;  // the scale of the values that O is beside, as a byte
-      // The two warps of an SM quarter take turns at its exponentials, a tile each: side by side they would both be slow at these, and then leave the unit idle together (8192 rows 596 and
-      // 591 us).
-      const bool turns = 128 < rows;  // (both row tiles have rows)
-      if (turns && g == 1) asm volatile("bar.arrive %0, 64;" ::"r"(mine_turn ^ 1u) : "memory");
+      // the references of the row's weights, and beside that one (rel) of its weights times the values' scales, of O; whole numbers, of what the row sees
+      float m_ref = -INFINITY, m_off = 0.f, rel = 0.f, l_run = 0.f;  // m_off: what is added to scores for it
+      bool again;         // the tile
+      bool huge = false;  // some row's reference is so large that scores round to fewer bits than their differences need
 #pragma unroll 1
-      for (int i = p.begin; i < p.end; ++i, ++T, ++tg) {
+      for (int i = p.begin, first = 1; i < p.end; i += !again, first = 0, ++tg) {
         const int b = tg & 1;
         const uint32_t ts = t_s(g, b) + la, ph = (uint32_t)((tg >> 1) & 1);
         const int key = p.key0 + i * TK, last = my_pos - key, low = my_low - key;  // the first key of the tile; the last and the first that the row sees
@@ -837,18 +906,16 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
         uint32_t r[TK];
         tmem_ld32_tc(ts, r);
         tmem_ld32_tc(ts + 32, r + 32);
-        const float s = fmaxf(sl2 * __uint_as_float((uint32_t)s_kt[T % SLOTS] << 23), 1e-37f);  // (zero must not meet minus infinity)
-        const int vt = s_vt[T % SLOTS];
+        const int tile = s_tile[g][tg % SLOTS];
+        const float s = fmaxf(sl2 * __uint_as_float(tile & 0x7f800000u), 1e-37f), vt = __uint_as_float(0x4b000000u | (tile & 255)) - 8388735.f;  // (zero must not meet minus infinity; 2^23 + 127)
         tmem_wait_ld_tc();
-        if (last < TK - 1) {
+        if (last < TK - 1 || low > 0 || tile & TILE_PART) {
+          unsigned long long in = last < 0 || low >= TK ? 0 : ~0ull >> max(TK - 1 - last, 0) & ~0ull << max(low, 0);
+          if (tile & TILE_PART) in &= s_in[g][tg % SLOTS];
+          const uint32_t in0 = (uint32_t)in, in1 = (uint32_t)(in >> 32);
 #pragma unroll
           for (int j = 0; j < TK; ++j)
-            if (j > last) r[j] = 0xff800000u;  // -inf
-        }
-        if (low > 0) {
-#pragma unroll
-          for (int j = 0; j < TK; ++j)
-            if (j < low) r[j] = 0xff800000u;
+            if (!((j < 32 ? in0 : in1) & 1u << (j & 31))) r[j] = 0xff800000u;  // -inf
         }
         float mx[4];
 #pragma unroll
@@ -859,19 +926,27 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
           for (int e = 0; e < 4; ++e) mx[e] = max3_tc(mx[e], __uint_as_float(r[j + e]), __uint_as_float(r[j + 4 + e]));
 #pragma unroll
         for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(r[60 + e]));
-        const float m_new = fmaxf(m_ref, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * s);
-        const bool grow = __any_sync(0xffffffffu, m_new > m_ref + LAG && mine) || vt > lr;
-        float f = 1.f;
+        const float top = __fmul_rn(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), s);
+        const bool grow = __any_sync(0xffffffffu, ((top > m_ref + LAG || (top - m_ref) + vt > rel + LAG) && mine) || huge || tile & TILE_AGAIN);  // (one vote for all that is rare)
+        float f = 1.f, sx = s;
+        again = false;
         if (grow) {
-          if (m_new > -INFINITY) f = ex2_tc(m_ref - m_new);  // (nothing before: 0)
-          m_ref = m_new;
-          l_run *= f;
-          if (vt > lr) f *= vt - lr < 127 ? __uint_as_float((uint32_t)(127 - (vt - lr)) << 23) : 0.f, lr = vt;
+          again = once_more(tile);
+          const float up = ceilf(top), m_new = fmaxf(m_ref, up);
+          if (m_new > -INFINITY) {
+            const float by = m_ref - m_new, before = rel + by, rel_new = fmaxf(before, (up - m_new) + vt);  // (nothing before: by minus infinity)
+            l_run *= ex2_tc(by), f = ex2_tc(before - rel_new), rel = rel_new, m_ref = m_new, m_off = -m_new;
+          }
+          huge = __any_sync(0xffffffffu, fabsf(m_off) >= 4194304.f);
+          if (huge) {  // the score rounded, as the maximum was, and then the difference
+#pragma unroll
+            for (int j = 0; j < TK; ++j) r[j] = __float_as_uint(__fadd_rn(__fmul_rn(__uint_as_float(r[j]), s), m_off));
+            sx = 1.f, m_off = 0.f;
+          }
         }
-        // weights by 2^7 and their values' scale beside the largest; 2^-64 of that is none in fp16, and one in the sum
-        const int d = max(vt - lr, -64) + P_EXP;
-        const unsigned long long s2 = twice_tc(s), n2 = twice_tc((m_ref > -INFINITY ? -m_ref : 0.f) + (float)d);
-        if (turns) asm volatile("bar.sync %0, 64;" ::"r"(mine_turn) : "memory");
+        // weights by 2^7 and their values' scale beside the reference of those; 2^-64 of that is none in fp16, and one in the sum
+        const float d = fmaxf(vt - rel, -64.f) + (float)P_EXP;
+        const unsigned long long s2 = twice_tc(sx), n2 = twice_tc(m_off + d);
         float rs[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < TK; c += 32) {
@@ -886,9 +961,8 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
           }
           tmem_st16_tc(ts + c / 2, wt);
         }
-        if (turns && (g == 0 || i + 1 < p.end)) asm volatile("bar.arrive %0, 64;" ::"r"(mine_turn ^ 1u) : "memory");
-        l_run += ((rs[0] + rs[1]) + (rs[2] + rs[3])) * __uint_as_float((uint32_t)(127 - d) << 23);
-        if (grow && i > p.begin) {  // O, behind the product of the tile before
+        l_run += ((rs[0] + rs[1]) + (rs[2] + rs[3])) * ex2_tc(-d);
+        if (grow && !first) {  // O, behind the product of the tile before
           mbar_wait_short_tc(bar_o + 16u * g + 8u * (b ^ 1), (uint32_t)(((tg - 1) >> 1) & 1), dead);
           __syncwarp();
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -916,8 +990,8 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
       mbar_wait_short_tc(bar_o + 16u * g + 8u * ((tg - 1) & 1), (uint32_t)(((tg - 1) >> 1) & 1), dead);
       __syncwarp();
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const float back = __uint_as_float((uint32_t)lr << 23) * (1.f / (1 << P_EXP)), nan = __int_as_float(0x7fc00000);
-      const float scale = *dead ? nan : !whole ? back : l_run > 0.f ? back / l_run : l_run;
+      const float back = m_ref > -INFINITY ? result_scale(rel) : 0.f, nan = __int_as_float(0x7fc00000);
+      const float scale = *dead ? nan : !whole ? back * (1 << LAG_EXP) : l_run > 0.f ? back * ((1 << LAG_EXP) / l_run) : l_run;
       if (!whole) part[ROWS_P * HD + row] = m_ref, part[ROWS_P * HD + ROWS_P + row] = *dead ? nan : l_run;
 #pragma unroll
       for (int c = 0; c < HD; c += 32) {

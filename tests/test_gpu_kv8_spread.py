@@ -1,8 +1,9 @@
 """Attention over a cache in 8 bits where scales lie far apart: a row's result hangs on the keys and values that it sees, each by its own scale, and on nothing beside them.
 
 Bound, of each column of a row's result.  Weights and their sums are fp32 of scores in fp32: 2^-9 of sum w |v| for scores below 2^6 (derived in test_gpu_kv8.py); a weight is rounded to fp16 in the
-product, 2^-11 of itself.  It is there by 2^7 and its value's scale s beside the row's largest w s, of which the reference is at most twice as much:
-below 2^-14 it is off by 2^-25, so by 2^-32 of the reference, times the code beside it, at most 448: of n keys n * 448 * 2^-31 of the largest w s.  The result is rounded to bf16, 2^-8 of itself."""
+product, 2^-11 of itself.  It is there by 2^7 and its value's scale s beside the row's largest w s, of which the reference is at most twice as much (blocks of few rows) or 2^9 times (larger
+blocks: a tile's largest weight and largest scale, which are one another's within 2^8, and a whole number): below 2^-14 it is off by 2^-25, so by 2^-32 of the reference, times the code beside it, at
+most 448: of n keys n * 448 * 2^-31 (2^-23) of the largest w s.  The result is rounded to bf16, 2^-8 of itself."""
 import numpy as np
 import pytest
 import torch
@@ -11,8 +12,9 @@ from kv8_util import DTYPES, Requests8, i32, values
 
 pytestmark = pytest.mark.gpu
 KINDS = ["e4m3", "int8"]
-# (cached, new) of requests, query heads, kv heads; room for more rows than requests, all of them in blocks of few rows
+# (cached, new) of requests, query heads, kv heads; room for more rows than requests: blocks of few rows, and larger ones
 FEW = [([(300, 3), (70, 8), (40, 1)], 2, 2), ([(200, 2), (9, 1)], 14, 2), ([(90, 1), (50, 1)], 16, 1)]
+MANY = [([(300, 100), (9, 1)], 4, 2), ([(100, 333)], 14, 2)]
 
 
 @pytest.fixture(scope="module")
@@ -82,7 +84,7 @@ def requests(L, lens, nq, nkv, hd, kind, room=4, ps=16, **k):
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("j", [0, 1])
 @pytest.mark.parametrize("d", [9, 15, 16, 20, 24, 25, 40])
-@pytest.mark.parametrize("few,case", [(True, c) for c in FEW[:2]])
+@pytest.mark.parametrize("few,case", [(True, c) for c in FEW[:2]] + [(False, c) for c in MANY])
 def test_tokens_that_a_row_does_not_see(L, kind, hd, j, d, few, case):
     """a later token's key or value 2^d times as large: the rows before it are those of the formula over what they see"""
     lens, nq, nkv = case
@@ -100,7 +102,7 @@ def test_tokens_that_a_row_does_not_see(L, kind, hd, j, d, few, case):
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("j", [0, 1])
 @pytest.mark.parametrize("d", [15, 25, 40])
-@pytest.mark.parametrize("few,lens,nq,nkv,window,at", [(True, [(200, 8), (9, 1)], 2, 2, 50, 152)])
+@pytest.mark.parametrize("few,lens,nq,nkv,window,at", [(True, [(200, 8), (9, 1)], 2, 2, 50, 152), (False, [(200, 200)], 4, 2, 70, 140), (False, [(0, 300)], 14, 2, 30, 100)])
 def test_tokens_behind_the_window(L, kind, j, d, few, lens, nq, nkv, window, at):
     r = requests(L, lens, nq, nkv, 64, kind, seed=d + 1)
     raised(r, 0, at, j, d)
@@ -111,7 +113,7 @@ def test_tokens_behind_the_window(L, kind, j, d, few, lens, nq, nkv, window, at)
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("d", [9, 15, 20, 24, 25, 33, 40])
-@pytest.mark.parametrize("few,case", [(True, c) for c in FEW])
+@pytest.mark.parametrize("few,case", [(True, c) for c in FEW] + [(False, c) for c in MANY])
 def test_values_of_weights_that_vanish(L, kind, hd, d, few, case):
     """a value 2^d times as large under a weight of 2^-80 or so: its part of the result is nothing, and takes nothing from the others"""
     lens, nq, nkv = case
@@ -132,7 +134,7 @@ def test_values_of_weights_that_vanish(L, kind, hd, d, few, case):
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("d", [9, 15, 16, 20, 24, 25, 40])
-@pytest.mark.parametrize("few,case", [(True, c) for c in FEW])
+@pytest.mark.parametrize("few,case", [(True, c) for c in FEW] + [(False, c) for c in MANY])
 def test_keys_beside_a_far_larger_one(L, kind, hd, d, few, case):
     """queries that lie on keys of small scales, beside one that all rows see, 2^d times as large, with a score far below theirs"""
     lens, nq, nkv = case
@@ -152,7 +154,7 @@ def test_keys_beside_a_far_larger_one(L, kind, hd, d, few, case):
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("d", [12, 18, 20, 24, 40, 60])
-@pytest.mark.parametrize("few,case", [(True, c) for c in FEW])
+@pytest.mark.parametrize("few,case", [(True, c) for c in FEW] + [(False, c) for c in MANY])
 def test_scores_beyond_their_differences(L, kind, hd, d, few, case):
     """two keys alike, far above the others, with scores of 2^d and more, and values 2^3 apart: their mean, however few bits a score has behind its point"""
     lens, nq, nkv = case
@@ -174,7 +176,7 @@ def test_scores_beyond_their_differences(L, kind, hd, d, few, case):
 
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("hd,ps", [(64, 16), (128, 24), (128, 16)])
-@pytest.mark.parametrize("few,case", [(True, c) for c in FEW])
+@pytest.mark.parametrize("few,case", [(True, c) for c in FEW] + [(False, c) for c in MANY] + [(False, ([(0, 700)], 7, 1))])
 @pytest.mark.parametrize("window", [0, 90])
 def test_scales_of_any_distance(L, kind, hd, ps, few, case, window):
     """each key's scale is any of 2^-60 .. 1 of the usual one's and each value's any of 2^-40 .. 2^40, zeros and vectors of no numbers that no row sees among them: every key counts once, by its own scale"""
@@ -196,7 +198,7 @@ def test_scales_of_any_distance(L, kind, hd, ps, few, case, window):
 
 
 @pytest.mark.parametrize("j", [0, 1])
-@pytest.mark.parametrize("few,lens,at", [(True, [(100, 5), (9, 1)], 102)])
+@pytest.mark.parametrize("few,lens,at", [(True, [(100, 5), (9, 1)], 102), (False, [(100, 60), (9, 1)], 130), (False, [(0, 200)], 3)])
 def test_no_numbers_beside_scales_far_apart(L, j, few, lens, at):
     """a vector of no numbers: the rows that see it are none, the others are as without it, though scales are of any distance"""
     r = requests(L, lens, 4, 2, 64, "e4m3", seed=11)
@@ -211,8 +213,8 @@ def test_no_numbers_beside_scales_far_apart(L, j, few, lens, at):
 
 
 def test_a_step_of_rows_that_end_apart(L):
-    """scales far apart at the cuts between CTAs"""
-    for lens, few in (([(5000, 1), (3000, 1)], True),):
+    """wide tiles at the cuts between CTAs: one long prompt and long decode rows, single and in the same call"""
+    for lens, few in (([(5000, 1), (3000, 1)], True), ([(2000, 600), (4000, 1)], False)):
         r = requests(L, lens, 8, 1, 128, "e4m3", seed=13, room=0)
         for i, (c, m) in enumerate(lens):
             for j, step in ((0, 5), (1, 7)):
