@@ -641,7 +641,7 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
           const unsigned char *vc = smem + SM::C + (rs * 2 + 1) * SM::CODES, *sc = smem + SM::SC + rs * 2 * TK;
           unsigned long long bad = 0;  // keys whose values are no numbers, where these must not meet a zero weight: zero values and scores that are no numbers
           if (edge && CODE == KV8_E4M3) {
-#pragma unroll 4
+#pragma unroll 1
             for (int e = 0; e < TK * HD / 512; ++e) {
               const uint4 c = *reinterpret_cast<const uint4*>(vc + (e * 32 + lane) * 16);
               if (kv8_nans(c.x) | kv8_nans(c.y) | kv8_nans(c.z) | kv8_nans(c.w)) bad |= 1ull << ((e * 32 + lane) * 16 / HD);
@@ -751,8 +751,8 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
         }
         mbar_wait_short_tc(bar_q + 8u * g, (uint32_t)(items & 1), dead);
         ++items;
-        issue_s();
-        if (left > 0) issue_s();
+#pragma unroll 1  // (every place that has these instructions costs the other roles some of theirs: written out twice 8192 rows took 581 us instead of 570)
+        for (int k = 0; k < 2 && left > 0; ++k) issue_s();
         for (bool first = true; ahead > 0; first = false, --ahead, ++T, ++tg) {
           const uint32_t st = (uint32_t)(T % ST), ph = (uint32_t)((tg >> 1) & 1);
           const int b = tg & 1;
@@ -938,9 +938,13 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
             l_run *= ex2_tc(by), f = ex2_tc(before - rel_new), rel = rel_new, m_ref = m_new, m_off = -m_new;
           }
           huge = __any_sync(0xffffffffu, fabsf(m_off) >= 4194304.f);
-          if (huge) {  // the score rounded, as the maximum was, and then the difference
+          if (huge) {  // the score rounded, as the maximum was, and then the difference (a packed product beside the packed sum would be fused with it)
 #pragma unroll
-            for (int j = 0; j < TK; ++j) r[j] = __float_as_uint(__fadd_rn(__fmul_rn(__uint_as_float(r[j]), s), m_off));
+            for (int j = 0; j < TK; j += 2) {
+              float e0 = __fmul_rn(__uint_as_float(r[j]), s), e1 = __fmul_rn(__uint_as_float(r[j + 1]), s);
+              add2_tc(e0, e1, m_off, m_off);
+              r[j] = __float_as_uint(e0), r[j + 1] = __float_as_uint(e1);
+            }
             sx = 1.f, m_off = 0.f;
           }
         }

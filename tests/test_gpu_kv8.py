@@ -583,3 +583,10 @@ def test_calls_that_do_not_fit(L):
         with pytest.raises(AssertionError):
             bad()
     torch.cuda.synchronize()
+
+
+def test_no_wait_ran_out_to_the_end(L):
+    """in the kernels of any test of this file"""
+    from qwen_inference_engine_b200 import _lib
+    torch.cuda.synchronize()
+    assert _lib.lib().qie_kernel_status() == 0
