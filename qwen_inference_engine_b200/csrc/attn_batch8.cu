@@ -891,7 +891,7 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
         mbar_arrive_tc(bar_q + 8u * g);
       }
       const int my_pos = p.pos0 + min(tok, p.tokens - 1), my_low = a.window > 0 ? max(0, my_pos - a.window + 1) : 0;
-      // the references of the row's weights, and beside that one (rel) of its weights times the values' scales, of O; whole numbers, of what the row sees
+      // the references of the row's weights, and beside that one (rel, a whole number) of its weights times the values' scales, of O; both of what the row sees
       float m_ref = -INFINITY, m_off = 0.f, rel = 0.f, l_run = 0.f;  // m_off: what is added to scores for it
       bool again;         // the tile
       bool huge = false;  // some row's reference is so large that scores round to fewer bits than their differences need
@@ -932,9 +932,9 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
         again = false;
         if (grow) {
           again = once_more(tile);
-          const float up = ceilf(top), m_new = fmaxf(m_ref, up);
+          const float m_new = fmaxf(m_ref, top);
           if (m_new > -INFINITY) {
-            const float by = m_ref - m_new, before = rel + by, rel_new = fmaxf(before, (up - m_new) + vt);  // (nothing before: by minus infinity)
+            const float by = m_ref - m_new, before = rel + by, rel_new = fmaxf(floorf(before), ceilf((top - m_new) + vt));  // (nothing before: by minus infinity)
             l_run *= ex2_tc(by), f = ex2_tc(before - rel_new), rel = rel_new, m_ref = m_new, m_off = -m_new;
           }
           huge = __any_sync(0xffffffffu, fabsf(m_off) >= 4194304.f);
