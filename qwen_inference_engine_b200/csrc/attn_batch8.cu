@@ -4,7 +4,7 @@
 //   out_t = sum_j 2^(x_tj - m) 2^ev_j v_j / sum_j 2^(x_tj - m),  x_tj = s 2^ek_j (q_t . k_j) over the positions j that row t sees, m their running maximum, k_j and v_j codes
 //
 // Codes become fp16 exactly, in larger blocks with a power of two beside them that a tile's keys, or values, have in common.  A row's query is brought to fp16 by a power of two of its own, which
-// loses nothing, and scores are summed in fp32.  A row goes by what it sees and by nothing beside it: m is its own running maximum, and its weights, which are fp16 in the product with the values
+// loses nothing down to 2^-31 of its largest element, and scores are summed in fp32.  A row goes by what it sees and by nothing beside it: m is its own running maximum, and its weights, which are fp16 in the product with the values
 // (2^-11 of themselves), stand there times their values' scales beside the largest such product that the row itself has met (a reference of their own), so that none is off by more than 2^-31 of that,
 // in larger blocks 2^-23, where a tile has one scale for values that are at most 2^8 apart.  Weights' sums are fp32.
 //
@@ -12,13 +12,14 @@
 // of at most 16 rows (decode), which memory bounds, one that keeps a unit of keys and values in registers between loads and products, and for larger blocks one on tcgen05 / TMEM.
 //
 // What bounds them (B200, in a graph; the cache as it is read, with its scales).
-//   Few rows.  64 at 1434 positions on average, 28 heads of 128 on 4, e4m3, 96 MB: 29.6 us (over a bf16 cache 42.8).  2.3 us pass before the first copies (the requests' numbers, the search for a
+//   Few rows.  64 at 1434 positions on average, 28 heads of 128 on 4, e4m3, 96 MB: 30.2 us (over a bf16 cache 42.8).  2.3 us pass before the first copies (the requests' numbers, the search for a
 //   CTA's stretch), then units come at 4.9 TB/s until the median CTA ends at 21 us and the last one at 25, and the kernel that joins takes the rest.  4 at 70000 positions, 12 heads on 2, int8,
-//   144 MB: 38.0 (62.3).  One at 700, 14 heads of 64 on 2: 8.8 (9.4), the plan, one tile's latency and the join.
-//   Larger blocks.  8192 rows of 28 heads of 128 on 4: e4m3 564 us, 853 TFLOP/s, int8 553 (over a bf16 cache 491, which has nothing to convert).  A tile of 64 keys of 256 rows has 1024 cycles
+//   144 MB: 38.3 (62.3).  One at 700, 14 heads of 64 on 2: 9.1 (9.4), the plan, one tile's latency and the join.
+//   Larger blocks.  8192 rows of 28 heads of 128 on 4: e4m3 563 us, 855 TFLOP/s, int8 573 (over a bf16 cache 491, which has nothing to convert).  A tile of 64 keys of 256 rows has 1024 cycles
 //   of exponentials, 1280 of products and 1500 of shared memory's bandwidth (its products' operands, codes and fp16 in and out) and takes 2600.  At 586 us it was 6 % less without the exponentials'
 //   instructions, 13 % without the conversion's arithmetic, 6 % without maxima, 11 % with an eighth of Q K^T: several chains of a tile (scores, softmax, product; copy, conversion) are about as
-//   long as each other.  An item's beginning and end, at which both row tiles drain, cost 7 us.
+//   long as each other, and their code only just has room in the instruction caches: forms of the same instructions in other places took from 547 to 890 us.  An item's beginning and end, at
+//   which both row tiles drain, cost 7 us.  A tile that is gone through twice takes twice as long: one key or value of each 64 2^20 below the others 1041 us, all values of 2^0 .. 2^60 4614.
 #include <cuda.h>
 
 #include <algorithm>
@@ -986,7 +987,7 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         mbar_arrive_tc(bar_p + 16u * g + 8u * b);
       }
-      // ---- the row of the result, and (heads of 128) the next piece while the last product is under way: 8192 rows 586 -> 562 us; with heads of 64 16 portions 107 -> 108
+      // ---- the row of the result, and (heads of 128) the next piece while the last product is under way: 8192 rows 586 -> 564 us; with heads of 64 16 portions 107 -> 108
       const bool whole = p.whole();
       bf16* dst = a.out + (size_t)(p.t0 + tok) * a.out_stride + (size_t)(p.kvh * G + gh) * HD;
       float* part = parts + ((size_t)blockIdx.x * 2 + (p.begin == 0)) * PART<HD, ROWS_P>;
@@ -1075,8 +1076,9 @@ size_t attention_batch8_work(int hd, int num_sms) { return work_few(hd, num_sms)
 cudaError_t launch_attention_batch8(const BatchAttnArgs& a, const Kv8Geom& kv, cudaStream_t st) {
   const int group = a.n_q / kv.n_kv, g = std::min(group, ROWS_F), P = kv.page_size;
   const JoinShape sh{g, group, (group + g - 1) / g};
-  // Requests of so many rows that their keys and values are read once or twice by blocks of few rows are theirs, the others have blocks of up to 256 (a decode row in one of those costs
-  // what 256 rows do: 48 of them at 2800 positions on average beside four portions of a prompt 105 us, by both kernels 82; 16 portions without decode rows 104 and 105).  Where the step has no more rows than requests, all of them
+  // Requests of at most 16 rows of a kv head are for blocks of few rows, which read their keys and values once to three times (once for each 16 heads of a larger group); the others have blocks
+  // of up to 256 (a decode row in one of those costs what 256 rows do: 48 of them at 2800 positions on average beside four portions of a prompt 105 us, by both kernels 92; 16 portions without
+  // decode rows 104 and 111, of which 6 are the kernel that finds nothing and begins when the other one has ended).  Where the step has no more rows than requests, all of them
   // are blocks of few rows (a request with many rows reads its keys and values that much more often); the room counts, which the host knows, and not the step's rows, which it does not.
   const bool few = a.n_tok <= a.n_req;
   // boxes of the most rows, a power of two, that divide a page and a unit or tile; a tile's scales come by bulk copies of a multiple of 16 bytes
