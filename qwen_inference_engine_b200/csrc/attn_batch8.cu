@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(Ring<HD>::THR, NB == 1 ? 2 : 1) attn_few8_kern
             float rx = fmaxf(fmaxf((x[nb][0][e] - to) + ve[0], (x[nb][0][e + 2] - to) + ve[1]), fmaxf((x[nb][1][e] - to) + ve[2], (x[nb][1][e + 2] - to) + ve[3]));
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) rx = fmaxf(rx, __shfl_xor_sync(0xffffffffu, rx, d));
-            const float before = rel[nb][e] + (m[nb][e] - to), f = ex2_tc(before - fmaxf(before, rx));  // (nothing before: 0, of zeros)
+            const float before = fmaxf(rel[nb][e] + (m[nb][e] - to), NOTHING), f = ex2_tc(before - fmaxf(before, rx));  // (a number, where all values so far are zeros too)
             l[nb][e] *= ex2_tc(m[nb][e] - to);
             m[nb][e] = to, rel[nb][e] = fmaxf(before, rx);
 #pragma unroll

@@ -226,3 +226,19 @@ def test_a_step_of_rows_that_end_apart(L):
         out = r.attend(L)
         for i in range(len(lens)):
             check(r, i, out, few or lens[i][1] == 1)
+
+
+@pytest.mark.parametrize("lens,nq,nkv,few", [([(9000, 1)] * 4, 8, 4, True), ([(600, 300)], 4, 2, False)])
+@pytest.mark.parametrize("first", [150, 4000])
+@pytest.mark.parametrize("j", [0, 1])
+def test_first_keys_of_zeros(L, j, first, lens, nq, nkv, few):
+    """the first positions' keys, or values, are zeros: whole units and tiles of them ahead of others of the same stretch"""
+    r = requests(L, lens, nq, nkv, 128, "e4m3", seed=16, room=0 if few else 4)
+    for i, (c, m) in enumerate(lens):
+        pg, at = r.kv_at[i]
+        n = min(first, c - 10)
+        r.scale[pg[:n], r.layer, j, :, at[:n]] = 0
+        (r.k, r.v)[j][i][:n] = 0
+    out = r.attend(L)
+    for i in range(len(lens)):
+        check(r, i, out, few)
