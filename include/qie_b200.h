@@ -257,7 +257,7 @@ int qie_kv8_read(const qie_kv8_view* kv, int layer, const int* row, int n_rows, 
  * scores and sums are fp32, weights are fp16 in the product with the values: a key's part of the result, weight * scale * code, is off by at most 2^-11 of itself or, times its code, by 2^-31 of the
  * row's largest weight * scale (2^-23 in larger blocks: of requests with more than 16 / min(16, n_q / n_kv) rows, where max_tokens is above n_req), whatever the scales of the others and
  * whatever lies at positions that the row does not see.  In larger blocks 64 keys next to each other are gone through in one step where their keys' scales are at most 2^15 (int8 2^24) apart
- * and their values' at most 2^8, and otherwise in a step for each of their groups that are.  Codes of e4m3 that are no numbers make rows that see them no numbers, in that column at least, and
+ * and their values' at most 2^8 (values of zeros have a group of their own), and otherwise in a step for each of their groups that are.  Codes of e4m3 that are no numbers make rows that see them no numbers, in that column at least, and
  * no other row. */
 int qie_attention_batch8(const qie_kv8_view* kv, int layer, const qie_batch* b, const qie_bf16* Q, size_t q_stride, qie_bf16* out, size_t out_stride,
                          int n_q_heads, int window, float scale, qie_stream st);

@@ -468,7 +468,10 @@ template <int CODE>
 constexpr uint32_t KEYS_APART = CODE == KV8_E4M3 ? 15 : 24;
 constexpr uint32_t VALUES_APART = 8;
 constexpr uint32_t NONE_H2 = 0x7e007e00u, CLEAR_H2 = 0xffffffffu;  // factors: no numbers; (of values) zeros, whatever the codes
-__device__ __forceinline__ bool far_below(uint32_t byte, uint32_t top, uint32_t apart) { return byte != 0 && byte + apart < top; }  // (zeros: at any scale; no numbers: above all)
+__device__ __forceinline__ bool far_below(uint32_t byte, uint32_t top, uint32_t apart) { return byte + apart < top; }  // (no numbers: above all)
+// a key of zeros has its score beside any scale; a value of zeros is far below others, as its weight says nothing about their products
+template <int CODE>
+__device__ __forceinline__ bool key_far(uint32_t byte, uint32_t top) { return byte != 0 && far_below(byte, top, KEYS_APART<CODE>); }
 template <int HD>
 struct SmemP {
   static constexpr bool Q_TMEM = HD == 64;
@@ -668,13 +671,13 @@ __global__ void __launch_bounds__(THR_P, 1) attn_prompt8_kernel(BatchAttnArgs a,
               if (in[h] && vb[h] != 255) vt = max(vt, vb[h]);
             }
             kt = __reduce_max_sync(0xffffffffu, kt), vt = __reduce_max_sync(0xffffffffu, vt);
-            auto far = [&](int h) { return in[h] && (far_below(kb[h], kt, KEYS_APART<CODE>) || far_below(vb[h], vt, VALUES_APART)); };
+            auto far = [&](int h) { return in[h] && (key_far<CODE>(kb[h], kt) || far_below(vb[h], vt, VALUES_APART)); };
             word = 0;
             if (__any_sync(0xffffffffu, far(0) || far(1))) {  // of the keys near the largest those whose values are near the largest of theirs; the others another time
               vt = 1;
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
-                now[h] = in[h] && !far_below(kb[h], kt, KEYS_APART<CODE>);
+                now[h] = in[h] && !key_far<CODE>(kb[h], kt);
                 if (now[h] && vb[h] != 255) vt = max(vt, vb[h]);
               }
               vt = __reduce_max_sync(0xffffffffu, vt);

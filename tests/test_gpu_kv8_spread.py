@@ -228,7 +228,25 @@ def test_a_step_of_rows_that_end_apart(L):
             check(r, i, out, few or lens[i][1] == 1)
 
 
-@pytest.mark.parametrize("lens,nq,nkv,few", [([(9000, 1)] * 4, 8, 4, True), ([(600, 300)], 4, 2, False)])
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("few,case", [(True, c) for c in FEW] + [(False, c) for c in MANY])
+@pytest.mark.parametrize("zeros", [40, 10 ** 6])
+def test_values_that_are_zeros(L, kind, hd, few, case, zeros):
+    """many values in a row that are zeros, at the beginning or all of them, with keys that are none"""
+    lens, nq, nkv = case
+    r = requests(L, lens, nq, nkv, hd, kind, seed=15)
+    for i, (c, m) in enumerate(lens):
+        for p in range(0 if zeros > c + m else max(0, c - zeros) // 2, min(zeros + c // 2, c + m)):
+            scaled(r, i, p, 1, torch.zeros(nkv))
+    out = r.attend(L)
+    for i in range(len(lens)):
+        check(r, i, out, few)
+        if zeros > sum(lens[i]):
+            assert (out[r.start[i]:r.start[i + 1]] == 0).all()
+
+
+@pytest.mark.parametrize("lens,nq,nkv,few", [([(9000, 1)] * 4, 8, 4, True), ([(100, 333)], 14, 2, False), ([(600, 300)], 4, 2, False)])
 @pytest.mark.parametrize("first", [150, 4000])
 @pytest.mark.parametrize("j", [0, 1])
 def test_first_keys_of_zeros(L, j, first, lens, nq, nkv, few):
@@ -242,3 +260,20 @@ def test_first_keys_of_zeros(L, j, first, lens, nq, nkv, few):
     out = r.attend(L)
     for i in range(len(lens)):
         check(r, i, out, few)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("few,case", [(True, c) for c in FEW] + [(False, c) for c in MANY])
+def test_a_value_of_zeros_that_takes_the_weight(L, hd, few, case):
+    """a key that every row lies on, e^40 above the others, with a value of zeros: the result is the others', small as it is"""
+    lens, nq, nkv = case
+    r = requests(L, lens, nq, nkv, hd, "e4m3", seed=17)
+    r.q.view(-1, nq, hd)[..., 0] = 4.0
+    at = lens[0][0] // 2
+    pg, slot = int(r.kv_at[0][0][at]), int(r.kv_at[0][1][at])
+    codes = torch.zeros(hd, device="cuda")
+    codes[0] = 112.0 if hd == 128 else 80.0  # 4 * 112 / sqrt(128), 4 * 80 / 8: about 40
+    r.codes[pg, r.layer, 0, :, slot] = codes.to(DTYPES["e4m3"]).view(torch.uint8)
+    scaled(r, 0, at, 0, torch.full((nkv,), 127))
+    scaled(r, 0, at, 1, torch.zeros(nkv))
+    check(r, 0, r.attend(L), few)
